@@ -224,7 +224,7 @@ def prepare(case, seed):
             nbytes = o.attn_tree_ws_bytes(T, nqh, nkvh, n_ctx)
         elif kind == "blocks":
             st["idx"] = torch.empty(T, nkvh, case["nsel"], dtype=torch.int32, device=DEV)
-            nbytes = max(o.attn_select_ws_bytes(T, nqh, nkvh, n_ctx), o.attn_blocks_ws_bytes(T, nqh, nkvh, case["nsel"]))
+            nbytes = max(o.attn_select_ws_bytes(T, nkvh, n_ctx), o.attn_blocks_ws_bytes(T, nqh, nkvh, case["nsel"]))
         else:
             nbytes = 0
         st["ws"] = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
