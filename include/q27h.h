@@ -171,6 +171,75 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
                    int n_ctx, int q8, q27h_stream_t s, const void* pf, size_t pf_bytes, const int* rope3,
                    const int* rdelta);
 
+/* ---------------------------------------------------------------- attention over the cache
+ * No counterpart in the reference's launchers (its attn_decode / attn_prefill are other functions). All of them read
+ * caches in the layout that attn_prep writes (f16, or q8_0 where q8 != 0), qn [T][nqh][256] as attn_prep leaves it, and
+ * the device integer *pos0 = rows of the context before this batch. Rows outside [0, n_ctx) are never read or written.
+ * float32 results: no operand is rounded to fewer bits than the cache holds.
+ * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
+ * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
+ * at the same time, need one each.
+ *
+ * attn_tree: attention of T <= 64 drafted tokens whose K / V attn_prep wrote to rows *pos0 + t. Token t sees every row
+ * before *pos0 and row *pos0 + u where bit u of tree[t] (device, 64-bit; bits >= T are ignored) is set: its ancestors
+ * and, usually, itself. tree NULL: a chain (bits 0 .. t); T = 1 with NULL is plain decoding.
+ * o [T][nqh][256] = sum_j p_j v_j, p = softmax over the rows seen of scale * q . k_j; lse [T][nqh] (may be NULL) =
+ * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. o may not overlap qn. nqh % nkvh == 0: query head h reads kv
+ * head h / (nqh / nkvh). Rotary positions of a tree are given to attn_prep through rope3. */
+size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx);
+int q27h_attn_tree(const float* qn, const void* kcache, const void* vcache, const int* pos0, const uint64_t* tree, int T,
+                   float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws, size_t ws_bytes,
+                   q27h_stream_t s);
+/* attn_weights: the attention each cache row received, acc [nkvh][n_ctx]. For the tokens t of `rows` (device, 64-bit mask;
+ * NULL = all T) and the query heads h of a kv head, with lse as attn_tree gave it for the same arguments:
+ * acc[j] += sum_t sum_h exp(scale * q . k_j - lse[t][h]) for rows j < *pos0, and acc[j] = that sum for the batch's own
+ * rows *pos0 .. *pos0 + T - 1, whose weights begin here. The same bits on every call. */
+int q27h_attn_weights(const float* qn, const float* lse, const void* kcache, const int* pos0, const uint64_t* tree,
+                      const uint64_t* rows, int T, float scale, int nqh, int nkvh, int n_ctx, int q8, float* acc,
+                      q27h_stream_t s);
+/* kv_evict: of the n = min(*pos0, n_ctx) rows, each kv head keeps the first `first`, the last `last` and, of those
+ * between, the keep - first - last of the largest acc (equal ones: the lower row; NaN below all); all where n <= keep.
+ * Kept rows move, in order, to rows 0 .. of kout / vout / acc_out, whose context is n_ctx_out >= keep rows; rows behind
+ * them are left as they were. The outputs are the inputs themselves (all three, n_ctx_out = n_ctx: in place) or overlap
+ * none of them. kept [nkvh][keep] (may be NULL): the kept rows' numbers, -1 behind the last.
+ * acc is only read between its ends: attn_weights starts the weights of rows written later. */
+size_t q27h_kv_evict_ws_bytes(int nkvh, int n_ctx, int keep, int q8, int in_place);
+int q27h_kv_evict(const void* kcache, const void* vcache, const float* acc, const int* pos0, int keep, int first, int last,
+                  void* kout, void* vout, float* acc_out, int n_ctx_out, int* kept, int nkvh, int n_ctx, int q8, void* ws,
+                  size_t ws_bytes, q27h_stream_t s);
+/* kv_evict_pos: after the caches of every layer were evicted, *pos0 = min(*pos0, keep), and *rdelta (may be NULL) falls
+ * by the rows that went, so that attn_prep's rotary position *pos0 + t - *rdelta goes on where it was. */
+int q27h_kv_evict_pos(int* pos0, int* rdelta, int keep, q27h_stream_t s);
+/* kv_accept: moves the accepted path of a verified tree to its place: row *pos0 + path[i] to row *pos0 + i, for
+ * i < *n_path <= T <= 64 (path, n_path: device), in each of n_caches K or V caches and n_accs acc arrays (host arrays of
+ * device pointers, read during the call; no two may overlap), one launch for up to 64 of each. The path ends at its first
+ * entry outside [0, T). *pos0 is not moved. */
+int q27h_kv_accept(void* const* caches, int n_caches, float* const* accs, int n_accs, const int* pos0, const int* path,
+                   const int* n_path, int T, int nkvh, int n_ctx, int q8, q27h_stream_t s);
+/* kv_block_bounds: bounds of the blocks of 64 K rows that the batch's rows *pos0 .. *pos0 + T - 1 touch, from their rows
+ * before *pos0 + T (any T; with *pos0 = 0 the whole context). kb, q27h_kv_block_bytes() bytes, 16-byte aligned:
+ * lo int8 [nkvh][nblk][256], hi the same, d f32 [nkvh][nblk], nblk = ceil(n_ctx / 64). Per block, over its channels'
+ * least and greatest values: d = amax / 127 (0 for amax < 2^-100), code = roundf(x * (1 / d)); a block with an infinity
+ * or NaN gets codes 0 and d = +inf, and scores +inf. Rows moved by kv_evict or kv_accept need new bounds. */
+size_t q27h_kv_block_bytes(int nkvh, int n_ctx);
+int q27h_kv_block_bounds(const void* kcache, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* kb, q27h_stream_t s);
+/* attn_select: the blocks that token t (at row *pos0 + t) reads, per kv head: idx [T][nkvh][nsel], ascending, -1 behind
+ * the last. Candidates are the blocks up to its own; always taken are the first `first` and the last `last` >= 1 of them
+ * (first + last <= nsel), the rest by score, equal ones the lower block. score = max over the kv head's query heads
+ * (at most 16) of float(sum_c max(q_c lo_c, q_c hi_c)) * dq, times d, with q quantized over its 256 values as the bounds
+ * are (codes 0 where it is not finite): whole numbers and three float roundings, the same on every call.
+ * n_ctx <= 1024000. */
+size_t q27h_attn_select_ws_bytes(int T, int nkvh, int n_ctx);
+int q27h_attn_select(const float* qn, const void* kb, const int* pos0, int T, int nqh, int nkvh, int n_ctx, int nsel, int first,
+                     int last, int* idx, void* ws, size_t ws_bytes, q27h_stream_t s);
+/* attn_blocks: attn_tree's o and lse of a causal batch of any T (token t sees rows <= *pos0 + t), over the rows of the
+ * listed blocks only: idx [T][nkvh][nsel], any order; entries that are no block of the token's context are skipped, a
+ * block listed twice counts twice. At most 16 query heads per kv head. */
+size_t q27h_attn_blocks_ws_bytes(int T, int nqh, int nkvh, int nsel);
+int q27h_attn_blocks(const float* qn, const void* kcache, const void* vcache, const int* pos0, const int* idx, int T, int nsel,
+                     float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws, size_t ws_bytes,
+                     q27h_stream_t s);
+
 /* ---------------------------------------------------------------- quantized embedding gather */
 /* get_rows_iq2_s (src/ops.h:22-23, src/ops.cu:756-766): rows ids[t] (device) of an IQ2_S table (82-byte
  * super-blocks, row_bytes apart) -> f32 y [T][n], n % 256 == 0; id < 0 copies row (-id - 1) of img [..][n]

@@ -62,6 +62,19 @@ SIGNATURES = {
     "q27h_add_norm_rows_q8": [_p, _p, _p, _i, _i, _p, _f, _p, _p, _p, _p, _i, _p],
     "q27h_kv_cache_bytes": [_i, _i, _i],
     "q27h_attn_prep": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _f, _i, _i, _i, _i, _p, _p, _sz, _p, _p],
+    "q27h_attn_tree_ws_bytes": [_i, _i, _i, _i],
+    "q27h_attn_tree": [_p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _p, _p, _p, _sz, _p],
+    "q27h_attn_weights": [_p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _p, _p],
+    "q27h_kv_evict_ws_bytes": [_i, _i, _i, _i, _i],
+    "q27h_kv_evict": [_p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _i, _p, _i, _i, _i, _p, _sz, _p],
+    "q27h_kv_evict_pos": [_p, _p, _i, _p],
+    "q27h_kv_accept": [_p, _i, _p, _i, _p, _p, _p, _i, _i, _i, _i, _p],
+    "q27h_kv_block_bytes": [_i, _i],
+    "q27h_kv_block_bounds": [_p, _p, _i, _i, _i, _i, _p, _p],
+    "q27h_attn_select_ws_bytes": [_i, _i, _i],
+    "q27h_attn_select": [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _sz, _p],
+    "q27h_attn_blocks_ws_bytes": [_i, _i, _i, _i],
+    "q27h_attn_blocks": [_p, _p, _p, _p, _p, _i, _i, _f, _i, _i, _i, _i, _p, _p, _p, _sz, _p],
     "q27h_get_rows_iq2_s": [_p, _i64, _p, _i, _p, _i, _p, _p],
     "q27h_get_rows_q4_k": [_p, _i64, _p, _i, _p, _i, _p, _p],
     "q27h_get_rows_q6_k": [_p, _i64, _p, _i, _p, _i, _p, _p],
@@ -89,7 +102,9 @@ SIGNATURES = {
     "q27h_last_error": [],
     "q27h_abi_version": [],
 }
-_RESTYPE = {"q27h_kv_cache_bytes": _sz, "q27h_qmat_bytes": _sz, "q27h_last_error": C.c_char_p,
+_RESTYPE = {"q27h_kv_cache_bytes": _sz, "q27h_attn_tree_ws_bytes": _sz, "q27h_kv_evict_ws_bytes": _sz,
+            "q27h_kv_block_bytes": _sz, "q27h_attn_select_ws_bytes": _sz, "q27h_attn_blocks_ws_bytes": _sz,
+            "q27h_qmat_bytes": _sz, "q27h_last_error": C.c_char_p,
             "q27h_gtype_name": C.c_char_p, "q27h_gguf_close": None, "q27h_gguf_n_tensors": _i64, "q27h_gguf_find": _i64,
             "q27h_gguf_n_kv": _i64}
 

@@ -1,0 +1,476 @@
+// One wave's work on a tile of 32 rows of the K/V cache, shared by the kernels that read it (attn_tree.hip).
+//
+// Scores and outputs are float32 results of 16-bit matrix instructions. The cache's values enter them exactly: an f16
+// cache as it is, a q8_0 cache as its codes (|code| <= 127 is exact in f16), with the f16 scales applied outside. The
+// other operand (q, or the weight p times V's scale) is split in two f16 terms, x = hi + lo, each product exact in the
+// instruction's float32 sum, so what is lost is below 2^-21 of a term; one f16 term would lose 2^-12 of it.
+//
+// mfma_f32_16x16x32_f16: lane l holds row (A) or column (B) l & 15 and the eight k = 8 (l >> 4) + e; of the result it
+// holds column l & 15, rows 4 (l >> 4) + i. Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a
+// lane holds scores, weights and outputs of ONE query row n = l & 15: the softmax needs no exchange between lanes but
+// the sum and the (rare) new maximum over its 4 lanes g = l >> 4, and the scores of a lane are already the second
+// product's operand. Row numbers of the tile in a lane: 16 u + 4 g + i (u = 0, 1; i = 0..3), in the order e = 4 u + i.
+#pragma once
+#include "q27h_device.h"
+
+namespace q27h {
+
+constexpr int kHD = 256;       // head width
+constexpr int kTileKeys = 32;  // cache rows of one wave's step
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ uint32_t pk_rtz(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// x - (float)h, exact for h = x rounded towards zero. The opaque -1 keeps the fma, which v_fma_mix_f32 does on the half
+// itself; a plain difference is two instructions (measured: 64 fewer of 690 in a tile).
+__device__ __forceinline__ float minus_half(float x, uint32_t pair, int hi) {
+  const h2 v = __builtin_bit_cast(h2, pair);
+  float m1 = -1.0f;
+  asm("" : "+s"(m1));
+  return __builtin_fmaf((float)(hi ? v[1] : v[0]), m1, x);
+}
+__device__ __forceinline__ float half_of(uint32_t pair, int hi) {
+  const h2 v = __builtin_bit_cast(h2, pair);
+  return (float)(hi ? v[1] : v[0]);
+}
+// Four int8 codes -> four halves of value code * 2^-9: byte ^ 0x80 = code + 128 = u, which as the low byte of a half is
+// the subnormal u 2^-24; fma(u 2^-24, 2^15, -2^-2) = (u - 128) 2^-9, exact. ev = codes 0, 2; od = codes 1, 3.
+__device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& ev, uint32_t& od) {
+  const h2 k = {(_Float16)32768.0f, (_Float16)32768.0f}, m = {(_Float16)-0.25f, (_Float16)-0.25f};
+  x ^= 0x80808080u;
+  const h2 a = __builtin_bit_cast(h2, x & 0x00ff00ffu);
+  const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, x, 0x0c030c01u));
+  ev = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(a, k, m));
+  od = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, k, m));
+}
+// Eight codes in two dwords -> the operand of eight halves; the order of the eight is 0, 2, 1, 3, 4, 6, 5, 7.
+__device__ __forceinline__ h8 codes8(uint32_t x, uint32_t y) {
+  uint32_t r[4];
+  codes_to_half(x, r[0], r[1]);
+  codes_to_half(y, r[2], r[3]);
+  return __builtin_bit_cast(h8, (u4){r[0], r[1], r[2], r[3]});
+}
+
+// Where a K or V cache of one kv head lies.
+struct KvHead {
+  const uint8_t* rows;   // q8: int8 [n_ctx][256]; else f16 [n_ctx][256]
+  const uint8_t* scale;  // q8: f16 [n_ctx][8]
+};
+template <bool Q8>
+__device__ __forceinline__ KvHead kv_head(const void* cache, int kh, int nkvh, int n_ctx) {
+  KvHead h;
+  h.rows = (const uint8_t*)cache + (size_t)kh * n_ctx * (Q8 ? kHD : 2 * kHD);
+  h.scale = (const uint8_t*)cache + (size_t)nkvh * n_ctx * kHD + (size_t)kh * n_ctx * 16;
+  return h;
+}
+
+// ---------------------------------------------------------------- queries
+// LDS image of 16 query rows: [hi, lo][b = 32-dim block][lane] of 16 bytes, and per row the factor that takes a score from
+// the operands' units to log2 units. A row is scaled by the power of two that brings its largest value into [1, 2) before
+// the split, so neither very large nor very small queries leave f16's range.
+struct QTile {
+  alignas(16) uint32_t v[2][8][64][4];
+  float c[16];
+};
+
+// All WAVES waves of the workgroup. Row r (0 .. 16 tiles - 1) is `row_ptr(r)` (nullptr: zeros). q8 caches: the eight
+// values of a lane are stored in the order of codes8, and the factor carries codes8's 2^-9.
+template <bool Q8, int WAVES, typename F>
+__device__ __forceinline__ void load_queries(QTile* im, int tiles, float mult, F row_ptr) {
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
+  for (int r = w; r < tiles * 16; r += WAVES) {
+    const float* src = row_ptr(r);
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (src) {
+      const float4 t = ld4(src + 4 * l);
+      x[0] = t.x * mult, x[1] = t.y * mult, x[2] = t.z * mult, x[3] = t.w * mult;
+    }
+    float a = __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
+                              __builtin_fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
+    a = __builtin_fmaxf(a, lane_xor<1>(a));
+    a = __builtin_fmaxf(a, lane_xor<2>(a));
+    a = __builtin_fmaxf(a, lane_xor<7>(a));
+    a = __builtin_fmaxf(a, lane_xor<8>(a));
+    a = __builtin_fmaxf(a, lane_xor<16>(a));
+    a = __builtin_fmaxf(a, lane_xor32(a));
+    int e = (int)((__builtin_bit_cast(uint32_t, a) >> 23) & 255) - 127;
+    e = e > 110 ? 110 : e < -110 ? -110 : e;  // a zero row keeps -110 (its scores are 0); inf and NaN stay what they are
+    const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] *= down;
+    const int o[4] = {0, Q8 ? 2 : 1, Q8 ? 1 : 2, 3};
+    const int b = l >> 3, slot = ((l >> 1) & 3) * 16 + (r & 15), at = (l & 1) * 2;
+    const uint32_t h0 = pk_rtz(x[o[0]], x[o[1]]), h1 = pk_rtz(x[o[2]], x[o[3]]);
+    const uint32_t l0 = pk_rtz(minus_half(x[o[0]], h0, 0), minus_half(x[o[1]], h0, 1));
+    const uint32_t l1 = pk_rtz(minus_half(x[o[2]], h1, 0), minus_half(x[o[3]], h1, 1));
+    *(u2*)&im[r >> 4].v[0][b][slot][at] = (u2){h0, h1};
+    *(u2*)&im[r >> 4].v[1][b][slot][at] = (u2){l0, l1};
+    if (l == 0) im[r >> 4].c[r & 15] = __builtin_bit_cast(float, (uint32_t)(127 + e + (Q8 ? 9 : 0)) << 23);
+  }
+}
+
+// ---------------------------------------------------------------- 32 rows of K or V
+// Rows of a tile are addressed from its first row j0 (the same in the whole wave). TAIL: only `left` rows of the tile
+// exist; a row behind them reads the last one (it is hidden, and must not be read outside the cache).
+template <bool TAIL>
+__device__ __forceinline__ int tile_row(int j, int left) {
+  return TAIL ? (j < left ? j : left - 1) : j;
+}
+
+// q8: rows of codes as they lie, 16 bytes a lane (row 4 r + g, bytes 16 n ..), and four of the 256 scales (row l >> 1,
+// blocks 4 (l & 1) .. + 3). Both go through LDS: the codes to be regrouped (K: 8 bytes of a row per lane, V: 8 rows of a
+// column), the scales so that a lane's registers hold 4 and not the 64 it uses.
+struct QRows {
+  u4 x[8];
+  u2 s;
+};
+// One wave's LDS: 272 bytes a row of codes (4 banks on), the upper 16 rows 128 bytes (32 banks) on: the 32 lanes that read
+// together touch every bank once, for K (16 rows, two 8-byte pieces) as for V (two lane groups, 8 rows of 16 bytes).
+// K's codes are consumed before V's are staged in their place. Then the scales of K and of V: halves [block b][32 rows].
+constexpr int kRow = 272, kUpper = 16 * kRow + 128, kCodes = kUpper + 16 * kRow;
+constexpr int kScales = 8 * 64;
+struct WaveLds {
+  alignas(16) uint8_t codes[kCodes];
+  alignas(16) uint8_t ks[kScales], vs[kScales];
+};
+
+// TAIL: scales of rows that do not exist are 0: whatever the memory behind the last row holds, NaN included, must not meet
+// a weight of 0 in the product.
+template <bool TAIL>
+__device__ __forceinline__ void load_rows(QRows& t, const KvHead& h, int j0, int left) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const uint8_t* rows = h.rows + (size_t)j0 * kHD;
+#pragma unroll
+  for (int r = 0; r < 8; r++) {
+    if (TAIL) t.x[r] = *(const u4*)(rows + (unsigned)(tile_row<TAIL>(4 * r + g, left) * kHD + 16 * n));
+    else t.x[r] = *(const u4*)(rows + (r >> 2) * 16 * kHD + (unsigned)(g * kHD + 16 * n) + (r & 3) * 4 * kHD);
+  }
+  t.s = *(const u2*)(h.scale + (size_t)j0 * 16 + (unsigned)(tile_row<TAIL>(l >> 1, left) * 16 + 8 * (l & 1)));
+  if (TAIL && (l >> 1) >= left) t.s = (u2){0u, 0u};
+}
+__device__ __forceinline__ void stage_rows(const QRows& t, uint8_t* codes, uint8_t* scales) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+#pragma unroll
+  for (int r = 0; r < 8; r++)
+    *(u4*)(codes + (r >= 4 ? kUpper + (4 * (r - 4) + g) * kRow : (4 * r + g) * kRow) + 16 * n) = t.x[r];
+  uint16_t* p = (uint16_t*)scales + 4 * (l & 1) * 32 + (l >> 1);
+  p[0] = (uint16_t)t.s.x;
+  p[32] = (uint16_t)(t.s.x >> 16);
+  p[64] = (uint16_t)t.s.y;
+  p[96] = (uint16_t)(t.s.y >> 16);
+  __builtin_amdgcn_wave_barrier();
+}
+// Scales of block b of the lane's rows 16 u + 4 g + i, four halves.
+__device__ __forceinline__ u2 scales_of(const uint8_t* scales, int b, int u) {
+  const int g = (threadIdx.x & 63) >> 4;
+  return *(const u2*)(scales + b * 64 + 32 * u + 8 * g);
+}
+
+// f16: K as operand rows (row 16 u + n, dims 32 b + 8 g .. + 7); V as halves 8 n .. + 7 and 128 + 8 n .. + 7 of the lane's
+// rows 16 u + 4 g + i.
+struct HKeys {
+  u4 x[2][8];
+};
+struct HValues {
+  u4 x[8][2];
+};
+template <bool TAIL>
+__device__ __forceinline__ void load_rows(HKeys& t, const KvHead& h, int j0, int left) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    // one offset register and immediate offsets: separate offsets for the 16 loads would cost as many registers
+    const uint8_t* p = h.rows + (size_t)j0 * (2 * kHD) + (unsigned)(tile_row<TAIL>(16 * u + n, left) * (2 * kHD) + 16 * g);
+#pragma unroll
+    for (int b = 0; b < 8; b++) t.x[u][b] = *(const u4*)(p + 64 * b);
+  }
+}
+template <bool TAIL>  // rows that do not exist are zeros, as the scales above
+__device__ __forceinline__ void load_rows(HValues& t, const KvHead& h, int j0, int left) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const uint8_t* rows = h.rows + (size_t)j0 * (2 * kHD);
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int j = 16 * (e >> 2) + 4 * g + (e & 3);
+    const uint8_t* p = TAIL ? rows + (unsigned)(tile_row<TAIL>(j, left) * (2 * kHD) + 16 * n)
+                            : rows + (e >> 2) * 32 * kHD + (unsigned)(8 * g * kHD + 16 * n) + (e & 3) * 2 * kHD;
+    t.x[e][0] = *(const u4*)p;
+    t.x[e][1] = *(const u4*)(p + kHD);
+    if (TAIL && j >= left) t.x[e][0] = t.x[e][1] = (u4){0u, 0u, 0u, 0u};
+  }
+}
+template <bool Q8>
+struct Tiles;
+template <>
+struct Tiles<true> {
+  typedef QRows K;
+  typedef QRows V;
+};
+template <>
+struct Tiles<false> {
+  typedef HKeys K;
+  typedef HValues V;
+};
+
+// Scores in the operands' units: s[rt][u][i] of tile row 16 u + 4 g + i and query row n of im[rt]. q8: `w` holds the
+// staged codes and scales.
+template <int RT>
+__device__ __forceinline__ void scores(const WaveLds& w, const QTile* im, f4 (&s)[RT][2]) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  const uint8_t* row = w.codes + n * kRow + 8 * g;
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    if (b) __builtin_amdgcn_sched_barrier(0);  // block by block: all eight at once would not fit the registers
+    h8 k[2];
+    u2 ks[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const u2 x = *(const u2*)(row + kUpper * u + 32 * b);
+      k[u] = codes8(x.x, x.y);
+      ks[u] = scales_of(w.ks, b, u);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+      const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        f4 c = mfma16(k[u], ql, (f4){0.0f, 0.0f, 0.0f, 0.0f});
+        c = mfma16(k[u], qh, c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[rt][u][i] = __builtin_fmaf(half_of(ks[u][i >> 1], i & 1), c[i], s[rt][u][i]);
+        asm("" : "+v"(s[rt][u]));  // formed here: sunk to their first use, the eight blocks' products would pile up
+      }
+    }
+  }
+}
+template <int RT>
+__device__ __forceinline__ void scores(const HKeys& t, const QTile* im, f4 (&s)[RT][2]) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    if (b) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+      const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), ql, s[rt][u]);
+        s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), qh, s[rt][u]);
+      }
+    }
+  }
+}
+
+// Which rows of a tile a query row sees: every one before n, and row n0 + t where bit t of `tree` is set (rows at or
+// behind `end` are none).
+struct Vis {
+  int n;    // rows [0, n) are seen by all
+  int n0;   // first drafted row (may lie outside the cache)
+  int end;  // one past the last row that exists
+};
+template <int RT>
+__device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint64_t (&tree)[RT], int j0) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int j = j0 + 16 * u + 4 * g + i;
+      const unsigned d = (unsigned)(j - vis.n0);
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) {
+        const bool seen = j < vis.n || (j < vis.end && d < 64u && ((tree[rt] >> (d & 63u)) & 1));
+        s[rt][u][i] = seen ? s[rt][u][i] : -__builtin_huge_valf();
+      }
+    }
+}
+
+// ---------------------------------------------------------------- online softmax
+// State of 16 query rows in a wave: lane (n, g) holds of row n the reference M (the same in its four lanes), its own part
+// of the sum l and 64 outputs. Weights are p = 2^(s - M). M is not the maximum itself: it is only moved when p times the
+// largest V scale seen would leave f16's range, that is when s - M > 15 - k (largest scale < 2^k; k = 0 for an f16 cache,
+// whose values multiply p inside the instruction), and then to s - (12 - k), so that the largest products lie near 2^12,
+// where the two f16 terms hold 22 bits, and small ones down to 2^-36 of them are still in range.
+// O, l and M of different waves and workgroups are joined by M alone.
+struct Rows {
+  f4 o[16];
+  float m, l, c;
+  int k;
+  float lim;  // 2^k; 0 before the first nonzero scale
+};
+
+template <bool Q8>
+__device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) st.o[i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  st.m = -3.0e38f;
+  st.l = 0.0f;
+  st.c = im.c[threadIdx.x & 15];
+  st.k = Q8 ? -24 : 0;
+  st.lim = Q8 ? 0.0f : 1.0f;
+}
+
+// Keeps k and 2^k above the finite scales of a q8 tile's V rows (one that is not makes its own block's outputs what they
+// are; it must not push the other products out of range).
+__device__ __forceinline__ void widen(Rows& st, u2 scales) {
+  const h2 c = __builtin_elementwise_max(__builtin_bit_cast(h2, scales.x), __builtin_bit_cast(h2, scales.y));
+  float d = __builtin_fmaxf((float)c[0], (float)c[1]);
+  if (__any(d > st.lim)) {  // a larger V scale than any so far
+    d = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float x = half_of(i < 2 ? scales.x : scales.y, i & 1);
+      d = x < 65536.0f ? __builtin_fmaxf(d, x) : d;
+    }
+    d = __builtin_fmaxf(d, lane_xor<1>(d));
+    d = __builtin_fmaxf(d, lane_xor<2>(d));
+    d = __builtin_fmaxf(d, lane_xor<7>(d));
+    d = __builtin_fmaxf(d, lane_xor<8>(d));
+    d = __builtin_fmaxf(d, lane_xor<16>(d));
+    d = __builtin_fmaxf(d, lane_xor32(d));
+    const int e = __builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, d) >> 23) - 126);  // d < 2^e
+    if (e > st.k) st.k = e, st.lim = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+  }
+}
+// p[u][i] from the scores (hidden ones are -inf), with the reference moved where it has to be.
+__device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
+  float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0][0], s[0][1]), __builtin_fmaxf(s[0][2], s[0][3])),
+                             __builtin_fmaxf(__builtin_fmaxf(s[1][0], s[1][1]), __builtin_fmaxf(s[1][2], s[1][3])));
+  mx *= st.c;
+  if (__any(mx - st.m > (float)(15 - st.k))) {
+    mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
+    mx = __builtin_fmaxf(mx, lane_xor32(mx));
+    const float m1 = __builtin_fmaxf(st.m, mx - (float)(12 - st.k));
+    const float a = __builtin_amdgcn_exp2f(st.m - m1);
+    st.m = m1;
+    st.l *= a;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= a;
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], st.c, -st.m));
+      sum += s[u][i];
+    }
+  st.l += sum;
+}
+
+// O += P V. Output o[i][j]: q8: dim 16 i + 4 g + j; f16: dim 128 (i >> 3) + 8 (4 g + j) + (i & 7).
+// q8: `w` holds the staged codes and scales. TAIL: a hidden row's scale may be anything (a weight of 0 times an infinite
+// scale is no part of the sum).
+template <bool TAIL>
+__device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const WaveLds& w) {
+  const int l = threadIdx.x & 63, j = l & 15, g = l >> 4;
+  // the transposing read: in a group of 16 lanes, lane j gives the address of 8 bytes of row j >> 1 and gets column j of
+  // the 8 rows by 16 columns
+  const uint8_t* base = w.codes + ((j >> 1) >= 4 ? kUpper + (4 * g + (j >> 1) - 4) * kRow : (4 * g + (j >> 1)) * kRow) + 8 * (j & 1);
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    if (b) __builtin_amdgcn_sched_barrier(0);
+    h8 v[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; hh++) {
+      typedef int v2i __attribute__((ext_vector_type(2)));
+      const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(base + 32 * b + 16 * hh));
+      v[hh] = codes8((uint32_t)r.x, (uint32_t)r.y);
+    }
+    const u2 vs[2] = {scales_of(w.vs, b, 0), scales_of(w.vs, b, 1)};
+    float x[8];  // in the order of codes8: 0, 2, 1, 3, 4, 6, 5, 7
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int e = 4 * u + ((i & 1) << 1 | i >> 1);
+        x[e] = __builtin_fmaf(p[u][i], half_of(vs[u][i >> 1], i & 1), 0.0f);
+        if (TAIL) x[e] = p[u][i] == 0.0f ? 0.0f : x[e];
+      }
+    u4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      hi[e] = pk_rtz(x[2 * e], x[2 * e + 1]);
+      lo[e] = pk_rtz(minus_half(x[2 * e], hi[e], 0), minus_half(x[2 * e + 1], hi[e], 1));
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; hh++) {
+      st.o[2 * b + hh] = mfma16(v[hh], __builtin_bit_cast(h8, lo), st.o[2 * b + hh]);
+      st.o[2 * b + hh] = mfma16(v[hh], __builtin_bit_cast(h8, hi), st.o[2 * b + hh]);
+    }
+  }
+}
+__device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const HValues& v) {
+  u4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float w0 = p[e >> 1][2 * (e & 1)], w1 = p[e >> 1][2 * (e & 1) + 1];
+    hi[e] = pk_rtz(w0, w1);
+    lo[e] = pk_rtz(minus_half(w0, hi[e], 0), minus_half(w1, hi[e], 1));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    u4 x;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      x[e] = __builtin_amdgcn_perm(v.x[2 * e + 1][i >> 3][(i & 7) >> 1], v.x[2 * e][i >> 3][(i & 7) >> 1],
+                                   i & 1 ? 0x07060302u : 0x05040100u);
+    st.o[i] = mfma16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, lo), st.o[i]);
+    st.o[i] = mfma16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, hi), st.o[i]);
+  }
+}
+
+// f16, tiles with hidden rows: infinities and NaN of a drafted row's values must reach the rows that see it and no
+// other, but 0 times infinity in the product would reach all. They are taken out of the tile here and added one by one.
+// (A tile without them, practically every one, pays the test.) `w`: 2 KB of this wave's LDS.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x, uint32_t& odd) {
+  // a half is infinite or NaN where its exponent field is all ones: adding one to the field then carries into the sign
+  const uint32_t c = ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+  odd |= c;
+  return x & ~((c >> 15) * 0xffffu);
+}
+__device__ __forceinline__ void accumulate_tail(Rows& st, const f4 (&p)[2], HValues& v, const KvHead& h, int j0, int left,
+                                                float* w) {
+  uint32_t odd = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) v.x[e][q][c] = finite_halves(v.x[e][q][c], odd);
+  accumulate(st, p, v);
+  if (!__any(odd != 0)) return;
+  const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int e = 0; e < 8; e++) w[(16 * (e >> 2) + 4 * g + (e & 3)) * 16 + n] = p[e >> 2][e & 3];  // [row][n]
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int j = 0; j < left && j < kTileKeys; j++) {
+    const float wt = w[j * 16 + n];
+    const u4* row = (const u4*)(h.rows + (size_t)(j0 + j) * (2 * kHD));
+#pragma unroll
+    for (int q = 0; q < 8; q++) {  // dims 128 (q >> 2) + 8 (4 g + (q & 3)) + 0 .. 7
+      const u4 x = row[16 * (q >> 2) + 4 * g + (q & 3)];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float f = half_of(x[e >> 1], e & 1);
+        const bool add = (__builtin_bit_cast(uint32_t, f) & 0x7f800000u) == 0x7f800000u && wt != 0.0f;
+        st.o[8 * (q >> 2) + e][q & 3] += add ? wt * f : 0.0f;
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+}  // namespace q27h

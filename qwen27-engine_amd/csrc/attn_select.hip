@@ -1,0 +1,296 @@
+// Which blocks of 64 cache rows a token's sparse attention (attn_blocks) reads: bounds of every block, kept beside the
+// cache (kv_block_bounds), and the choice by a score of the query against them (attn_select).
+//
+// A block's bounds are, per channel, the least and the greatest K value of its rows, in int8 with one scale for the block:
+// d = amax / 127, code = roundf(x * (1 / d)). The query head is quantized the same way. The score of a head is
+// sum_c max(q_c lo_c, q_c hi_c) = sum_c max(q_c, 0) hi_c + min(q_c, 0) lo_c, an upper bound of its products with the
+// block's rows up to the rounding to int8; a whole number below 2^24, computed exactly. The block's score for the kv head is
+// max over the heads of float(sum) * dq, times d of the block: every rounding is fixed, so the choice is the same
+// whatever the order of the work, and equal scores go to the lower block.
+#include "pick.h"
+#include "q27h_device.h"
+#include "q27h_internal.h"
+
+namespace q27h {
+namespace {
+
+constexpr int kHD = 256;
+constexpr int kBlockRows = 64;
+constexpr int kMaxBlocks = 16000;  // blocks of a context that attn_select takes (its keys lie in 64 KB of LDS)
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+// Blocks kept for n_ctx rows: lo int8 [nkvh][nblk][256], hi the same, d f32 [nkvh][nblk].
+__host__ __device__ inline int blocks_of(int n_ctx) { return (n_ctx + kBlockRows - 1) / kBlockRows; }
+
+__device__ __forceinline__ float wave_max(float a) {
+  a = __builtin_fmaxf(a, lane_xor<1>(a));
+  a = __builtin_fmaxf(a, lane_xor<2>(a));
+  a = __builtin_fmaxf(a, lane_xor<7>(a));
+  a = __builtin_fmaxf(a, lane_xor<8>(a));
+  a = __builtin_fmaxf(a, lane_xor<16>(a));
+  return __builtin_fmaxf(a, lane_xor32(a));
+}
+__device__ __forceinline__ bool not_finite(float x) {
+  return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u;
+}
+// The scale of values up to amax, and its reciprocal; both 0 below 2^-100 (every code is then 0).
+__device__ __forceinline__ float scale_of(float amax, float& inv) {
+  const float d = amax >= 0x1p-100f ? div127(amax) : 0.0f;
+  inv = d != 0.0f ? 1.0f / d : 0.0f;
+  return d;
+}
+__device__ __forceinline__ int code_of(float x, float inv) { return (int)__builtin_roundf(x * inv); }
+
+// One workgroup per block: a lane holds 4 channels, a wave every fourth row.
+__global__ void __launch_bounds__(256) block_bounds_kernel(const uint8_t* __restrict__ kcache, const int* __restrict__ dpos0,
+                                                           int T, int nkvh, int n_ctx, int q8, int8_t* __restrict__ lo,
+                                                           int8_t* __restrict__ hi, float* __restrict__ kd) {
+  __shared__ float s_lo[4][kHD], s_hi[4][kHD];
+  __shared__ int s_odd[4];
+  const int kh = blockIdx.y, w = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const long long p0 = *dpos0, e = p0 + T;
+  const int begin = p0 < 0 ? 0 : p0 > n_ctx ? n_ctx : (int)p0, end = e < 0 ? 0 : e > n_ctx ? n_ctx : (int)e;
+  if (end <= begin) return;
+  const int b = begin / kBlockRows + blockIdx.x, nblk = blocks_of(n_ctx);
+  const int r0 = b * kBlockRows, r1 = r0 + kBlockRows < end ? r0 + kBlockRows : end;
+  if (r0 >= end) return;
+  float a[4], z[4];
+  bool odd = false;
+#pragma unroll
+  for (int c = 0; c < 4; c++) a[c] = __builtin_huge_valf(), z[c] = -__builtin_huge_valf();
+  for (int r = r0 + w; r < r1; r += 4) {
+    const size_t row = (size_t)kh * n_ctx + r;
+    float x[4];
+    if (q8) {
+      const uint32_t v = *(const uint32_t*)(kcache + row * kHD + 4 * l);
+      const float d = h2f_bits(*(const uint16_t*)(kcache + (size_t)nkvh * n_ctx * kHD + row * 16 + 2 * (l >> 3)));
+#pragma unroll
+      for (int c = 0; c < 4; c++) x[c] = (float)(int8_t)(v >> (8 * c)) * d;
+    } else {
+      const uint2 v = *(const uint2*)(kcache + (row * kHD + 4 * l) * 2);
+      x[0] = h2f_bits((uint16_t)v.x), x[1] = h2f_bits((uint16_t)(v.x >> 16));
+      x[2] = h2f_bits((uint16_t)v.y), x[3] = h2f_bits((uint16_t)(v.y >> 16));
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      odd |= not_finite(x[c]);
+      a[c] = __builtin_fminf(a[c], x[c]);
+      z[c] = __builtin_fmaxf(z[c], x[c]);
+    }
+  }
+  const int any = __any(odd);
+#pragma unroll
+  for (int c = 0; c < 4; c++) s_lo[w][4 * l + c] = a[c], s_hi[w][4 * l + c] = z[c];
+  if (l == 0) s_odd[w] = any;
+  __syncthreads();
+  if (w) return;
+  float amax = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const int i = 4 * l + c;
+    a[c] = __builtin_fminf(__builtin_fminf(s_lo[0][i], s_lo[1][i]), __builtin_fminf(s_lo[2][i], s_lo[3][i]));
+    z[c] = __builtin_fmaxf(__builtin_fmaxf(s_hi[0][i], s_hi[1][i]), __builtin_fmaxf(s_hi[2][i], s_hi[3][i]));
+    amax = __builtin_fmaxf(amax, __builtin_fmaxf(__builtin_fabsf(a[c]), __builtin_fabsf(z[c])));
+  }
+  amax = wave_max(amax);
+  const bool bad = s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3];  // an infinity or NaN: the block scores +inf and is read
+  float inv;
+  const float d = scale_of(bad ? 0.0f : amax, inv);
+  int ca[4], cz[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    ca[c] = bad ? 0 : code_of(a[c], inv);
+    cz[c] = bad ? 0 : code_of(z[c], inv);
+  }
+  const size_t at = (size_t)kh * nblk + b;
+  *(uint32_t*)(lo + at * kHD + 4 * l) = pack4_i8(ca[0], ca[1], ca[2], ca[3]);
+  *(uint32_t*)(hi + at * kHD + 4 * l) = pack4_i8(cz[0], cz[1], cz[2], cz[3]);
+  if (l == 0) kd[at] = bad ? __builtin_huge_valf() : d;
+}
+
+// Scores: one int8 matrix instruction (16 query rows x 16 blocks x 64 channels) per 64 channels of hi and of lo. A token's
+// heads are padded to gp = 4, 8 or 16 rows, so that 16 / gp tokens fill a row tile and the maximum over a token's heads
+// stays inside a lane and its neighbours 16 and 32 lanes on. A workgroup quantizes the queries of kRowTiles row tiles
+// into LDS and walks its blocks, 16 to a wave.
+constexpr int kRowTiles = 4;
+__global__ void __launch_bounds__(256) select_score_kernel(const float* __restrict__ qn, const int8_t* __restrict__ lo,
+                                                           const int8_t* __restrict__ hi, const float* __restrict__ kd,
+                                                           const int* __restrict__ dpos0, int T, int nqh, int nkvh, int n_ctx,
+                                                           int gp, int splits, float* __restrict__ score) {
+  // [row tile][positive, negative part][64-channel step][lane] of 16 codes
+  __shared__ __attribute__((aligned(16))) uint8_t s_q[kRowTiles][2][4][64][16];
+  __shared__ float s_d[kRowTiles * 16];
+  const int group = nqh / nkvh, per_tile = 16 / gp, per_wg = kRowTiles * per_tile;
+  const int kh = blockIdx.x % nkvh, split = (blockIdx.x / nkvh) % splits, t0 = (int)(blockIdx.x / nkvh / splits) * per_wg;
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4, nblk = blocks_of(n_ctx);
+  // blocks up to the one of the group's last token
+  const long long last = (long long)*dpos0 + (t0 + per_wg < T ? t0 + per_wg : T) - 1;
+  const int nb = last < 0 ? 0 : last >= n_ctx ? nblk : (int)(last / kBlockRows) + 1;
+  const int tiles = (nb + 15) / 16, per = (tiles + splits - 1) / splits;
+  const int b1 = split * per + per < tiles ? split * per + per : tiles;
+  if (split * per >= b1) return;
+  const int used = (T - t0 + per_tile - 1) / per_tile < kRowTiles ? (T - t0 + per_tile - 1) / per_tile : kRowTiles;
+  for (int r = w; r < used * 16; r += 4) {
+    const int t = t0 + r / gp, h = r % gp;
+    const bool on = t < T && h < group;
+    const float4 v = on ? ld4(qn + ((size_t)t * nqh + kh * group + h) * kHD + 4 * l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    const float amax = wave_max(__builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
+                                                __builtin_fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3]))));
+    const bool bad = __any(not_finite(x[0]) || not_finite(x[1]) || not_finite(x[2]) || not_finite(x[3]));
+    float inv;
+    const float d = scale_of(bad ? 0.0f : amax, inv);
+    int p[4], m[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int q = bad ? 0 : code_of(x[c], inv);
+      p[c] = q > 0 ? q : 0;
+      m[c] = q < 0 ? q : 0;
+    }
+    const int slot = ((l >> 2) & 3) * 16 + (r & 15), at = (l & 3) * 4;
+    *(uint32_t*)&s_q[r >> 4][0][l >> 4][slot][at] = pack4_i8(p[0], p[1], p[2], p[3]);
+    *(uint32_t*)&s_q[r >> 4][1][l >> 4][slot][at] = pack4_i8(m[0], m[1], m[2], m[3]);
+    if (l == 0) s_d[r] = d;
+  }
+  __syncthreads();
+  for (int bt = split * per + w; bt < b1; bt += 4) {
+    const int b = bt * 16 + n, bb = b < nb ? b : nb - 1;  // this lane's block (column)
+    const int8_t* ph = hi + ((size_t)kh * nblk + bb) * kHD + 16 * g;
+    const int8_t* pl = lo + ((size_t)kh * nblk + bb) * kHD + 16 * g;
+    v4i vh[4], vl[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) vh[i] = *(const v4i*)(ph + 64 * i), vl[i] = *(const v4i*)(pl + 64 * i);
+    const float d = kd[(size_t)kh * nblk + bb];
+    for (int rt = 0; rt < used; rt++) {
+      v4i c = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][0][i][l], vh[i], c, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][1][i][l], vl[i], c, 0, 0, 0);
+      float m = -__builtin_huge_valf();
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int r = 4 * g + i;
+        if ((r & (gp - 1)) < group) m = __builtin_fmaxf(m, (float)c[i] * s_d[rt * 16 + r]);
+      }
+      if (gp >= 8) m = __builtin_fmaxf(m, lane_xor<16>(m));
+      if (gp >= 16) m = __builtin_fmaxf(m, lane_xor32(m));
+      const int t = t0 + rt * per_tile + 4 * g / gp;
+      if (b < nb && t < T && (4 * g & (gp - 1)) == 0)
+        score[((size_t)t * nkvh + kh) * nblk + b] = d == __builtin_huge_valf() ? d : m * d;
+    }
+  }
+}
+
+// One workgroup per (token, kv head): the nsel-th largest key by four 8-bit digits over keys in LDS, then the chosen
+// blocks in order. The first `first` blocks and the last `last` ones up to the token's own rank above every score.
+__global__ void __launch_bounds__(256) select_pick_kernel(const float* __restrict__ score, const int* __restrict__ dpos0, int nkvh,
+                                                          int n_ctx, int nsel, int first, int last, int* __restrict__ idx) {
+  extern __shared__ uint32_t s_key[];
+  __shared__ int s_hist[256], s_scan[4], s_pick[2];
+  const int t = blockIdx.x / nkvh, tid = threadIdx.x, nblk = blocks_of(n_ctx);
+  const long long pos = (long long)*dpos0 + t;
+  const int nb = pos < 0 ? 0 : pos >= n_ctx ? nblk : (int)(pos / kBlockRows) + 1;
+  int* out = idx + (size_t)blockIdx.x * nsel;
+  if (nb <= nsel) {
+    for (int i = tid; i < nsel; i += 256) out[i] = i < nb ? i : -1;
+    return;
+  }
+  const float* row = score + (size_t)blockIdx.x * nblk;
+  for (int b = tid; b < nb; b += 256)
+    s_key[b] = b < first || b >= nb - last ? order_key(__builtin_huge_valf()) : order_key(row[b]);
+  uint32_t prefix = 0;
+  int need = nsel;  // keys still to take among those that share the prefix
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    s_hist[tid] = 0;
+    __syncthreads();
+    for (int b = tid; b < nb; b += 256) {
+      const uint32_t k = s_key[b];
+      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255], 1);
+    }
+    __syncthreads();
+    const int bin = 255 - tid, h = s_hist[bin];
+    int total;
+    const int above = scan256(h, s_scan, total);
+    if (above < need && need <= above + h) s_pick[0] = bin, s_pick[1] = need - above;
+    __syncthreads();
+    prefix |= (uint32_t)s_pick[0] << shift;
+    need = s_pick[1];
+    __syncthreads();
+  }
+  // keys above `prefix`, and the first `need` equal to it
+  int done = 0, equal = 0;
+  for (int b0 = 0; b0 < nb; b0 += 256) {
+    const int b = b0 + tid;
+    const uint32_t k = b < nb ? s_key[b] : 0u;
+    const bool eq = b < nb && k == prefix;
+    int total_eq, total;
+    const int rank = equal + scan256(eq, s_scan, total_eq);
+    const bool take = (b < nb && k > prefix) || (eq && rank < need);
+    const int at = done + scan256(take, s_scan, total);
+    if (take) out[at] = b;
+    done += total;
+    equal += total_eq;
+  }
+}
+
+int padded_group(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
+
+}  // namespace
+}  // namespace q27h
+
+using namespace q27h;
+
+extern "C" size_t q27h_kv_block_bytes(int nkvh, int n_ctx) {
+  if (nkvh <= 0 || n_ctx <= 0) return 0;
+  return (size_t)nkvh * blocks_of(n_ctx) * (2 * kHD + 4);
+}
+
+extern "C" int q27h_kv_block_bounds(const void* kcache, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* kb,
+                                    q27h_stream_t s) {
+  if (T < 0 || nkvh <= 0 || nkvh > 65535 || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "kv_block_bounds: bad shape");
+  if (T == 0) return Q27H_OK;
+  if (!kcache || !pos0 || !kb) return fail(Q27H_ERR_ARG, "kv_block_bounds: null pointer");
+  if (!aligned16(kcache) || !aligned16(kb)) return fail(Q27H_ERR_ARG, "kv_block_bounds: tensors need 16-byte alignment");
+  const int nblk = blocks_of(n_ctx);
+  const long touched = (long)(T + kBlockRows - 1) / kBlockRows + 1;
+  int8_t* lo = (int8_t*)kb;
+  int8_t* hi = lo + (size_t)nkvh * nblk * kHD;
+  hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)(touched < nblk ? touched : nblk), (unsigned)nkvh), dim3(256), 0,
+                     stream_of(s), (const uint8_t*)kcache, pos0, T, nkvh, n_ctx, q8, lo, hi,
+                     (float*)(hi + (size_t)nkvh * nblk * kHD));
+  return check_launch("kv_block_bounds");
+}
+
+extern "C" size_t q27h_attn_select_ws_bytes(int T, int nkvh, int n_ctx) {
+  if (T <= 0 || nkvh <= 0 || n_ctx <= 0) return 0;
+  return (size_t)T * nkvh * blocks_of(n_ctx) * sizeof(float);
+}
+
+extern "C" int q27h_attn_select(const float* qn, const void* kb, const int* pos0, int T, int nqh, int nkvh, int n_ctx, int nsel,
+                                int first, int last, int* idx, void* ws, size_t ws_bytes, q27h_stream_t s) {
+  if (T < 0 || nkvh <= 0 || nqh <= 0 || nqh % nkvh || nqh / nkvh > 16 || n_ctx <= 0 || nsel <= 0)
+    return fail(Q27H_ERR_SHAPE, "attn_select: bad shape (at most 16 query heads per kv head)");
+  if (first < 0 || last < 1 || (long long)first + last > nsel)
+    return fail(Q27H_ERR_SHAPE, "attn_select: first >= 0, last >= 1 and first + last <= nsel");
+  const int nblk = blocks_of(n_ctx);
+  if (nblk > kMaxBlocks) return fail(Q27H_ERR_SHAPE, "attn_select: n_ctx must be <= 1024000");
+  if ((long long)T * nkvh > 0x7fffffffLL / 64) return fail(Q27H_ERR_SHAPE, "attn_select: T too large");
+  if (T == 0) return Q27H_OK;
+  if (!qn || !kb || !pos0 || !idx || !ws) return fail(Q27H_ERR_ARG, "attn_select: null pointer");
+  if (!aligned16(qn) || !aligned16(kb) || !aligned4(ws)) return fail(Q27H_ERR_ARG, "attn_select: tensors need 16-byte alignment");
+  if (ws_bytes < q27h_attn_select_ws_bytes(T, nkvh, n_ctx)) return fail(Q27H_ERR_ARG, "attn_select: workspace too small");
+  const int8_t* lo = (const int8_t*)kb;
+  const int8_t* hi = lo + (size_t)nkvh * nblk * kHD;
+  const float* kd = (const float*)(hi + (size_t)nkvh * nblk * kHD);
+  const int gp = padded_group(nqh / nkvh), per_wg = kRowTiles * 16 / gp;
+  const int tg = (T + per_wg - 1) / per_wg, most = (nblk + 63) / 64;  // 4 waves of 16 blocks
+  int splits = (int)(2L * kCUs / ((long)tg * nkvh));
+  splits = splits > most ? most : splits < 1 ? 1 : splits;
+  hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)((long)tg * nkvh * splits)), dim3(256), 0, stream_of(s), qn, lo, hi, kd,
+                     pos0, T, nqh, nkvh, n_ctx, gp, splits, (float*)ws);
+  hipLaunchKernelGGL(select_pick_kernel, dim3((unsigned)(T * nkvh)), dim3(256), (size_t)nblk * 4, stream_of(s), (const float*)ws,
+                     pos0, nkvh, n_ctx, nsel, first, last, idx);
+  return check_launch("attn_select");
+}

@@ -1,0 +1,516 @@
+// Attention over the K/V cache that attn_prep writes: a tree of drafted tokens (attn_tree; one token is plain decoding),
+// blocks of 64 rows chosen per token (attn_blocks), and the sums of attention weights per cache row (attn_weights).
+//
+// The rows of the cache are split over workgroups and, in each, over its 4 waves; a wave walks its tiles of 32 rows with
+// the online softmax of attn_core.h, the next tile's loads in flight behind the current one's arithmetic. The query rows
+// of a kv head (tokens x query heads of the group) are 16 or 32 to a wave; more are spread over workgroups that read the
+// same cache rows on the same XCD, so that its L2 serves all but the first. A second launch joins the splits.
+#include "attn_core.h"
+#include "q27h_internal.h"
+
+namespace q27h {
+namespace {
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr int kMaxTree = 64;   // tokens of a tree: a 64-bit mask per token
+constexpr int kBlockRows = 64;  // rows of a block of attn_blocks
+constexpr int kWaves = 4;      // waves of a workgroup of attn_blocks and attn_weights
+
+// How the cache rows are split. Host: `max` splits are launched. Device: rows become tiles; a split takes `per` tiles,
+// at least one for each of its `waves` while there are few, and the splits behind the last one have nothing to do.
+struct Split {
+  int per, used;
+};
+__device__ __forceinline__ Split split_of(int tiles, int max, int waves) {
+  int per = (tiles + max - 1) / max;
+  per = per < waves ? waves : per;
+  return {per, (tiles + per - 1) / per};
+}
+
+// Rows that every drafted token sees, and the rows that exist.
+__device__ __forceinline__ Vis vis_of(long long pos0, int T, int n_ctx) {
+  Vis v;
+  v.n0 = pos0 > n_ctx ? n_ctx : (int)pos0;
+  v.n = pos0 < 0 ? 0 : pos0 > n_ctx ? n_ctx : (int)pos0;
+  const long long e = pos0 + T;
+  v.end = e < 0 ? 0 : e > n_ctx ? n_ctx : (int)e;
+  return v;
+}
+__device__ __forceinline__ uint64_t tree_of(const uint64_t* tree, int t, int T) {
+  const uint64_t all = T >= 64 ? ~0ull : (1ull << T) - 1;
+  return (tree ? tree[t] : ~0ull >> (63 - t)) & all;
+}
+
+struct AttnArgs {
+  const float* qn;
+  const void *kcache, *vcache;
+  const int* pos0;
+  const uint64_t* tree;  // attn_tree
+  const int* idx;        // attn_blocks
+  float *o, *lse;        // lse may be null
+  float *part, *ml;      // [row][split][256], [row][split][2]; row = token * nqh + query head
+  int T, nqh, nkvh, n_ctx, nsel;
+  int splits, groups, waves;  // attn_tree: workgroups over the query rows of a kv head, waves over the cache rows of one
+  float scale;
+};
+
+// WR * WK waves: WR row tiles of 16 query rows, and for each of them WK waves that share the workgroup's cache rows.
+template <int WR, int WK>
+struct AttnShared {
+  QTile q[WR];
+  WaveLds w[WR * WK];
+};
+
+// A wave's tile of which some rows are hidden or do not exist.
+template <bool Q8>
+__device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const QTile& im, WaveLds& w,
+                                          const Vis& vis, uint64_t tree, int j0) {
+  typename Tiles<Q8>::K k;
+  typename Tiles<Q8>::V v;
+  f4 s[1][2];
+  const int left = vis.end - j0;
+  const uint64_t trees[1] = {tree};
+  load_rows<true>(k, kc, j0, left);
+  if constexpr (Q8) {
+    stage_rows(k, w.codes, w.ks);
+    scores<1>(w, &im, s);
+  } else {
+    scores<1>(k, &im, s);
+  }
+  hide<1>(s, vis, trees, j0);
+  load_rows<true>(v, vc, j0, left);
+  if constexpr (Q8) {
+    widen(st, v.s);
+    weights(st, s[0]);
+    stage_rows(v, w.codes, w.vs);
+    accumulate<true>(st, s[0], w);
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    weights(st, s[0]);
+    accumulate_tail(st, s[0], v, vc, j0, left, (float*)w.codes);
+  }
+}
+
+// The wave's tiles that are wholly visible; next() gives the first cache row of one after the other, then -1. The next
+// tile's K is requested once this one's is in LDS (q8) or its scores are formed, its V once this one's is in LDS or
+// consumed, so that one set of registers each is enough and the loads fly behind the arithmetic.
+template <bool Q8, typename F>
+__device__ __forceinline__ void full_tiles(Rows& st, const KvHead& kc, const KvHead& vc, const QTile& im, WaveLds& w, F next) {
+  int j0 = next();
+  if (j0 < 0) return;
+  typename Tiles<Q8>::K k;
+  typename Tiles<Q8>::V v;
+  load_rows<false>(k, kc, j0, 0);
+  load_rows<false>(v, vc, j0, 0);
+  do {
+    f4 s[1][2];
+    j0 = next();
+    asm volatile("" ::: "memory");  // the queries are read from LDS for each tile: held in registers they would spill
+    if constexpr (Q8) {
+      stage_rows(k, w.codes, w.ks);
+      if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
+      loads_issued();
+      scores<1>(w, &im, s);
+      widen(st, v.s);
+      weights(st, s[0]);
+      __builtin_amdgcn_wave_barrier();
+      stage_rows(v, w.codes, w.vs);
+      if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
+      loads_issued();
+      accumulate<false>(st, s[0], w);
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      scores<1>(k, &im, s);
+      if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
+      loads_issued();
+      weights(st, s[0]);
+      accumulate(st, s[0], v);
+      if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
+      loads_issued();
+    }
+  } while (j0 >= 0);
+}
+
+// Joins the WK waves of each row tile and writes its rows: as a split's part, or as the result where there is one split
+// only. gr: the global row (token * nqh + head) of this lane's query row, or -1.
+template <bool Q8, int WR, int WK>
+__device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const AttnArgs& a, int split, bool single, int gr) {
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4, wr = w % WR, wk = w / WR;
+  float(*ml)[16][2] = (float(*)[16][2])sh.q;       // [wave][row]
+  f4(*ex)[16][64] = (f4(*)[16][64])sh.w;           // outputs of half the waves
+  static_assert(sizeof(sh.w) >= WR * WK / 2 * sizeof(f4) * 16 * 64 && sizeof(sh.q) >= WR * WK * 16 * 8);
+  st.l += lane_xor<16>(st.l);
+  st.l += lane_xor32(st.l);
+  __syncthreads();  // every wave is done with the queries and its tile
+  if (g == 0) ml[w][n][0] = st.m, ml[w][n][1] = st.l;
+  __syncthreads();
+  float m = -3.0e38f, sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < WK; k++) m = __builtin_fmaxf(m, ml[k * WR + wr][n][0]);
+#pragma unroll
+  for (int k = 0; k < WK; k++) sum += ml[k * WR + wr][n][1] * __builtin_amdgcn_exp2f(ml[k * WR + wr][n][0] - m);
+  const float f = __builtin_amdgcn_exp2f(st.m - m) * (Q8 ? 512.0f : 1.0f);  // codes8's 2^-9
+#pragma unroll
+  for (int i = 0; i < 16; i++) st.o[i] *= f;
+#pragma unroll
+  for (int h = WK / 2; h > 0; h /= 2) {  // the upper half of the waves hands over, the lower adds: always in the same order
+    if (wk >= h && wk < 2 * h) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) ex[w - h * WR][i][l] = st.o[i];
+    }
+    __syncthreads();
+    if (wk < h) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) st.o[i] += ex[w][i][l];
+    }
+    __syncthreads();
+  }
+  if (wk != 0 || gr < 0) return;
+  float* dst;
+  if (single) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= inv;
+    dst = a.o + (size_t)gr * kHD;
+    if (a.lse && g == 0) a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  } else {
+    const size_t at = (size_t)gr * a.splits + split;
+    dst = a.part + at * kHD;
+    if (g == 0) *(float2*)(a.ml + at * 2) = make_float2(m, sum);
+  }
+  if constexpr (Q8) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) *(f4*)(dst + 16 * i + 4 * g) = st.o[i];
+  } else {
+#pragma unroll
+    for (int hr = 0; hr < 2; hr++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+          *(f4*)(dst + 128 * hr + 8 * (4 * g + c) + 4 * q) =
+              (f4){st.o[8 * hr + 4 * q][c], st.o[8 * hr + 4 * q + 1][c], st.o[8 * hr + 4 * q + 2][c], st.o[8 * hr + 4 * q + 3][c]};
+  }
+}
+
+template <bool Q8, int WR, int WK>
+__global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) {
+  __shared__ AttnShared<WR, WK> sh;
+  // workgroups 8 apart run on one XCD: those of one (kv head, split) follow each other there
+  const int unit = (int)(blockIdx.x / (8 * a.groups)) * 8 + (int)(blockIdx.x & 7), rg = (int)(blockIdx.x >> 3) % a.groups;
+  if (unit >= a.nkvh * a.splits) return;
+  const int kh = unit % a.nkvh, split = unit / a.nkvh;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = w % WR, wk = w / WR;
+  const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
+  const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
+  const Split sp = split_of(tiles, a.splits, WK);
+  if (split >= sp.used) return;
+  const int group = a.nqh / a.nkvh, rows = a.T * group;
+  auto row = [&](int r) {
+    r += rg * WR * 16;
+    return r < rows ? (r / group) * a.nqh + kh * group + r % group : -1;
+  };
+  load_queries<Q8, WR * WK>(sh.q, WR, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
+  });
+  const int mine = wr * 16 + (threadIdx.x & 15);
+  const uint64_t tree = row(mine) >= 0 ? tree_of(a.tree, (rg * WR * 16 + mine) / group, a.T) : 0ull;
+  __syncthreads();
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
+  Rows st;
+  rows_init<Q8>(st, sh.q[wr]);
+  if ((rg * WR + wr) * 16 < rows) {  // the last group's row tiles may be fewer
+    const int t1 = split * sp.per + sp.per < tiles ? split * sp.per + sp.per : tiles;
+    const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
+    int t = split * sp.per + wk;
+    full_tiles<Q8>(st, kc, vc, sh.q[wr], sh.w[w], [&] {
+      if (t >= full) return -1;
+      t += WK;
+      return (t - WK) * kTileKeys;
+    });
+    for (; t < t1; t += WK) tail_tile<Q8>(st, kc, vc, sh.q[wr], sh.w[w], vis, tree, t * kTileKeys);
+  }
+  finish<Q8, WR, WK>(st, sh, a, split, sp.used == 1, row(mine));
+}
+
+// attn_blocks: one workgroup per (token, kv head, split of its list); the group's query heads are one row tile.
+template <bool Q8>
+__global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a) {
+  __shared__ AttnShared<1, kWaves> sh;
+  const int unit = (int)(blockIdx.x / a.splits), split = (int)(blockIdx.x % a.splits);
+  const int kh = unit % a.nkvh, t = unit / a.nkvh;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Vis vis = vis_of((long long)*a.pos0 + t + 1, 0, a.n_ctx);
+  const int group = a.nqh / a.nkvh;
+  auto row = [&](int r) { return r < group ? t * a.nqh + kh * group + r : -1; };
+  load_queries<Q8, kWaves>(sh.q, 1, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
+  });
+  __syncthreads();
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
+  Rows st;
+  rows_init<Q8>(st, sh.q[0]);
+  const int per = (2 * a.nsel + a.splits - 1) / a.splits;
+  const int t1 = split * per + per < 2 * a.nsel ? split * per + per : 2 * a.nsel;
+  const int* list = a.idx + ((size_t)t * a.nkvh + kh) * a.nsel;
+  // the first cache row of the list's i-th tile, or -1: an entry that is no block of the context, or one seen in part
+  // where a whole one is asked for (and the other way round)
+  const int nb = (vis.n + kBlockRows - 1) / kBlockRows;
+  auto tile = [&](int i, bool part) {
+    const int b = __builtin_amdgcn_readfirstlane(list[i >> 1]);
+    const int j0 = b * kBlockRows + (i & 1) * kTileKeys;
+    return b >= 0 && b < nb && j0 < vis.n && (j0 + kTileKeys > vis.n) == part ? j0 : -1;
+  };
+  int i = split * per + w;
+  full_tiles<Q8>(st, kc, vc, sh.q[0], sh.w[w], [&] {
+    for (; i < t1; i += kWaves) {
+      const int j0 = tile(i, false);
+      if (j0 >= 0) {
+        i += kWaves;
+        return j0;
+      }
+    }
+    return -1;
+  });
+  for (i = split * per + w; i < t1; i += kWaves) {
+    const int j0 = tile(i, true);
+    if (j0 >= 0) tail_tile<Q8>(st, kc, vc, sh.q[0], sh.w[w], vis, 0ull, j0);
+  }
+  finish<Q8, 1, kWaves>(st, sh, a, split, a.splits == 1, row(threadIdx.x & 15));
+}
+
+// Joins the splits of one query row: one workgroup each, a thread per dim. FIXED: every split was written; else those
+// that split_of used, and nothing is left to do where that is one.
+template <bool FIXED>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+  const int gr = blockIdx.x, d = threadIdx.x;
+  int used = a.splits;
+  if (!FIXED) {
+    const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
+    used = split_of((vis.end + kTileKeys - 1) / kTileKeys, a.splits, a.waves).used;
+    if (used == 1) return;
+  }
+  const float* ml = a.ml + (size_t)gr * a.splits * 2;
+  const float* part = a.part + (size_t)gr * a.splits * kHD + d;
+  float m = -3.0e38f;
+  for (int s = 0; s < used; s++) m = __builtin_fmaxf(m, ml[2 * s]);
+  float sum = 0.0f, o = 0.0f;
+  for (int s = 0; s < used; s++) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
+    sum += ml[2 * s + 1] * f;
+    o += part[(size_t)s * kHD] * f;
+  }
+  a.o[(size_t)gr * kHD + d] = sum == 0.0f ? 0.0f : o / sum;
+  if (a.lse && d == 0) a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+struct WeightArgs {
+  const float *qn, *lse;
+  const void* kcache;
+  const int* pos0;
+  const uint64_t *tree, *rows;
+  float* acc;
+  int T, nqh, nkvh, n_ctx, splits, groups;
+  float scale;
+};
+
+// attn_weights: a workgroup takes a split of the cache rows of one kv head, walks the query rows in groups of 16 RT and,
+// for each, its tiles; the sum over the 16 query rows of a tile is a lane reduction, that over row tiles and groups is
+// taken in order, and a row of the cache belongs to one wave: the same bits always.
+template <bool Q8, int RT>
+__global__ void __launch_bounds__(kWaves * 64, RT == 4 ? 1 : 2) attn_weights_kernel(WeightArgs a) {
+  __shared__ QTile im[RT];
+  __shared__ float s_lse[RT * 16];
+  __shared__ WaveLds s_w[Q8 ? kWaves : 1];
+  const int kh = blockIdx.x % a.nkvh, split = blockIdx.x / a.nkvh;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
+  const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
+  const Split sp = split_of(tiles, a.splits, kWaves);
+  if (split >= sp.used) return;
+  const int t1 = split * sp.per + sp.per < tiles ? split * sp.per + sp.per : tiles;
+  const int group = a.nqh / a.nkvh, rows = a.T * group;
+  const uint64_t used = a.rows ? *a.rows : ~0ull;
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx);
+  float* acc = a.acc + (size_t)kh * a.n_ctx;
+  for (int rg = 0; rg < a.groups; rg++) {
+    __syncthreads();
+    load_queries<Q8, kWaves>(im, RT, a.scale * kLog2e, [&](int r) {
+      r += rg * RT * 16;
+      return r < rows ? a.qn + ((size_t)(r / group) * a.nqh + kh * group + r % group) * kHD : nullptr;
+    });
+    if (threadIdx.x < RT * 16) {
+      const int r = rg * RT * 16 + threadIdx.x;
+      const bool on = r < rows && ((used >> (r / group)) & 1);
+      s_lse[threadIdx.x] = on ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : __builtin_huge_valf();
+    }
+    __syncthreads();
+    uint64_t tree[RT];
+    float c[RT], lse[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+      const int r = rg * RT * 16 + rt * 16 + n;
+      tree[rt] = r < rows ? tree_of(a.tree, r / group, a.T) : 0ull;
+      c[rt] = im[rt].c[n];
+      lse[rt] = s_lse[rt * 16 + n];
+    }
+    for (int t = split * sp.per + w; t < t1; t += kWaves) {
+      const int j0 = t * kTileKeys;
+      const bool full = j0 + kTileKeys <= vis.n;
+      typename Tiles<Q8>::K k;
+      f4 s[RT][2];
+      if (full) load_rows<false>(k, kc, j0, 0);
+      else load_rows<true>(k, kc, j0, vis.end - j0);
+      const int j = j0 + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);  // the row this lane stores (n < 8)
+      const bool mine = n < 8 && j < vis.end;
+      const float old = mine && (j < vis.n || rg) ? acc[j] : 0.0f;  // the weights of a drafted row begin here
+      asm volatile("" ::: "memory");
+      if constexpr (Q8) {
+        __builtin_amdgcn_wave_barrier();
+        stage_rows(k, s_w[w].codes, s_w[w].ks);
+        scores<RT>(s_w[w], im, s);
+      } else {
+        scores<RT>(k, im, s);
+      }
+      if (!full) hide<RT>(s, vis, tree, j0);
+      float sum[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        sum[e] = 0.0f;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+          const float x = s[rt][e >> 2][e & 3];
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[rt], -lse[rt]));
+          // rows not asked for, and hidden cache rows (of a query row that sees none lse is -inf too)
+          sum[e] += lse[rt] == __builtin_huge_valf() || x == -__builtin_huge_valf() ? 0.0f : p;
+        }
+        sum[e] += lane_xor<1>(sum[e]);
+        sum[e] += lane_xor<2>(sum[e]);
+        sum[e] += lane_xor<7>(sum[e]);
+        sum[e] += lane_xor<8>(sum[e]);
+      }
+      float v = sum[0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) v = n == e ? sum[e] : v;
+      if (mine) acc[j] = old + v;
+    }
+  }
+}
+
+// How attn_tree's workgroups are laid out: 1, 2 or 4 row tiles of 16 query rows.
+struct TreeLayout {
+  int wr, wk, groups, splits;
+};
+TreeLayout tree_layout(int T, int nqh, int nkvh, int n_ctx) {
+  TreeLayout t;
+  const int tiles = (T * (nqh / nkvh) + 15) / 16;
+  t.wr = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4;
+  t.wk = t.wr == 4 ? 2 : 4;
+  t.groups = (tiles + t.wr - 1) / t.wr;
+  // enough workgroups for every compute unit: two of 4 waves on each, or one of 8
+  const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + t.wk - 1) / t.wk;
+  int s = (t.wr == 1 ? 2 * kCUs : kCUs) / (nkvh * t.groups);
+  s = s > most ? most : s;
+  t.splits = s < 1 ? 1 : s;
+  return t;
+}
+int blocks_splits(int T, int nkvh, int nsel) {
+  const long units = (long)T * nkvh;
+  long s = 2 * kCUs / units;
+  const long most = (2L * nsel + kWaves - 1) / kWaves;
+  s = s > most ? most : s;
+  return s < 1 ? 1 : (int)s;
+}
+size_t part_bytes(size_t rows, int splits) { return splits <= 1 ? 0 : rows * splits * (kHD + 2) * sizeof(float); }
+
+bool heads_ok(int nqh, int nkvh) { return nkvh > 0 && nqh > 0 && nqh % nkvh == 0; }
+
+}  // namespace
+}  // namespace q27h
+
+using namespace q27h;
+
+extern "C" size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx) {
+  if (T <= 0 || T > kMaxTree || !heads_ok(nqh, nkvh) || n_ctx <= 0) return 0;
+  return part_bytes((size_t)T * nqh, tree_layout(T, nqh, nkvh, n_ctx).splits);
+}
+
+extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* vcache, const int* pos0, const uint64_t* tree,
+                              int T, float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws,
+                              size_t ws_bytes, q27h_stream_t s) {
+  if (T < 0 || T > kMaxTree) return fail(Q27H_ERR_SHAPE, "attn_tree: T must be 0..64");
+  if (!heads_ok(nqh, nkvh) || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "attn_tree: bad shape");
+  if (T == 0) return Q27H_OK;
+  if (!qn || !kcache || !vcache || !pos0 || !o) return fail(Q27H_ERR_ARG, "attn_tree: null pointer");
+  if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
+    return fail(Q27H_ERR_ARG, "attn_tree: tensors need 16-byte alignment");
+  if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_tree: o overlaps qn");
+  const size_t need = q27h_attn_tree_ws_bytes(T, nqh, nkvh, n_ctx);
+  if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_tree: workspace too small");
+  AttnArgs a = {};
+  a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.tree = tree, a.o = o, a.lse = lse;
+  a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
+  const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  a.splits = lay.splits, a.groups = lay.groups, a.waves = lay.wk;
+  a.part = (float*)ws, a.ml = a.part + (size_t)T * nqh * a.splits * kHD;
+  const unsigned grid = (unsigned)((nkvh * a.splits + 7) / 8 * 8 * a.groups);
+  const auto kern = lay.wr == 1   ? (q8 ? attn_tree_kernel<true, 1, 4> : attn_tree_kernel<false, 1, 4>)
+                    : lay.wr == 2 ? (q8 ? attn_tree_kernel<true, 2, 4> : attn_tree_kernel<false, 2, 4>)
+                                  : (q8 ? attn_tree_kernel<true, 4, 2> : attn_tree_kernel<false, 4, 2>);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3((unsigned)(lay.wr * lay.wk * 64)), 0, stream_of(s), a);
+  hipLaunchKernelGGL(attn_join_kernel<false>, dim3((unsigned)(T * nqh)), dim3(256), 0, stream_of(s), a);
+  return check_launch("attn_tree");
+}
+
+extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* kcache, const int* pos0, const uint64_t* tree,
+                                 const uint64_t* rows, int T, float scale, int nqh, int nkvh, int n_ctx, int q8, float* acc,
+                                 q27h_stream_t s) {
+  if (T < 0 || T > kMaxTree) return fail(Q27H_ERR_SHAPE, "attn_weights: T must be 0..64");
+  if (!heads_ok(nqh, nkvh) || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "attn_weights: bad shape");
+  if (T == 0) return Q27H_OK;
+  if (!qn || !lse || !kcache || !pos0 || !acc) return fail(Q27H_ERR_ARG, "attn_weights: null pointer");
+  if (!aligned16(qn) || !aligned16(kcache)) return fail(Q27H_ERR_ARG, "attn_weights: tensors need 16-byte alignment");
+  WeightArgs a = {};
+  a.qn = qn, a.lse = lse, a.kcache = kcache, a.pos0 = pos0, a.tree = tree, a.rows = rows, a.acc = acc;
+  a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
+  const int n_rows = T * (nqh / nkvh), rt = n_rows <= 16 ? 1 : n_rows <= 32 ? 2 : 4;
+  a.groups = (n_rows + rt * 16 - 1) / (rt * 16);
+  const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + kWaves - 1) / kWaves;
+  a.splits = 4 * kCUs / nkvh;
+  a.splits = a.splits > most ? most : a.splits < 1 ? 1 : a.splits;
+  const auto kern = q8 ? (rt == 1 ? attn_weights_kernel<true, 1> : rt == 2 ? attn_weights_kernel<true, 2> : attn_weights_kernel<true, 4>)
+                       : (rt == 1 ? attn_weights_kernel<false, 1> : rt == 2 ? attn_weights_kernel<false, 2> : attn_weights_kernel<false, 4>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(nkvh * a.splits)), dim3(256), 0, stream_of(s), a);
+  return check_launch("attn_weights");
+}
+
+extern "C" size_t q27h_attn_blocks_ws_bytes(int T, int nqh, int nkvh, int nsel) {
+  if (T <= 0 || !heads_ok(nqh, nkvh) || nqh / nkvh > 16 || nsel <= 0) return 0;
+  return part_bytes((size_t)T * nqh, blocks_splits(T, nkvh, nsel));
+}
+
+extern "C" int q27h_attn_blocks(const float* qn, const void* kcache, const void* vcache, const int* pos0, const int* idx, int T,
+                                int nsel, float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws,
+                                size_t ws_bytes, q27h_stream_t s) {
+  if (T < 0 || nsel <= 0 || !heads_ok(nqh, nkvh) || nqh / nkvh > 16 || n_ctx <= 0)
+    return fail(Q27H_ERR_SHAPE, "attn_blocks: bad shape (at most 16 query heads per kv head)");
+  if (nsel > (1 << 20) || (long long)T * nqh > 0x7fffffffLL / 64) return fail(Q27H_ERR_SHAPE, "attn_blocks: T or nsel too large");
+  if (T == 0) return Q27H_OK;
+  if (!qn || !kcache || !vcache || !pos0 || !idx || !o) return fail(Q27H_ERR_ARG, "attn_blocks: null pointer");
+  if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
+    return fail(Q27H_ERR_ARG, "attn_blocks: tensors need 16-byte alignment");
+  if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_blocks: o overlaps qn");
+  const size_t need = q27h_attn_blocks_ws_bytes(T, nqh, nkvh, nsel);
+  if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_blocks: workspace too small");
+  AttnArgs a = {};
+  a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.idx = idx, a.o = o, a.lse = lse;
+  a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.nsel = nsel, a.scale = scale;
+  a.splits = blocks_splits(T, nkvh, nsel);
+  a.part = (float*)ws, a.ml = a.part + (size_t)T * nqh * a.splits * kHD;
+  const auto kern = q8 ? attn_blocks_kernel<true> : attn_blocks_kernel<false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((long)T * nkvh * a.splits)), dim3(256), 0, stream_of(s), a);
+  if (a.splits > 1) hipLaunchKernelGGL(attn_join_kernel<true>, dim3((unsigned)(T * nqh)), dim3(256), 0, stream_of(s), a);
+  return check_launch("attn_blocks");
+}

@@ -1,0 +1,361 @@
+// Which rows of the K/V cache stay, and moving them: eviction by accumulated attention weight (kv_evict) and the move of
+// an accepted path of drafted tokens to its place (kv_accept).
+//
+// kv_evict keeps, per kv head, the first `first` rows, the last `last` rows and the heaviest of those between, in their
+// order. The weights' exact order is found by three histograms (11, 11 and 10 bits of the integer key, counted with
+// integer atomics, so in any order to the same result) over workgroups that each hold a segment of the rows; then each
+// segment counts its rows above and at the threshold and writes its own part of the list behind the segments before it.
+// Rows are moved by 16 bytes a lane. In place they pass through the workspace, since a row's place may be another row's
+// source.
+#include "pick.h"
+#include "q27h_device.h"
+#include "q27h_internal.h"
+
+namespace q27h {
+namespace {
+
+constexpr int kHD = 256;
+constexpr int kBins = 2048;
+constexpr int kSegRows = 2048;  // rows of a segment, while there are fewer than kMaxSegs of them
+constexpr int kMaxSegs = 128;
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+__host__ __device__ inline int segs_of(int n_ctx) {
+  const int s = (n_ctx + kSegRows - 1) / kSegRows;
+  return s > kMaxSegs ? kMaxSegs : s;
+}
+
+struct EvictArgs {
+  const void *kc, *vc;
+  const float* acc;
+  const int* pos0;
+  void *ko, *vo;
+  float* acc_o;
+  int* kept;
+  int* hist;    // [nkvh][3][kBins]
+  int2* count;  // [nkvh][segs]: rows above, rows at the threshold
+  int keep, first, last, n_out, nkvh, n_ctx, q8, segs, in_place;
+};
+
+__device__ __forceinline__ int rows_of(const EvictArgs& a) {
+  const int n = *a.pos0;
+  return n < 0 ? 0 : n > a.n_ctx ? a.n_ctx : n;
+}
+
+// The bin (from the top) in which the need-th value of a histogram lies, and how many of that bin are needed.
+__device__ __forceinline__ void find_bin(const int* hist, int bins, int& need, int& bin, int* s_scan, int* s_pick) {
+  const int per = bins / 256;
+  int h[kBins / 256], mine = 0;
+#pragma unroll
+  for (int i = 0; i < kBins / 256; i++)
+    if (i < per) h[i] = hist[bins - 1 - (int)threadIdx.x * per - i], mine += h[i];
+  int total;
+  int above = scan256(mine, s_scan, total);
+#pragma unroll
+  for (int i = 0; i < kBins / 256; i++) {
+    if (i < per) {
+      if (above < need && need <= above + h[i]) s_pick[0] = bins - 1 - (int)threadIdx.x * per - i, s_pick[1] = need - above;
+      above += h[i];
+    }
+  }
+  __syncthreads();
+  bin = s_pick[0];
+  need = s_pick[1];
+  __syncthreads();
+}
+__device__ __forceinline__ int digit_of(uint32_t key, int pass) {
+  return pass == 0 ? key >> 21 : pass == 1 ? (key >> 10) & 2047 : key & 1023;
+}
+__device__ __forceinline__ uint32_t above_digit(uint32_t key, int pass) { return pass == 0 ? 0u : pass == 1 ? key >> 21 : key >> 10; }
+
+// The key's digits found by the first `passes` histograms, and how many of the rows that share them are kept.
+__device__ __forceinline__ uint32_t prefix_of(const EvictArgs& a, int kh, int passes, int& need, int* s_scan, int* s_pick) {
+  uint32_t key = 0;
+  const int* h = a.hist + (size_t)kh * 3 * kBins;
+  for (int p = 0; p < passes; p++) {
+    int bin;
+    find_bin(h + p * kBins, p == 2 ? 1024 : kBins, need, bin, s_scan, s_pick);
+    key |= (uint32_t)bin << (p == 0 ? 21 : p == 1 ? 10 : 0);
+  }
+  return key;
+}
+
+__global__ void __launch_bounds__(256) evict_clear_kernel(int* hist) {
+  *(int4*)(hist + 4 * ((size_t)blockIdx.x * 256 + threadIdx.x)) = make_int4(0, 0, 0, 0);
+}
+
+// One digit's histogram of the rows between the fixed ends; a workgroup per (segment, kv head).
+__global__ void __launch_bounds__(256) evict_hist_kernel(EvictArgs a, int pass) {
+  __shared__ int s_hist[kBins], s_scan[4], s_pick[2];
+  const int kh = blockIdx.y, n = rows_of(a);
+  int need = a.keep - a.first - a.last;
+  if (n <= a.keep || need == 0) return;
+  const int r0 = a.first, r1 = n - a.last, per = (r1 - r0 + a.segs - 1) / a.segs;
+  const int b = r0 + blockIdx.x * per, e = b + per < r1 ? b + per : r1;
+  if (b >= e) return;
+  for (int i = threadIdx.x; i < kBins; i += 256) s_hist[i] = 0;
+  const uint32_t key = prefix_of(a, kh, pass, need, s_scan, s_pick);
+  __syncthreads();
+  const float* acc = a.acc + (size_t)kh * a.n_ctx;
+  for (int r = b + threadIdx.x; r < e; r += 256) {
+    const uint32_t k = order_key(acc[r]);
+    if (above_digit(k, pass) == above_digit(key, pass)) atomicAdd(&s_hist[digit_of(k, pass)], 1);
+  }
+  __syncthreads();
+  int* h = a.hist + ((size_t)kh * 3 + pass) * kBins;
+  for (int i = threadIdx.x; i < kBins; i += 256)
+    if (s_hist[i]) atomicAdd(h + i, s_hist[i]);
+}
+
+__global__ void __launch_bounds__(256) evict_count_kernel(EvictArgs a) {
+  __shared__ int s_scan[4], s_pick[2];
+  const int kh = blockIdx.y, n = rows_of(a);
+  int need = a.keep - a.first - a.last;
+  if (n <= a.keep) return;
+  const int r0 = a.first, r1 = n - a.last, per = (r1 - r0 + a.segs - 1) / a.segs;
+  const int b = r0 + blockIdx.x * per, e = b + per < r1 ? b + per : r1;
+  int above = 0, equal = 0;
+  if (need) {
+    const uint32_t key = prefix_of(a, kh, 3, need, s_scan, s_pick);
+    const float* acc = a.acc + (size_t)kh * a.n_ctx;
+    for (int r = b + threadIdx.x; r < e; r += 256) {
+      const uint32_t k = order_key(acc[r]);
+      above += k > key;
+      equal += k == key;
+    }
+    int t0, t1;
+    scan256(above, s_scan, t0);
+    scan256(equal, s_scan, t1);
+    above = t0, equal = t1;
+  }
+  if (threadIdx.x == 0) a.count[kh * a.segs + blockIdx.x] = make_int2(above, equal);
+}
+
+// The list of kept rows: a segment's part starts behind the rows kept by the segments before it.
+__global__ void __launch_bounds__(256) evict_list_kernel(EvictArgs a) {
+  __shared__ int s_scan[4], s_pick[2];
+  const int kh = blockIdx.y, n = rows_of(a), seg = blockIdx.x;
+  int* out = a.kept + (size_t)kh * a.keep;
+  if (n <= a.keep) {
+    for (int i = seg * 256 + threadIdx.x; i < a.keep; i += a.segs * 256) out[i] = i < n ? i : -1;
+    return;
+  }
+  for (int i = seg * 256 + threadIdx.x; i < a.first; i += a.segs * 256) out[i] = i;
+  for (int i = seg * 256 + threadIdx.x; i < a.last; i += a.segs * 256) out[a.keep - a.last + i] = n - a.last + i;
+  int need = a.keep - a.first - a.last;
+  if (need == 0) return;
+  const int r0 = a.first, r1 = n - a.last, per = (r1 - r0 + a.segs - 1) / a.segs;
+  const int b = r0 + seg * per, e = b + per < r1 ? b + per : r1;
+  if (b >= e) return;
+  const uint32_t key = prefix_of(a, kh, 3, need, s_scan, s_pick);
+  int above = 0, equal = 0;  // of the segments before this one
+  for (int i = threadIdx.x; i < seg; i += 256) above += a.count[kh * a.segs + i].x, equal += a.count[kh * a.segs + i].y;
+  int t0, t1;
+  scan256(above, s_scan, t0);
+  scan256(equal, s_scan, t1);
+  equal = t1;
+  int done = a.first + t0 + (equal < need ? equal : need);
+  const float* acc = a.acc + (size_t)kh * a.n_ctx;
+  for (int base = b; base < e; base += 256) {
+    const int r = base + threadIdx.x;
+    const uint32_t k = r < e ? order_key(acc[r]) : 0u;
+    const bool eq = r < e && k == key;
+    int total_eq, total;
+    const int rank = equal + scan256(eq, s_scan, total_eq);
+    const bool take = (r < e && k > key) || (eq && rank < need);
+    const int at = done + scan256(take, s_scan, total);
+    if (take) out[at] = r;
+    done += total;
+    equal += total_eq;
+  }
+}
+
+// Rows of one cache: `lanes` 16-byte pieces a row (16 or 32) at `stride`, then for q8 the row's 16 bytes of scales.
+// MODE 0: kept rows to their places in another cache (or the workspace); 1: rows 0 .. keep - 1 of the workspace back.
+template <int MODE>
+__global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
+  const int kh = blockIdx.y, n = MODE == 0 ? rows_of(a) : *a.pos0, m = n < a.keep ? n : a.keep;
+  if (a.in_place && n <= a.keep) return;  // nothing evicted: every row is where it belongs
+  const bool v = blockIdx.z;
+  const uint8_t* src = (const uint8_t*)(v ? a.vc : a.kc);
+  uint8_t* dst = (uint8_t*)(v ? a.vo : a.ko);
+  const int lanes = a.q8 ? 16 : 32, sub = threadIdx.x % lanes, rows = 256 / lanes;
+  const size_t stride = (size_t)lanes * 16;
+  const uint8_t* ss = src + (size_t)a.nkvh * a.n_ctx * kHD;
+  uint8_t* ds = dst + (size_t)a.nkvh * a.n_out * kHD;
+  for (int i = blockIdx.x * rows + threadIdx.x / lanes; i < m; i += gridDim.x * rows) {
+    const int r = MODE == 0 ? a.kept[(size_t)kh * a.keep + i] : i;
+    const size_t from = (size_t)kh * a.n_ctx + r, to = (size_t)kh * a.n_out + i;
+    *(u4*)(dst + to * stride + sub * 16) = *(const u4*)(src + from * stride + sub * 16);
+    if (a.q8 && sub == 0) *(u4*)(ds + to * 16) = *(const u4*)(ss + from * 16);
+    if (!v && sub == 1) a.acc_o[to] = a.acc[from];
+  }
+}
+
+__global__ void evict_pos_kernel(int* pos0, int* rdelta, int keep) {
+  const int n = *pos0, m = n < keep ? n : keep;
+  *pos0 = m;
+  if (rdelta) *rdelta -= n - m;
+}
+
+// kv_accept: one workgroup per (cache or weight array, kv head) holds all the path's rows in registers before it writes
+// the first of them, so a path in any order is right.
+constexpr int kMaxPath = 64, kMaxPtrs = 64;
+struct AcceptArgs {
+  void* cache[kMaxPtrs];
+  float* acc[kMaxPtrs];
+  const int *pos0, *path, *n_path;
+  int n_cache, T, nkvh, n_ctx, q8;
+};
+__global__ void __launch_bounds__(256) accept_kernel(AcceptArgs a) {
+  __shared__ int s_src[kMaxPath], s_n;
+  const int kh = blockIdx.y, tid = threadIdx.x, pos0 = *a.pos0;
+  if (tid < 64) {
+    const int want = *a.n_path < a.T ? *a.n_path : a.T;
+    const int p = tid < want ? a.path[tid] : -1;
+    const bool ok = p >= 0 && p < a.T;
+    const uint64_t good = __ballot(ok);
+    if (tid == 0) s_n = good == ~0ull ? 64 : __builtin_ctzll(~good);  // the path ends at its first entry outside the tree
+    s_src[tid] = p;
+  }
+  __syncthreads();
+  const int n = s_n;
+  // row i of the path: from cache row pos0 + path[i] to pos0 + i, where both exist
+  auto rows = [&](int i, size_t& from, size_t& to) {
+    const long long f = (long long)pos0 + s_src[i], t = (long long)pos0 + i;
+    from = (size_t)kh * a.n_ctx + (size_t)(f < 0 ? 0 : f);
+    to = (size_t)kh * a.n_ctx + (size_t)(t < 0 ? 0 : t);
+    return f >= 0 && f < a.n_ctx && t >= 0 && t < a.n_ctx;
+  };
+  if ((int)blockIdx.x >= a.n_cache) {
+    float* acc = a.acc[blockIdx.x - a.n_cache];
+    size_t from = 0, to = 0;
+    const bool ok = tid < n && rows(tid, from, to);
+    const float x = ok ? acc[from] : 0.0f;
+    __syncthreads();
+    if (ok) acc[to] = x;
+    return;
+  }
+  uint8_t* c = (uint8_t*)a.cache[blockIdx.x];
+  const int lanes = a.q8 ? 16 : 32, sub = tid % lanes, step = 256 / lanes;
+  const size_t stride = (size_t)lanes * 16;
+  uint8_t* sc = c + (size_t)a.nkvh * a.n_ctx * kHD;
+  u4 x[8], d = {0u, 0u, 0u, 0u};
+  size_t from = 0, to = 0;
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const int i = k * step + tid / lanes;
+    if (i < n && rows(i, from, to)) x[k] = *(const u4*)(c + from * stride + sub * 16);
+  }
+  if (a.q8 && tid < n && rows(tid, from, to)) d = *(const u4*)(sc + from * 16);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const int i = k * step + tid / lanes;
+    if (i < n && rows(i, from, to)) *(u4*)(c + to * stride + sub * 16) = x[k];
+  }
+  if (a.q8 && tid < n && rows(tid, from, to)) *(u4*)(sc + to * 16) = d;
+}
+
+size_t cache_bytes(int nkvh, int n_ctx, int q8) { return q27h_kv_cache_bytes(nkvh, n_ctx, q8); }
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace q27h
+
+using namespace q27h;
+
+extern "C" size_t q27h_kv_evict_ws_bytes(int nkvh, int n_ctx, int keep, int q8, int in_place) {
+  if (nkvh <= 0 || n_ctx <= 0 || keep <= 0) return 0;
+  size_t b = up256((size_t)nkvh * 3 * kBins * 4) + up256((size_t)nkvh * segs_of(n_ctx) * 8) + up256((size_t)nkvh * keep * 4);
+  if (in_place) b += 2 * up256(cache_bytes(nkvh, keep, q8)) + up256((size_t)nkvh * keep * 4);
+  return b;
+}
+
+extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float* acc, const int* pos0, int keep, int first,
+                             int last, void* kout, void* vout, float* acc_out, int n_ctx_out, int* kept, int nkvh, int n_ctx,
+                             int q8, void* ws, size_t ws_bytes, q27h_stream_t s) {
+  if (nkvh <= 0 || nkvh > 65535 || n_ctx <= 0 || n_ctx_out <= 0) return fail(Q27H_ERR_SHAPE, "kv_evict: bad shape");
+  if (keep <= 0 || first < 0 || last < 0 || (long long)first + last > keep)
+    return fail(Q27H_ERR_SHAPE, "kv_evict: keep >= 1 and 0 <= first + last <= keep");
+  if (keep > n_ctx_out || keep > n_ctx) return fail(Q27H_ERR_SHAPE, "kv_evict: keep must be <= n_ctx and n_ctx_out");
+  if (!kcache || !vcache || !acc || !pos0 || !kout || !vout || !acc_out || !ws)
+    return fail(Q27H_ERR_ARG, "kv_evict: null pointer");
+  if (!aligned16(kcache) || !aligned16(vcache) || !aligned16(kout) || !aligned16(vout) || !aligned16(ws))
+    return fail(Q27H_ERR_ARG, "kv_evict: tensors need 16-byte alignment");
+  const size_t in = cache_bytes(nkvh, n_ctx, q8), out = cache_bytes(nkvh, n_ctx_out, q8);
+  const size_t ain = (size_t)nkvh * n_ctx * 4, aout = (size_t)nkvh * n_ctx_out * 4;
+  const bool in_place = kout == kcache && vout == vcache && acc_out == acc && n_ctx_out == n_ctx;
+  if (overlaps(kcache, in, vcache, in) || (!in_place && (overlaps(kcache, in, kout, out) || overlaps(kcache, in, vout, out) ||
+      overlaps(vcache, in, kout, out) || overlaps(vcache, in, vout, out) || overlaps(acc, ain, acc_out, aout) ||
+      overlaps(kout, out, vout, out))))
+    return fail(Q27H_ERR_ARG, "kv_evict: the outputs overlap the inputs (all of them in place, or none)");
+  if (ws_bytes < q27h_kv_evict_ws_bytes(nkvh, n_ctx, keep, q8, in_place)) return fail(Q27H_ERR_ARG, "kv_evict: workspace too small");
+  EvictArgs a = {};
+  uint8_t* p = (uint8_t*)ws;
+  auto take = [&](size_t n) {
+    uint8_t* r = p;
+    p += up256(n);
+    return r;
+  };
+  a.kc = kcache, a.vc = vcache, a.acc = acc, a.pos0 = pos0;
+  a.keep = keep, a.first = first, a.last = last, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8, a.segs = segs_of(n_ctx), a.in_place = in_place;
+  a.hist = (int*)take((size_t)nkvh * 3 * kBins * 4);
+  a.count = (int2*)take((size_t)nkvh * a.segs * 8);
+  int* list = (int*)take((size_t)nkvh * keep * 4);
+  a.kept = kept ? kept : list;
+  const dim3 grid((unsigned)a.segs, (unsigned)nkvh), block(256);
+  hipStream_t st = stream_of(s);
+  hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)(nkvh * 3 * kBins / 1024)), block, 0, st, a.hist);
+  for (int pass = 0; pass < 3; pass++) hipLaunchKernelGGL(evict_hist_kernel, grid, block, 0, st, a, pass);
+  hipLaunchKernelGGL(evict_count_kernel, grid, block, 0, st, a);
+  hipLaunchKernelGGL(evict_list_kernel, grid, block, 0, st, a);
+  const int rows = q8 ? 16 : 8;
+  int chunks = (keep + rows - 1) / rows;
+  const int most = 16 * kCUs / (2 * nkvh) < 1 ? 1 : 16 * kCUs / (2 * nkvh);
+  chunks = chunks > most ? most : chunks;
+  const dim3 mgrid((unsigned)chunks, (unsigned)nkvh, 2);
+  if (!in_place) {
+    a.ko = kout, a.vo = vout, a.acc_o = acc_out, a.n_out = n_ctx_out;
+    hipLaunchKernelGGL(evict_move_kernel<0>, mgrid, block, 0, st, a);
+  } else {
+    a.ko = take(cache_bytes(nkvh, keep, q8)), a.vo = take(cache_bytes(nkvh, keep, q8));
+    a.acc_o = (float*)take((size_t)nkvh * keep * 4), a.n_out = keep;
+    hipLaunchKernelGGL(evict_move_kernel<0>, mgrid, block, 0, st, a);
+    EvictArgs b = a;
+    b.kc = a.ko, b.vc = a.vo, b.acc = a.acc_o, b.n_ctx = keep;
+    b.ko = kout, b.vo = vout, b.acc_o = acc_out, b.n_out = n_ctx;
+    hipLaunchKernelGGL(evict_move_kernel<1>, mgrid, block, 0, st, b);
+  }
+  return check_launch("kv_evict");
+}
+
+extern "C" int q27h_kv_evict_pos(int* pos0, int* rdelta, int keep, q27h_stream_t s) {
+  if (keep <= 0) return fail(Q27H_ERR_SHAPE, "kv_evict_pos: keep >= 1");
+  if (!pos0) return fail(Q27H_ERR_ARG, "kv_evict_pos: null pointer");
+  hipLaunchKernelGGL(evict_pos_kernel, dim3(1), dim3(1), 0, stream_of(s), pos0, rdelta, keep);
+  return check_launch("kv_evict_pos");
+}
+
+extern "C" int q27h_kv_accept(void* const* caches, int n_caches, float* const* accs, int n_accs, const int* pos0, const int* path,
+                              const int* n_path, int T, int nkvh, int n_ctx, int q8, q27h_stream_t s) {
+  if (T < 0 || T > kMaxPath) return fail(Q27H_ERR_SHAPE, "kv_accept: T must be 0..64");
+  if (n_caches < 0 || n_accs < 0 || nkvh <= 0 || nkvh > 65535 || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "kv_accept: bad shape");
+  if (T == 0 || n_caches + n_accs == 0) return Q27H_OK;
+  if (!pos0 || !path || !n_path || (n_caches && !caches) || (n_accs && !accs)) return fail(Q27H_ERR_ARG, "kv_accept: null pointer");
+  for (int i = 0; i < n_caches; i++) {
+    if (!caches[i]) return fail(Q27H_ERR_ARG, "kv_accept: null pointer");
+    if (!aligned16(caches[i])) return fail(Q27H_ERR_ARG, "kv_accept: caches need 16-byte alignment");
+  }
+  for (int i = 0; i < n_accs; i++)
+    if (!accs[i]) return fail(Q27H_ERR_ARG, "kv_accept: null pointer");
+  for (int c = 0, w = 0; c < n_caches || w < n_accs;) {
+    AcceptArgs a = {};
+    a.pos0 = pos0, a.path = path, a.n_path = n_path, a.T = T, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8;
+    int n_w = 0;
+    while (c < n_caches && a.n_cache < kMaxPtrs) a.cache[a.n_cache++] = caches[c++];
+    while (w < n_accs && n_w < kMaxPtrs) a.acc[n_w++] = accs[w++];
+    hipLaunchKernelGGL(accept_kernel, dim3((unsigned)(a.n_cache + n_w), (unsigned)nkvh), dim3(256), 0, stream_of(s), a);
+  }
+  return check_launch("kv_accept");
+}

@@ -110,6 +110,97 @@ def attn_prep(qg, k, v, q_norm, k_norm, qn, kcache, vcache, pos0, T, eps, theta_
                                _ptr(pf), pf_bytes, _ptr(rope3), _ptr(rdelta)))
 
 
+# ---------------------------------------------------------------- attention over the cache that attn_prep writes
+def _bytes(ws):
+    return 0 if ws is None else ws.numel() * ws.element_size()
+
+
+def attn_tree_ws_bytes(T, nqh, nkvh, n_ctx):
+    return int(lib().q27h_attn_tree_ws_bytes(T, nqh, nkvh, n_ctx))
+
+
+def attn_tree(qn, kcache, vcache, pos0, tree, T, scale, nqh, nkvh, n_ctx, q8, o, ws, s=None, lse=None):
+    """Attention of T <= 64 drafted tokens (cache rows *pos0 + t) over the cache: every row before *pos0, and of the
+    drafted rows those of the token's 64-bit mask in `tree` (int64 / uint64 tensor; None: a chain). o f32 [T][nqh][256],
+    lse f32 [T][nqh]; ws: a tensor of attn_tree_ws_bytes() bytes, one per call that may run at a time."""
+    check(lib().q27h_attn_tree(_ptr(qn), _ptr(kcache), _ptr(vcache), _ptr(pos0), _ptr(tree), T, scale, nqh, nkvh, n_ctx,
+                               int(q8), _ptr(o), _ptr(lse), _ptr(ws), _bytes(ws), _stream(s)))
+
+
+def attn_weights(qn, lse, kcache, pos0, tree, T, scale, nqh, nkvh, n_ctx, q8, acc, s=None, rows=None):
+    """acc f32 [nkvh][n_ctx]: adds the attention weight each cache row got from the tokens of attn_tree's call (of those
+    in the 64-bit device mask `rows`, if given); the weights of the batch's own rows begin here."""
+    check(lib().q27h_attn_weights(_ptr(qn), _ptr(lse), _ptr(kcache), _ptr(pos0), _ptr(tree), _ptr(rows), T, scale, nqh, nkvh,
+                                  n_ctx, int(q8), _ptr(acc), _stream(s)))
+
+
+def kv_evict_ws_bytes(nkvh, n_ctx, keep, q8, in_place):
+    return int(lib().q27h_kv_evict_ws_bytes(nkvh, n_ctx, keep, int(q8), int(in_place)))
+
+
+def kv_evict(kcache, vcache, acc, pos0, keep, first, last, kout, vout, acc_out, n_ctx_out, kept, nkvh, n_ctx, q8, ws, s=None):
+    """Keeps, per kv head, the first `first`, the last `last` and the heaviest rows between, `keep` in all, moved in order
+    to kout / vout / acc_out (the inputs themselves, or others); kept int32 [nkvh][keep] (may be None) lists them."""
+    check(lib().q27h_kv_evict(_ptr(kcache), _ptr(vcache), _ptr(acc), _ptr(pos0), keep, first, last, _ptr(kout), _ptr(vout),
+                              _ptr(acc_out), n_ctx_out, _ptr(kept), nkvh, n_ctx, int(q8), _ptr(ws), _bytes(ws), _stream(s)))
+
+
+def kv_evict_pos(pos0, rdelta, keep, s=None):
+    """After every layer's kv_evict: *pos0 = min(*pos0, keep), *rdelta (may be None) less the rows that went."""
+    check(lib().q27h_kv_evict_pos(_ptr(pos0), _ptr(rdelta), keep, _stream(s)))
+
+
+class KvPointers:
+    """Addresses of caches or weight arrays for kv_accept, listed once; holds the tensors."""
+
+    def __init__(self, tensors):
+        import ctypes
+
+        self.tensors, self.n = list(tensors), len(tensors)
+        self.addr = (ctypes.c_void_p * max(1, self.n))(*(_ptr(t) for t in self.tensors))
+
+
+def kv_pointers(tensors):
+    return KvPointers(tensors)
+
+
+def kv_accept(caches, accs, pos0, path, n_path, T, nkvh, n_ctx, q8, s=None):
+    """Rows *pos0 + path[i] of every cache (and weight array) to *pos0 + i, i < *n_path <= T; caches and accs: KvPointers,
+    lists of tensors or None."""
+    c, a = (x if isinstance(x, KvPointers) else KvPointers(x or []) for x in (caches, accs))
+    check(lib().q27h_kv_accept(c.addr, c.n, a.addr, a.n, _ptr(pos0), _ptr(path), _ptr(n_path), T, nkvh, n_ctx, int(q8), _stream(s)))
+
+
+def kv_block_bytes(nkvh, n_ctx):
+    return int(lib().q27h_kv_block_bytes(nkvh, n_ctx))
+
+
+def kv_block_bounds(kcache, pos0, T, nkvh, n_ctx, q8, kb, s=None):
+    """Bounds (int8, one scale) of the 64-row blocks that rows *pos0 .. *pos0 + T - 1 touch, into kb."""
+    check(lib().q27h_kv_block_bounds(_ptr(kcache), _ptr(pos0), T, nkvh, n_ctx, int(q8), _ptr(kb), _stream(s)))
+
+
+def attn_select_ws_bytes(T, nkvh, n_ctx):
+    return int(lib().q27h_attn_select_ws_bytes(T, nkvh, n_ctx))
+
+
+def attn_select(qn, kb, pos0, T, nqh, nkvh, n_ctx, nsel, first, last, idx, ws, s=None):
+    """idx int32 [T][nkvh][nsel]: the blocks each token reads, ascending, -1 behind the last: the first `first`, the last
+    `last` and the best scored ones between."""
+    check(lib().q27h_attn_select(_ptr(qn), _ptr(kb), _ptr(pos0), T, nqh, nkvh, n_ctx, nsel, first, last, _ptr(idx), _ptr(ws),
+                                 _bytes(ws), _stream(s)))
+
+
+def attn_blocks_ws_bytes(T, nqh, nkvh, nsel):
+    return int(lib().q27h_attn_blocks_ws_bytes(T, nqh, nkvh, nsel))
+
+
+def attn_blocks(qn, kcache, vcache, pos0, idx, T, nsel, scale, nqh, nkvh, n_ctx, q8, o, ws, s=None, lse=None):
+    """Causal attention of T tokens over the rows of the blocks in idx only."""
+    check(lib().q27h_attn_blocks(_ptr(qn), _ptr(kcache), _ptr(vcache), _ptr(pos0), _ptr(idx), T, nsel, scale, nqh, nkvh, n_ctx,
+                                 int(q8), _ptr(o), _ptr(lse), _ptr(ws), _bytes(ws), _stream(s)))
+
+
 def rmsnorm_q8(x, w, h, xq, xd, n, rows, eps, s=None, xs=None):
     check(lib().q27h_rmsnorm_q8(_ptr(x), _ptr(w), _ptr(h), _ptr(xq), _ptr(xd), n, rows, eps, _stream(s), _ptr(xs)))
 
