@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(const uint8_t* __rest
   bool odd = false;
 #pragma unroll
   for (int c = 0; c < 4; c++) a[c] = __builtin_huge_valf(), z[c] = -__builtin_huge_valf();
+#pragma unroll 8
   for (int r = r0 + w; r < r1; r += 4) {
     const size_t row = (size_t)kh * n_ctx + r;
     float x[4];
@@ -131,27 +132,34 @@ __global__ void __launch_bounds__(256) select_score_kernel(const float* __restri
   const int b1 = split * per + per < tiles ? split * per + per : tiles;
   if (split * per >= b1) return;
   const int used = (T - t0 + per_tile - 1) / per_tile < kRowTiles ? (T - t0 + per_tile - 1) / per_tile : kRowTiles;
-  for (int r = w; r < used * 16; r += 4) {
-    const int t = t0 + r / gp, h = r % gp;
-    const bool on = t < T && h < group;
-    const float4 v = on ? ld4(qn + ((size_t)t * nqh + kh * group + h) * kHD + 4 * l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float x[4] = {v.x, v.y, v.z, v.w};
-    const float amax = wave_max(__builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
-                                                __builtin_fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3]))));
-    const bool bad = __any(not_finite(x[0]) || not_finite(x[1]) || not_finite(x[2]) || not_finite(x[3]));
-    float inv;
-    const float d = scale_of(bad ? 0.0f : amax, inv);
-    int p[4], m[4];
+  for (int rt = 0; rt < used; rt++) {
+    float4 in[4];  // the wave's four rows of the tile, requested together
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const int q = bad ? 0 : code_of(x[c], inv);
-      p[c] = q > 0 ? q : 0;
-      m[c] = q < 0 ? q : 0;
+    for (int k = 0; k < 4; k++) {
+      const int r = rt * 16 + w + 4 * k, t = t0 + r / gp, h = r % gp;
+      in[k] = t < T && h < group ? ld4(qn + ((size_t)t * nqh + kh * group + h) * kHD + 4 * l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const int slot = ((l >> 2) & 3) * 16 + (r & 15), at = (l & 3) * 4;
-    *(uint32_t*)&s_q[r >> 4][0][l >> 4][slot][at] = pack4_i8(p[0], p[1], p[2], p[3]);
-    *(uint32_t*)&s_q[r >> 4][1][l >> 4][slot][at] = pack4_i8(m[0], m[1], m[2], m[3]);
-    if (l == 0) s_d[r] = d;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int r = w + 4 * k;
+      const float x[4] = {in[k].x, in[k].y, in[k].z, in[k].w};
+      const float amax = wave_max(__builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
+                                                  __builtin_fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3]))));
+      const bool bad = __any(not_finite(x[0]) || not_finite(x[1]) || not_finite(x[2]) || not_finite(x[3]));
+      float inv;
+      const float d = scale_of(bad ? 0.0f : amax, inv);
+      int p[4], m[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int q = bad ? 0 : code_of(x[c], inv);
+        p[c] = q > 0 ? q : 0;
+        m[c] = q < 0 ? q : 0;
+      }
+      const int slot = ((l >> 2) & 3) * 16 + r, at = (l & 3) * 4;
+      *(uint32_t*)&s_q[rt][0][l >> 4][slot][at] = pack4_i8(p[0], p[1], p[2], p[3]);
+      *(uint32_t*)&s_q[rt][1][l >> 4][slot][at] = pack4_i8(m[0], m[1], m[2], m[3]);
+      if (l == 0) s_d[rt * 16 + r] = d;
+    }
   }
   __syncthreads();
   for (int bt = split * per + w; bt < b1; bt += 4) {
@@ -183,13 +191,18 @@ __global__ void __launch_bounds__(256) select_score_kernel(const float* __restri
   }
 }
 
-// One workgroup per (token, kv head): the nsel-th largest key by four 8-bit digits over keys in LDS, then the chosen
-// blocks in order. The first `first` blocks and the last `last` ones up to the token's own rank above every score.
+// One workgroup per (token, kv head). Always taken are the first `first` blocks and the last `last` ones up to the token's
+// own; of the others, keys in LDS, the need-th largest is found by 8-bit digits of key - (least key), so that the first
+// digit already tells them apart (digits of the key itself would put most scores, which share their exponents, in one
+// histogram bin, and its counter's updates one behind another). It ends as soon as a bin is taken whole. Then a thread
+// counts and lists a stretch of consecutive blocks of its own. (2345 blocks: 18 us with the key's own digits and a
+// workgroup sum for every 256 blocks, 6 us so.)
 __global__ void __launch_bounds__(256) select_pick_kernel(const float* __restrict__ score, const int* __restrict__ dpos0, int nkvh,
                                                           int n_ctx, int nsel, int first, int last, int* __restrict__ idx) {
   extern __shared__ uint32_t s_key[];
-  __shared__ int s_hist[256], s_scan[4], s_pick[2];
-  const int t = blockIdx.x / nkvh, tid = threadIdx.x, nblk = blocks_of(n_ctx);
+  __shared__ int s_hist[256], s_scan[4], s_pick[3];
+  __shared__ uint32_t s_end[8];
+  const int t = blockIdx.x / nkvh, tid = threadIdx.x, w = tid >> 6, nblk = blocks_of(n_ctx);
   const long long pos = (long long)*dpos0 + t;
   const int nb = pos < 0 ? 0 : pos >= n_ctx ? nblk : (int)(pos / kBlockRows) + 1;
   int* out = idx + (size_t)blockIdx.x * nsel;
@@ -198,41 +211,73 @@ __global__ void __launch_bounds__(256) select_pick_kernel(const float* __restric
     return;
   }
   const float* row = score + (size_t)blockIdx.x * nblk;
-  for (int b = tid; b < nb; b += 256)
-    s_key[b] = b < first || b >= nb - last ? order_key(__builtin_huge_valf()) : order_key(row[b]);
-  uint32_t prefix = 0;
-  int need = nsel;  // keys still to take among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  const int b0 = first, b1 = nb - last;  // the blocks chosen from
+  uint32_t least = ~0u, most = 0u;
+#pragma unroll 4
+  for (int b = b0 + tid; b < b1; b += 256) {
+    const uint32_t k = order_key(row[b]);
+    s_key[b] = k;
+    least = least < k ? least : k;
+    most = most > k ? most : k;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t x = __shfl_xor(least, d), y = __shfl_xor(most, d);
+    least = least < x ? least : x;
+    most = most > y ? most : y;
+  }
+  if ((tid & 63) == 0) s_end[w] = least, s_end[4 + w] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    least = least < s_end[i] ? least : s_end[i];
+    most = most > s_end[4 + i] ? most : s_end[4 + i];
+  }
+  // `need` blocks are still to be taken among the keys whose digits above `shift` are those of `prefix`
+  int need = nsel - first - last, shift = need && least < most ? 32 - __builtin_clz(most - least) : 0;
+  uint32_t prefix = need ? 0u : ~0u;
+  auto upper = [](uint32_t k, int by) { return (uint32_t)((uint64_t)k >> by); };
+  while (shift > 0) {
+    const int next = shift > 8 ? shift - 8 : 0;
     s_hist[tid] = 0;
     __syncthreads();
-    for (int b = tid; b < nb; b += 256) {
-      const uint32_t k = s_key[b];
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255], 1);
+    for (int b = b0 + tid; b < b1; b += 256) {
+      const uint32_t k = s_key[b] - least;
+      if (upper(k, shift) == upper(prefix, shift)) atomicAdd(&s_hist[(k >> next) & ((1u << (shift - next)) - 1u)], 1);
     }
     __syncthreads();
     const int bin = 255 - tid, h = s_hist[bin];
     int total;
     const int above = scan256(h, s_scan, total);
-    if (above < need && need <= above + h) s_pick[0] = bin, s_pick[1] = need - above;
+    if (above < need && need <= above + h) s_pick[0] = bin, s_pick[1] = need - above, s_pick[2] = h;
     __syncthreads();
-    prefix |= (uint32_t)s_pick[0] << shift;
+    prefix |= (uint32_t)s_pick[0] << next;
     need = s_pick[1];
+    shift = next;
+    if (need == s_pick[2]) break;  // every key with these digits is taken
     __syncthreads();
   }
-  // keys above `prefix`, and the first `need` equal to it
-  int done = 0, equal = 0;
-  for (int b0 = 0; b0 < nb; b0 += 256) {
-    const int b = b0 + tid;
-    const uint32_t k = b < nb ? s_key[b] : 0u;
-    const bool eq = b < nb && k == prefix;
-    int total_eq, total;
-    const int rank = equal + scan256(eq, s_scan, total_eq);
-    const bool take = (b < nb && k > prefix) || (eq && rank < need);
-    const int at = done + scan256(take, s_scan, total);
-    if (take) out[at] = b;
-    done += total;
-    equal += total_eq;
+  __syncthreads();
+  // taken: keys above the digits found; of those with them the first `need`
+  const int per = (b1 - b0 + 255) / 256, c0 = b0 + tid * per, c1 = c0 + per < b1 ? c0 + per : b1;
+  const uint32_t p = upper(prefix, shift);
+  int above = 0, equal = 0;
+  for (int b = c0; b < c1; b++) {
+    const uint32_t k = upper(s_key[b] - least, shift);
+    above += k > p;
+    equal += k == p;
   }
+  int total;
+  int at = scan256(above, s_scan, total), rank = scan256(equal, s_scan, total);
+  at += first + (rank < need ? rank : need);
+  for (int b = c0; b < c1; b++) {
+    const uint32_t k = upper(s_key[b] - least, shift);
+    const bool take = k > p || (k == p && rank < need);
+    rank += k == p;
+    if (take) out[at++] = b;
+  }
+  for (int i = tid; i < first; i += 256) out[i] = i;
+  for (int i = tid; i < last; i += 256) out[nsel - last + i] = b1 + i;
 }
 
 int padded_group(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }

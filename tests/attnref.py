@@ -189,7 +189,7 @@ def select(q, lo, hi, d, pos0, n_ctx, nsel, first, last):
             with np.errstate(invalid="ignore"):
                 score = np.where(np.isinf(d[kh, :nb]), np.float32(np.inf), best * d[kh, :nb])
             b = np.arange(nb)
-            score = np.where((b < first) | (b >= nb - last), np.inf, score)
-            chosen = np.sort(np.argsort(-score, kind="stable")[:nsel])
+            must = (b < first) | (b >= nb - last)
+            chosen = np.sort(np.lexsort((b, -score, ~must))[:nsel])  # the ends, then by score, then the lower one
             out[t, kh, :len(chosen)] = chosen
     return out
