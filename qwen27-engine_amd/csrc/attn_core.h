@@ -231,33 +231,43 @@ struct Tiles<false> {
 };
 
 // Scores in the operands' units: s[rt][u][i] of tile row 16 u + 4 g + i and query row n of im[rt]. q8: `w` holds the
-// staged codes and scales.
+// staged codes and scales. A block's codes and scales are requested from LDS before the block before it is worked on, and
+// neighbouring products do not depend on each other: a wave has only one other to hide these latencies behind.
 template <int RT>
 __device__ __forceinline__ void scores(const WaveLds& w, const QTile* im, f4 (&s)[RT][2]) {
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = zero;
   const uint8_t* row = w.codes + n * kRow + 8 * g;
-#pragma unroll
-  for (int b = 0; b < 8; b++) {
-    if (b) __builtin_amdgcn_sched_barrier(0);  // block by block: all eight at once would not fit the registers
-    h8 k[2];
-    u2 ks[2];
+  u2 x[2][2], ks[2][2];
+  auto ask = [&](int b) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const u2 x = *(const u2*)(row + kUpper * u + 32 * b);
-      k[u] = codes8(x.x, x.y);
-      ks[u] = scales_of(w.ks, b, u);
+      x[b & 1][u] = *(const u2*)(row + kUpper * u + 32 * b);
+      ks[b & 1][u] = scales_of(w.ks, b, u);
     }
+  };
+  ask(0);
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    if (b < 7) ask(b + 1);
+    __builtin_amdgcn_sched_barrier(0);  // block by block: all eight at once would not fit the registers
+    h8 k[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) k[u] = codes8(x[b & 1][u].x, x[b & 1][u].y);
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
       const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
+      f4 c[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[u] = mfma16(k[u], ql, zero);
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[u] = mfma16(k[u], qh, c[u]);
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        f4 c = mfma16(k[u], ql, (f4){0.0f, 0.0f, 0.0f, 0.0f});
-        c = mfma16(k[u], qh, c);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[rt][u][i] = __builtin_fmaf(half_of(ks[u][i >> 1], i & 1), c[i], s[rt][u][i]);
+        for (int i = 0; i < 4; i++) s[rt][u][i] = __builtin_fmaf(half_of(ks[b & 1][u][i >> 1], i & 1), c[u][i], s[rt][u][i]);
         asm("" : "+v"(s[rt][u]));  // formed here: sunk to their first use, the eight blocks' products would pile up
       }
     }
@@ -266,21 +276,24 @@ __device__ __forceinline__ void scores(const WaveLds& w, const QTile* im, f4 (&s
 template <int RT>
 __device__ __forceinline__ void scores(const HKeys& t, const QTile* im, f4 (&s)[RT][2]) {
   const int l = threadIdx.x & 63;
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  f4 lo[RT][2];
 #pragma unroll
-  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = lo[rt][0] = lo[rt][1] = zero;
 #pragma unroll
   for (int b = 0; b < 8; b++) {
-    if (b) __builtin_amdgcn_sched_barrier(0);
+    if (b && !(b & 1)) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
       const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), ql, s[rt][u]);
-        s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), qh, s[rt][u]);
-      }
+      for (int u = 0; u < 2; u++) lo[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), ql, lo[rt][u]);
+#pragma unroll
+      for (int u = 0; u < 2; u++) s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), qh, s[rt][u]);
     }
   }
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) s[rt][0] += lo[rt][0], s[rt][1] += lo[rt][1];
 }
 
 // Which rows of a tile a query row sees: every one before n, and row n0 + t where bit t of `tree` is set (rows at or
@@ -389,24 +402,28 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
   // the transposing read: in a group of 16 lanes, lane j gives the address of 8 bytes of row j >> 1 and gets column j of
   // the 8 rows by 16 columns
   const uint8_t* base = w.codes + ((j >> 1) >= 4 ? kUpper + (4 * g + (j >> 1) - 4) * kRow : (4 * g + (j >> 1)) * kRow) + 8 * (j & 1);
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  v2i c[2][2];
+  u2 vs[2][2];
+  auto ask = [&](int b) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      c[b & 1][h] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(base + 32 * b + 16 * h));
+      vs[b & 1][h] = scales_of(w.vs, b, h);
+    }
+  };
+  ask(0);
 #pragma unroll
   for (int b = 0; b < 8; b++) {
-    if (b) __builtin_amdgcn_sched_barrier(0);
-    h8 v[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; hh++) {
-      typedef int v2i __attribute__((ext_vector_type(2)));
-      const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(base + 32 * b + 16 * hh));
-      v[hh] = codes8((uint32_t)r.x, (uint32_t)r.y);
-    }
-    const u2 vs[2] = {scales_of(w.vs, b, 0), scales_of(w.vs, b, 1)};
+    if (b < 7) ask(b + 1);
+    __builtin_amdgcn_sched_barrier(0);
     float x[8];  // in the order of codes8: 0, 2, 1, 3, 4, 6, 5, 7
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int e = 4 * u + ((i & 1) << 1 | i >> 1);
-        x[e] = __builtin_fmaf(p[u][i], half_of(vs[u][i >> 1], i & 1), 0.0f);
+        x[e] = __builtin_fmaf(p[u][i], half_of(vs[b & 1][u][i >> 1], i & 1), 0.0f);
         if (TAIL) x[e] = p[u][i] == 0.0f ? 0.0f : x[e];
       }
     u4 hi, lo;
@@ -415,11 +432,13 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
       hi[e] = pk_rtz(x[2 * e], x[2 * e + 1]);
       lo[e] = pk_rtz(minus_half(x[2 * e], hi[e], 0), minus_half(x[2 * e + 1], hi[e], 1));
     }
+    h8 v[2];
 #pragma unroll
-    for (int hh = 0; hh < 2; hh++) {
-      st.o[2 * b + hh] = mfma16(v[hh], __builtin_bit_cast(h8, lo), st.o[2 * b + hh]);
-      st.o[2 * b + hh] = mfma16(v[hh], __builtin_bit_cast(h8, hi), st.o[2 * b + hh]);
-    }
+    for (int h = 0; h < 2; h++) v[h] = codes8((uint32_t)c[b & 1][h].x, (uint32_t)c[b & 1][h].y);
+#pragma unroll
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[h], __builtin_bit_cast(h8, lo), st.o[2 * b + h]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[h], __builtin_bit_cast(h8, hi), st.o[2 * b + h]);
   }
 }
 __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const HValues& v) {

@@ -5,7 +5,10 @@
 // the online softmax of attn_core.h, the next tile's loads in flight behind the current one's arithmetic. The query rows
 // of a kv head (tokens x query heads of the group) are 16 or 32 to a wave; more are spread over workgroups that read the
 // same cache rows on the same XCD, so that its L2 serves all but the first. A second launch joins the splits.
+#include <type_traits>
+
 #include "attn_core.h"
+#include "attn_shared.h"
 #include "q27h_internal.h"
 
 namespace q27h {
@@ -50,7 +53,8 @@ struct AttnArgs {
   float *o, *lse;        // lse may be null
   float *part, *ml;      // [row][split][256], [row][split][2]; row = token * nqh + query head
   int T, nqh, nkvh, n_ctx, nsel;
-  int splits, groups, waves;  // attn_tree: workgroups over the query rows of a kv head, waves over the cache rows of one
+  int splits, groups, waves;  // attn_tree: workgroups over the query rows of a kv head; waves over the cache rows of one
+  int tiles;                  // attn_wide_kernel: row tiles of a workgroup
   float scale;
 };
 
@@ -131,8 +135,40 @@ __device__ __forceinline__ void full_tiles(Rows& st, const KvHead& kc, const KvH
   } while (j0 >= 0);
 }
 
-// Joins the WK waves of each row tile and writes its rows: as a split's part, or as the result where there is one split
-// only. gr: the global row (token * nqh + head) of this lane's query row, or -1.
+// Writes a wave's rows: as a split's part, or as the result where there is one split only. gr: the global row (token * nqh
+// + head) of this lane's query row, or -1. BY16: outputs o[i][j] are dims 16 i + 4 g + j; else attn_core.h's f16 order.
+template <bool BY16>
+__device__ __forceinline__ void write_rows(Rows& st, const AttnArgs& a, int split, bool single, int gr, float m, float sum) {
+  const int g = (threadIdx.x & 63) >> 4;
+  if (gr < 0) return;
+  float* dst;
+  if (single) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= inv;
+    dst = a.o + (size_t)gr * kHD;
+    if (a.lse && g == 0) a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  } else {
+    const size_t at = (size_t)gr * a.splits + split;
+    dst = a.part + at * kHD;
+    if (g == 0) *(float2*)(a.ml + at * 2) = make_float2(m, sum);
+  }
+  if constexpr (BY16) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) *(f4*)(dst + 16 * i + 4 * g) = st.o[i];
+  } else {
+#pragma unroll
+    for (int hr = 0; hr < 2; hr++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+          *(f4*)(dst + 128 * hr + 8 * (4 * g + c) + 4 * q) =
+              (f4){st.o[8 * hr + 4 * q][c], st.o[8 * hr + 4 * q + 1][c], st.o[8 * hr + 4 * q + 2][c], st.o[8 * hr + 4 * q + 3][c]};
+  }
+}
+
+// Joins the WK waves of each row tile and writes its rows.
 template <bool Q8, int WR, int WK>
 __device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const AttnArgs& a, int split, bool single, int gr) {
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4, wr = w % WR, wk = w / WR;
@@ -165,32 +201,7 @@ __device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const A
     }
     __syncthreads();
   }
-  if (wk != 0 || gr < 0) return;
-  float* dst;
-  if (single) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < 16; i++) st.o[i] *= inv;
-    dst = a.o + (size_t)gr * kHD;
-    if (a.lse && g == 0) a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
-  } else {
-    const size_t at = (size_t)gr * a.splits + split;
-    dst = a.part + at * kHD;
-    if (g == 0) *(float2*)(a.ml + at * 2) = make_float2(m, sum);
-  }
-  if constexpr (Q8) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) *(f4*)(dst + 16 * i + 4 * g) = st.o[i];
-  } else {
-#pragma unroll
-    for (int hr = 0; hr < 2; hr++)
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-          *(f4*)(dst + 128 * hr + 8 * (4 * g + c) + 4 * q) =
-              (f4){st.o[8 * hr + 4 * q][c], st.o[8 * hr + 4 * q + 1][c], st.o[8 * hr + 4 * q + 2][c], st.o[8 * hr + 4 * q + 3][c]};
-  }
+  if (wk == 0) write_rows<Q8>(st, a, split, single, gr, m, sum);
 }
 
 template <bool Q8, int WR, int WK>
@@ -232,6 +243,88 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) 
     for (; t < t1; t += WK) tail_tile<Q8>(st, kc, vc, sh.q[wr], sh.w[w], vis, tree, t * kTileKeys);
   }
   finish<Q8, WR, WK>(st, sh, a, split, sp.used == 1, row(mine));
+}
+
+// More than 32 query rows: a row tile per wave, the cache rows shared (attn_shared.h). While the waves work on one tile, the
+// next one is in registers or on its way; it goes to the other LDS buffer behind the wave's own work, and one barrier a
+// tile keeps the two apart.
+template <bool Q8, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
+  constexpr size_t kLds = sizeof(SharedTile) * 2 > sizeof(QTile) * WAVES ? sizeof(SharedTile) * 2 : sizeof(QTile) * WAVES;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kLds];  // the queries' image, then the tiles
+  __shared__ int s_odd[2];
+  QTile* im = (QTile*)s_mem;
+  SharedTile* buf = (SharedTile*)s_mem;
+  const int unit = (int)(blockIdx.x / (8 * a.groups)) * 8 + (int)(blockIdx.x & 7), rg = (int)(blockIdx.x >> 3) % a.groups;
+  if (unit >= a.nkvh * a.splits) return;
+  const int kh = unit % a.nkvh, split = unit / a.nkvh;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
+  const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
+  const Split sp = split_of(tiles, a.splits, a.waves);
+  if (split >= sp.used) return;
+  const int t0 = split * sp.per, t1 = t0 + sp.per < tiles ? t0 + sp.per : tiles;
+  const int group = a.nqh / a.nkvh, rows = a.T * group, first = rg * a.tiles * 16;
+  auto row = [&](int r) {  // global row of the workgroup's query row r
+    const int q = first + r;
+    return r < a.tiles * 16 && q < rows ? (q / group) * a.nqh + kh * group + q % group : -1;
+  };
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
+  auto left_of = [&](int t) { return vis.end - t * kTileKeys < kTileKeys ? vis.end - t * kTileKeys : kTileKeys; };
+  auto part_of = [&](int t) { return (t + 1) * kTileKeys > vis.n; };
+  Staged<Q8, WAVES> next;
+  if (t0 < t1) request<Q8, WAVES, true, true>(next, kc, vc, t0 * kTileKeys, left_of(t0));
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
+  });
+  __syncthreads();
+  QRegs q;
+  take_queries(q, im[w]);
+  Rows st;
+  rows_init<Q8>(st, im[w]);
+  const int mine = w * 16 + (threadIdx.x & 15), gr = row(mine);
+  const uint64_t tree[1] = {gr >= 0 ? tree_of(a.tree, (first + mine) / group, a.T) : 0ull};
+  const bool active = w < a.tiles && first + w * 16 < rows;
+  __syncthreads();
+  if (t0 < t1) stage<Q8, WAVES, true, true>(next, buf[0], part_of(t0), left_of(t0), &s_odd[0]);
+  if (t0 + 1 < t1) request<Q8, WAVES, true, true>(next, kc, vc, (t0 + 1) * kTileKeys, left_of(t0 + 1));
+  __syncthreads();
+  // two loops: a tile with hidden rows takes another form of the product, and with both in one loop the outputs' registers
+  // are copied between them (and spill)
+  int t = t0;
+  auto walk = [&](auto hidden, int end) {
+    constexpr bool kPart = decltype(hidden)::value;
+    for (; t < end; t++) {
+      const int at = (t - t0) & 1;
+      if (active) {
+        f4 s[1][2];
+        scores<Q8>(buf[at], q, s[0]);
+        if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
+        if constexpr (Q8) widen(st, *(const u2*)(buf[at].vs + 8 * (threadIdx.x & 63)));
+        weights(st, s[0]);
+        accumulate<Q8, kPart>(st, s[0], buf[at]);
+        if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
+      }
+      if (t + 1 < t1) {
+        stage<Q8, WAVES, true, true>(next, buf[at ^ 1], part_of(t + 1), left_of(t + 1), &s_odd[at ^ 1]);
+        if (t + 2 < t1) request<Q8, WAVES, true, true>(next, kc, vc, (t + 2) * kTileKeys, left_of(t + 2));
+      }
+      __syncthreads();
+    }
+  };
+  const int full = vis.n / kTileKeys;
+  walk(std::false_type(), full < t1 ? full : t1);
+  walk(std::true_type(), t1);
+  if (!active) return;
+  st.l += lane_xor<16>(st.l);
+  st.l += lane_xor32(st.l);
+  if constexpr (Q8) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= 512.0f;  // codes8's 2^-9
+  }
+  write_rows<true>(st, a, split, sp.used == 1, gr, st.m, st.l);
 }
 
 // attn_blocks: one workgroup per (token, kv head, split of its list); the group's query heads are one row tile.
@@ -363,7 +456,7 @@ struct WeightArgs {
   const int* pos0;
   const uint64_t *tree, *rows;
   float* acc;
-  int T, nqh, nkvh, n_ctx, splits, groups;
+  int T, nqh, nkvh, n_ctx, splits, groups, tiles;
   float scale;
 };
 
@@ -371,7 +464,7 @@ struct WeightArgs {
 // for each, its tiles; the sum over the 16 query rows of a tile is a lane reduction, that over row tiles and groups is
 // taken in order, and a row of the cache belongs to one wave: the same bits always.
 template <bool Q8, int RT>
-__global__ void __launch_bounds__(kWaves * 64, RT == 4 ? 1 : 2) attn_weights_kernel(WeightArgs a) {
+__global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs a) {
   __shared__ QTile im[RT];
   __shared__ float s_lse[RT * 16];
   __shared__ WaveLds s_w[Q8 ? kWaves : 1];
@@ -450,19 +543,108 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 4 ? 1 : 2) attn_weights_ker
   }
 }
 
-// How attn_tree's workgroups are laid out: 1, 2 or 4 row tiles of 16 query rows.
+// attn_weights of more than 32 query rows: a row tile per wave, K shared; a wave leaves its sums per cache row in LDS, and
+// the first wave adds them up, in the waves' order, behind the barrier that ends the tile.
+template <bool Q8, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(WeightArgs a) {
+  constexpr size_t kLds = sizeof(SharedTile) * 2 > sizeof(QTile) * WAVES ? sizeof(SharedTile) * 2 : sizeof(QTile) * WAVES;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kLds];
+  __shared__ float s_sum[2][WAVES][kTileKeys];
+  QTile* im = (QTile*)s_mem;
+  SharedTile* buf = (SharedTile*)s_mem;
+  const int kh = blockIdx.x % a.nkvh, split = blockIdx.x / a.nkvh;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
+  const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
+  const Split sp = split_of(tiles, a.splits, kWaves);
+  if (split >= sp.used) return;
+  const int t0 = split * sp.per, t1 = t0 + sp.per < tiles ? t0 + sp.per : tiles;
+  if (t0 >= t1) return;
+  const int group = a.nqh / a.nkvh, rows = a.T * group;
+  const uint64_t used = a.rows ? *a.rows : ~0ull;
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx);
+  float* acc = a.acc + (size_t)kh * a.n_ctx;
+  auto left_of = [&](int t) { return vis.end - t * kTileKeys < kTileKeys ? vis.end - t * kTileKeys : kTileKeys; };
+  for (int rg = 0; rg < a.groups; rg++) {
+    const int first = rg * a.tiles * 16;
+    Staged<Q8, WAVES> next;
+    request<Q8, WAVES, true, false>(next, kc, kc, t0 * kTileKeys, left_of(t0));
+    load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
+      const int q = first + r;
+      return r < a.tiles * 16 && q < rows ? a.qn + ((size_t)(q / group) * a.nqh + kh * group + q % group) * kHD : nullptr;
+    });
+    __syncthreads();
+    QRegs q;
+    take_queries(q, im[w]);
+    const float c = im[w].c[n];
+    const int r = first + w * 16 + n;
+    const bool mine = w < a.tiles && r < rows, on = mine && ((used >> (r / group)) & 1);
+    const float lse = on ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : 0.0f;
+    const uint64_t tree[1] = {mine ? tree_of(a.tree, r / group, a.T) : 0ull};
+    const bool active = __any(on);  // a row tile of which no row is asked for adds nothing
+    __syncthreads();
+    stage<Q8, WAVES, true, false>(next, buf[0], false, 0, nullptr);
+    if (t0 + 1 < t1) request<Q8, WAVES, true, false>(next, kc, kc, (t0 + 1) * kTileKeys, left_of(t0 + 1));
+    __syncthreads();
+    float old = 0.0f, old1 = 0.0f;
+    for (int t = t0; t <= t1; t++) {
+      // threads 0 .. 31: a row's weight before this tile's sums, and the sums of the tile before
+      const int j = t * kTileKeys + threadIdx.x;
+      old = old1;
+      if (threadIdx.x < kTileKeys && t < t1 && j < vis.end) old1 = j < vis.n || rg ? acc[j] : 0.0f;
+      if (t > t0 && threadIdx.x < kTileKeys && j - kTileKeys < vis.end) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) v += s_sum[(t - 1 - t0) & 1][k][threadIdx.x];
+        acc[j - kTileKeys] = old + v;
+      }
+      if (t == t1) break;
+      float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      if (active) {
+        f4 s[1][2];
+        scores<Q8>(buf[(t - t0) & 1], q, s[0]);
+        if ((t + 1) * kTileKeys > vis.n) hide<1>(s, vis, tree, t * kTileKeys);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float x = s[0][e >> 2][e & 3];
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse));
+          sum[e] = !on || x == -__builtin_huge_valf() ? 0.0f : p;
+          sum[e] += lane_xor<1>(sum[e]);
+          sum[e] += lane_xor<2>(sum[e]);
+          sum[e] += lane_xor<7>(sum[e]);
+          sum[e] += lane_xor<8>(sum[e]);
+        }
+      }
+      float v = sum[0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) v = n == e ? sum[e] : v;
+      if (n < 8) s_sum[(t - t0) & 1][w][16 * (n >> 2) + 4 * g + (n & 3)] = v;
+      if (t + 1 < t1) {
+        stage<Q8, WAVES, true, false>(next, buf[(t - t0 + 1) & 1], false, 0, nullptr);
+        if (t + 2 < t1) request<Q8, WAVES, true, false>(next, kc, kc, (t + 2) * kTileKeys, left_of(t + 2));
+      }
+      __syncthreads();
+    }
+    __syncthreads();  // the sums are read, the buffers free for the next group's queries
+  }
+}
+
+// How attn_tree's and attn_weights' workgroups are laid out by the row tiles of 16 query rows. Up to two: each wave walks
+// cache rows of its own. More: up to 8 waves of a row tile each share them, in as few groups as that takes, of equal size.
 struct TreeLayout {
-  int wr, wk, groups, splits;
+  int row_tiles, wide, groups, tiles, splits, waves;
 };
 TreeLayout tree_layout(int T, int nqh, int nkvh, int n_ctx) {
   TreeLayout t;
-  const int tiles = (T * (nqh / nkvh) + 15) / 16;
-  t.wr = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4;
-  t.wk = t.wr == 4 ? 2 : 4;
-  t.groups = (tiles + t.wr - 1) / t.wr;
+  t.row_tiles = (T * (nqh / nkvh) + 15) / 16;
+  t.wide = t.row_tiles > 2;
+  t.groups = t.wide ? (t.row_tiles + 7) / 8 : 1;
+  t.tiles = (t.row_tiles + t.groups - 1) / t.groups;
+  t.waves = 4;
   // enough workgroups for every compute unit: two of 4 waves on each, or one of 8
-  const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + t.wk - 1) / t.wk;
-  int s = (t.wr == 1 ? 2 * kCUs : kCUs) / (nkvh * t.groups);
+  const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + t.waves - 1) / t.waves;
+  const bool half = t.wide ? t.tiles <= 4 : t.row_tiles == 1;
+  int s = (half ? 2 * kCUs : kCUs) / t.groups / 8 * 8 / nkvh;  // the grid has 8 units (kv head, split) a round, see the kernels
   s = s > most ? most : s;
   t.splits = s < 1 ? 1 : s;
   return t;
@@ -504,13 +686,17 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
   a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.tree = tree, a.o = o, a.lse = lse;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
   const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
-  a.splits = lay.splits, a.groups = lay.groups, a.waves = lay.wk;
+  a.splits = lay.splits, a.groups = lay.groups, a.waves = lay.waves, a.tiles = lay.tiles;
   a.part = (float*)ws, a.ml = a.part + (size_t)T * nqh * a.splits * kHD;
-  const unsigned grid = (unsigned)((nkvh * a.splits + 7) / 8 * 8 * a.groups);
-  const auto kern = lay.wr == 1   ? (q8 ? attn_tree_kernel<true, 1, 4> : attn_tree_kernel<false, 1, 4>)
-                    : lay.wr == 2 ? (q8 ? attn_tree_kernel<true, 2, 4> : attn_tree_kernel<false, 2, 4>)
-                                  : (q8 ? attn_tree_kernel<true, 4, 2> : attn_tree_kernel<false, 4, 2>);
-  hipLaunchKernelGGL(kern, dim3(grid), dim3((unsigned)(lay.wr * lay.wk * 64)), 0, stream_of(s), a);
+  const dim3 grid((unsigned)((nkvh * a.splits + 7) / 8 * 8 * a.groups));
+  if (lay.row_tiles == 1)
+    hipLaunchKernelGGL((q8 ? attn_tree_kernel<true, 1, 4> : attn_tree_kernel<false, 1, 4>), grid, dim3(256), 0, stream_of(s), a);
+  else if (lay.row_tiles == 2)
+    hipLaunchKernelGGL((q8 ? attn_tree_kernel<true, 2, 4> : attn_tree_kernel<false, 2, 4>), grid, dim3(512), 0, stream_of(s), a);
+  else if (lay.tiles <= 4)
+    hipLaunchKernelGGL((q8 ? attn_wide_kernel<true, 4> : attn_wide_kernel<false, 4>), grid, dim3(256), 0, stream_of(s), a);
+  else
+    hipLaunchKernelGGL((q8 ? attn_wide_kernel<true, 8> : attn_wide_kernel<false, 8>), grid, dim3(512), 0, stream_of(s), a);
   if (lay.splits > 1) hipLaunchKernelGGL(attn_join_kernel<false>, dim3((unsigned)(T * nqh), 4), dim3(256), 0, stream_of(s), a);
   return check_launch("attn_tree");
 }
@@ -526,14 +712,23 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   WeightArgs a = {};
   a.qn = qn, a.lse = lse, a.kcache = kcache, a.pos0 = pos0, a.tree = tree, a.rows = rows, a.acc = acc;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
-  const int n_rows = T * (nqh / nkvh), rt = n_rows <= 16 ? 1 : n_rows <= 32 ? 2 : 4;
-  a.groups = (n_rows + rt * 16 - 1) / (rt * 16);
+  const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  a.groups = lay.groups, a.tiles = lay.tiles;
   const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + kWaves - 1) / kWaves;
-  a.splits = 4 * kCUs / nkvh;
+  // narrow: small workgroups, four to a compute unit; wide: as many as are resident
+  a.splits = (!lay.wide ? 4 * kCUs : lay.tiles <= 4 ? 2 * kCUs : kCUs) / nkvh;
   a.splits = a.splits > most ? most : a.splits < 1 ? 1 : a.splits;
-  const auto kern = q8 ? (rt == 1 ? attn_weights_kernel<true, 1> : rt == 2 ? attn_weights_kernel<true, 2> : attn_weights_kernel<true, 4>)
-                       : (rt == 1 ? attn_weights_kernel<false, 1> : rt == 2 ? attn_weights_kernel<false, 2> : attn_weights_kernel<false, 4>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)(nkvh * a.splits)), dim3(256), 0, stream_of(s), a);
+  const dim3 grid((unsigned)(nkvh * a.splits));
+  if (lay.row_tiles == 1)
+    hipLaunchKernelGGL((q8 ? attn_weights_kernel<true, 1> : attn_weights_kernel<false, 1>), grid, dim3(256), 0, stream_of(s), a);
+  else if (lay.row_tiles == 2)
+    hipLaunchKernelGGL((q8 ? attn_weights_kernel<true, 2> : attn_weights_kernel<false, 2>), grid, dim3(256), 0, stream_of(s), a);
+  else if (lay.tiles <= 4)
+    hipLaunchKernelGGL((q8 ? attn_weights_wide_kernel<true, 4> : attn_weights_wide_kernel<false, 4>), grid, dim3(256), 0,
+                       stream_of(s), a);
+  else
+    hipLaunchKernelGGL((q8 ? attn_weights_wide_kernel<true, 8> : attn_weights_wide_kernel<false, 8>), grid, dim3(512), 0,
+                       stream_of(s), a);
   return check_launch("attn_weights");
 }
 
