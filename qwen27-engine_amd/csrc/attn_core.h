@@ -24,6 +24,8 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
+// By value: __builtin_bit_cast of a vector's element, as an lvalue, would take the vector's first.
+__device__ __forceinline__ h2 as_h2(uint32_t x) { return __builtin_bit_cast(h2, x); }
 __device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ uint32_t pk_rtz(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
@@ -31,13 +33,13 @@ __device__ __forceinline__ uint32_t pk_rtz(float a, float b) {
 // x - (float)h, exact for h = x rounded towards zero. The opaque -1 keeps the fma, which v_fma_mix_f32 does on the half
 // itself; a plain difference is two instructions (measured: 64 fewer of 690 in a tile).
 __device__ __forceinline__ float minus_half(float x, uint32_t pair, int hi) {
-  const h2 v = __builtin_bit_cast(h2, pair);
+  const h2 v = as_h2(pair);
   float m1 = -1.0f;
   asm("" : "+s"(m1));
   return __builtin_fmaf((float)(hi ? v[1] : v[0]), m1, x);
 }
 __device__ __forceinline__ float half_of(uint32_t pair, int hi) {
-  const h2 v = __builtin_bit_cast(h2, pair);
+  const h2 v = as_h2(pair);
   return (float)(hi ? v[1] : v[0]);
 }
 // Four int8 codes -> four halves of value code * 2^-9: byte ^ 0x80 = code + 128 = u, which as the low byte of a half is
@@ -56,6 +58,16 @@ __device__ __forceinline__ h8 codes8(uint32_t x, uint32_t y) {
   codes_to_half(x, r[0], r[1]);
   codes_to_half(y, r[2], r[3]);
   return __builtin_bit_cast(h8, (u4){r[0], r[1], r[2], r[3]});
+}
+
+// The scheduler's order for a step of a pipeline over the 8 blocks: four matrix instructions, N vector ones behind each.
+template <int N>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, N, 0);
+  }
 }
 
 // Where a K or V cache of one kv head lies.
@@ -83,7 +95,7 @@ struct QTile {
 // All WAVES waves of the workgroup. Row r (0 .. 16 TILES - 1) is `row_ptr(r)` (nullptr: zeros). q8 caches: the eight
 // values of a lane are stored in the order of codes8, and the factor carries codes8's 2^-9. A wave requests up to 8 rows
 // before it works on the first: one round trip to memory instead of one a row (attn_weights of 32 tokens, 20001 rows:
-// 84 -> 37 us).
+// 84 -> 67 us).
 template <bool Q8, int WAVES, int TILES, typename F>
 __device__ __forceinline__ void load_queries(QTile* im, float mult, F row_ptr) {
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
@@ -144,12 +156,14 @@ struct QRows {
 };
 // One wave's LDS: 272 bytes a row of codes (4 banks on), the upper 16 rows 128 bytes (32 banks) on: the 32 lanes that read
 // together touch every bank once, for K (16 rows, two 8-byte pieces) as for V (two lane groups, 8 rows of 16 bytes).
-// K's codes are consumed before V's are staged in their place. Then the scales of K and of V: halves [block b][32 rows].
+// K's codes are consumed before V's are staged in their place. Then the scales of K and of V: halves [block b][32 rows],
+// four rows in the order 0, 2, 1, 3 of codes8.
 constexpr int kRow = 272, kUpper = 16 * kRow + 128, kCodes = kUpper + 16 * kRow;
 constexpr int kScales = 8 * 64;
 struct WaveLds {
   alignas(16) uint8_t codes[kCodes];
   alignas(16) uint8_t ks[kScales], vs[kScales];
+  alignas(16) float vf[kTileKeys];  // V's scales are stored as d / f, f the row's own power of two above them
 };
 
 // TAIL: scales of rows that do not exist are 0: whatever the memory behind the last row holds, NaN included, must not meet
@@ -166,43 +180,94 @@ __device__ __forceinline__ void load_rows(QRows& t, const KvHead& h, int j0, int
   t.s = *(const u2*)(h.scale + (size_t)j0 * 16 + (unsigned)(tile_row<TAIL>(l >> 1, left) * 16 + 8 * (l & 1)));
   if (TAIL && (l >> 1) >= left) t.s = (u2){0u, 0u};
 }
-__device__ __forceinline__ void stage_rows(const QRows& t, uint8_t* codes, uint8_t* scales) {
+__device__ __forceinline__ void put_scales(u2 s, uint8_t* scales) {
+  const int l = threadIdx.x & 63, r = l >> 1;
+  uint16_t* p = (uint16_t*)scales + 4 * (l & 1) * 32 + ((r & ~3) | (r & 1) << 1 | (r >> 1 & 1));
+  p[0] = (uint16_t)s.x;
+  p[32] = (uint16_t)(s.x >> 16);
+  p[64] = (uint16_t)s.y;
+  p[96] = (uint16_t)(s.y >> 16);
+}
+// V's: brought to |d / f| <= 1 by the power of two f above the finite scales of the row's 8 blocks, f beside them (0 for
+// a row of zeros, which leaves the others' unit alone). f meets the weight in float32, so a row of large values does not
+// coarsen another, and d / f is a half without loss unless the block's scale is below 2^-14 of f; then it is off by less
+// than 2^-24 of f.
+__device__ __forceinline__ float exp2i(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
+__device__ __forceinline__ void put_value_scales(u2 s, uint8_t* scales, float* factors) {
+  const int l = threadIdx.x & 63;
+  float x[4], m = 0.0f, odd = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[i] = half_of(i < 2 ? s.x : s.y, i & 1);
+    const bool finite = __builtin_fabsf(x[i]) < 65536.0f;
+    m = finite ? __builtin_fmaxf(m, __builtin_fabsf(x[i])) : m;
+    odd = finite ? odd : 1.0f;
+  }
+  m = __builtin_fmaxf(m, lane_xor<1>(m));
+  odd = __builtin_fmaxf(odd, lane_xor<1>(odd));
+  const uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;  // 2^(e - 127) <= m < 2^(e - 126); 0 for m = 0
+  const float down = exp2i(253u - e);
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = e ? x[i] * down : x[i];  // m = 0: zeros, or values that are not finite
+  put_scales((u2){pk_rtz(x[0], x[1]), pk_rtz(x[2], x[3])}, scales);
+  if (!(l & 1)) factors[l >> 1] = e ? exp2i(e + 1) : odd;
+}
+__device__ __forceinline__ void stage_codes(const QRows& t, WaveLds& w) {
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
 #pragma unroll
   for (int r = 0; r < 8; r++)
-    *(u4*)(codes + (r >= 4 ? kUpper + (4 * (r - 4) + g) * kRow : (4 * r + g) * kRow) + 16 * n) = t.x[r];
-  uint16_t* p = (uint16_t*)scales + 4 * (l & 1) * 32 + (l >> 1);
-  p[0] = (uint16_t)t.s.x;
-  p[32] = (uint16_t)(t.s.x >> 16);
-  p[64] = (uint16_t)t.s.y;
-  p[96] = (uint16_t)(t.s.y >> 16);
+    *(u4*)(w.codes + (r >= 4 ? kUpper + (4 * (r - 4) + g) * kRow : (4 * r + g) * kRow) + 16 * n) = t.x[r];
+}
+__device__ __forceinline__ void stage_keys(const QRows& t, WaveLds& w) {
+  stage_codes(t, w);
+  put_scales(t.s, w.ks);
   __builtin_amdgcn_wave_barrier();
 }
-// Scales of block b of the lane's rows 16 u + 4 g + i, four halves.
+__device__ __forceinline__ void stage_values(const QRows& t, WaveLds& w) {
+  stage_codes(t, w);
+  put_value_scales(t.s, w.vs, w.vf);
+  __builtin_amdgcn_wave_barrier();
+}
+// Scales of block b of the lane's rows 16 u + 4 g + i: rows i = 0, 2 in x, 1, 3 in y.
 __device__ __forceinline__ u2 scales_of(const uint8_t* scales, int b, int u) {
   const int g = (threadIdx.x & 63) >> 4;
   return *(const u2*)(scales + b * 64 + 32 * u + 8 * g);
 }
 
-// f16: K as operand rows (row 16 u + n, dims 32 b + 8 g .. + 7); V as halves 8 n .. + 7 and 128 + 8 n .. + 7 of the lane's
-// rows 16 u + 4 g + i.
-struct HKeys {
-  u4 x[2][8];
-};
+// f16: V as halves 8 n .. + 7 and 128 + 8 n .. + 7 of the lane's rows 16 u + 4 g + i, in registers. K goes from memory to LDS
+// without passing registers (16 KB a tile and wave): as operand loads a lane would read its own row, 16 rows for every 16
+// lanes, and the vector cache takes a cycle for each (1280 a tile, which bound attn_blocks: 650 us for 1027 tokens of 32
+// blocks; 400 us so). A row of 512 bytes lies in LDS as 32 pieces of 16, piece c at c ^ (row & 15), so that the
+// operand reads, the same piece of 16 rows, touch every bank once.
 struct HValues {
   u4 x[8][2];
 };
+struct HKeysLds {
+  alignas(16) uint8_t k[kTileKeys * 2 * kHD];
+};
 template <bool TAIL>
-__device__ __forceinline__ void load_rows(HKeys& t, const KvHead& h, int j0, int left) {
-  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
-#pragma unroll
-  for (int u = 0; u < 2; u++) {
-    // one offset register and immediate offsets: separate offsets for the 16 loads would cost as many registers
-    const uint8_t* p = h.rows + (size_t)j0 * (2 * kHD) + (unsigned)(tile_row<TAIL>(16 * u + n, left) * (2 * kHD) + 16 * g);
-#pragma unroll
-    for (int b = 0; b < 8; b++) t.x[u][b] = *(const u4*)(p + 64 * b);
+__device__ __forceinline__ void request_keys(HKeysLds& w, const KvHead& h, int j0, int left) {
+  const int l = threadIdx.x & 63, up = l >> 5;
+  int c = (l & 31) ^ up;
+  asm volatile("" : "+v"(c));  // the 16 offsets are formed for each tile: kept over the loop they would take 16 registers
+  const uint8_t* rows = h.rows + (size_t)j0 * (2 * kHD);
+#pragma unroll TAIL ? 2 : kTileKeys / 2
+  for (int r = 0; r < kTileKeys / 2; r++) {  // rows 2 r and 2 r + 1
+    const uint8_t* p = rows + (unsigned)(tile_row<TAIL>(2 * r + up, left) * (2 * kHD) + (c ^ (2 * r & 14)) * 16);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)p,
+                                     (__attribute__((address_space(3))) uint32_t*)(w.k + r * 4 * kHD), 16, 0, 0);
   }
 }
+// Waits until the wave's K tile has arrived while at most NEWER loads that were issued behind it have not (they return in
+// order), and keeps the reads of it behind that.
+template <int NEWER>
+__device__ __forceinline__ void keys_there() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((NEWER & 15) | (NEWER >> 4) << 14 | 0x0f70);  // vmcnt(NEWER)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+constexpr int kValueLoads = 16;  // loads of load_rows(HValues)
 template <bool TAIL>  // rows that do not exist are zeros, as the scales above
 __device__ __forceinline__ void load_rows(HValues& t, const KvHead& h, int j0, int left) {
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
@@ -217,22 +282,25 @@ __device__ __forceinline__ void load_rows(HValues& t, const KvHead& h, int j0, i
     if (TAIL && j >= left) t.x[e][0] = t.x[e][1] = (u4){0u, 0u, 0u, 0u};
   }
 }
-template <bool Q8>
-struct Tiles;
-template <>
-struct Tiles<true> {
-  typedef QRows K;
-  typedef QRows V;
+// A wave's query rows as operands in registers, from their LDS image.
+struct QRegs {
+  h8 hi[8], lo[8];
+  __device__ __forceinline__ h8 low(int b) const { return lo[b]; }
 };
-template <>
-struct Tiles<false> {
-  typedef HKeys K;
-  typedef HValues V;
+// The same with the second terms left in LDS, where 32 registers more would spill.
+struct QHalf {
+  h8 hi[8];
+  const uint32_t (*lo)[64][4];
+  __device__ __forceinline__ h8 low(int b) const { return *(const h8*)lo[b][threadIdx.x & 63]; }
 };
+__device__ __forceinline__ void take_queries(QRegs& q, const QTile& im) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int b = 0; b < 8; b++) q.hi[b] = *(const h8*)im.v[0][b][l], q.lo[b] = *(const h8*)im.v[1][b][l];
+}
 
 // Scores in the operands' units: s[rt][u][i] of tile row 16 u + 4 g + i and query row n of im[rt]. q8: `w` holds the
-// staged codes and scales. A block's codes and scales are requested from LDS before the block before it is worked on, and
-// neighbouring products do not depend on each other: a wave has only one other to hide these latencies behind.
+// staged codes and scales. The blocks are a pipeline (see interleave): a wave has only one other to hide latencies behind.
 template <int RT>
 __device__ __forceinline__ void scores(const WaveLds& w, const QTile* im, f4 (&s)[RT][2]) {
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
@@ -240,57 +308,84 @@ __device__ __forceinline__ void scores(const WaveLds& w, const QTile* im, f4 (&s
 #pragma unroll
   for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = zero;
   const uint8_t* row = w.codes + n * kRow + 8 * g;
-  u2 x[2][2], ks[2][2];
+  u2 x[2][2], ks[3][2];
+  h8 k[2][2];
+  f4 c[2][RT][2];
   auto ask = [&](int b) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       x[b & 1][u] = *(const u2*)(row + kUpper * u + 32 * b);
-      ks[b & 1][u] = scales_of(w.ks, b, u);
+      ks[b % 3][u] = scales_of(w.ks, b, u);
     }
+  };
+  auto turn = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) k[b & 1][u] = codes8(x[b & 1][u].x, x[b & 1][u].y);
+  };
+  auto scale = [&](int b) {
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          s[rt][u][i] = __builtin_fmaf(half_of(ks[b % 3][u][i & 1], i >> 1), c[b & 1][rt][u][i], s[rt][u][i]);
+        asm("" : "+v"(s[rt][u]));  // formed here: sunk to their first use, the eight blocks' products would pile up
+      }
+  };
+  // a step per block: its products, the scaling of the block before, the next block's codes turned, the one after's read
+  h8 q[2][RT][2];
+  auto ask_q = [&](int b) {
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) q[b & 1][rt][0] = *(const h8*)im[rt].v[0][b][l], q[b & 1][rt][1] = *(const h8*)im[rt].v[1][b][l];
+  };
+  ask(0);
+  ask_q(0);
+  turn(0);
+  ask(1);
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    __builtin_amdgcn_sched_barrier(0);  // block by block: all eight at once would not fit the registers
+    if (b < 7) ask_q(b + 1);
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[b & 1][rt][u] = mfma16(k[b & 1][u], q[b & 1][rt][1], zero);
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[b & 1][rt][u] = mfma16(k[b & 1][u], q[b & 1][rt][0], c[b & 1][rt][u]);
+    }
+    if (b) scale(b - 1);
+    if (b < 7) turn(b + 1);
+    if (b < 6) ask(b + 2);
+    if (RT == 1) interleave<7>();
+  }
+  scale(7);
+}
+template <int RT, typename Q>
+__device__ __forceinline__ void scores(const HKeysLds& w, const Q (&q)[RT], f4 (&s)[RT][2]) {
+  const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  f4 lo[RT][2];
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = lo[rt][0] = lo[rt][1] = zero;
+  h8 k[2][2];
+  auto ask = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) k[b & 1][u] = *(const h8*)(w.k + (16 * u + n) * 2 * kHD + ((4 * b + g) ^ n) * 16);
   };
   ask(0);
 #pragma unroll
   for (int b = 0; b < 8; b++) {
     if (b < 7) ask(b + 1);
-    __builtin_amdgcn_sched_barrier(0);  // block by block: all eight at once would not fit the registers
-    h8 k[2];
-#pragma unroll
-    for (int u = 0; u < 2; u++) k[u] = codes8(x[b & 1][u].x, x[b & 1][u].y);
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-      const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
-      f4 c[2];
+      const h8 ql = q[rt].low(b);  // there by the time the products with the first terms are issued
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[u] = mfma16(k[u], ql, zero);
+      for (int u = 0; u < 2; u++) s[rt][u] = mfma16(k[b & 1][u], q[rt].hi[b], s[rt][u]);
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[u] = mfma16(k[u], qh, c[u]);
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[rt][u][i] = __builtin_fmaf(half_of(ks[b & 1][u][i >> 1], i & 1), c[u][i], s[rt][u][i]);
-        asm("" : "+v"(s[rt][u]));  // formed here: sunk to their first use, the eight blocks' products would pile up
-      }
+      for (int u = 0; u < 2; u++) lo[rt][u] = mfma16(k[b & 1][u], ql, lo[rt][u]);
     }
-  }
-}
-template <int RT>
-__device__ __forceinline__ void scores(const HKeys& t, const QTile* im, f4 (&s)[RT][2]) {
-  const int l = threadIdx.x & 63;
-  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  f4 lo[RT][2];
-#pragma unroll
-  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = lo[rt][0] = lo[rt][1] = zero;
-#pragma unroll
-  for (int b = 0; b < 8; b++) {
-    if (b && !(b & 1)) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-      const h8 qh = *(const h8*)im[rt].v[0][b][l], ql = *(const h8*)im[rt].v[1][b][l];
-#pragma unroll
-      for (int u = 0; u < 2; u++) lo[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), ql, lo[rt][u]);
-#pragma unroll
-      for (int u = 0; u < 2; u++) s[rt][u] = mfma16(__builtin_bit_cast(h8, t.x[u][b]), qh, s[rt][u]);
-    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int rt = 0; rt < RT; rt++) s[rt][0] += lo[rt][0], s[rt][1] += lo[rt][1];
@@ -322,17 +417,16 @@ __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint6
 
 // ---------------------------------------------------------------- online softmax
 // State of 16 query rows in a wave: lane (n, g) holds of row n the reference M (the same in its four lanes), its own part
-// of the sum l and 64 outputs. Weights are p = 2^(s - M). M is not the maximum itself: it is only moved when p times the
-// largest V scale seen would leave f16's range, that is when s - M > 15 - k (largest scale < 2^k; k = 0 for an f16 cache,
-// whose values multiply p inside the instruction), and then to s - (12 - k), so that the largest products lie near 2^12,
-// where the two f16 terms hold 22 bits, and small ones down to 2^-36 of them are still in range.
+// of the sum l and 64 outputs. Weights are p = 2^(s - M). M is not the maximum itself: it is only moved when p would leave
+// f16's range, that is when s - M > 15, and then to s - 12, so that the largest weights lie near 2^12, where two f16 terms
+// hold 22 bits, and small ones down to 2^-36 of them are still in range. q8: the outputs are in units of `unit`, the
+// largest row factor f of the V rows seen so far (a power of two), and a row's weight enters the product as p f / unit.
 // O, l and M of different waves and workgroups are joined by M alone.
 struct Rows {
   f4 o[16];
-  float m, l, c;
-  int k;
-  float lim;  // 2^k; 0 before the first nonzero scale
+  float m, l, c, unit;
 };
+constexpr float kLeastUnit = 0x1p-24f;
 
 template <bool Q8>
 __device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
@@ -341,41 +435,58 @@ __device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
   st.m = -3.0e38f;
   st.l = 0.0f;
   st.c = im.c[threadIdx.x & 15];
-  st.k = Q8 ? -24 : 0;
-  st.lim = Q8 ? 0.0f : 1.0f;
+  st.unit = kLeastUnit;
 }
 
-// Keeps k and 2^k above the finite scales of a q8 tile's V rows (one that is not makes its own block's outputs what they
-// are; it must not push the other products out of range).
-__device__ __forceinline__ void widen(Rows& st, u2 scales) {
-  const h2 c = __builtin_elementwise_max(__builtin_bit_cast(h2, scales.x), __builtin_bit_cast(h2, scales.y));
-  float d = __builtin_fmaxf((float)c[0], (float)c[1]);
-  if (__any(d > st.lim)) {  // a larger V scale than any so far
-    d = 0.0f;
+// Raises the unit to f where that is larger (powers of two: the quotient's exponent is their difference's).
+__device__ __forceinline__ void raise_unit(Rows& st, float f) {
+  f = __builtin_fmaxf(f, st.unit);
+  const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, f));
+  st.unit = f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float x = half_of(i < 2 ? scales.x : scales.y, i & 1);
-      d = x < 65536.0f ? __builtin_fmaxf(d, x) : d;
+  for (int i = 0; i < 16; i++) st.o[i] *= a;
+}
+// The row factors of a q8 tile (in LDS) and the unit. HIDDEN: a query row counts those of the rows that it sees, so that
+// what a hidden row holds cannot coarsen its outputs.
+template <bool HIDDEN>
+__device__ __forceinline__ void widen(Rows& st, const f4 (&p)[2], const float* factors) {
+  if constexpr (HIDDEN) {
+    float f = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const f4 x = *(const f4*)(factors + 16 * u + 4 * ((threadIdx.x & 63) >> 4));
+#pragma unroll
+      for (int i = 0; i < 4; i++) f = p[u][i] != 0.0f ? __builtin_fmaxf(f, x[i]) : f;
     }
-    d = __builtin_fmaxf(d, lane_xor<1>(d));
-    d = __builtin_fmaxf(d, lane_xor<2>(d));
-    d = __builtin_fmaxf(d, lane_xor<7>(d));
-    d = __builtin_fmaxf(d, lane_xor<8>(d));
-    d = __builtin_fmaxf(d, lane_xor<16>(d));
-    d = __builtin_fmaxf(d, lane_xor32(d));
-    const int e = __builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, d) >> 23) - 126);  // d < 2^e
-    if (e > st.k) st.k = e, st.lim = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    if (__any(f > st.unit)) {
+      f = __builtin_fmaxf(f, lane_xor<16>(f));
+      raise_unit(st, __builtin_fmaxf(f, lane_xor32(f)));
+    }
+  } else {
+    float f = factors[threadIdx.x & 31];
+    if (__any(f > st.unit)) {
+      f = __builtin_fmaxf(f, lane_xor<1>(f));
+      f = __builtin_fmaxf(f, lane_xor<2>(f));
+      f = __builtin_fmaxf(f, lane_xor<7>(f));
+      f = __builtin_fmaxf(f, lane_xor<8>(f));
+      raise_unit(st, __builtin_fmaxf(f, lane_xor<16>(f)));
+    }
   }
+}
+// What the outputs have to be multiplied by in the end: the unit, and 2^9 for codes8's 2^-9.
+template <bool Q8>
+__device__ __forceinline__ float unit_of(const Rows& st) {
+  return Q8 ? st.unit * 512.0f : 1.0f;
 }
 // p[u][i] from the scores (hidden ones are -inf), with the reference moved where it has to be.
 __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0][0], s[0][1]), __builtin_fmaxf(s[0][2], s[0][3])),
                              __builtin_fmaxf(__builtin_fmaxf(s[1][0], s[1][1]), __builtin_fmaxf(s[1][2], s[1][3])));
   mx *= st.c;
-  if (__any(mx - st.m > (float)(15 - st.k))) {
+  if (__any(mx - st.m > 15.0f)) {
     mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
     mx = __builtin_fmaxf(mx, lane_xor32(mx));
-    const float m1 = __builtin_fmaxf(st.m, mx - (float)(12 - st.k));
+    const float m1 = __builtin_fmaxf(st.m, mx - 12.0f);
     const float a = __builtin_amdgcn_exp2f(st.m - m1);
     st.m = m1;
     st.l *= a;
@@ -393,6 +504,48 @@ __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   st.l += sum;
 }
 
+// Weights as operands: two f16 terms, p = hi + lo, each the rest cut off to f16. f16 caches: rows in order.
+__device__ __forceinline__ void split(const f4 (&p)[2], u4& hi, u4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float w0 = p[e >> 1][2 * (e & 1)], w1 = p[e >> 1][2 * (e & 1) + 1];
+    hi[e] = pk_rtz(w0, w1);
+    lo[e] = pk_rtz(minus_half(w0, hi[e], 0), minus_half(w1, hi[e], 1));
+  }
+}
+
+// q8: the same of p f / unit, pairs of rows (0, 2), (1, 3) of u = 0, then of u = 1, as codes8 orders them.
+__device__ __forceinline__ void split8(const f4 (&p)[2], const float* factors, float unit, u4& hi, u4& lo) {
+  const int g = (threadIdx.x & 63) >> 4;
+  const float inv = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, unit));  // 1 / unit
+  f4 w[2];
+#pragma unroll
+  for (int u = 0; u < 2; u++) w[u] = p[u] * (*(const f4*)(factors + 16 * u + 4 * g) * inv);
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float w0 = w[e >> 1][e & 1], w1 = w[e >> 1][(e & 1) + 2];
+    hi[e] = pk_rtz(w0, w1);
+    lo[e] = pk_rtz(minus_half(w0, hi[e], 0), minus_half(w1, hi[e], 1));
+  }
+}
+// Times the stored scales d <= 1 of a block of V: hi' = hi d, rounded; the fma gives what that lost, exactly (11 by 11 bits
+// leave at most 11 below the first 11), and lo' = lo d + that. HIDDEN: a row with weight 0 is left out whatever its scale
+// is (0 times infinity is no part of the sum).
+template <bool HIDDEN>
+__device__ __forceinline__ void weigh(const u4& ph, const u4& pl, const u2 (&vs)[2], u4& hi, u4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    uint32_t x = vs[e >> 1][e & 1];
+    const uint32_t any = ph[e] | pl[e];
+    if (HIDDEN) x &= (any & 0xffffu ? 0xffffu : 0u) | (any >> 16 ? 0xffff0000u : 0u);
+    const h2 d = as_h2(x), p = as_h2(ph[e]);
+    const h2 h = p * d;
+    const h2 lost = __builtin_elementwise_fma(p, d, -h);
+    hi[e] = __builtin_bit_cast(uint32_t, h);
+    lo[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_h2(pl[e]), d, lost));
+  }
+}
+
 // O += P V. Output o[i][j]: q8: dim 16 i + 4 g + j; f16: dim 128 (i >> 3) + 8 (4 g + j) + (i & 7).
 // q8: `w` holds the staged codes and scales. TAIL: a hidden row's scale may be anything (a weight of 0 times an infinite
 // scale is no part of the sum).
@@ -405,6 +558,9 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
   typedef int v2i __attribute__((ext_vector_type(2)));
   v2i c[2][2];
   u2 vs[2][2];
+  h8 v[2][2];
+  u4 ph, pl, hi[2], lo[2];
+  split8(p, w.vf, st.unit, ph, pl);
   auto ask = [&](int b) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -412,43 +568,31 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
       vs[b & 1][h] = scales_of(w.vs, b, h);
     }
   };
+  auto turn = [&](int b) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) v[b & 1][h] = codes8((uint32_t)c[b & 1][h].x, (uint32_t)c[b & 1][h].y);
+    weigh<TAIL>(ph, pl, vs[b & 1], hi[b & 1], lo[b & 1]);
+  };
   ask(0);
+  turn(0);
+  ask(1);
 #pragma unroll
   for (int b = 0; b < 8; b++) {
-    if (b < 7) ask(b + 1);
     __builtin_amdgcn_sched_barrier(0);
-    float x[8];  // in the order of codes8: 0, 2, 1, 3, 4, 6, 5, 7
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, lo[b & 1]), st.o[2 * b + h]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int e = 4 * u + ((i & 1) << 1 | i >> 1);
-        x[e] = __builtin_fmaf(p[u][i], half_of(vs[b & 1][u][i >> 1], i & 1), 0.0f);
-        if (TAIL) x[e] = p[u][i] == 0.0f ? 0.0f : x[e];
-      }
-    u4 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      hi[e] = pk_rtz(x[2 * e], x[2 * e + 1]);
-      lo[e] = pk_rtz(minus_half(x[2 * e], hi[e], 0), minus_half(x[2 * e + 1], hi[e], 1));
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, hi[b & 1]), st.o[2 * b + h]);
+    if (b < 7) {
+      turn(b + 1);
+      if (b < 6) ask(b + 2);
+      interleave<8>();
     }
-    h8 v[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) v[h] = codes8((uint32_t)c[b & 1][h].x, (uint32_t)c[b & 1][h].y);
-#pragma unroll
-    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[h], __builtin_bit_cast(h8, lo), st.o[2 * b + h]);
-#pragma unroll
-    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[h], __builtin_bit_cast(h8, hi), st.o[2 * b + h]);
   }
 }
 __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const HValues& v) {
   u4 hi, lo;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const float w0 = p[e >> 1][2 * (e & 1)], w1 = p[e >> 1][2 * (e & 1) + 1];
-    hi[e] = pk_rtz(w0, w1);
-    lo[e] = pk_rtz(minus_half(w0, hi[e], 0), minus_half(w1, hi[e], 1));
-  }
+  split(p, hi, lo);
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     u4 x;

@@ -11,21 +11,22 @@
 namespace q27h {
 
 struct SharedTile {
-  // operand of rows 16 u + n, dims 32 b + 8 g ..: [8 u + b][lane]
+  // operand of rows 16 u + n, dims 32 b + 8 g ..: [8 u + b][16 g + (n ^ ((4 b + g) & 15))]
   alignas(16) uint32_t k[16][64][4];
-  // operand of dims 16 i + m, rows 16 u + 4 g + 0 .. 3 at 8 u: [i][16 g + (m ^ i)]; the exchange spreads the writes of one
-  // m over the banks (a wave writes one m of many i)
+  // operand of dims 16 i + m, rows 16 u + 4 g + 0 .. 3 at 8 u: [i][16 g + (m ^ i)]. The exchanges (here and in k)
+  // spread a wave's writes over the banks: it writes one row's piece of many b, g, or one m of many i
   alignas(16) uint32_t v[16][64][4];
   alignas(16) uint8_t ks[kScales], vs[kScales];
+  alignas(16) float vf[kTileKeys];
 };
 
 // What a thread holds of the next tile on its way to LDS. 256 threads carry K (and 64 of them its scales), 256 carry V;
 // with 4 waves each thread has both parts, with 8 one. Rows behind the last one that exists are read from the last one.
 template <bool Q8, int WAVES>
 struct Staged {
-  static constexpr bool kBoth = WAVES == 4;
-  u4 k[Q8 ? 2 : 4], v[4];
-  u2 s;  // q8: scales (K in one wave, V in another)
+  static constexpr int kV = WAVES == 4 ? 4 : 0;
+  u4 x[kV + 4];  // K from 0, V from kV on
+  u2 s;          // q8: scales (K in one wave, V in another)
 };
 template <int WAVES>
 __device__ __forceinline__ bool carries_k() {
@@ -47,15 +48,15 @@ __device__ __forceinline__ void request(Staged<Q8, WAVES>& t, const KvHead& kc, 
   if (K && carries_k<WAVES>()) {
 #pragma unroll
     for (int j = 0; j < (Q8 ? 2 : 4); j++) {
-      if constexpr (Q8) t.k[j] = *(const u4*)at(kc.rows, 16 * (f >> 1) + n, 64 * (2 * (f & 1) + j) + 16 * g);
-      else t.k[j] = *(const u4*)at(kc.rows, 16 * (f >> 1) + n, 64 * (4 * (f & 1) + j) + 16 * g);
+      if constexpr (Q8) t.x[j] = *(const u4*)at(kc.rows, 16 * j + (q >> 4), 16 * n);
+      else t.x[j] = *(const u4*)at(kc.rows, 8 * j + (q >> 5), 16 * (q & 31));
     }
   }
   if (V && carries_v<WAVES>()) {
     if (!Q8 || f < 2) {
       const int u = Q8 ? f : f >> 1, g4 = Q8 ? g : (q >> 5) & 3, c = Q8 ? n : q & 31;
 #pragma unroll
-      for (int e = 0; e < 4; e++) t.v[e] = *(const u4*)at(vc.rows, 16 * u + 4 * g4 + e, 16 * c);
+      for (int e = 0; e < 4; e++) t.x[t.kV + e] = *(const u4*)at(vc.rows, 16 * u + 4 * g4 + e, 16 * c);
     }
   }
   if constexpr (Q8) {
@@ -68,15 +69,6 @@ __device__ __forceinline__ void request(Staged<Q8, WAVES>& t, const KvHead& kc, 
   }
 }
 
-__device__ __forceinline__ void put_scales(u2 s, uint8_t* scales) {
-  const int l = threadIdx.x & 63;
-  uint16_t* p = (uint16_t*)scales + 4 * (l & 1) * 32 + (l >> 1);
-  p[0] = (uint16_t)s.x;
-  p[32] = (uint16_t)(s.x >> 16);
-  p[64] = (uint16_t)s.y;
-  p[96] = (uint16_t)(s.y >> 16);
-}
-
 // Staged rows into LDS as operands. part: some rows of the tile are hidden from some query rows, or do not exist; then f16
 // values that are not finite are taken out of V, and *s_odd is set.
 template <bool Q8, int WAVES, bool K, bool V>
@@ -87,12 +79,13 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
 #pragma unroll
     for (int j = 0; j < (Q8 ? 2 : 4); j++) {
       if constexpr (Q8) {
-        // 16 codes: dims 64 (2 (f & 1) + j) + 16 g: the two 8-dim operands 2 (g & 1), + 1 of a block
-        auto* dst = &sh.k[8 * (f >> 1) + 2 * (2 * (f & 1) + j) + (g >> 1)][32 * (g & 1) + n];
-        *(h8*)dst[0] = codes8(t.k[j].x, t.k[j].y);
-        *(h8*)dst[16] = codes8(t.k[j].z, t.k[j].w);
+        // 16 codes: dims 16 n .. of row 16 j + (q >> 4): the 8-dim operands 2 (n & 1) and the next of block n >> 1
+        const int b = n >> 1, g0 = 2 * (n & 1), r = q >> 4;
+        *(h8*)sh.k[8 * j + b][16 * g0 + (r ^ ((4 * b + g0) & 15))] = codes8(t.x[j].x, t.x[j].y);
+        *(h8*)sh.k[8 * j + b][16 * g0 + 16 + (r ^ ((4 * b + g0 + 1) & 15))] = codes8(t.x[j].z, t.x[j].w);
       } else {
-        *(u4*)sh.k[8 * (f >> 1) + 4 * (f & 1) + j][l] = t.k[j];
+        const int c = q & 31, r = 8 * j + (q >> 5);  // dims 8 c .. of row r
+        *(u4*)sh.k[8 * (r >> 4) + (c >> 2)][16 * (c & 3) + ((r & 15) ^ (c & 15))] = t.x[j];
       }
     }
   }
@@ -101,7 +94,7 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
       if (f < 2) {  // 4 rows x 16 dims: 4 x 4 codes turned at a time
 #pragma unroll
         for (int d = 0; d < 4; d++) {
-          const uint32_t a = t.v[0][d], b = t.v[1][d], c = t.v[2][d], e = t.v[3][d];
+          const uint32_t a = t.x[t.kV + 0][d], b = t.x[t.kV + 1][d], c = t.x[t.kV + 2][d], e = t.x[t.kV + 3][d];
           const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
           const uint32_t ce0 = __builtin_amdgcn_perm(e, c, 0x05010400u), ce1 = __builtin_amdgcn_perm(e, c, 0x07030602u);
           const uint32_t x[4] = {__builtin_amdgcn_perm(ce0, ab0, 0x05040100u), __builtin_amdgcn_perm(ce0, ab0, 0x07060302u),
@@ -122,8 +115,8 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
         for (int e = 0; e < 4; e++)
 #pragma unroll
           for (int d = 0; d < 4; d++) {
-            uint32_t x = finite_halves(t.v[e][d], odd);
-            t.v[e][d] = 16 * u + 4 * g4 + e < left ? x : 0u;
+            uint32_t x = finite_halves(t.x[t.kV + e][d], odd);
+            t.x[t.kV + e][d] = 16 * u + 4 * g4 + e < left ? x : 0u;
           }
         if (odd) *s_odd = 1;  // a row that does not exist repeats the last one: nothing is lost by marking it
       }
@@ -131,117 +124,108 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
       for (int d = 0; d < 8; d++) {
         const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
         *(u2*)&sh.v[i][16 * g4 + ((8 * half + d) ^ i)][2 * u] =
-            (u2){__builtin_amdgcn_perm(t.v[1][d >> 1], t.v[0][d >> 1], sel), __builtin_amdgcn_perm(t.v[3][d >> 1], t.v[2][d >> 1], sel)};
+            (u2){__builtin_amdgcn_perm(t.x[t.kV + 1][d >> 1], t.x[t.kV + 0][d >> 1], sel), __builtin_amdgcn_perm(t.x[t.kV + 3][d >> 1], t.x[t.kV + 2][d >> 1], sel)};
       }
     }
   }
   if constexpr (Q8) {
     if ((f == 2 && K && carries_v<WAVES>()) || (K && !V && f == 2)) put_scales(t.s, sh.ks);
-    if (f == 3 && V && carries_v<WAVES>()) put_scales(t.s, sh.vs);
+    if (f == 3 && V && carries_v<WAVES>()) put_value_scales(t.s, sh.vs, sh.vf);
   }
 }
 
-// The wave's query rows as operands, from their LDS image.
-struct QRegs {
-  h8 hi[8], lo[8];
-};
-__device__ __forceinline__ void take_queries(QRegs& q, const QTile& im) {
-  const int l = threadIdx.x & 63;
-#pragma unroll
-  for (int b = 0; b < 8; b++) q.hi[b] = *(const h8*)im.v[0][b][l], q.lo[b] = *(const h8*)im.v[1][b][l];
-}
-
-// The operands of a block are requested from LDS before the block before it is worked on, and the four products of a block
-// are issued so that no two neighbours depend on each other: with two waves to a SIMD little else hides either latency.
+// Both products walk the 8 blocks of 32 dims as a pipeline, a step per block: its four matrix instructions (no two
+// neighbours depend on each other), the vector work that feeds the next block's or finishes the one's before, between
+// them, and the LDS reads for the block after the next. A wave has one other beside it on its SIMD at the most, so it
+// has to hide these latencies itself (64 tokens, 65536 q8_0 rows: 329 us with each block done in turn, 305 so, and 300
+// with the weights' products in pairs of halves, see weigh()).
 template <bool Q8>
 __device__ __forceinline__ void scores(const SharedTile& t, const QRegs& q, f4 (&s)[2]) {
-  const int l = threadIdx.x & 63;
+  const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  f4 lo[2] = {zero, zero};
+  f4 lo[2] = {zero, zero}, c[2][2];
   s[0] = s[1] = zero;
   h8 k[2][2];
-  u2 ks[2][2];
+  u2 ks[3][2];
   auto ask = [&](int b) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      k[b & 1][u] = *(const h8*)t.k[8 * u + b][l];
-      if constexpr (Q8) ks[b & 1][u] = scales_of(t.ks, b, u);
+      k[b & 1][u] = *(const h8*)t.k[8 * u + b][16 * g + (n ^ g ^ (4 * b & 12))];
+      if constexpr (Q8) ks[b % 3][u] = scales_of(t.ks, b, u);
+    }
+  };
+  auto scale = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[u][i] = __builtin_fmaf(half_of(ks[b % 3][u][i & 1], i >> 1), c[b & 1][u][i], s[u][i]);
+      asm("" : "+v"(s[u]));  // formed here, as in attn_core.h
     }
   };
   ask(0);
 #pragma unroll
   for (int b = 0; b < 8; b++) {
     if (b < 7) ask(b + 1);
-    __builtin_amdgcn_sched_barrier(0);
     if constexpr (Q8) {
-      f4 c[2];
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[u] = mfma16(k[b & 1][u], q.lo[b], zero);
+      for (int u = 0; u < 2; u++) c[b & 1][u] = mfma16(k[b & 1][u], q.lo[b], zero);
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[u] = mfma16(k[b & 1][u], q.hi[b], c[u]);
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[u][i] = __builtin_fmaf(half_of(ks[b & 1][u][i >> 1], i & 1), c[u][i], s[u][i]);
-        asm("" : "+v"(s[u]));  // formed here, as in attn_core.h
-      }
+      for (int u = 0; u < 2; u++) c[b & 1][u] = mfma16(k[b & 1][u], q.hi[b], c[b & 1][u]);
+      if (b) scale(b - 1);
+      interleave<2>();
     } else {
 #pragma unroll
       for (int u = 0; u < 2; u++) lo[u] = mfma16(k[b & 1][u], q.lo[b], lo[u]);
 #pragma unroll
       for (int u = 0; u < 2; u++) s[u] = mfma16(k[b & 1][u], q.hi[b], s[u]);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
-  if constexpr (!Q8) s[0] += lo[0], s[1] += lo[1];
+  if constexpr (Q8) scale(7);
+  else s[0] += lo[0], s[1] += lo[1];
 }
 
 // PART: some rows of the tile are hidden.
 template <bool Q8, bool PART>
 __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const SharedTile& t) {
   const int l = threadIdx.x & 63, m = l & 15, g = l >> 4;
-  u4 hi, lo;
-  if constexpr (!Q8) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float w0 = p[e >> 1][2 * (e & 1)], w1 = p[e >> 1][2 * (e & 1) + 1];
-      hi[e] = pk_rtz(w0, w1);
-      lo[e] = pk_rtz(minus_half(w0, hi[e], 0), minus_half(w1, hi[e], 1));
-    }
-  }
+  u4 ph, pl, hi[2], lo[2];
   h8 v[2][2];
   u2 vs[2][2];
-  auto ask = [&](int b) {
+  if constexpr (Q8) split8(p, t.vf, st.unit, ph, pl);
+  auto ask_v = [&](int b) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      v[b & 1][h] = *(const h8*)t.v[2 * b + h][16 * g + (m ^ (2 * b + h))];
-      if constexpr (Q8) vs[b & 1][h] = scales_of(t.vs, b, h);
-    }
+    for (int h = 0; h < 2; h++) v[b & 1][h] = *(const h8*)t.v[2 * b + h][16 * g + (m ^ (2 * b + h))];
   };
-  ask(0);
+  auto ask_s = [&](int b) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) vs[b & 1][h] = scales_of(t.vs, b, h);
+  };
+  if constexpr (Q8) {
+    ask_s(0);
+    ask_v(0);
+    ask_s(1);
+    weigh<PART>(ph, pl, vs[0], hi[0], lo[0]);
+  } else {
+    ask_v(0);
+    split(p, hi[0], lo[0]);
+  }
 #pragma unroll
   for (int b = 0; b < 8; b++) {
-    if (b < 7) ask(b + 1);
     __builtin_amdgcn_sched_barrier(0);
+    const int w = Q8 ? b & 1 : 0;
+    if (b < 7) ask_v(b + 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, lo[w]), st.o[2 * b + h]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, hi[w]), st.o[2 * b + h]);
     if constexpr (Q8) {
-      float x[8];  // in the order of codes8: 0, 2, 1, 3, 4, 6, 5, 7
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int e = 4 * u + ((i & 1) << 1 | i >> 1);
-          x[e] = __builtin_fmaf(p[u][i], half_of(vs[b & 1][u][i >> 1], i & 1), 0.0f);
-          if (PART) x[e] = p[u][i] == 0.0f ? 0.0f : x[e];  // a hidden row's scale may be anything
-        }
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        hi[e] = pk_rtz(x[2 * e], x[2 * e + 1]);
-        lo[e] = pk_rtz(minus_half(x[2 * e], hi[e], 0), minus_half(x[2 * e + 1], hi[e], 1));
+      if (b < 7) {
+        weigh<PART>(ph, pl, vs[(b + 1) & 1], hi[w ^ 1], lo[w ^ 1]);
+        if (b < 6) ask_s(b + 2);
+        interleave<3>();
       }
     }
-#pragma unroll
-    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, lo), st.o[2 * b + h]);
-#pragma unroll
-    for (int h = 0; h < 2; h++) st.o[2 * b + h] = mfma16(v[b & 1][h], __builtin_bit_cast(h8, hi), st.o[2 * b + h]);
   }
 }
 

@@ -58,82 +58,162 @@ struct AttnArgs {
   float scale;
 };
 
-// WR * WK waves: WR row tiles of 16 query rows, and for each of them WK waves that share the workgroup's cache rows.
+// LDS of WR * WK waves: WR row tiles of 16 query rows, and for each of them WK waves that share the workgroup's cache rows.
+// f16: the queries' image is taken apart before the first K tile takes its place: first terms to registers, second to `lo`.
+template <bool Q8, int WR, int WK>
+struct AttnShared;
 template <int WR, int WK>
-struct AttnShared {
+struct AttnShared<true, WR, WK> {
   QTile q[WR];
   WaveLds w[WR * WK];
+  float ml[WR * WK][16][2];
+};
+template <int WR, int WK>
+struct AttnShared<false, WR, WK> {
+  union {
+    QTile q[WR];
+    HKeysLds w[WR * WK];
+  };
+  alignas(16) uint32_t lo[WR][8][64][4];
+  float ml[WR * WK][16][2];
 };
 
-// A wave's tile of which some rows are hidden or do not exist.
+// What a wave has of its queries, by the cache's type.
 template <bool Q8>
-__device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const QTile& im, WaveLds& w,
+struct Queries;
+template <>
+struct Queries<true> {
+  const QTile* im;
+};
+template <>
+struct Queries<false> {
+  QHalf r[1];
+};
+
+// A wave's rows at their start; all waves of the workgroup, behind the barrier that ends load_queries.
+template <int WR, int WK>
+__device__ __forceinline__ void begin_rows(Rows& st, Queries<true>& q, AttnShared<true, WR, WK>& sh, int wr, int wk) {
+  rows_init<true>(st, sh.q[wr]);
+  q.im = &sh.q[wr];
+}
+template <int WR, int WK>
+__device__ __forceinline__ void begin_rows(Rows& st, Queries<false>& q, AttnShared<false, WR, WK>& sh, int wr, int wk) {
+  const int l = threadIdx.x & 63;
+  rows_init<false>(st, sh.q[wr]);
+#pragma unroll
+  for (int b = 0; b < 8; b++) q.r[0].hi[b] = *(const h8*)sh.q[wr].v[0][b][l];
+  q.r[0].lo = sh.lo[wr];
+#pragma unroll
+  for (int b = 0; b < 8; b += WK)  // each of the row tile's waves moves its share
+    *(h8*)sh.lo[wr][b + wk][l] = *(const h8*)sh.q[wr].v[1][b + wk][l];
+  __syncthreads();
+}
+
+// A wave's tile of which some rows are hidden or do not exist.
+__device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<true>& q, WaveLds& w,
                                           const Vis& vis, uint64_t tree, int j0) {
-  typename Tiles<Q8>::K k;
-  typename Tiles<Q8>::V v;
+  QRows k, v;
   f4 s[1][2];
   const int left = vis.end - j0;
   const uint64_t trees[1] = {tree};
   load_rows<true>(k, kc, j0, left);
-  if constexpr (Q8) {
-    stage_rows(k, w.codes, w.ks);
-    scores<1>(w, &im, s);
-  } else {
-    scores<1>(k, &im, s);
-  }
-  hide<1>(s, vis, trees, j0);
   load_rows<true>(v, vc, j0, left);
-  if constexpr (Q8) {
-    widen(st, v.s);
-    weights(st, s[0]);
-    stage_rows(v, w.codes, w.vs);
-    accumulate<true>(st, s[0], w);
-    __builtin_amdgcn_wave_barrier();
-  } else {
-    weights(st, s[0]);
-    accumulate_tail(st, s[0], v, vc, j0, left, (float*)w.codes);
-  }
+  stage_keys(k, w);
+  scores<1>(w, q.im, s);
+  hide<1>(s, vis, trees, j0);
+  weights(st, s[0]);
+  __builtin_amdgcn_wave_barrier();
+  stage_values(v, w);
+  widen<true>(st, s[0], w.vf);
+  accumulate<true>(st, s[0], w);
+  __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<false>& q, HKeysLds& w,
+                                          const Vis& vis, uint64_t tree, int j0) {
+  HValues v;
+  f4 s[1][2];
+  const int left = vis.end - j0;
+  const uint64_t trees[1] = {tree};
+  request_keys<true>(w, kc, j0, left);
+  keys_there<0>();
+  scores(w, q.r, s);
+  load_rows<true>(v, vc, j0, left);
+  hide<1>(s, vis, trees, j0);
+  weights(st, s[0]);
+  accumulate_tail(st, s[0], v, vc, j0, left, (float*)w.k);
 }
 
-// The wave's tiles that are wholly visible; next() gives the first cache row of one after the other, then -1. The next
-// tile's K is requested once this one's is in LDS (q8) or its scores are formed, its V once this one's is in LDS or
-// consumed, so that one set of registers each is enough and the loads fly behind the arithmetic.
-template <bool Q8, typename F>
-__device__ __forceinline__ void full_tiles(Rows& st, const KvHead& kc, const KvHead& vc, const QTile& im, WaveLds& w, F next) {
-  int j0 = next();
-  if (j0 < 0) return;
-  typename Tiles<Q8>::K k;
-  typename Tiles<Q8>::V v;
-  load_rows<false>(k, kc, j0, 0);
-  load_rows<false>(v, vc, j0, 0);
-  do {
-    f4 s[1][2];
+// The wave's tiles that are wholly visible: next() gives the first cache row of one after the other, then -1. begin()
+// requests the first one (q8), ahead of the queries' own round trip to memory; run() takes them all.
+// q8: the next tile's K is requested once this one's is in LDS, its V once this one's is, so that one set of registers each
+// is enough and the loads fly behind the arithmetic. f16: K's place in LDS is free once the scores are formed (and only
+// after the queries' image is taken apart), V's registers once it is consumed.
+template <bool Q8>
+struct FullTiles;
+template <>
+struct FullTiles<true> {
+  QRows k, v;
+  int j0;
+  template <typename F>
+  __device__ __forceinline__ void begin(const KvHead& kc, const KvHead& vc, F next) {
     j0 = next();
-    asm volatile("" ::: "memory");  // the queries are read from LDS for each tile: held in registers they would spill
-    if constexpr (Q8) {
-      stage_rows(k, w.codes, w.ks);
+    if (j0 < 0) return;
+    load_rows<false>(k, kc, j0, 0);
+    load_rows<false>(v, vc, j0, 0);
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<true>& q, WaveLds& w, F next) {
+    if (j0 < 0) return;
+    do {
+      f4 s[1][2];
+      j0 = next();
+      asm volatile("" ::: "memory");  // the queries are read from LDS for each tile: held in registers they would spill
+      stage_keys(k, w);
       if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
       loads_issued();
-      scores<1>(w, &im, s);
-      widen(st, v.s);
+      scores<1>(w, q.im, s);
       weights(st, s[0]);
       __builtin_amdgcn_wave_barrier();
-      stage_rows(v, w.codes, w.vs);
+      stage_values(v, w);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
+      widen<false>(st, s[0], w.vf);
       accumulate<false>(st, s[0], w);
       __builtin_amdgcn_wave_barrier();
-    } else {
-      scores<1>(k, &im, s);
-      if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
+    } while (j0 >= 0);
+  }
+};
+template <>
+struct FullTiles<false> {
+  HValues v;
+  int j0;
+  template <typename F>
+  __device__ __forceinline__ void begin(const KvHead& kc, const KvHead& vc, F next) {
+    j0 = next();
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<false>& q, HKeysLds& w, F next) {
+    if (j0 < 0) return;
+    request_keys<false>(w, kc, j0, 0);
+    loads_issued();
+    load_rows<false>(v, vc, j0, 0);
+    do {
+      f4 s[1][2];
+      j0 = next();
+      keys_there<kValueLoads>();
+      scores(w, q.r, s);
+      // V, asked for behind this tile's K, is waited for before the next K is: waited for at its use, it would be with a
+      // count of zero, the next K included (the compiler does not count loads to LDS)
+      keys_there<0>();
+      if (j0 >= 0) request_keys<false>(w, kc, j0, 0);
       loads_issued();
       weights(st, s[0]);
       accumulate(st, s[0], v);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
-    }
-  } while (j0 >= 0);
-}
+    } while (j0 >= 0);
+  }
+};
 
 // Writes a wave's rows: as a split's part, or as the result where there is one split only. gr: the global row (token * nqh
 // + head) of this lane's query row, or -1. BY16: outputs o[i][j] are dims 16 i + 4 g + j; else attn_core.h's f16 order.
@@ -170,11 +250,11 @@ __device__ __forceinline__ void write_rows(Rows& st, const AttnArgs& a, int spli
 
 // Joins the WK waves of each row tile and writes its rows.
 template <bool Q8, int WR, int WK>
-__device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const AttnArgs& a, int split, bool single, int gr) {
+__device__ __forceinline__ void finish(Rows& st, AttnShared<Q8, WR, WK>& sh, const AttnArgs& a, int split, bool single, int gr) {
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63, n = l & 15, g = l >> 4, wr = w % WR, wk = w / WR;
-  float(*ml)[16][2] = (float(*)[16][2])sh.q;       // [wave][row]
-  f4(*ex)[16][64] = (f4(*)[16][64])sh.w;           // outputs of half the waves
-  static_assert(sizeof(sh.w) >= WR * WK / 2 * sizeof(f4) * 16 * 64 && sizeof(sh.q) >= WR * WK * 16 * 8);
+  auto& ml = sh.ml;                       // [wave][row]
+  f4(*ex)[16][64] = (f4(*)[16][64])sh.w;  // outputs of half the waves
+  static_assert(sizeof(sh.w) >= WR * WK / 2 * sizeof(f4) * 16 * 64);
   st.l += lane_xor<16>(st.l);
   st.l += lane_xor32(st.l);
   __syncthreads();  // every wave is done with the queries and its tile
@@ -185,7 +265,7 @@ __device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const A
   for (int k = 0; k < WK; k++) m = __builtin_fmaxf(m, ml[k * WR + wr][n][0]);
 #pragma unroll
   for (int k = 0; k < WK; k++) sum += ml[k * WR + wr][n][1] * __builtin_amdgcn_exp2f(ml[k * WR + wr][n][0] - m);
-  const float f = __builtin_amdgcn_exp2f(st.m - m) * (Q8 ? 512.0f : 1.0f);  // codes8's 2^-9
+  const float f = __builtin_amdgcn_exp2f(st.m - m) * unit_of<Q8>(st);
 #pragma unroll
   for (int i = 0; i < 16; i++) st.o[i] *= f;
 #pragma unroll
@@ -206,7 +286,7 @@ __device__ __forceinline__ void finish(Rows& st, AttnShared<WR, WK>& sh, const A
 
 template <bool Q8, int WR, int WK>
 __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) {
-  __shared__ AttnShared<WR, WK> sh;
+  __shared__ AttnShared<Q8, WR, WK> sh;
   // workgroups 8 apart run on one XCD: those of one (kv head, split) follow each other there
   const int unit = (int)(blockIdx.x / (8 * a.groups)) * 8 + (int)(blockIdx.x & 7), rg = (int)(blockIdx.x >> 3) % a.groups;
   if (unit >= a.nkvh * a.splits) return;
@@ -221,6 +301,17 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) 
     r += rg * WR * 16;
     return r < rows ? (r / group) * a.nqh + kh * group + r % group : -1;
   };
+  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
+  const int t1 = split * sp.per + sp.per < tiles ? split * sp.per + sp.per : tiles;
+  const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
+  int t = split * sp.per + wk;
+  auto next = [&] {
+    if (t >= full) return -1;
+    t += WK;
+    return (t - WK) * kTileKeys;
+  };
+  FullTiles<Q8> ft;
+  ft.begin(kc, vc, next);
   load_queries<Q8, WR * WK, WR>(sh.q, a.scale * kLog2e, [&](int r) {
     const int gr = row(r);
     return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
@@ -228,20 +319,11 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) 
   const int mine = wr * 16 + (threadIdx.x & 15);
   const uint64_t tree = row(mine) >= 0 ? tree_of(a.tree, (rg * WR * 16 + mine) / group, a.T) : 0ull;
   __syncthreads();
-  const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
   Rows st;
-  rows_init<Q8>(st, sh.q[wr]);
-  if ((rg * WR + wr) * 16 < rows) {  // the last group's row tiles may be fewer
-    const int t1 = split * sp.per + sp.per < tiles ? split * sp.per + sp.per : tiles;
-    const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
-    int t = split * sp.per + wk;
-    full_tiles<Q8>(st, kc, vc, sh.q[wr], sh.w[w], [&] {
-      if (t >= full) return -1;
-      t += WK;
-      return (t - WK) * kTileKeys;
-    });
-    for (; t < t1; t += WK) tail_tile<Q8>(st, kc, vc, sh.q[wr], sh.w[w], vis, tree, t * kTileKeys);
-  }
+  Queries<Q8> q;
+  begin_rows(st, q, sh, wr, wk);
+  ft.run(st, kc, vc, q, sh.w[w], next);
+  for (; t < t1; t += WK) tail_tile(st, kc, vc, q, sh.w[w], vis, tree, t * kTileKeys);
   finish<Q8, WR, WK>(st, sh, a, split, sp.used == 1, row(mine));
 }
 
@@ -272,8 +354,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
   const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
   auto left_of = [&](int t) { return vis.end - t * kTileKeys < kTileKeys ? vis.end - t * kTileKeys : kTileKeys; };
   auto part_of = [&](int t) { return (t + 1) * kTileKeys > vis.n; };
-  Staged<Q8, WAVES> next;
-  if (t0 < t1) request<Q8, WAVES, true, true>(next, kc, vc, t0 * kTileKeys, left_of(t0));
+  auto ask = [&](Staged<Q8, WAVES>& n, int t) {
+    if (t < t1) request<Q8, WAVES, true, true>(n, kc, vc, t * kTileKeys, left_of(t));
+  };
+  // tiles on their way beside the one in LDS: 8 waves of f16 two (64 tokens, 65536 rows: 221 -> 215 us); q8's arithmetic
+  // takes longer than a load, and 4 waves carry twice as much each, whose registers spill: one
+  constexpr int kAhead = WAVES == 8 && !Q8 ? 2 : 1;
+  Staged<Q8, WAVES> even, two;
+  Staged<Q8, WAVES>& odd = kAhead == 2 ? two : even;
+  ask(even, t0);
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
     const int gr = row(r);
@@ -288,41 +377,51 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
   const uint64_t tree[1] = {gr >= 0 ? tree_of(a.tree, (first + mine) / group, a.T) : 0ull};
   const bool active = w < a.tiles && first + w * 16 < rows;
   __syncthreads();
-  if (t0 < t1) stage<Q8, WAVES, true, true>(next, buf[0], part_of(t0), left_of(t0), &s_odd[0]);
-  if (t0 + 1 < t1) request<Q8, WAVES, true, true>(next, kc, vc, (t0 + 1) * kTileKeys, left_of(t0 + 1));
+  if (t0 < t1) stage<Q8, WAVES, true, true>(even, buf[0], part_of(t0), left_of(t0), &s_odd[0]);
+  ask(even, t0 + 1);
+  if (kAhead == 2) ask(odd, t0 + 2);
   __syncthreads();
-  // two loops: a tile with hidden rows takes another form of the product, and with both in one loop the outputs' registers
-  // are copied between them (and spill)
+  // `next` holds tile t + 1 and is given the one kAhead behind it. Two loops: a tile with hidden rows takes another form of the product,
+  // and with both in one loop the outputs' registers are copied between them (and spill); the first takes an even number
+  // of tiles, so that either begins with `even`.
   int t = t0;
-  auto walk = [&](auto hidden, int end) {
+  auto step = [&](auto hidden, int at, Staged<Q8, WAVES>& next) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(hidden)::value;
-    for (; t < end; t++) {
-      const int at = (t - t0) & 1;
-      if (active) {
-        f4 s[1][2];
-        scores<Q8>(buf[at], q, s[0]);
-        if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
-        if constexpr (Q8) widen(st, *(const u2*)(buf[at].vs + 8 * (threadIdx.x & 63)));
-        weights(st, s[0]);
-        accumulate<Q8, kPart>(st, s[0], buf[at]);
-        if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
+    if (active) {
+      f4 s[1][2];
+      scores<Q8>(buf[at], q, s[0]);
+      if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
+      weights(st, s[0]);
+      if constexpr (Q8) widen<kPart>(st, s[0], buf[at].vf);
+      accumulate<Q8, kPart>(st, s[0], buf[at]);
+      if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
+    }
+    if (t + 1 < t1) stage<Q8, WAVES, true, true>(next, buf[at ^ 1], part_of(t + 1), left_of(t + 1), &s_odd[at ^ 1]);
+    ask(next, t + 1 + kAhead);
+    __syncthreads();
+    t++;
+  };
+  auto walk = [&](auto hidden, int end) __attribute__((always_inline)) {
+    if constexpr (kAhead == 1) {
+      while (t < end) step(hidden, (t - t0) & 1, even);
+    } else {
+      while (t + 1 < end) {
+        step(hidden, 0, even);
+        step(hidden, 1, odd);
       }
-      if (t + 1 < t1) {
-        stage<Q8, WAVES, true, true>(next, buf[at ^ 1], part_of(t + 1), left_of(t + 1), &s_odd[at ^ 1]);
-        if (t + 2 < t1) request<Q8, WAVES, true, true>(next, kc, vc, (t + 2) * kTileKeys, left_of(t + 2));
-      }
-      __syncthreads();
+      if (t < end) step(hidden, 0, even);
     }
   };
-  const int full = vis.n / kTileKeys;
-  walk(std::false_type(), full < t1 ? full : t1);
+  const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
+  if (full > t0) walk(std::false_type(), t0 + (full - t0) / 2 * 2);
   walk(std::true_type(), t1);
   if (!active) return;
   st.l += lane_xor<16>(st.l);
   st.l += lane_xor32(st.l);
   if constexpr (Q8) {
+    const float f = unit_of<Q8>(st);
 #pragma unroll
-    for (int i = 0; i < 16; i++) st.o[i] *= 512.0f;  // codes8's 2^-9
+    for (int i = 0; i < 16; i++) st.o[i] *= f;
   }
   write_rows<true>(st, a, split, sp.used == 1, gr, st.m, st.l);
 }
@@ -330,21 +429,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
 // attn_blocks: one workgroup per (token, kv head, split of its list); the group's query heads are one row tile.
 template <bool Q8>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a) {
-  __shared__ AttnShared<1, kWaves> sh;
+  __shared__ AttnShared<Q8, 1, kWaves> sh;
   const int unit = (int)(blockIdx.x / a.splits), split = (int)(blockIdx.x % a.splits);
   const int kh = unit % a.nkvh, t = unit / a.nkvh;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Vis vis = vis_of((long long)*a.pos0 + t + 1, 0, a.n_ctx);
   const int group = a.nqh / a.nkvh;
   auto row = [&](int r) { return r < group ? t * a.nqh + kh * group + r : -1; };
-  load_queries<Q8, kWaves, 1>(sh.q, a.scale * kLog2e, [&](int r) {
-    const int gr = row(r);
-    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
-  });
-  __syncthreads();
   const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx), vc = kv_head<Q8>(a.vcache, kh, a.nkvh, a.n_ctx);
-  Rows st;
-  rows_init<Q8>(st, sh.q[0]);
   const int per = (2 * a.nsel + a.splits - 1) / a.splits;
   const int t1 = split * per + per < 2 * a.nsel ? split * per + per : 2 * a.nsel;
   const int* list = a.idx + ((size_t)t * a.nkvh + kh) * a.nsel;
@@ -352,12 +444,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a)
   // where a whole one is asked for (and the other way round)
   const int nb = (vis.n + kBlockRows - 1) / kBlockRows;
   auto tile = [&](int i, bool part) {
-    const int b = __builtin_amdgcn_readfirstlane(list[i >> 1]);
+    // a scalar load: a vector load's wait would be for the tiles on their way as well
+    const int b = *(const __attribute__((address_space(4))) int*)(list + (i >> 1));
     const int j0 = b * kBlockRows + (i & 1) * kTileKeys;
     return b >= 0 && b < nb && j0 < vis.n && (j0 + kTileKeys > vis.n) == part ? j0 : -1;
   };
   int i = split * per + w;
-  full_tiles<Q8>(st, kc, vc, sh.q[0], sh.w[w], [&] {
+  auto next = [&] {
     for (; i < t1; i += kWaves) {
       const int j0 = tile(i, false);
       if (j0 >= 0) {
@@ -366,10 +459,21 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a)
       }
     }
     return -1;
+  };
+  FullTiles<Q8> ft;
+  ft.begin(kc, vc, next);
+  load_queries<Q8, kWaves, 1>(sh.q, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
   });
+  __syncthreads();
+  Rows st;
+  Queries<Q8> q;
+  begin_rows(st, q, sh, 0, w);
+  ft.run(st, kc, vc, q, sh.w[w], next);
   for (i = split * per + w; i < t1; i += kWaves) {
     const int j0 = tile(i, true);
-    if (j0 >= 0) tail_tile<Q8>(st, kc, vc, sh.q[0], sh.w[w], vis, 0ull, j0);
+    if (j0 >= 0) tail_tile(st, kc, vc, q, sh.w[w], vis, 0ull, j0);
   }
   finish<Q8, 1, kWaves>(st, sh, a, split, a.splits == 1, row(threadIdx.x & 15));
 }
@@ -377,10 +481,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a)
 // Joins the splits of one query row: a workgroup takes 64 of the 256 dims (16 lanes of 4), its 16 groups of lanes every
 // 16th split, all requested at once; then the groups' sums are added in order. FIXED: every split was written; else those
 // that split_of used, and nothing is left to do where that is one. (128 splits of 24 rows: 38 us with a thread per dim
-// that walks the splits, 4.6 us so.)
+// that walks the splits, 4.7 us so.)
 constexpr int kMaxSplits = 2 * kCUs;
 template <bool FIXED>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, 8) attn_join_kernel(AttnArgs a) {
   __shared__ float s_f[kMaxSplits], s_red[8];
   __shared__ f4 s_o[16][16];
   const int gr = blockIdx.x, tid = threadIdx.x, c = tid & 15, sg = tid >> 4, w = tid >> 6;
@@ -450,6 +554,25 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
+// Sums of eight values over the 16 query rows (lanes n) of a lane group: lanes n and n ^ 8 leave with value n & 7 in x[0].
+// At each exchange a lane hands over the half of its values that the other keeps, so 4 + 2 + 1 + 1 exchanges, not 32.
+__device__ __forceinline__ void sum_rows(float (&x)[8]) {
+  const int n = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float keep = n & 4 ? x[i + 4] : x[i], give = n & 4 ? x[i] : x[i + 4];
+    x[i] = keep + __shfl_xor(give, 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const float keep = n & 2 ? x[i + 2] : x[i], give = n & 2 ? x[i] : x[i + 2];
+    x[i] = keep + lane_xor<2>(give);
+  }
+  const float keep = n & 1 ? x[1] : x[0], give = n & 1 ? x[0] : x[1];
+  x[0] = keep + lane_xor<1>(give);
+  x[0] += lane_xor<8>(x[0]);
+}
+
 struct WeightArgs {
   const float *qn, *lse;
   const void* kcache;
@@ -465,9 +588,13 @@ struct WeightArgs {
 // taken in order, and a row of the cache belongs to one wave: the same bits always.
 template <bool Q8, int RT>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs a) {
-  __shared__ QTile im[RT];
+  __shared__ union {
+    QTile im[RT];
+    HKeysLds w[Q8 ? 1 : kWaves];  // f16: the queries move to registers before the first K tile takes their place
+  } sh;
   __shared__ float s_lse[RT * 16];
   __shared__ WaveLds s_w[Q8 ? kWaves : 1];
+  QTile(&im)[RT] = sh.im;
   const int kh = blockIdx.x % a.nkvh, split = blockIdx.x / a.nkvh;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
@@ -500,23 +627,35 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs
       c[rt] = im[rt].c[n];
       lse[rt] = s_lse[rt * 16 + n];
     }
+    QRegs q[RT];
+    if constexpr (!Q8) {
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) take_queries(q[rt], im[rt]);
+      __syncthreads();
+    }
     for (int t = split * sp.per + w; t < t1; t += kWaves) {
       const int j0 = t * kTileKeys;
       const bool full = j0 + kTileKeys <= vis.n;
-      typename Tiles<Q8>::K k;
+      QRows k;
       f4 s[RT][2];
-      if (full) load_rows<false>(k, kc, j0, 0);
-      else load_rows<true>(k, kc, j0, vis.end - j0);
+      if constexpr (Q8) {
+        if (full) load_rows<false>(k, kc, j0, 0);
+        else load_rows<true>(k, kc, j0, vis.end - j0);
+      } else {
+        if (full) request_keys<false>(sh.w[w], kc, j0, 0);
+        else request_keys<true>(sh.w[w], kc, j0, vis.end - j0);
+      }
       const int j = j0 + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);  // the row this lane stores (n < 8)
       const bool mine = n < 8 && j < vis.end;
       const float old = mine && (j < vis.n || rg) ? acc[j] : 0.0f;  // the weights of a drafted row begin here
       asm volatile("" ::: "memory");
       if constexpr (Q8) {
         __builtin_amdgcn_wave_barrier();
-        stage_rows(k, s_w[w].codes, s_w[w].ks);
+        stage_keys(k, s_w[w]);
         scores<RT>(s_w[w], im, s);
       } else {
-        scores<RT>(k, im, s);
+        keys_there<0>();
+        scores(sh.w[w], q, s);
       }
       if (!full) hide<RT>(s, vis, tree, j0);
       float sum[8];
@@ -530,15 +669,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs
           // rows not asked for, and hidden cache rows (of a query row that sees none lse is -inf too)
           sum[e] += lse[rt] == __builtin_huge_valf() || x == -__builtin_huge_valf() ? 0.0f : p;
         }
-        sum[e] += lane_xor<1>(sum[e]);
-        sum[e] += lane_xor<2>(sum[e]);
-        sum[e] += lane_xor<7>(sum[e]);
-        sum[e] += lane_xor<8>(sum[e]);
       }
-      float v = sum[0];
-#pragma unroll
-      for (int e = 1; e < 8; e++) v = n == e ? sum[e] : v;
-      if (mine) acc[j] = old + v;
+      sum_rows(sum);
+      if (mine) acc[j] = old + sum[0];
     }
   }
 }
@@ -567,8 +700,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
   auto left_of = [&](int t) { return vis.end - t * kTileKeys < kTileKeys ? vis.end - t * kTileKeys : kTileKeys; };
   for (int rg = 0; rg < a.groups; rg++) {
     const int first = rg * a.tiles * 16;
-    Staged<Q8, WAVES> next;
-    request<Q8, WAVES, true, false>(next, kc, kc, t0 * kTileKeys, left_of(t0));
+    auto ask = [&](Staged<Q8, WAVES>& n, int t) {
+      if (t < t1) request<Q8, WAVES, true, false>(n, kc, kc, t * kTileKeys, left_of(t));
+    };
+    Staged<Q8, WAVES> even, odd;
+    ask(even, t0);
     load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
       const int q = first + r;
       return r < a.tiles * 16 && q < rows ? a.qn + ((size_t)(q / group) * a.nqh + kh * group + q % group) * kHD : nullptr;
@@ -583,48 +719,49 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
     const uint64_t tree[1] = {mine ? tree_of(a.tree, r / group, a.T) : 0ull};
     const bool active = __any(on);  // a row tile of which no row is asked for adds nothing
     __syncthreads();
-    stage<Q8, WAVES, true, false>(next, buf[0], false, 0, nullptr);
-    if (t0 + 1 < t1) request<Q8, WAVES, true, false>(next, kc, kc, (t0 + 1) * kTileKeys, left_of(t0 + 1));
+    stage<Q8, WAVES, true, false>(even, buf[0], false, 0, nullptr);
+    ask(even, t0 + 1);
+    ask(odd, t0 + 2);
     __syncthreads();
-    float old = 0.0f, old1 = 0.0f;
-    for (int t = t0; t <= t1; t++) {
-      // threads 0 .. 31: a row's weight before this tile's sums, and the sums of the tile before
+    float old = 0.0f;
+    // threads 0 .. 31, behind the barrier of the tile before: its sums are added to its rows' weights
+    auto add_up = [&](int t, int at) {
       const int j = t * kTileKeys + threadIdx.x;
-      old = old1;
-      if (threadIdx.x < kTileKeys && t < t1 && j < vis.end) old1 = j < vis.n || rg ? acc[j] : 0.0f;
-      if (t > t0 && threadIdx.x < kTileKeys && j - kTileKeys < vis.end) {
-        float v = 0.0f;
+      if (t < t0 || threadIdx.x >= kTileKeys || j >= vis.end) return;
+      float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < WAVES; k++) v += s_sum[(t - 1 - t0) & 1][k][threadIdx.x];
-        acc[j - kTileKeys] = old + v;
-      }
-      if (t == t1) break;
+      for (int k = 0; k < WAVES; k++) v += s_sum[at][k][threadIdx.x];
+      acc[j] = old + v;
+    };
+    auto step = [&](int t, int at, Staged<Q8, WAVES>& next) __attribute__((always_inline)) {
+      add_up(t - 1, at ^ 1);
+      const int j = t * kTileKeys + threadIdx.x;
+      if (threadIdx.x < kTileKeys && j < vis.end) old = j < vis.n || rg ? acc[j] : 0.0f;  // the weights of new rows begin here
       float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
       if (active) {
         f4 s[1][2];
-        scores<Q8>(buf[(t - t0) & 1], q, s[0]);
+        scores<Q8>(buf[at], q, s[0]);
         if ((t + 1) * kTileKeys > vis.n) hide<1>(s, vis, tree, t * kTileKeys);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const float x = s[0][e >> 2][e & 3];
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse));
           sum[e] = !on || x == -__builtin_huge_valf() ? 0.0f : p;
-          sum[e] += lane_xor<1>(sum[e]);
-          sum[e] += lane_xor<2>(sum[e]);
-          sum[e] += lane_xor<7>(sum[e]);
-          sum[e] += lane_xor<8>(sum[e]);
         }
+        sum_rows(sum);
       }
-      float v = sum[0];
-#pragma unroll
-      for (int e = 1; e < 8; e++) v = n == e ? sum[e] : v;
-      if (n < 8) s_sum[(t - t0) & 1][w][16 * (n >> 2) + 4 * g + (n & 3)] = v;
-      if (t + 1 < t1) {
-        stage<Q8, WAVES, true, false>(next, buf[(t - t0 + 1) & 1], false, 0, nullptr);
-        if (t + 2 < t1) request<Q8, WAVES, true, false>(next, kc, kc, (t + 2) * kTileKeys, left_of(t + 2));
-      }
+      if (n < 8) s_sum[at][w][16 * (n >> 2) + 4 * g + (n & 3)] = sum[0];
+      if (t + 1 < t1) stage<Q8, WAVES, true, false>(next, buf[at ^ 1], false, 0, nullptr);
+      ask(next, t + 3);
       __syncthreads();
+    };
+    int t = t0;
+    for (; t + 1 < t1; t += 2) {
+      step(t, 0, even);
+      step(t + 1, 1, odd);
     }
+    if (t < t1) step(t++, 0, even);
+    add_up(t1 - 1, (t1 - 1 - t0) & 1);
     __syncthreads();  // the sums are read, the buffers free for the next group's queries
   }
 }

@@ -5,8 +5,10 @@
 // order. The weights' exact order is found by three histograms (11, 11 and 10 bits of the integer key, counted with
 // integer atomics, so in any order to the same result) over workgroups that each hold a segment of the rows; then each
 // segment counts its rows above and at the threshold and writes its own part of the list behind the segments before it.
-// Rows are moved by 16 bytes a lane. In place they pass through the workspace, since a row's place may be another row's
-// source.
+// Up to 32768 rows of context one workgroup a kv head does all of that over keys in LDS (20001 rows: 7 launches, 29 us;
+// two, 24 us, 16 of them the choice). Rows are moved by 16 bytes a lane. In place, the kept rows that lie before row
+// `keep` go through the workspace, since a row's place may be another one's source there; the others are read where no
+// row is written.
 #include "pick.h"
 #include "q27h_device.h"
 #include "q27h_internal.h"
@@ -32,9 +34,11 @@ struct EvictArgs {
   void *ko, *vo;
   float* acc_o;
   int* kept;
+  uint8_t *k_aside, *v_aside;  // in place: workspace of `keep` rows
+  float* acc_aside;
   int* hist;    // [nkvh][3][kBins]
   int2* count;  // [nkvh][segs]: rows above, rows at the threshold
-  int keep, first, last, n_out, nkvh, n_ctx, q8, segs, in_place;
+  int keep, first, last, n_out, nkvh, n_ctx, q8, segs;
 };
 
 __device__ __forceinline__ int rows_of(const EvictArgs& a) {
@@ -131,9 +135,106 @@ __global__ void __launch_bounds__(256) evict_count_kernel(EvictArgs a) {
   if (threadIdx.x == 0) a.count[kh * a.segs + blockIdx.x] = make_int2(above, equal);
 }
 
+// The whole choice of a kv head by one workgroup, for contexts of up to kLdsRows: keys in LDS, digits of key - (least key)
+// from the top (see select_pick_kernel in attn_select.hip), until a bin is kept whole; then each thread lists a stretch
+// of consecutive rows, an odd number of them, so that the lanes' reads fall in different banks.
+constexpr int kLdsRows = 32768, kListThreads = 1024;
+__global__ void __launch_bounds__(kListThreads) evict_choose_kernel(EvictArgs a) {
+  __shared__ uint32_t s_key[kLdsRows];
+  __shared__ int s_hist[kBins], s_scan[kListThreads / 64], s_pick[3];
+  __shared__ uint32_t s_end[2 * kListThreads / 64];
+  const int kh = blockIdx.x, tid = threadIdx.x, w = tid >> 6, n = rows_of(a);
+  int* out = a.kept + (size_t)kh * a.keep;
+  if (n <= a.keep) {
+    for (int i = tid; i < a.keep; i += kListThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int r0 = a.first, rows = n - a.last - r0;
+  const float* acc = a.acc + (size_t)kh * a.n_ctx + r0;
+  uint32_t least = ~0u, most = 0u;
+  for (int r = tid; r < rows; r += 16 * kListThreads) {
+    float x[16];  // requested together
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (r + i * kListThreads < rows) x[i] = acc[r + i * kListThreads];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      if (r + i * kListThreads >= rows) break;
+      const uint32_t k = order_key(x[i]);
+      s_key[r + i * kListThreads] = k;
+      least = least < k ? least : k;
+      most = most > k ? most : k;
+    }
+  }
+  for (int i = tid; i < a.first; i += kListThreads) out[i] = i;
+  for (int i = tid; i < a.last; i += kListThreads) out[a.keep - a.last + i] = n - a.last + i;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t x = __shfl_xor(least, d), y = __shfl_xor(most, d);
+    least = least < x ? least : x;
+    most = most > y ? most : y;
+  }
+  if ((tid & 63) == 0) s_end[2 * w] = least, s_end[2 * w + 1] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kListThreads / 64; i++) {
+    const uint32_t x = s_end[2 * i], y = s_end[2 * i + 1];
+    least = least < x ? least : x;
+    most = most > y ? most : y;
+  }
+  int need = a.keep - a.first - a.last, shift = need && least < most ? 32 - __builtin_clz(most - least) : 0;
+  uint32_t prefix = need ? 0u : ~0u;
+  auto upper = [](uint32_t k, int by) { return (uint32_t)((uint64_t)k >> by); };
+  while (shift > 0) {
+    const int next = shift > 11 ? shift - 11 : 0;
+    s_hist[tid] = s_hist[tid + 1024] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int r = tid; r < rows; r += kListThreads) {
+      const uint32_t k = s_key[r] - least;
+      if (upper(k, shift) == upper(prefix, shift)) atomicAdd(&s_hist[(k >> next) & ((1u << (shift - next)) - 1u)], 1);
+    }
+    __syncthreads();
+    const int hi = s_hist[kBins - 1 - 2 * tid], lo = s_hist[kBins - 2 - 2 * tid];
+    int total;
+    int above = scan_waves<kListThreads / 64>(hi + lo, s_scan, total);
+    if (above < need && need <= above + hi) s_pick[0] = kBins - 1 - 2 * tid, s_pick[1] = need - above, s_pick[2] = hi;
+    above += hi;
+    if (above < need && need <= above + lo) s_pick[0] = kBins - 2 - 2 * tid, s_pick[1] = need - above, s_pick[2] = lo;
+    __syncthreads();
+    prefix |= (uint32_t)s_pick[0] << next;
+    need = s_pick[1];
+    shift = next;
+    if (need == s_pick[2]) break;
+    __syncthreads();
+  }
+  __syncthreads();
+  const int per = (rows + kListThreads - 1) / kListThreads | 1, c0 = tid * per < rows ? tid * per : rows;
+  const int c1 = c0 + per < rows ? c0 + per : rows;
+  const uint32_t p = upper(prefix, shift);
+  int above = 0, equal = 0;
+#pragma unroll 8
+  for (int r = c0; r < c1; r++) {
+    const uint32_t k = upper(s_key[r] - least, shift);
+    above += k > p;
+    equal += k == p;
+  }
+  int total;
+  int at = scan_waves<kListThreads / 64>(above, s_scan, total), rank = scan_waves<kListThreads / 64>(equal, s_scan, total);
+  at += a.first + (rank < need ? rank : need);
+#pragma unroll 4
+  for (int r = c0; r < c1; r++) {
+    const uint32_t k = upper(s_key[r] - least, shift);
+    const bool take = k > p || (k == p && rank < need);
+    rank += k == p;
+    if (take) out[at++] = r0 + r;
+  }
+}
+
 // The list of kept rows: a segment's part starts behind the rows kept by the segments before it.
 __global__ void __launch_bounds__(256) evict_list_kernel(EvictArgs a) {
   __shared__ int s_scan[4], s_pick[2];
+  __shared__ uint32_t s_key[8 * 256];
   const int kh = blockIdx.y, n = rows_of(a), seg = blockIdx.x;
   int* out = a.kept + (size_t)kh * a.keep;
   if (n <= a.keep) {
@@ -156,39 +257,75 @@ __global__ void __launch_bounds__(256) evict_list_kernel(EvictArgs a) {
   equal = t1;
   int done = a.first + t0 + (equal < need ? equal : need);
   const float* acc = a.acc + (size_t)kh * a.n_ctx;
-  for (int base = b; base < e; base += 256) {
-    const int r = base + threadIdx.x;
-    const uint32_t k = r < e ? order_key(acc[r]) : 0u;
-    const bool eq = r < e && k == key;
-    int total_eq, total;
-    const int rank = equal + scan256(eq, s_scan, total_eq);
-    const bool take = (r < e && k > key) || (eq && rank < need);
-    const int at = done + scan256(take, s_scan, total);
-    if (take) out[at] = r;
-    done += total;
-    equal += total_eq;
+  // 2048 rows at a time: each thread counts and lists 8 consecutive ones
+  for (int base = b; base < e; base += 8 * 256) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int r = base + 256 * i + threadIdx.x;
+      s_key[256 * i + threadIdx.x] = r < e ? order_key(acc[r]) : 0u;
+    }
+    __syncthreads();
+    uint32_t k[8];
+    int n_above = 0, n_equal = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const bool is = base + 8 * (int)threadIdx.x + i < e;
+      k[i] = s_key[8 * threadIdx.x + i];
+      n_above += is && k[i] > key;
+      n_equal += is && k[i] == key;
+    }
+    int total_above, total_equal;
+    int at = scan256(n_above, s_scan, total_above), rank = scan256(n_equal, s_scan, total_equal);
+    const int start = equal < need ? equal : need;  // equal rows taken before this stretch of 2048
+    rank += equal;
+    at += done + (rank < need ? rank : need) - start;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int r = base + 8 * (int)threadIdx.x + i;
+      const bool take = r < e && (k[i] > key || (k[i] == key && rank < need));
+      rank += r < e && k[i] == key;
+      if (take) out[at++] = r;
+    }
+    equal += total_equal;
+    done += total_above + (equal < need ? equal : need) - start;
   }
 }
 
-// Rows of one cache: `lanes` 16-byte pieces a row (16 or 32) at `stride`, then for q8 the row's 16 bytes of scales.
-// MODE 0: kept rows to their places in another cache (or the workspace); 1: rows 0 .. keep - 1 of the workspace back.
+// Rows of K and V (blockIdx.z), 16 or 32 lanes of 16 bytes a row, then for q8 the row's 16 bytes of scales; the weights
+// with K. OUT: kept rows to their places in other buffers. In place: ASIDE: those of rows before `keep` that have to move,
+// to the workspace; BACK: those to their places, and the others from where they lie.
+enum { OUT, ASIDE, BACK };
 template <int MODE>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
-  const int kh = blockIdx.y, n = MODE == 0 ? rows_of(a) : *a.pos0, m = n < a.keep ? n : a.keep;
-  if (a.in_place && n <= a.keep) return;  // nothing evicted: every row is where it belongs
+  const int kh = blockIdx.y, n = rows_of(a), m = n < a.keep ? n : a.keep;
+  if (MODE != OUT && n <= a.keep) return;  // nothing evicted: every row is where it belongs
   const bool v = blockIdx.z;
-  const uint8_t* src = (const uint8_t*)(v ? a.vc : a.kc);
-  uint8_t* dst = (uint8_t*)(v ? a.vo : a.ko);
+  const uint8_t* cache = (const uint8_t*)(v ? a.vc : a.kc);
+  uint8_t* aside = (uint8_t*)(v ? a.v_aside : a.k_aside);
+  uint8_t* out = (uint8_t*)(v ? a.vo : a.ko);
   const int lanes = a.q8 ? 16 : 32, sub = threadIdx.x % lanes, rows = 256 / lanes;
   const size_t stride = (size_t)lanes * 16;
-  const uint8_t* ss = src + (size_t)a.nkvh * a.n_ctx * kHD;
-  uint8_t* ds = dst + (size_t)a.nkvh * a.n_out * kHD;
+  // where row r of kv head kh lies in a buffer of so many rows, and its scales
+  auto row = [&](auto* base, int n_rows, int r) { return base + ((size_t)kh * n_rows + r) * stride + sub * 16; };
+  auto scale = [&](auto* base, int n_rows, int r) {
+    return base + (size_t)a.nkvh * n_rows * kHD + ((size_t)kh * n_rows + r) * 16;
+  };
+  const int out_rows = MODE == ASIDE ? a.keep : a.n_out;
+  uint8_t* to = MODE == ASIDE ? aside : out;
+  float* acc_to = MODE == ASIDE ? a.acc_aside : a.acc_o;
+#pragma unroll 4
   for (int i = blockIdx.x * rows + threadIdx.x / lanes; i < m; i += gridDim.x * rows) {
-    const int r = MODE == 0 ? a.kept[(size_t)kh * a.keep + i] : i;
-    const size_t from = (size_t)kh * a.n_ctx + r, to = (size_t)kh * a.n_out + i;
-    *(u4*)(dst + to * stride + sub * 16) = *(const u4*)(src + from * stride + sub * 16);
-    if (a.q8 && sub == 0) *(u4*)(ds + to * 16) = *(const u4*)(ss + from * 16);
-    if (!v && sub == 1) a.acc_o[to] = a.acc[from];
+    const int r = a.kept[(size_t)kh * a.keep + i];
+    const bool near = MODE != OUT && r < a.keep;
+    if (MODE != OUT && (r == i || (MODE == ASIDE && !near))) continue;
+    const bool ws = MODE == BACK && near;
+    const uint8_t* from = ws ? aside : cache;
+    const int from_rows = ws ? a.keep : a.n_ctx, fr = ws ? i : r;
+    *(u4*)row(to, out_rows, i) = *(const u4*)row(from, from_rows, fr);
+    if (a.q8 && sub == 0) *(u4*)scale(to, out_rows, i) = *(const u4*)scale(from, from_rows, fr);
+    if (!v && sub == 1)
+      acc_to[(size_t)kh * out_rows + i] = ws ? a.acc_aside[(size_t)kh * a.keep + i] : a.acc[(size_t)kh * a.n_ctx + r];
   }
 }
 
@@ -299,33 +436,34 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
     return r;
   };
   a.kc = kcache, a.vc = vcache, a.acc = acc, a.pos0 = pos0;
-  a.keep = keep, a.first = first, a.last = last, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8, a.segs = segs_of(n_ctx), a.in_place = in_place;
+  a.keep = keep, a.first = first, a.last = last, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8, a.segs = segs_of(n_ctx);
   a.hist = (int*)take((size_t)nkvh * 3 * kBins * 4);
   a.count = (int2*)take((size_t)nkvh * a.segs * 8);
   int* list = (int*)take((size_t)nkvh * keep * 4);
   a.kept = kept ? kept : list;
   const dim3 grid((unsigned)a.segs, (unsigned)nkvh), block(256);
   hipStream_t st = stream_of(s);
-  hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)(nkvh * 3 * kBins / 1024)), block, 0, st, a.hist);
-  for (int pass = 0; pass < 3; pass++) hipLaunchKernelGGL(evict_hist_kernel, grid, block, 0, st, a, pass);
-  hipLaunchKernelGGL(evict_count_kernel, grid, block, 0, st, a);
-  hipLaunchKernelGGL(evict_list_kernel, grid, block, 0, st, a);
+  if (n_ctx <= kLdsRows) {
+    hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)nkvh), dim3(kListThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)(nkvh * 3 * kBins / 1024)), block, 0, st, a.hist);
+    for (int pass = 0; pass < 3; pass++) hipLaunchKernelGGL(evict_hist_kernel, grid, block, 0, st, a, pass);
+    hipLaunchKernelGGL(evict_count_kernel, grid, block, 0, st, a);
+    hipLaunchKernelGGL(evict_list_kernel, grid, block, 0, st, a);
+  }
   const int rows = q8 ? 16 : 8;
   int chunks = (keep + rows - 1) / rows;
   const int most = 16 * kCUs / (2 * nkvh) < 1 ? 1 : 16 * kCUs / (2 * nkvh);
   chunks = chunks > most ? most : chunks;
   const dim3 mgrid((unsigned)chunks, (unsigned)nkvh, 2);
+  a.ko = kout, a.vo = vout, a.acc_o = acc_out, a.n_out = n_ctx_out;
   if (!in_place) {
-    a.ko = kout, a.vo = vout, a.acc_o = acc_out, a.n_out = n_ctx_out;
-    hipLaunchKernelGGL(evict_move_kernel<0>, mgrid, block, 0, st, a);
+    hipLaunchKernelGGL(evict_move_kernel<OUT>, mgrid, block, 0, st, a);
   } else {
-    a.ko = take(cache_bytes(nkvh, keep, q8)), a.vo = take(cache_bytes(nkvh, keep, q8));
-    a.acc_o = (float*)take((size_t)nkvh * keep * 4), a.n_out = keep;
-    hipLaunchKernelGGL(evict_move_kernel<0>, mgrid, block, 0, st, a);
-    EvictArgs b = a;
-    b.kc = a.ko, b.vc = a.vo, b.acc = a.acc_o, b.n_ctx = keep;
-    b.ko = kout, b.vo = vout, b.acc_o = acc_out, b.n_out = n_ctx;
-    hipLaunchKernelGGL(evict_move_kernel<1>, mgrid, block, 0, st, b);
+    a.k_aside = take(cache_bytes(nkvh, keep, q8)), a.v_aside = take(cache_bytes(nkvh, keep, q8));
+    a.acc_aside = (float*)take((size_t)nkvh * keep * 4);
+    hipLaunchKernelGGL(evict_move_kernel<ASIDE>, mgrid, block, 0, st, a);
+    hipLaunchKernelGGL(evict_move_kernel<BACK>, mgrid, block, 0, st, a);
   }
   return check_launch("kv_evict");
 }

@@ -13,8 +13,9 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the workgroup's threads before this one, and over all of them. `s` is 4 words of LDS.
-__device__ __forceinline__ int scan256(int v, int* s, int& total) {
+// Sum over the threads of WAVES waves before this one, and over all of them. `s` is WAVES words of LDS.
+template <int WAVES>
+__device__ __forceinline__ int scan_waves(int v, int* s, int& total) {
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
   int x = v;
 #pragma unroll
@@ -27,11 +28,13 @@ __device__ __forceinline__ int scan256(int v, int* s, int& total) {
   __syncthreads();
   int before = 0;
   total = 0;
-  for (int i = 0; i < 4; i++) {
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) {
     if (i < w) before += s[i];
     total += s[i];
   }
   return before + x - v;
 }
+__device__ __forceinline__ int scan256(int v, int* s, int& total) { return scan_waves<4>(v, s, total); }
 
 }  // namespace q27h

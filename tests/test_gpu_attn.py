@@ -171,6 +171,48 @@ def test_odd_drafted_rows_reach_only_those_that_see_them(G, where, bad, q8):
 
 
 @pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("T", [5, 12])
+def test_large_drafted_rows_do_not_coarsen_those_that_do_not_see_them(G, T, q8):
+    """Token 1's V row is 2^30 times as large as the others; only tokens 1 and 3 see it."""
+    r = np.random.default_rng(6)
+    pos0, n_ctx, nqh, nkvh = 40, 64, 24, 4
+    k, v = R.make_cache(r, nkvh, n_ctx, q8), R.make_cache(r, nkvh, n_ctx, q8, std=2.0 ** -10)
+    tree = np.array([1 << t for t in range(T)], np.uint64)
+    tree[3] |= np.uint64(2)
+    big = v.copy()
+    if q8:
+        R.split_q8(big, nkvh, n_ctx)[1][:, pos0 + 1] = 20000
+    else:
+        big.view(np.float16).reshape(nkvh, n_ctx, 256)[:, pos0 + 1] *= np.float16(1024)
+        big.view(np.float16).reshape(nkvh, n_ctx, 256)[:, pos0 + 1] *= np.float16(1024)
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    run = lambda v: [G.down(x) for x in G.tree(G.up(q), G.up(k), G.up(v), G.i32(pos0), G.u64(tree), T, nqh, nkvh,  # noqa: E731
+                                                n_ctx, q8)]
+    (o, lse), (eo, elze) = run(big), run(v)
+    others = [t for t in range(T) if t not in (1, 3)]
+    assert_bits_equal(o[others], eo[others], "o")
+    assert_bits_equal(lse, elze, "lse")
+    assert (np.abs(o[1]) > 100 * np.abs(eo[1])).any()
+
+
+@pytest.mark.parametrize("T,nqh", [(1, 24), (4, 24), (12, 24)])
+def test_tree_of_blocks_of_different_size(G, T, nqh):
+    """q8_0: the scales of a V row's 8 blocks span 2^28."""
+    r = np.random.default_rng(8)
+    pos0, n_ctx, nkvh = 300, 320, 4
+    k, (c, d) = R.make_cache(r, nkvh, n_ctx, True), R.split_q8(R.make_cache(r, nkvh, n_ctx, True, std=64), nkvh, n_ctx)
+    d = (d.astype(np.float32) * 2.0 ** (6 - 4 * np.arange(8))).astype(np.float16)
+    v = R.join_q8(c, d)
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    o, _ = G.tree(G.up(q), G.up(k), G.up(v), G.i32(pos0), None, T, nqh, nkvh, n_ctx, True)
+    eo, _, bo, _ = R.attend(q, R.values(k, nkvh, n_ctx, True), R.values(v, nkvh, n_ctx, True), R.visible(T, pos0, n_ctx, None), SCALE)
+    # a scale enters as a half relative to its row's largest, cut off: below 2^-14 of that by 2^-24 of it (f < 2 largest, so
+    # 2^-23), times a code of at most 127; the weights sum to 1. A product with it rounds to a half again, 2^-25 of f
+    # whatever its size, twice (both terms).
+    near(G.down(o), eo, bo + d.astype(np.float64).max() * 127 * (2.0 ** -23 + 2 * 2.0 ** -24), "o")
+
+
+@pytest.mark.parametrize("q8", [True, False])
 def test_tree_is_the_same_alone_and_among_others(G, q8):
     """A token's result depends on its mask alone, bit for bit, and two calls at once on two streams do not disturb each
     other."""

@@ -41,7 +41,10 @@ def evict(G, k, v, acc, pos0, keep, first, last, nkvh, n_ctx, q8, n_out=None, wi
 @pytest.mark.parametrize("n_ctx,pos0,keep,first,last,kind", [
     (300, 200, 64, 4, 16, "random"), (300, 300, 1, 0, 0, "random"), (300, 250, 40, 20, 20, "random"), (300, 250, 249, 4, 16, "random"),
     (300, 250, 250, 4, 16, "random"), (300, 60, 100, 4, 16, "random"), (300, 0, 10, 1, 1, "random"), (300, 500, 17, 3, 5, "random"),
-    (5000, 4999, 700, 0, 0, "equal"), (5000, 4999, 700, 4, 64, "few"), (5000, 4800, 1000, 4, 64, "odd"), (9000, 8999, 4100, 4, 64, "close")])
+    (5000, 4999, 700, 0, 0, "equal"), (5000, 4999, 700, 4, 64, "few"), (5000, 4800, 1000, 4, 64, "odd"), (9000, 8999, 4100, 4, 64, "close"),
+    (32768, 32768, 5000, 4, 64, "random"), (33000, 32990, 9000, 4, 64, "close"), (33000, 20000, 300, 4, 64, "odd"),
+    (33000, 33000, 300, 0, 0, "equal"), (33000, 25000, 30000, 4, 64, "random"), (33000, 32999, 32998, 4, 64, "few"),
+    (33000, 33000, 64, 32, 32, "random")])
 def test_evict(G, n_ctx, pos0, keep, first, last, kind, in_place, q8):  # noqa: F811
     r = np.random.default_rng(n_ctx + pos0 + keep)
     nkvh, n = 2, min(pos0, n_ctx)
