@@ -409,7 +409,8 @@ __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint6
       const unsigned d = (unsigned)(j - vis.n0);
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
-        const bool seen = j < vis.n || (j < vis.end && d < 64u && ((tree[rt] >> (d & 63u)) & 1));
+        // no branches: eight of them a lane cost more than the shift, and hipcc has lost one's value
+        const bool seen = (j < vis.n) | ((j < vis.end) & (d < 64u) & (bool)((tree[rt] >> (d & 63u)) & 1));
         s[rt][u][i] = seen ? s[rt][u][i] : -__builtin_huge_valf();
       }
     }

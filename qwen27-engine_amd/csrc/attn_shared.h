@@ -139,12 +139,14 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
 // them, and the LDS reads for the block after the next. A wave has one other beside it on its SIMD at the most, so it
 // has to hide these latencies itself (64 tokens, 65536 q8_0 rows: 329 us with each block done in turn, 305 so, and 300
 // with the weights' products in pairs of halves, see weigh()).
-template <bool Q8>
-__device__ __forceinline__ void scores(const SharedTile& t, const QRegs& q, f4 (&s)[2]) {
+// RT: row tiles of 16 query rows that the wave holds.
+template <bool Q8, int RT>
+__device__ __forceinline__ void scores(const SharedTile& t, const QRegs* q, f4 (&s)[RT][2]) {
   const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  f4 lo[2] = {zero, zero}, c[2][2];
-  s[0] = s[1] = zero;
+  f4 c[2][RT][2];
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = zero;
   h8 k[2][2];
   u2 ks[3][2];
   auto ask = [&](int b) {
@@ -156,11 +158,14 @@ __device__ __forceinline__ void scores(const SharedTile& t, const QRegs& q, f4 (
   };
   auto scale = [&](int b) {
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) s[u][i] = __builtin_fmaf(half_of(ks[b % 3][u][i & 1], i >> 1), c[b & 1][u][i], s[u][i]);
-      asm("" : "+v"(s[u]));  // formed here, as in attn_core.h
-    }
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          s[rt][u][i] = __builtin_fmaf(half_of(ks[b % 3][u][i & 1], i >> 1), c[b & 1][rt][u][i], s[rt][u][i]);
+        asm("" : "+v"(s[rt][u]));  // formed here, as in attn_core.h
+      }
   };
   ask(0);
 #pragma unroll
@@ -168,21 +173,29 @@ __device__ __forceinline__ void scores(const SharedTile& t, const QRegs& q, f4 (
     if (b < 7) ask(b + 1);
     if constexpr (Q8) {
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[b & 1][u] = mfma16(k[b & 1][u], q.lo[b], zero);
+      for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[b & 1][u] = mfma16(k[b & 1][u], q.hi[b], c[b & 1][u]);
+        for (int u = 0; u < 2; u++) c[b & 1][rt][u] = mfma16(k[b & 1][u], q[rt].lo[b], zero);
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) c[b & 1][rt][u] = mfma16(k[b & 1][u], q[rt].hi[b], c[b & 1][rt][u]);
       if (b) scale(b - 1);
       interleave<2>();
+      if (RT == 2) interleave<2>();
     } else {
 #pragma unroll
-      for (int u = 0; u < 2; u++) lo[u] = mfma16(k[b & 1][u], q.lo[b], lo[u]);
+      for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) s[u] = mfma16(k[b & 1][u], q.hi[b], s[u]);
+        for (int u = 0; u < 2; u++) s[rt][u] = mfma16(k[b & 1][u], q[rt].lo[b], s[rt][u]);
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) s[rt][u] = mfma16(k[b & 1][u], q[rt].hi[b], s[rt][u]);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
   if constexpr (Q8) scale(7);
-  else s[0] += lo[0], s[1] += lo[1];
 }
 
 // PART: some rows of the tile are hidden.

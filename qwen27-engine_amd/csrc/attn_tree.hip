@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
     constexpr bool kPart = decltype(hidden)::value;
     if (active) {
       f4 s[1][2];
-      scores<Q8>(buf[at], q, s[0]);
+      scores<Q8>(buf[at], &q, s);
       if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
       weights(st, s[0]);
       if constexpr (Q8) widen<kPart>(st, s[0], buf[at].vf);
@@ -676,9 +676,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs
   }
 }
 
-// attn_weights of more than 32 query rows: a row tile per wave, K shared; a wave leaves its sums per cache row in LDS, and
-// the first wave adds them up, in the waves' order, behind the barrier that ends the tile.
-template <bool Q8, int WAVES>
+// attn_weights of more than 32 query rows: K shared, row tiles w and WAVES + w in wave w (so that with 12 row tiles every
+// SIMD, which runs waves w and w + 4, has three); a wave leaves its sums per cache row in LDS, and the first wave adds them
+// up, in the waves' order, behind the barrier that ends the tile.
+template <bool Q8, int WAVES, int RT>
 __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(WeightArgs a) {
   constexpr size_t kLds = sizeof(SharedTile) * 2 > sizeof(QTile) * WAVES ? sizeof(SharedTile) * 2 : sizeof(QTile) * WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[kLds];
@@ -703,25 +704,36 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
     auto ask = [&](Staged<Q8, WAVES>& n, int t) {
       if (t < t1) request<Q8, WAVES, true, false>(n, kc, kc, t * kTileKeys, left_of(t));
     };
-    Staged<Q8, WAVES> even, odd;
+    constexpr int kAhead = RT == 2 ? 1 : 2;  // tiles on their way; two row tiles' queries leave registers for one
+    Staged<Q8, WAVES> even, two;
+    Staged<Q8, WAVES>& odd = kAhead == 2 ? two : even;
     ask(even, t0);
-    load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
-      const int q = first + r;
-      return r < a.tiles * 16 && q < rows ? a.qn + ((size_t)(q / group) * a.nqh + kh * group + q % group) * kHD : nullptr;
-    });
-    __syncthreads();
-    QRegs q;
-    take_queries(q, im[w]);
-    const float c = im[w].c[n];
-    const int r = first + w * 16 + n;
-    const bool mine = w < a.tiles && r < rows, on = mine && ((used >> (r / group)) & 1);
-    const float lse = on ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : 0.0f;
-    const uint64_t tree[1] = {mine ? tree_of(a.tree, r / group, a.T) : 0ull};
-    const bool active = __any(on);  // a row tile of which no row is asked for adds nothing
-    __syncthreads();
+    QRegs q[RT];
+    float c[RT], lse[RT];
+    bool on[RT], active[RT];
+    auto row = [&](int rt) { return first + (rt * WAVES + w) * 16 + n; };  // this lane's query row, where it is one
+    auto is_row = [&](int rt) { return rt * WAVES + w < a.tiles && row(rt) < rows; };
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+      on[rt] = active[rt] = false;
+      if (rt * WAVES >= a.tiles) continue;
+      load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
+        r += rt * WAVES * 16;
+        const int q = first + r;
+        return r < a.tiles * 16 && q < rows ? a.qn + ((size_t)(q / group) * a.nqh + kh * group + q % group) * kHD : nullptr;
+      });
+      __syncthreads();
+      take_queries(q[rt], im[w]);
+      c[rt] = im[w].c[n];
+      const int r = row(rt);
+      on[rt] = is_row(rt) && ((used >> (r / group)) & 1);
+      lse[rt] = on[rt] ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : 0.0f;
+      active[rt] = __any(on[rt]);  // a row tile of which no row is asked for adds nothing
+      __syncthreads();
+    }
     stage<Q8, WAVES, true, false>(even, buf[0], false, 0, nullptr);
     ask(even, t0 + 1);
-    ask(odd, t0 + 2);
+    if (kAhead == 2) ask(odd, t0 + 2);
     __syncthreads();
     float old = 0.0f;
     // threads 0 .. 31, behind the barrier of the tile before: its sums are added to its rows' weights
@@ -738,29 +750,44 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
       const int j = t * kTileKeys + threadIdx.x;
       if (threadIdx.x < kTileKeys && j < vis.end) old = j < vis.n || rg ? acc[j] : 0.0f;  // the weights of new rows begin here
       float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      if (active) {
-        f4 s[1][2];
-        scores<Q8>(buf[at], q, s[0]);
-        if ((t + 1) * kTileKeys > vis.n) hide<1>(s, vis, tree, t * kTileKeys);
+      auto add = [&](auto count) __attribute__((always_inline)) {  // the first `count` row tiles
+        constexpr int kN = decltype(count)::value;
+        f4 s[kN][2];
+        scores<Q8>(buf[at], q, s);
+        if ((t + 1) * kTileKeys > vis.n) {
+          uint64_t bits[kN];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float x = s[0][e >> 2][e & 3];
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse));
-          sum[e] = !on || x == -__builtin_huge_valf() ? 0.0f : p;
+          for (int rt = 0; rt < kN; rt++) bits[rt] = is_row(rt) ? tree_of(a.tree, row(rt) / group, a.T) : 0ull;
+          hide<kN>(s, vis, bits, t * kTileKeys);
         }
+#pragma unroll
+        for (int rt = 0; rt < kN; rt++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float x = s[rt][e >> 2][e & 3];
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[rt], -lse[rt]));
+            sum[e] += !on[rt] || x == -__builtin_huge_valf() ? 0.0f : p;
+          }
         sum_rows(sum);
-      }
+      };
+      if (RT == 2 && active[RT - 1]) add(std::integral_constant<int, RT>());
+      else if (active[0]) add(std::integral_constant<int, 1>());
       if (n < 8) s_sum[at][w][16 * (n >> 2) + 4 * g + (n & 3)] = sum[0];
       if (t + 1 < t1) stage<Q8, WAVES, true, false>(next, buf[at ^ 1], false, 0, nullptr);
-      ask(next, t + 3);
+      ask(next, t + 1 + kAhead);
       __syncthreads();
     };
     int t = t0;
-    for (; t + 1 < t1; t += 2) {
-      step(t, 0, even);
-      step(t + 1, 1, odd);
+    if constexpr (kAhead == 1) {
+#pragma unroll 1
+      for (; t < t1; t++) step(t, (t - t0) & 1, even);
+    } else {
+      for (; t + 1 < t1; t += 2) {
+        step(t, 0, even);
+        step(t + 1, 1, odd);
+      }
+      if (t < t1) step(t++, 0, even);
     }
-    if (t < t1) step(t++, 0, even);
     add_up(t1 - 1, (t1 - 1 - t0) & 1);
     __syncthreads();  // the sums are read, the buffers free for the next group's queries
   }
@@ -849,7 +876,12 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   WeightArgs a = {};
   a.qn = qn, a.lse = lse, a.kcache = kcache, a.pos0 = pos0, a.tree = tree, a.rows = rows, a.acc = acc;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
-  const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  // f16: without outputs a wave has registers for the queries of two row tiles. Taken where the fullest SIMD has less to do
+  // (32 tokens, 65536 rows: 100 -> 80 us), not at equal work (64 tokens: 149 us either way). q8's products in flight leave none.
+  const int two_groups = (lay.row_tiles + 15) / 16, two_tiles = (lay.row_tiles + two_groups - 1) / two_groups;
+  const bool two = !q8 && lay.tiles > 4 && two_groups * ((two_tiles + 3) / 4) < lay.groups * ((lay.tiles + 3) / 4);
+  if (two) lay.groups = two_groups, lay.tiles = two_tiles;
   a.groups = lay.groups, a.tiles = lay.tiles;
   const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + kWaves - 1) / kWaves;
   // narrow: small workgroups, four to a compute unit; wide: as many as are resident
@@ -861,11 +893,13 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   else if (lay.row_tiles == 2)
     hipLaunchKernelGGL((q8 ? attn_weights_kernel<true, 2> : attn_weights_kernel<false, 2>), grid, dim3(256), 0, stream_of(s), a);
   else if (lay.tiles <= 4)
-    hipLaunchKernelGGL((q8 ? attn_weights_wide_kernel<true, 4> : attn_weights_wide_kernel<false, 4>), grid, dim3(256), 0,
+    hipLaunchKernelGGL((q8 ? attn_weights_wide_kernel<true, 4, 1> : attn_weights_wide_kernel<false, 4, 1>), grid, dim3(256), 0,
                        stream_of(s), a);
   else
-    hipLaunchKernelGGL((q8 ? attn_weights_wide_kernel<true, 8> : attn_weights_wide_kernel<false, 8>), grid, dim3(512), 0,
-                       stream_of(s), a);
+    hipLaunchKernelGGL((q8    ? attn_weights_wide_kernel<true, 8, 1>
+                        : two ? attn_weights_wide_kernel<false, 8, 2>
+                              : attn_weights_wide_kernel<false, 8, 1>),
+                       grid, dim3(512), 0, stream_of(s), a);
   return check_launch("attn_weights");
 }
 

@@ -276,7 +276,7 @@ def test_far_rows_of_a_long_cache(G, q8, n_ctx):
 @pytest.mark.parametrize("T,pos0,n_ctx,nqh,nkvh,rows", [
     (1, 0, 40, 24, 4, None), (1, 33, 64, 24, 4, None), (4, 700, 1000, 24, 4, 0b1011), (5, 62, 65, 7, 1, None),
     (12, 95, 128, 16, 2, 0b100000000001), (64, 100, 200, 24, 4, None), (64, 130, 194, 6, 2, 1 << 63 | 5), (3, 50, 64, 24, 4, 0),
-    (3, -1, 64, 24, 4, None)])
+    (3, -1, 64, 24, 4, None), (27, 300, 400, 24, 4, 0x5ffffff), (9, 70, 200, 16, 1, None)])
 def test_weights(G, T, pos0, n_ctx, nqh, nkvh, rows, q8):
     r = np.random.default_rng(T * 1000 + pos0 + 7)
     end = min(pos0 + T, n_ctx)
