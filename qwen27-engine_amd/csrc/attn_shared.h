@@ -137,8 +137,8 @@ __device__ __forceinline__ void stage(Staged<Q8, WAVES>& t, SharedTile& sh, bool
 // Both products walk the 8 blocks of 32 dims as a pipeline, a step per block: its four matrix instructions (no two
 // neighbours depend on each other), the vector work that feeds the next block's or finishes the one's before, between
 // them, and the LDS reads for the block after the next. A wave has one other beside it on its SIMD at the most, so it
-// has to hide these latencies itself (64 tokens, 65536 q8_0 rows: 329 us with each block done in turn, 305 so, and 300
-// with the weights' products in pairs of halves, see weigh()).
+// has to hide these latencies itself (64 tokens, 65536 q8_0 rows: 329 us with each block done in turn, 305 so, 300
+// with the weights' products in pairs of halves, see weigh(), and 284 with one barrier for two tiles).
 // RT: row tiles of 16 query rows that the wave holds.
 template <bool Q8, int RT>
 __device__ __forceinline__ void scores(const SharedTile& t, const QRegs* q, f4 (&s)[RT][2]) {

@@ -327,14 +327,14 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) 
   finish<Q8, WR, WK>(st, sh, a, split, sp.used == 1, row(mine));
 }
 
-// More than 32 query rows: a row tile per wave, the cache rows shared (attn_shared.h). While the waves work on one tile, the
-// next one is in registers or on its way; it goes to the other LDS buffer behind the wave's own work, and one barrier a
-// tile keeps the two apart.
+// More than 32 query rows: a row tile per wave, the cache rows shared (attn_shared.h). While the waves work on kLag tiles,
+// the next ones are on their way through registers to the other LDS buffers, and one barrier keeps the two apart.
 template <bool Q8, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
-  constexpr size_t kLds = sizeof(SharedTile) * 2 > sizeof(QTile) * WAVES ? sizeof(SharedTile) * 2 : sizeof(QTile) * WAVES;
-  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kLds];  // the queries' image, then the tiles
-  __shared__ int s_odd[2];
+  constexpr int kLag = WAVES == 8 ? 2 : 1;  // tiles per barrier (4 waves: LDS for two workgroups on a compute unit)
+  constexpr size_t kTiles = sizeof(SharedTile) * 2 * kLag, kImages = sizeof(QTile) * WAVES;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kTiles > kImages ? kTiles : kImages];  // the queries' image, then the tiles
+  __shared__ int s_odd[2 * kLag];
   QTile* im = (QTile*)s_mem;
   SharedTile* buf = (SharedTile*)s_mem;
   const int unit = (int)(blockIdx.x / (8 * a.groups)) * 8 + (int)(blockIdx.x & 7), rg = (int)(blockIdx.x >> 3) % a.groups;
@@ -357,13 +357,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
   auto ask = [&](Staged<Q8, WAVES>& n, int t) {
     if (t < t1) request<Q8, WAVES, true, true>(n, kc, vc, t * kTileKeys, left_of(t));
   };
-  // tiles on their way beside the one in LDS: 8 waves of f16 two (64 tokens, 65536 rows: 221 -> 215 us); q8's arithmetic
+  // tiles on their way beside those in LDS: 8 waves of f16 two (64 tokens, 65536 rows: 221 -> 215 us); q8's arithmetic
   // takes longer than a load, and 4 waves carry twice as much each, whose registers spill: one
   constexpr int kAhead = WAVES == 8 && !Q8 ? 2 : 1;
-  Staged<Q8, WAVES> even, two;
-  Staged<Q8, WAVES>& odd = kAhead == 2 ? two : even;
+  Staged<Q8, WAVES> even, odd;
   ask(even, t0);
-  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  if (kLag == 2) ask(odd, t0 + 1);
+  if (threadIdx.x < 2 * kLag) s_odd[threadIdx.x] = 0;
   load_queries<Q8, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
     const int gr = row(r);
     return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
@@ -377,16 +377,22 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
   const uint64_t tree[1] = {gr >= 0 ? tree_of(a.tree, (first + mine) / group, a.T) : 0ull};
   const bool active = w < a.tiles && first + w * 16 < rows;
   __syncthreads();
-  if (t0 < t1) stage<Q8, WAVES, true, true>(even, buf[0], part_of(t0), left_of(t0), &s_odd[0]);
-  ask(even, t0 + 1);
-  if (kAhead == 2) ask(odd, t0 + 2);
+  auto put = [&](Staged<Q8, WAVES>& n, int t) __attribute__((always_inline)) {
+    const int at = (t - t0) & (2 * kLag - 1);
+    if (t < t1) stage<Q8, WAVES, true, true>(n, buf[at], part_of(t), left_of(t), &s_odd[at]);
+  };
+  put(even, t0);
+  if (kLag == 2) put(odd, t0 + 1);
+  ask(even, t0 + kLag);
+  if (kAhead == 2) ask(odd, t0 + kLag + 1);
   __syncthreads();
-  // `next` holds tile t + 1 and is given the one kAhead behind it. Two loops: a tile with hidden rows takes another form of the product,
+  // `next` holds tile t + kLag and is given the one kAhead behind it. Two loops: a tile with hidden rows takes another form of the product,
   // and with both in one loop the outputs' registers are copied between them (and spill); the first takes an even number
   // of tiles, so that either begins with `even`.
   int t = t0;
-  auto step = [&](auto hidden, int at, Staged<Q8, WAVES>& next) __attribute__((always_inline)) {
+  auto step = [&](auto hidden, Staged<Q8, WAVES>& next) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(hidden)::value;
+    const int at = (t - t0) & (2 * kLag - 1);
     if (active) {
       f4 s[1][2];
       scores<Q8>(buf[at], &q, s);
@@ -396,20 +402,20 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
       accumulate<Q8, kPart>(st, s[0], buf[at]);
       if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
     }
-    if (t + 1 < t1) stage<Q8, WAVES, true, true>(next, buf[at ^ 1], part_of(t + 1), left_of(t + 1), &s_odd[at ^ 1]);
-    ask(next, t + 1 + kAhead);
-    __syncthreads();
+    put(next, t + kLag);
+    ask(next, t + kLag + kAhead);
+    if (kLag == 1 || (at & 1)) __syncthreads();
     t++;
   };
   auto walk = [&](auto hidden, int end) __attribute__((always_inline)) {
     if constexpr (kAhead == 1) {
-      while (t < end) step(hidden, (t - t0) & 1, even);
+      while (t < end) step(hidden, even);
     } else {
       while (t + 1 < end) {
-        step(hidden, 0, even);
-        step(hidden, 1, odd);
+        step(hidden, even);
+        step(hidden, odd);
       }
-      if (t < end) step(hidden, 0, even);
+      if (t < end) step(hidden, even);
     }
   };
   const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
