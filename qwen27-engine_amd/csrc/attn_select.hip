@@ -42,72 +42,73 @@ __device__ __forceinline__ float scale_of(float amax, float& inv) {
 }
 __device__ __forceinline__ int code_of(float x, float inv) { return (int)__builtin_roundf(x * inv); }
 
-// One workgroup per block: a lane holds 4 channels, a wave every fourth row.
-__global__ void __launch_bounds__(256) block_bounds_kernel(const uint8_t* __restrict__ kcache, const int* __restrict__ dpos0,
-                                                           int T, int nkvh, int n_ctx, int q8, int8_t* __restrict__ lo,
+// One workgroup per block. A thread takes 16 bytes of every 16th (f16: 8th) row, all requested before the first is used: one
+// round trip to memory for the block; then thread c joins channel c's parts. (One token: 7.1 us with 4 bytes a lane and two
+// round trips, 4.0 us so.)
+template <bool Q8>
+__global__ void __launch_bounds__(kHD) block_bounds_kernel(const uint8_t* __restrict__ kcache, const int* __restrict__ dpos0,
+                                                           int T, int nkvh, int n_ctx, int8_t* __restrict__ lo,
                                                            int8_t* __restrict__ hi, float* __restrict__ kd) {
-  __shared__ float s_lo[4][kHD], s_hi[4][kHD];
-  __shared__ int s_odd[4];
-  const int kh = blockIdx.y, w = threadIdx.x >> 6, l = threadIdx.x & 63;
+  constexpr int kLanes = Q8 ? 16 : 32, kChans = kHD / kLanes, kGroups = kHD / kLanes, kRows = kBlockRows / kGroups;
+  __shared__ float s_lo[kGroups][kHD], s_hi[kGroups][kHD], s_max[kHD / 64];
+  __shared__ int s_odd[kHD / 64];
+  const int kh = blockIdx.y, tid = threadIdx.x, c = tid % kLanes, rg = tid / kLanes;
   const long long p0 = *dpos0, e = p0 + T;
   const int begin = p0 < 0 ? 0 : p0 > n_ctx ? n_ctx : (int)p0, end = e < 0 ? 0 : e > n_ctx ? n_ctx : (int)e;
   if (end <= begin) return;
   const int b = begin / kBlockRows + blockIdx.x, nblk = blocks_of(n_ctx);
   const int r0 = b * kBlockRows, r1 = r0 + kBlockRows < end ? r0 + kBlockRows : end;
   if (r0 >= end) return;
-  float a[4], z[4];
+  uint4 x[kRows];
+  uint16_t d[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; k++) {  // a row behind the last one that exists: the block's first again
+    const int r = r0 + rg + k * kGroups;
+    const size_t row = (size_t)kh * n_ctx + (r < r1 ? r : r0);
+    x[k] = *(const uint4*)(kcache + (row * kLanes + c) * 16);
+    if (Q8) d[k] = *(const uint16_t*)(kcache + (size_t)nkvh * n_ctx * kHD + row * 16 + 2 * (c >> 1));
+  }
+  loads_issued();
+  float a[kChans], z[kChans];
   bool odd = false;
 #pragma unroll
-  for (int c = 0; c < 4; c++) a[c] = __builtin_huge_valf(), z[c] = -__builtin_huge_valf();
-#pragma unroll 8
-  for (int r = r0 + w; r < r1; r += 4) {
-    const size_t row = (size_t)kh * n_ctx + r;
-    float x[4];
-    if (q8) {
-      const uint32_t v = *(const uint32_t*)(kcache + row * kHD + 4 * l);
-      const float d = h2f_bits(*(const uint16_t*)(kcache + (size_t)nkvh * n_ctx * kHD + row * 16 + 2 * (l >> 3)));
+  for (int i = 0; i < kChans; i++) a[i] = __builtin_huge_valf(), z[i] = -__builtin_huge_valf();
 #pragma unroll
-      for (int c = 0; c < 4; c++) x[c] = (float)(int8_t)(v >> (8 * c)) * d;
-    } else {
-      const uint2 v = *(const uint2*)(kcache + (row * kHD + 4 * l) * 2);
-      x[0] = h2f_bits((uint16_t)v.x), x[1] = h2f_bits((uint16_t)(v.x >> 16));
-      x[2] = h2f_bits((uint16_t)v.y), x[3] = h2f_bits((uint16_t)(v.y >> 16));
-    }
+  for (int k = 0; k < kRows; k++) {
+    const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      odd |= not_finite(x[c]);
-      a[c] = __builtin_fminf(a[c], x[c]);
-      z[c] = __builtin_fmaxf(z[c], x[c]);
+    for (int i = 0; i < kChans; i++) {
+      const float v = Q8 ? (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * h2f_bits(d[k]) : h2f_bits((uint16_t)(w[(i >> 1) & 3] >> (16 * (i & 1))));
+      odd |= not_finite(v);
+      a[i] = __builtin_fminf(a[i], v);
+      z[i] = __builtin_fmaxf(z[i], v);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < kChans; i += 4) {
+    *(float4*)&s_lo[rg][c * kChans + i] = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+    *(float4*)&s_hi[rg][c * kChans + i] = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
   }
   const int any = __any(odd);
-#pragma unroll
-  for (int c = 0; c < 4; c++) s_lo[w][4 * l + c] = a[c], s_hi[w][4 * l + c] = z[c];
-  if (l == 0) s_odd[w] = any;
+  if ((tid & 63) == 0) s_odd[tid >> 6] = any;
   __syncthreads();
-  if (w) return;
-  float amax = 0.0f;
+  float least = s_lo[0][tid], most = s_hi[0][tid];
 #pragma unroll
-  for (int c = 0; c < 4; c++) {
-    const int i = 4 * l + c;
-    a[c] = __builtin_fminf(__builtin_fminf(s_lo[0][i], s_lo[1][i]), __builtin_fminf(s_lo[2][i], s_lo[3][i]));
-    z[c] = __builtin_fmaxf(__builtin_fmaxf(s_hi[0][i], s_hi[1][i]), __builtin_fmaxf(s_hi[2][i], s_hi[3][i]));
-    amax = __builtin_fmaxf(amax, __builtin_fmaxf(__builtin_fabsf(a[c]), __builtin_fabsf(z[c])));
+  for (int k = 1; k < kGroups; k++) {
+    least = __builtin_fminf(least, s_lo[k][tid]);
+    most = __builtin_fmaxf(most, s_hi[k][tid]);
   }
-  amax = wave_max(amax);
+  const float m = wave_max(__builtin_fmaxf(__builtin_fabsf(least), __builtin_fabsf(most)));
+  if ((tid & 63) == 0) s_max[tid >> 6] = m;
+  __syncthreads();
+  const float amax = __builtin_fmaxf(__builtin_fmaxf(s_max[0], s_max[1]), __builtin_fmaxf(s_max[2], s_max[3]));
   const bool bad = s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3];  // an infinity or NaN: the block scores +inf and is read
   float inv;
-  const float d = scale_of(bad ? 0.0f : amax, inv);
-  int ca[4], cz[4];
-#pragma unroll
-  for (int c = 0; c < 4; c++) {
-    ca[c] = bad ? 0 : code_of(a[c], inv);
-    cz[c] = bad ? 0 : code_of(z[c], inv);
-  }
+  const float dk = scale_of(bad ? 0.0f : amax, inv);
   const size_t at = (size_t)kh * nblk + b;
-  *(uint32_t*)(lo + at * kHD + 4 * l) = pack4_i8(ca[0], ca[1], ca[2], ca[3]);
-  *(uint32_t*)(hi + at * kHD + 4 * l) = pack4_i8(cz[0], cz[1], cz[2], cz[3]);
-  if (l == 0) kd[at] = bad ? __builtin_huge_valf() : d;
+  lo[at * kHD + tid] = (int8_t)(bad ? 0 : code_of(least, inv));
+  hi[at * kHD + tid] = (int8_t)(bad ? 0 : code_of(most, inv));
+  if (tid == 0) kd[at] = bad ? __builtin_huge_valf() : dk;
 }
 
 // Scores: one int8 matrix instruction (16 query rows x 16 blocks x 64 channels) per 64 channels of hi and of lo. A token's
@@ -131,6 +132,19 @@ __global__ void __launch_bounds__(256) select_score_kernel(const float* __restri
   const int tiles = (nb + 15) / 16, per = (tiles + splits - 1) / splits;
   const int b1 = split * per + per < tiles ? split * per + per : tiles;
   if (split * per >= b1) return;
+  // this lane's block (column) of 16, requested ahead of the queries and then of the products before
+  v4i vh[4], vl[4];
+  float d;
+  auto ask = [&](int bt) {
+    const int b = bt * 16 + n, bb = b < nb ? b : nb - 1;
+    const int8_t* ph = hi + ((size_t)kh * nblk + bb) * kHD + 16 * g;
+    const int8_t* pl = lo + ((size_t)kh * nblk + bb) * kHD + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) vh[i] = *(const v4i*)(ph + 64 * i), vl[i] = *(const v4i*)(pl + 64 * i);
+    d = kd[(size_t)kh * nblk + bb];
+  };
+  ask(split * per + w);
+  loads_issued();
   const int used = (T - t0 + per_tile - 1) / per_tile < kRowTiles ? (T - t0 + per_tile - 1) / per_tile : kRowTiles;
   for (int rt = 0; rt < used; rt++) {
     float4 in[4];  // the wave's four rows of the tile, requested together
@@ -163,19 +177,18 @@ __global__ void __launch_bounds__(256) select_score_kernel(const float* __restri
   }
   __syncthreads();
   for (int bt = split * per + w; bt < b1; bt += 4) {
-    const int b = bt * 16 + n, bb = b < nb ? b : nb - 1;  // this lane's block (column)
-    const int8_t* ph = hi + ((size_t)kh * nblk + bb) * kHD + 16 * g;
-    const int8_t* pl = lo + ((size_t)kh * nblk + bb) * kHD + 16 * g;
-    v4i vh[4], vl[4];
+    const int b = bt * 16 + n;
+    v4i wh[4], wl[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) vh[i] = *(const v4i*)(ph + 64 * i), vl[i] = *(const v4i*)(pl + 64 * i);
-    const float d = kd[(size_t)kh * nblk + bb];
+    for (int i = 0; i < 4; i++) wh[i] = vh[i], wl[i] = vl[i];
+    const float db = d;
+    if (bt + 4 < b1) ask(bt + 4);
     for (int rt = 0; rt < used; rt++) {
       v4i c = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][0][i][l], vh[i], c, 0, 0, 0);
+      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][0][i][l], wh[i], c, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][1][i][l], vl[i], c, 0, 0, 0);
+      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)s_q[rt][1][i][l], wl[i], c, 0, 0, 0);
       float m = -__builtin_huge_valf();
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -186,35 +199,39 @@ __global__ void __launch_bounds__(256) select_score_kernel(const float* __restri
       if (gp >= 16) m = __builtin_fmaxf(m, lane_xor32(m));
       const int t = t0 + rt * per_tile + 4 * g / gp;
       if (b < nb && t < T && (4 * g & (gp - 1)) == 0)
-        score[((size_t)t * nkvh + kh) * nblk + b] = d == __builtin_huge_valf() ? d : m * d;
+        score[((size_t)t * nkvh + kh) * nblk + b] = db == __builtin_huge_valf() ? db : m * db;
     }
   }
 }
 
 // One workgroup per (token, kv head). Always taken are the first `first` blocks and the last `last` ones up to the token's
-// own; of the others, keys in LDS, the need-th largest is found by 8-bit digits of key - (least key), so that the first
+// own; of the others, keys in LDS, the need-th largest is found by digits of key - (least key), so that the first
 // digit already tells them apart (digits of the key itself would put most scores, which share their exponents, in one
 // histogram bin, and its counter's updates one behind another). It ends as soon as a bin is taken whole. Then a thread
-// counts and lists a stretch of consecutive blocks of its own. (2345 blocks: 18 us with the key's own digits and a
-// workgroup sum for every 256 blocks, 6 us so.)
-__global__ void __launch_bounds__(256) select_pick_kernel(const float* __restrict__ score, const int* __restrict__ dpos0, int nkvh,
+// counts and lists a stretch of consecutive blocks of its own. A digit has as many values as there are threads: 256, or 1024
+// while the workgroups leave compute units free. (2345 blocks: 18 us with the key's own digits and a workgroup sum for every
+// 256 blocks, 8 us so with 256 threads, 6.8 us with 1024.)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) select_pick_kernel(const float* __restrict__ score, const int* __restrict__ dpos0, int nkvh,
                                                           int n_ctx, int nsel, int first, int last, int* __restrict__ idx) {
   extern __shared__ uint32_t s_key[];
-  __shared__ int s_hist[256], s_scan[4], s_pick[3];
-  __shared__ uint32_t s_end[8];
+  constexpr int kWaves = THREADS / 64, kBits = THREADS == 256 ? 8 : 10;
+  static_assert(THREADS == 1 << kBits && kMaxBlocks < 1 << 15);
+  __shared__ int s_hist[THREADS], s_scan[kWaves], s_pick[3];
+  __shared__ uint32_t s_end[2 * kWaves];
   const int t = blockIdx.x / nkvh, tid = threadIdx.x, w = tid >> 6, nblk = blocks_of(n_ctx);
   const long long pos = (long long)*dpos0 + t;
   const int nb = pos < 0 ? 0 : pos >= n_ctx ? nblk : (int)(pos / kBlockRows) + 1;
   int* out = idx + (size_t)blockIdx.x * nsel;
   if (nb <= nsel) {
-    for (int i = tid; i < nsel; i += 256) out[i] = i < nb ? i : -1;
+    for (int i = tid; i < nsel; i += THREADS) out[i] = i < nb ? i : -1;
     return;
   }
   const float* row = score + (size_t)blockIdx.x * nblk;
   const int b0 = first, b1 = nb - last;  // the blocks chosen from
   uint32_t least = ~0u, most = 0u;
 #pragma unroll 4
-  for (int b = b0 + tid; b < b1; b += 256) {
+  for (int b = b0 + tid; b < b1; b += THREADS) {
     const uint32_t k = order_key(row[b]);
     s_key[b] = k;
     least = least < k ? least : k;
@@ -226,29 +243,29 @@ __global__ void __launch_bounds__(256) select_pick_kernel(const float* __restric
     least = least < x ? least : x;
     most = most > y ? most : y;
   }
-  if ((tid & 63) == 0) s_end[w] = least, s_end[4 + w] = most;
+  if ((tid & 63) == 0) s_end[w] = least, s_end[kWaves + w] = most;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < kWaves; i++) {
     least = least < s_end[i] ? least : s_end[i];
-    most = most > s_end[4 + i] ? most : s_end[4 + i];
+    most = most > s_end[kWaves + i] ? most : s_end[kWaves + i];
   }
   // `need` blocks are still to be taken among the keys whose digits above `shift` are those of `prefix`
   int need = nsel - first - last, shift = need && least < most ? 32 - __builtin_clz(most - least) : 0;
   uint32_t prefix = need ? 0u : ~0u;
   auto upper = [](uint32_t k, int by) { return (uint32_t)((uint64_t)k >> by); };
   while (shift > 0) {
-    const int next = shift > 8 ? shift - 8 : 0;
+    const int next = shift > kBits ? shift - kBits : 0;
     s_hist[tid] = 0;
     __syncthreads();
-    for (int b = b0 + tid; b < b1; b += 256) {
+    for (int b = b0 + tid; b < b1; b += THREADS) {
       const uint32_t k = s_key[b] - least;
       if (upper(k, shift) == upper(prefix, shift)) atomicAdd(&s_hist[(k >> next) & ((1u << (shift - next)) - 1u)], 1);
     }
     __syncthreads();
-    const int bin = 255 - tid, h = s_hist[bin];
+    const int bin = THREADS - 1 - tid, h = s_hist[bin];
     int total;
-    const int above = scan256(h, s_scan, total);
+    const int above = scan_waves<kWaves>(h, s_scan, total);
     if (above < need && need <= above + h) s_pick[0] = bin, s_pick[1] = need - above, s_pick[2] = h;
     __syncthreads();
     prefix |= (uint32_t)s_pick[0] << next;
@@ -259,16 +276,16 @@ __global__ void __launch_bounds__(256) select_pick_kernel(const float* __restric
   }
   __syncthreads();
   // taken: keys above the digits found; of those with them the first `need`
-  const int per = (b1 - b0 + 255) / 256, c0 = b0 + tid * per, c1 = c0 + per < b1 ? c0 + per : b1;
+  const int per = (b1 - b0 + THREADS - 1) / THREADS, c0 = b0 + tid * per, c1 = c0 + per < b1 ? c0 + per : b1;
   const uint32_t p = upper(prefix, shift);
-  int above = 0, equal = 0;
+  int mine = 0;  // above << 16 | equal: each below 2^15
   for (int b = c0; b < c1; b++) {
     const uint32_t k = upper(s_key[b] - least, shift);
-    above += k > p;
-    equal += k == p;
+    mine += (k > p ? 1 << 16 : 0) + (k == p);
   }
   int total;
-  int at = scan256(above, s_scan, total), rank = scan256(equal, s_scan, total);
+  const int before = scan_waves<kWaves>(mine, s_scan, total);
+  int at = before >> 16, rank = before & 0xffff;
   at += first + (rank < need ? rank : need);
   for (int b = c0; b < c1; b++) {
     const uint32_t k = upper(s_key[b] - least, shift);
@@ -276,8 +293,8 @@ __global__ void __launch_bounds__(256) select_pick_kernel(const float* __restric
     rank += k == p;
     if (take) out[at++] = b;
   }
-  for (int i = tid; i < first; i += 256) out[i] = i;
-  for (int i = tid; i < last; i += 256) out[nsel - last + i] = b1 + i;
+  for (int i = tid; i < first; i += THREADS) out[i] = i;
+  for (int i = tid; i < last; i += THREADS) out[nsel - last + i] = b1 + i;
 }
 
 int padded_group(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
@@ -302,9 +319,9 @@ extern "C" int q27h_kv_block_bounds(const void* kcache, const int* pos0, int T, 
   const long touched = (long)(T + kBlockRows - 1) / kBlockRows + 1;
   int8_t* lo = (int8_t*)kb;
   int8_t* hi = lo + (size_t)nkvh * nblk * kHD;
-  hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)(touched < nblk ? touched : nblk), (unsigned)nkvh), dim3(256), 0,
-                     stream_of(s), (const uint8_t*)kcache, pos0, T, nkvh, n_ctx, q8, lo, hi,
-                     (float*)(hi + (size_t)nkvh * nblk * kHD));
+  hipLaunchKernelGGL((q8 ? block_bounds_kernel<true> : block_bounds_kernel<false>),
+                     dim3((unsigned)(touched < nblk ? touched : nblk), (unsigned)nkvh), dim3(kHD), 0, stream_of(s),
+                     (const uint8_t*)kcache, pos0, T, nkvh, n_ctx, lo, hi, (float*)(hi + (size_t)nkvh * nblk * kHD));
   return check_launch("kv_block_bounds");
 }
 
@@ -335,7 +352,8 @@ extern "C" int q27h_attn_select(const float* qn, const void* kb, const int* pos0
   splits = splits > most ? most : splits < 1 ? 1 : splits;
   hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)((long)tg * nkvh * splits)), dim3(256), 0, stream_of(s), qn, lo, hi, kd,
                      pos0, T, nqh, nkvh, n_ctx, gp, splits, (float*)ws);
-  hipLaunchKernelGGL(select_pick_kernel, dim3((unsigned)(T * nkvh)), dim3(256), (size_t)nblk * 4, stream_of(s), (const float*)ws,
-                     pos0, nkvh, n_ctx, nsel, first, last, idx);
+  const bool few = T * nkvh <= kCUs;
+  hipLaunchKernelGGL((few ? select_pick_kernel<1024> : select_pick_kernel<256>), dim3((unsigned)(T * nkvh)), dim3(few ? 1024 : 256),
+                     (size_t)nblk * 4, stream_of(s), (const float*)ws, pos0, nkvh, n_ctx, nsel, first, last, idx);
   return check_launch("attn_select");
 }

@@ -800,15 +800,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
 }
 
 // How attn_tree's and attn_weights' workgroups are laid out by the row tiles of 16 query rows. Up to two: each wave walks
-// cache rows of its own. More: up to 8 waves of a row tile each share them, in as few groups as that takes, of equal size.
+// cache rows of its own. More: up to 8 waves of a row tile each share them, in as few groups as that takes, of equal size;
+// attn_tree over q8_0 takes groups of 4 waves, two to a compute unit, where the fullest SIMD has less to do then (32 tokens,
+// 65536 rows: 184 -> 170 us, 48: 275 -> 256 us; f16, bound by the matrix instructions and L2: 137 -> 140, 194 -> 206 us).
 struct TreeLayout {
   int row_tiles, wide, groups, tiles, splits, waves;
 };
-TreeLayout tree_layout(int T, int nqh, int nkvh, int n_ctx) {
+TreeLayout tree_layout(int T, int nqh, int nkvh, int n_ctx, bool quarter) {
   TreeLayout t;
   t.row_tiles = (T * (nqh / nkvh) + 15) / 16;
   t.wide = t.row_tiles > 2;
   t.groups = t.wide ? (t.row_tiles + 7) / 8 : 1;
+  const int quarters = (t.row_tiles + 3) / 4;
+  if (quarter && t.wide && quarters < t.groups * (((t.row_tiles + t.groups - 1) / t.groups + 3) / 4)) t.groups = quarters;
   t.tiles = (t.row_tiles + t.groups - 1) / t.groups;
   t.waves = 4;
   // enough workgroups for every compute unit: two of 4 waves on each, or one of 8
@@ -837,7 +841,8 @@ using namespace q27h;
 
 extern "C" size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx) {
   if (T <= 0 || T > kMaxTree || !heads_ok(nqh, nkvh) || n_ctx <= 0) return 0;
-  return part_bytes((size_t)T * nqh, tree_layout(T, nqh, nkvh, n_ctx).splits);
+  const int s0 = tree_layout(T, nqh, nkvh, n_ctx, false).splits, s1 = tree_layout(T, nqh, nkvh, n_ctx, true).splits;
+  return part_bytes((size_t)T * nqh, s0 > s1 ? s0 : s1);
 }
 
 extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* vcache, const int* pos0, const uint64_t* tree,
@@ -855,7 +860,7 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
   AttnArgs a = {};
   a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.tree = tree, a.o = o, a.lse = lse;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
-  const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  const TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx, q8 != 0);
   a.splits = lay.splits, a.groups = lay.groups, a.waves = lay.waves, a.tiles = lay.tiles;
   a.part = (float*)ws, a.ml = a.part + (size_t)T * nqh * a.splits * kHD;
   const dim3 grid((unsigned)((nkvh * a.splits + 7) / 8 * 8 * a.groups));
@@ -882,7 +887,7 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   WeightArgs a = {};
   a.qn = qn, a.lse = lse, a.kcache = kcache, a.pos0 = pos0, a.tree = tree, a.rows = rows, a.acc = acc;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
-  TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx);
+  TreeLayout lay = tree_layout(T, nqh, nkvh, n_ctx, false);
   // f16: without outputs a wave has registers for the queries of two row tiles. Taken where the fullest SIMD has less to do
   // (32 tokens, 65536 rows: 100 -> 80 us), not at equal work (64 tokens: 149 us either way). q8's products in flight leave none.
   const int two_groups = (lay.row_tiles + 15) / 16, two_tiles = (lay.row_tiles + two_groups - 1) / two_groups;

@@ -75,6 +75,8 @@ TREES = [
     (64, 65, 140, 24, 4, "random"),  # the widest tree
     (64, 513, 577, 1, 1, "random"),
     (17, 40, 64, 48, 2, "high"),     # mask bits of tokens that are none
+    (27, 300, 400, 24, 4, "random"),  # eleven row tiles
+    (45, 700, 1000, 24, 4, "random"),  # seventeen
 ]
 
 
