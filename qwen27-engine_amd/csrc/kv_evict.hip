@@ -6,7 +6,7 @@
 // integer atomics, so in any order to the same result) over workgroups that each hold a segment of the rows; then each
 // segment counts its rows above and at the threshold and writes its own part of the list behind the segments before it.
 // Up to 32768 rows of context one workgroup a kv head does all of that over keys in LDS (20001 rows: 7 launches, 29 us;
-// two, 24 us, 16 of them the choice). Rows are moved by 16 bytes a lane. In place, the kept rows that lie before row
+// two, 23 us, 15 of them the choice). Rows are moved by 16 bytes a lane. In place, the kept rows that lie before row
 // `keep` go through the workspace, since a row's place may be another one's source there; the others are read where no
 // row is written.
 #include "pick.h"
@@ -152,19 +152,18 @@ __global__ void __launch_bounds__(kListThreads) evict_choose_kernel(EvictArgs a)
   const int r0 = a.first, rows = n - a.last - r0;
   const float* acc = a.acc + (size_t)kh * a.n_ctx + r0;
   uint32_t least = ~0u, most = 0u;
-  for (int r = tid; r < rows; r += 16 * kListThreads) {
-    float x[16];  // requested together
+  constexpr int kEach = kLdsRows / kListThreads;
+  float x[kEach];  // requested together
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (r + i * kListThreads < rows) x[i] = acc[r + i * kListThreads];
+  for (int i = 0; i < kEach; i++)
+    if (tid + i * kListThreads < rows) x[i] = acc[tid + i * kListThreads];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      if (r + i * kListThreads >= rows) break;
-      const uint32_t k = order_key(x[i]);
-      s_key[r + i * kListThreads] = k;
-      least = least < k ? least : k;
-      most = most > k ? most : k;
-    }
+  for (int i = 0; i < kEach; i++) {
+    if (tid + i * kListThreads >= rows) break;
+    const uint32_t k = order_key(x[i]);
+    s_key[tid + i * kListThreads] = k;
+    least = least < k ? least : k;
+    most = most > k ? most : k;
   }
   for (int i = tid; i < a.first; i += kListThreads) out[i] = i;
   for (int i = tid; i < a.last; i += kListThreads) out[a.keep - a.last + i] = n - a.last + i;
@@ -212,15 +211,15 @@ __global__ void __launch_bounds__(kListThreads) evict_choose_kernel(EvictArgs a)
   const int per = (rows + kListThreads - 1) / kListThreads | 1, c0 = tid * per < rows ? tid * per : rows;
   const int c1 = c0 + per < rows ? c0 + per : rows;
   const uint32_t p = upper(prefix, shift);
-  int above = 0, equal = 0;
+  uint32_t mine = 0;  // above << 16 | equal, together at most kLdsRows
 #pragma unroll 8
   for (int r = c0; r < c1; r++) {
     const uint32_t k = upper(s_key[r] - least, shift);
-    above += k > p;
-    equal += k == p;
+    mine += (k > p ? 1u << 16 : 0u) + (k == p);
   }
   int total;
-  int at = scan_waves<kListThreads / 64>(above, s_scan, total), rank = scan_waves<kListThreads / 64>(equal, s_scan, total);
+  const uint32_t before = (uint32_t)scan_waves<kListThreads / 64>((int)mine, s_scan, total);
+  int at = (int)(before >> 16), rank = (int)(before & 0xffffu);
   at += a.first + (rank < need ? rank : need);
 #pragma unroll 4
   for (int r = c0; r < c1; r++) {
