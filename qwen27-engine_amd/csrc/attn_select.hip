@@ -316,7 +316,7 @@ extern "C" int q27h_kv_block_bounds(const void* kcache, const int* pos0, int T, 
   if (!kcache || !pos0 || !kb) return fail(Q27H_ERR_ARG, "kv_block_bounds: null pointer");
   if (!aligned16(kcache) || !aligned16(kb)) return fail(Q27H_ERR_ARG, "kv_block_bounds: tensors need 16-byte alignment");
   const int nblk = blocks_of(n_ctx);
-  const long touched = (long)(T + kBlockRows - 1) / kBlockRows + 1;
+  const long touched = ((long)T + kBlockRows - 1) / kBlockRows + 1;
   int8_t* lo = (int8_t*)kb;
   int8_t* hi = lo + (size_t)nkvh * nblk * kHD;
   hipLaunchKernelGGL((q8 ? block_bounds_kernel<true> : block_bounds_kernel<false>),
@@ -352,7 +352,7 @@ extern "C" int q27h_attn_select(const float* qn, const void* kb, const int* pos0
   splits = splits > most ? most : splits < 1 ? 1 : splits;
   hipLaunchKernelGGL(select_score_kernel, dim3((unsigned)((long)tg * nkvh * splits)), dim3(256), 0, stream_of(s), qn, lo, hi, kd,
                      pos0, T, nqh, nkvh, n_ctx, gp, splits, (float*)ws);
-  const bool few = T * nkvh <= kCUs;
+  const bool few = T * nkvh <= kCUs && nblk <= kMaxBlocks - 1024;  // the larger digits' counts take 3 KB of the 64
   hipLaunchKernelGGL((few ? select_pick_kernel<1024> : select_pick_kernel<256>), dim3((unsigned)(T * nkvh)), dim3(few ? 1024 : 256),
                      (size_t)nblk * 4, stream_of(s), (const float*)ws, pos0, nkvh, n_ctx, nsel, first, last, idx);
   return check_launch("attn_select");

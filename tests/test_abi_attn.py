@@ -96,6 +96,10 @@ def blocks(o, qn=F, T=4, nsel=16, nqh=24, nkvh=4, n_ctx=4096, out=F << 4, ws=W):
     (lambda o: accept(o, caches=(F, None)), -4, "null pointer"),
     (lambda o: accept(o, caches=(F, F + 8)), -4, "alignment"),
     (lambda o: accept(o, accs=(None,)), -4, "null pointer"),
+    (lambda o: accept(o, caches=(F, 2 * F, F)), -4, "overlap"),                   # a cache twice
+    (lambda o: accept(o, caches=(F, F + 4096)), -4, "overlap"),
+    (lambda o: accept(o, accs=(F + 4096,)), -4, "overlap"),
+    (lambda o: accept(o, caches=(2 * F,), accs=(F, F + 4)), -4, "overlap"),
     (lambda o: bounds(o, T=-1), -1, "bad shape"),
     (lambda o: bounds(o, n_ctx=0), -1, "bad shape"),
     (lambda o: bounds(o, kb=None), -4, "null pointer"),

@@ -58,6 +58,8 @@ def near(got, want, bound, what):
 
 # (T, rows before, n_ctx, query heads, kv heads, tree)
 TREES = [
+    (1, 0, 1, 24, 4, None),          # a cache of one row
+    (2, 0, 1, 6, 6, "random"),
     (1, 0, 40, 24, 4, None),         # the very first token sees itself alone
     (1, 1, 40, 24, 4, None),
     (1, 31, 64, 4, 4, None),         # a tile of 32 rows, exactly
@@ -276,7 +278,7 @@ def test_far_rows_of_a_long_cache(G, q8, n_ctx):
 
 @pytest.mark.parametrize("q8", [True, False])
 @pytest.mark.parametrize("T,pos0,n_ctx,nqh,nkvh,rows", [
-    (1, 0, 40, 24, 4, None), (1, 33, 64, 24, 4, None), (4, 700, 1000, 24, 4, 0b1011), (5, 62, 65, 7, 1, None),
+    (1, 0, 1, 24, 4, None), (1, 0, 40, 24, 4, None), (1, 33, 64, 24, 4, None), (4, 700, 1000, 24, 4, 0b1011), (5, 62, 65, 7, 1, None),
     (12, 95, 128, 16, 2, 0b100000000001), (64, 100, 200, 24, 4, None), (64, 130, 194, 6, 2, 1 << 63 | 5), (3, 50, 64, 24, 4, 0),
     (3, -1, 64, 24, 4, None), (27, 300, 400, 24, 4, 0x5ffffff), (9, 70, 200, 16, 1, None)])
 def test_weights(G, T, pos0, n_ctx, nqh, nkvh, rows, q8):
@@ -355,8 +357,24 @@ def test_select(G, T, pos0, n_ctx, nqh, nkvh, nsel, first, last):
     assert np.array_equal(G.down(idx), want)
 
 
+@pytest.mark.parametrize("n_ctx", [1024000, 958000])
+def test_select_of_the_longest_context(G, n_ctx):
+    """The bounds are written as they are; every block but the fixed ones is told apart by its scale."""
+    r = np.random.default_rng(n_ctx)
+    nblk, nsel, first, last = -(-n_ctx // 64), 40, 1, 2
+    one = r.integers(1, 128, 256).astype(np.int8)
+    d = r.permutation(nblk).astype(np.float32) + 1
+    kb = np.concatenate([np.tile(one, nblk).view(np.uint8), np.tile(one, nblk).view(np.uint8), d.view(np.uint8)])
+    q = np.abs(r.standard_normal((1, 2, 256))).astype(np.float32)  # scores: a positive constant times d
+    idx = G.full((1, 1, nsel), 99, dtype=__import__("torch").int32)
+    G.ops.attn_select(G.up(q), G.up(kb), G.i32(n_ctx - 1), 1, 2, 1, n_ctx, nsel, first, last, idx,
+                      G.ws(G.ops.attn_select_ws_bytes(1, 1, n_ctx)))
+    mid = first + np.argsort(-d[first:nblk - last])[:nsel - first - last]
+    assert G.down(idx)[0, 0].tolist() == sorted([0, *mid.tolist(), nblk - 2, nblk - 1])
+
+
 @pytest.mark.parametrize("q8", [True, False])
-@pytest.mark.parametrize("T,pos0,n_ctx,nqh,nkvh,nsel", [(1, 0, 40, 24, 4, 1), (1, 1000, 1100, 24, 4, 9), (3, 62, 70, 7, 1, 2),
+@pytest.mark.parametrize("T,pos0,n_ctx,nqh,nkvh,nsel", [(1, 0, 1, 24, 4, 2), (1, 0, 40, 24, 4, 1), (1, 1000, 1100, 24, 4, 9), (3, 62, 70, 7, 1, 2),
                                                         (40, 300, 340, 16, 2, 4), (300, 20, 320, 6, 2, 3), (2, 200, 201, 16, 1, 5)])
 def test_blocks(G, T, pos0, n_ctx, nqh, nkvh, nsel, q8):
     """Lists in any order, with entries that are no blocks, blocks behind the token, a block twice, and empty lists."""

@@ -39,7 +39,7 @@ def evict(G, k, v, acc, pos0, keep, first, last, nkvh, n_ctx, q8, n_out=None, wi
 @pytest.mark.parametrize("q8", [True, False])
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("n_ctx,pos0,keep,first,last,kind", [
-    (300, 200, 64, 4, 16, "random"), (300, 300, 1, 0, 0, "random"), (300, 250, 40, 20, 20, "random"), (300, 250, 249, 4, 16, "random"),
+    (1, 1, 1, 0, 0, "random"), (1, 0, 1, 1, 0, "random"), (300, 200, 64, 4, 16, "random"), (300, 300, 1, 0, 0, "random"), (300, 250, 40, 20, 20, "random"), (300, 250, 249, 4, 16, "random"),
     (300, 250, 250, 4, 16, "random"), (300, 60, 100, 4, 16, "random"), (300, 0, 10, 1, 1, "random"), (300, 500, 17, 3, 5, "random"),
     (5000, 4999, 700, 0, 0, "equal"), (5000, 4999, 700, 4, 64, "few"), (5000, 4800, 1000, 4, 64, "odd"), (9000, 8999, 4100, 4, 64, "close"),
     (32768, 32768, 5000, 4, 64, "random"), (33000, 32990, 9000, 4, 64, "close"), (33000, 20000, 300, 4, 64, "odd"),
@@ -116,6 +116,82 @@ def test_accept(G, T, pos0, path, n_path, q8):  # noqa: F811
         for a, b in moves:
             want[:, b] = src[:, a]
         assert_bits_equal(G.down(got), want, "acc")
+
+
+@pytest.mark.parametrize("q8,n_ctx", [(True, 3200000), (False, 1600000)])
+def test_far_rows(G, q8, n_ctx):  # noqa: F811
+    """The last head's last rows of a cache of more than 2^31 bytes: moved by kv_accept and kv_evict, bounded, chosen,
+    attended to and weighed. All rows before them are zeros."""
+    import torch
+
+    r = np.random.default_rng(4)
+    nkvh, tail = 4, 300
+    pos0, row = n_ctx - tail, 272 if q8 else 512
+    rest = [R.make_cache(r, 1, tail, q8) for _ in range(2)]
+    bufs = []
+    for x in rest:
+        buf = torch.zeros(nkvh * n_ctx * row, dtype=torch.uint8, device="cuda:0")
+        if q8:
+            buf[(nkvh * n_ctx - tail) * 256:nkvh * n_ctx * 256] = G.up(x[:tail * 256])
+            buf[-tail * 16:] = G.up(x[tail * 256:])
+        else:
+            buf[-tail * 512:] = G.up(x)
+        bufs.append(buf)
+
+    def rows(buf, a, b):  # of the last head
+        if not q8:
+            return G.down(buf[((nkvh - 1) * n_ctx + a) * 512:][:(b - a) * 512]).reshape(-1, 512)
+        codes = buf[((nkvh - 1) * n_ctx + a) * 256:][:(b - a) * 256]
+        scales = buf[nkvh * n_ctx * 256 + ((nkvh - 1) * n_ctx + a) * 16:][:(b - a) * 16]
+        return np.concatenate([G.down(codes).reshape(-1, 256), G.down(scales).reshape(-1, 16)], 1)
+
+    src = [rows(b, pos0, n_ctx) for b in bufs]
+    kv = [R.values(x, 1, tail, q8) for x in rest]
+    q = r.standard_normal((1, nkvh, 256)).astype(np.float32)
+    # the tail's blocks alone
+    idx = np.full((1, nkvh, 8), -1, np.int32)
+    b0 = -(-pos0 // 64)
+    idx[0, nkvh - 1, :3] = [b0, b0 + 2, b0 + 1]
+    o, lse = G.blocks(G.up(q), bufs[0], bufs[1], G.i32(n_ctx - 1), G.up(idx), 1, 8, nkvh, nkvh, n_ctx, q8)
+    at = 64 * b0 - pos0
+    seen = np.zeros((1, tail), bool)
+    seen[0, at:at + 192] = True
+    eo, el, bo, bl = R.attend(q[:, -1:], kv[0], kv[1], seen, SCALE)
+    near(G.down(o)[:, -1:], eo, bo, "o")
+    near(G.down(lse)[:, -1:], el, bl, "lse")
+    # their weights, by the blocks' lse
+    acc = torch.zeros((nkvh, n_ctx), device="cuda:0")
+    G.ops.attn_weights(G.up(q), lse, bufs[0], G.i32(n_ctx - 1), None, 1, SCALE, nkvh, nkvh, n_ctx, q8, acc,
+                       rows=G.u64([1]))
+    s = SCALE * (kv[0][0, at:at + 192] @ q[0, -1].astype(np.float64))
+    ds = SCALE * (np.abs(kv[0][0, at:at + 192]) @ np.abs(q[0, -1].astype(np.float64))) * (2.0 ** -21 + 16 * 2.0 ** -23)
+    p = np.exp(s - np.float64(G.down(lse)[0, -1]))
+    near(G.down(acc[-1, pos0 + at:pos0 + at + 192]), p, p * (ds + (np.abs(s) + 10) * 2.0 ** -22 + 2.0 ** -22), "acc")
+    # bounds of the tail's blocks
+    kb = torch.zeros(G.ops.kv_block_bytes(nkvh, n_ctx), dtype=torch.uint8, device="cuda:0")
+    G.ops.kv_block_bounds(bufs[0], G.i32(64 * b0), n_ctx - 64 * b0, nkvh, n_ctx, q8, kb)
+    nblk = -(-n_ctx // 64)
+    lo = G.down(kb[:nkvh * nblk * 256].view(torch.int8).view(nkvh, nblk, 256)[-1, b0:b0 + 3])
+    d = G.down(kb[2 * nkvh * nblk * 256:].view(torch.float32).view(nkvh, nblk)[-1, b0:b0 + 3])
+    for i in range(3):
+        x = kv[0][0, at + 64 * i:at + 64 * (i + 1)]
+        assert d[i] == np.float32(np.float32(np.abs(x).max()) / np.float32(127))
+        # a code is off by half a step and the three roundings of x * (1 / d)
+        assert np.all(np.abs(lo[i] - x.min(0) / np.float64(d[i])) <= 0.5 + 127 * 3 * 2.0 ** -24)
+    # a path of the tail
+    G.ops.kv_accept(bufs, [acc], G.i32(pos0 + 100), G.i32(3, 50, 60, *[0] * 61), G.i32(3), 64, nkvh, n_ctx, q8)
+    for x in src:
+        x[100:103] = x[[103, 150, 160]]
+    for b, x in zip(bufs, src):
+        assert np.array_equal(rows(b, pos0, n_ctx), x)
+    # the tail and the first rows stay
+    acc.zero_()
+    ws = G.ws(G.ops.kv_evict_ws_bytes(nkvh, n_ctx, 400, q8, True))
+    kept = G.full((nkvh, 400), 0, dtype=torch.int32)
+    G.ops.kv_evict(bufs[0], bufs[1], acc, G.i32(n_ctx), 400, 50, tail, bufs[0], bufs[1], acc, n_ctx, kept, nkvh, n_ctx, q8, ws)
+    assert np.array_equal(G.down(kept)[-1], np.r_[np.arange(100), pos0 + np.arange(tail)])
+    for b, x in zip(bufs, src):
+        assert np.array_equal(rows(b, 100, 400), x) and np.array_equal(rows(b, pos0, n_ctx), x)
 
 
 def test_accept_of_many_arrays(G):  # noqa: F811
