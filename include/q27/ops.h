@@ -4,7 +4,8 @@
 // launchers throw on bad shapes (src/ops.cu:699,704,724,734) and through CK (src/common.cuh:11-12).
 // Declared here: the fused per-layer ops and their unfused twins, the delta-rule recurrence gdn_step and the bf16
 // pair GEMV gemv_bf16_pair of src/ops.h. The quantized GEMV is in qmat.h, the prefill row ops in prefill.h; the
-// attention kernels of src/ops.h (attn_decode, attn_prefill) are outside this library.
+// attention kernels of src/ops.h (attn_decode, attn_prefill) are outside this library. What reads the K/V cache here, under
+// names and signatures of its own, is in attn.h.
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime_api.h>

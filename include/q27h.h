@@ -175,7 +175,8 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * No counterpart in the reference's launchers (its attn_decode / attn_prefill are other functions). All of them read
  * caches in the layout that attn_prep writes (f16, or q8_0 where q8 != 0), qn [T][nqh][256] as attn_prep leaves it, and
  * the device integer *pos0 = rows of the context before this batch. Rows outside [0, n_ctx) are never read or written.
- * float32 results: no operand is rounded to fewer bits than the cache holds.
+ * float32 results from the cache's values as they are; one exception: a q8_0 V scale below 2^-14 of the power of two above
+ * its row's largest is taken to 2^-24 of that.
  * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
  * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
  * at the same time, need one each.
@@ -184,8 +185,8 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * before *pos0 and row *pos0 + u where bit u of tree[t] (device, 64-bit; bits >= T are ignored) is set: its ancestors
  * and, usually, itself. tree NULL: a chain (bits 0 .. t); T = 1 with NULL is plain decoding.
  * o [T][nqh][256] = sum_j p_j v_j, p = softmax over the rows seen of scale * q . k_j; lse [T][nqh] (may be NULL) =
- * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. o may not overlap qn. nqh % nkvh == 0: query head h reads kv
- * head h / (nqh / nkvh). Rotary positions of a tree are given to attn_prep through rope3. */
+ * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. o may not overlap qn. nqh % nkvh == 0:
+ * query head h reads kv head h / (nqh / nkvh). Values that are not finite reach the tokens that see their row. Rotary positions of a tree are given to attn_prep through rope3. */
 size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx);
 int q27h_attn_tree(const float* qn, const void* kcache, const void* vcache, const int* pos0, const uint64_t* tree, int T,
                    float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws, size_t ws_bytes,

@@ -142,3 +142,46 @@ def test_workspace_sizes(q27):
     assert o.attn_select_ws_bytes(5, 4, 129) == 5 * 4 * 3 * 4
     assert o.attn_blocks_ws_bytes(1027, 24, 4, 32) == 0 and o.attn_blocks_ws_bytes(1, 24, 4, 64) > 0
     assert o.kv_evict_ws_bytes(4, 4096, 64, True, True) >= o.kv_evict_ws_bytes(4, 4096, 64, True, False) + 2 * 4 * 64 * 272
+
+
+def test_cpp_header_forwards(tmp_path):
+    """include/q27/attn.h: every function compiles in a caller, and a refusal arrives as an exception."""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "qwen27-engine_amd", "lib")
+    src, exe = tmp_path / "caller.cpp", tmp_path / "caller"
+    src.write_text(r'''
+#include <cstdio>
+#include "q27/attn.h"
+void step(const float* qn, void* k, void* v, int* pos0, const uint64_t* tree, float* o, float* lse, float* acc, void* kb, int* idx,
+          void* ws, size_t n, hipStream_t s) {
+  q27::attn_tree(qn, k, v, pos0, tree, 4, 0.0625f, 24, 4, 4096, true, o, ws, n, s, lse);
+  q27::attn_weights(qn, lse, k, pos0, tree, 4, 0.0625f, 24, 4, 4096, true, acc, s, tree);
+  q27::kv_evict(k, v, acc, pos0, 1024, 4, 64, k, v, acc, 4096, nullptr, 4, 4096, true, ws, n, s);
+  q27::kv_evict_pos(pos0, idx, 1024, s);
+  void* caches[2] = {k, v};
+  q27::kv_accept(caches, 2, &acc, 1, pos0, idx, idx, 4, 4, 4096, true, s);
+  q27::kv_block_bounds(k, pos0, 4, 4, 4096, true, kb, s);
+  q27::attn_select(qn, kb, pos0, 4, 24, 4, 4096, 32, 1, 2, idx, ws, n, s);
+  q27::attn_blocks(qn, k, v, pos0, idx, 4, 32, 0.0625f, 24, 4, 4096, true, o, ws, n, s, lse);
+}
+int main(int argc, char**) {
+  if (argc > 9) step(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr);
+  size_t n = q27::attn_tree_ws_bytes(4, 24, 4, 4096) + q27::kv_evict_ws_bytes(4, 4096, 64, true, false) +
+             q27::kv_block_bytes(4, 4096) + q27::attn_select_ws_bytes(4, 4, 4096) + q27::attn_blocks_ws_bytes(4, 24, 4, 32);
+  try {
+    q27::attn_tree(nullptr, nullptr, nullptr, nullptr, nullptr, 65, 1.0f, 24, 4, 4096, true, nullptr, nullptr, 0, nullptr);
+  } catch (const std::runtime_error& e) {
+    std::printf("%d %s\n", n > 0, e.what());
+    return 0;
+  }
+  return 1;
+}
+''')
+    subprocess.run(["/opt/rocm/llvm/bin/clang++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    f"-I{root}/include", str(src), f"-L{lib}", "-lq27h", "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{lib}",
+                    "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)], check=True, capture_output=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout
+    assert out.startswith("1 ") and "T must be 0..64" in out
