@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(256) evict_list_kernel(EvictArgs a) {
 // with K. OUT: kept rows to their places in other buffers. In place: ASIDE: those of rows before `keep` that have to move,
 // to the workspace; BACK: those to their places, and the others from where they lie.
 enum { OUT, ASIDE, BACK };
+constexpr int kMoves = 2;  // rows of a thread in flight at once
 template <int MODE>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
   const int kh = blockIdx.y, n = rows_of(a), m = n < a.keep ? n : a.keep;
@@ -313,18 +314,35 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
   const int out_rows = MODE == ASIDE ? a.keep : a.n_out;
   uint8_t* to = MODE == ASIDE ? aside : out;
   float* acc_to = MODE == ASIDE ? a.acc_aside : a.acc_o;
-#pragma unroll 4
-  for (int i = blockIdx.x * rows + threadIdx.x / lanes; i < m; i += gridDim.x * rows) {
-    const int r = a.kept[(size_t)kh * a.keep + i];
-    const bool near = MODE != OUT && r < a.keep;
-    if (MODE != OUT && (r == i || (MODE == ASIDE && !near))) continue;
-    const bool ws = MODE == BACK && near;
-    const uint8_t* from = ws ? aside : cache;
-    const int from_rows = ws ? a.keep : a.n_ctx, fr = ws ? i : r;
-    *(u4*)row(to, out_rows, i) = *(const u4*)row(from, from_rows, fr);
-    if (a.q8 && sub == 0) *(u4*)scale(to, out_rows, i) = *(const u4*)scale(from, from_rows, fr);
-    if (!v && sub == 1)
-      acc_to[(size_t)kh * out_rows + i] = ws ? a.acc_aside[(size_t)kh * a.keep + i] : a.acc[(size_t)kh * a.n_ctx + r];
+  const int* kept = a.kept + (size_t)kh * a.keep;
+  for (int i0 = blockIdx.x * rows * kMoves + threadIdx.x / lanes; i0 < m; i0 += gridDim.x * rows * kMoves) {
+    int r[kMoves];
+    bool go[kMoves], ws[kMoves];  // to be moved here; from the workspace
+    u4 x[kMoves], d[kMoves];
+    float w[kMoves];
+#pragma unroll
+    for (int k = 0; k < kMoves; k++) r[k] = i0 + k * rows < m ? kept[i0 + k * rows] : -1;
+#pragma unroll
+    for (int k = 0; k < kMoves; k++) {
+      const int i = i0 + k * rows;
+      const bool near = MODE != OUT && r[k] < a.keep;
+      go[k] = r[k] >= 0 && (MODE == OUT || (r[k] != i && (MODE != ASIDE || near)));
+      ws[k] = MODE == BACK && near;
+      const uint8_t* from = ws[k] ? aside : cache;
+      const int from_rows = ws[k] ? a.keep : a.n_ctx, fr = ws[k] ? i : r[k];
+      if (!go[k]) continue;
+      x[k] = *(const u4*)row(from, from_rows, fr);
+      if (a.q8 && sub == 0) d[k] = *(const u4*)scale(from, from_rows, fr);
+      if (!v && sub == 1) w[k] = ws[k] ? a.acc_aside[(size_t)kh * a.keep + i] : a.acc[(size_t)kh * a.n_ctx + r[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < kMoves; k++) {
+      const int i = i0 + k * rows;
+      if (!go[k]) continue;
+      *(u4*)row(to, out_rows, i) = x[k];
+      if (a.q8 && sub == 0) *(u4*)scale(to, out_rows, i) = d[k];
+      if (!v && sub == 1) acc_to[(size_t)kh * out_rows + i] = w[k];
+    }
   }
 }
 
@@ -450,7 +468,7 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
     hipLaunchKernelGGL(evict_count_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(evict_list_kernel, grid, block, 0, st, a);
   }
-  const int rows = q8 ? 16 : 8;
+  const int rows = (q8 ? 16 : 8) * kMoves;
   int chunks = (keep + rows - 1) / rows;
   const int most = 16 * kCUs / (2 * nkvh) < 1 ? 1 : 16 * kCUs / (2 * nkvh);
   chunks = chunks > most ? most : chunks;
