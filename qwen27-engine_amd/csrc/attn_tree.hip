@@ -331,7 +331,9 @@ __global__ void __launch_bounds__(WR * WK * 64, 2) attn_tree_kernel(AttnArgs a) 
 // the next ones are on their way through registers to the other LDS buffers, and one barrier keeps the two apart.
 template <bool Q8, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
-  constexpr int kLag = WAVES == 8 ? 2 : 1;  // tiles per barrier (4 waves: LDS for two workgroups on a compute unit)
+  // tiles per barrier. 4 waves: one, for two workgroups' LDS on a compute unit; f16: one, since the second tile's way at the
+  // start costs as much as the barriers do (12 tokens, 32771 rows: 49.1, 50.5 us; 64, 65536: 221 us either way)
+  constexpr int kLag = WAVES == 8 && Q8 ? 2 : 1;
   constexpr size_t kTiles = sizeof(SharedTile) * 2 * kLag, kImages = sizeof(QTile) * WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[kTiles > kImages ? kTiles : kImages];  // the queries' image, then the tiles
   __shared__ int s_odd[2 * kLag];

@@ -505,12 +505,14 @@ extern "C" int q27h_kv_accept(void* const* caches, int n_caches, float* const* a
   for (int i = 0; i < n_accs; i++)
     if (!accs[i]) return fail(Q27H_ERR_ARG, "kv_accept: null pointer");
   const size_t cb = cache_bytes(nkvh, n_ctx, q8), ab = (size_t)nkvh * n_ctx * 4;
-  for (int i = 0; i < n_caches + n_accs; i++)  // a row moved twice, by workgroups that run at once
-    for (int j = 0; j < i; j++) {
-      const void *x = i < n_caches ? caches[i] : accs[i - n_caches], *y = j < n_caches ? caches[j] : accs[j - n_caches];
-      if (overlaps(x, i < n_caches ? cb : ab, y, j < n_caches ? cb : ab))
-        return fail(Q27H_ERR_ARG, "kv_accept: caches or weight arrays overlap");
-    }
+  bool twice = false;  // a row moved twice, by workgroups that run at once
+  for (int i = 0; i < n_caches; i++)
+    for (int j = 0; j < i; j++) twice |= overlaps(caches[i], cb, caches[j], cb);
+  for (int i = 0; i < n_accs; i++) {
+    for (int j = 0; j < i; j++) twice |= overlaps(accs[i], ab, accs[j], ab);
+    for (int j = 0; j < n_caches; j++) twice |= overlaps(accs[i], ab, caches[j], cb);
+  }
+  if (twice) return fail(Q27H_ERR_ARG, "kv_accept: caches or weight arrays overlap");
   for (int c = 0, w = 0; c < n_caches || w < n_accs;) {
     AcceptArgs a = {};
     a.pos0 = pos0, a.path = path, a.n_path = n_path, a.T = T, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8;
