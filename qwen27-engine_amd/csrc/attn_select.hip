@@ -338,7 +338,7 @@ extern "C" int q27h_attn_select(const float* qn, const void* kb, const int* pos0
     return fail(Q27H_ERR_SHAPE, "attn_select: first >= 0, last >= 1 and first + last <= nsel");
   const int nblk = blocks_of(n_ctx);
   if (nblk > kMaxBlocks) return fail(Q27H_ERR_SHAPE, "attn_select: n_ctx must be <= 1024000");
-  if ((long long)T * nkvh > 0x7fffffffLL / 64) return fail(Q27H_ERR_SHAPE, "attn_select: T too large");
+  if ((long long)T * nkvh > 0x7fffffffLL / 128) return fail(Q27H_ERR_SHAPE, "attn_select: T too large");
   if (T == 0) return Q27H_OK;
   if (!qn || !kb || !pos0 || !idx || !ws) return fail(Q27H_ERR_ARG, "attn_select: null pointer");
   if (!aligned16(qn) || !aligned16(kb) || !aligned4(ws)) return fail(Q27H_ERR_ARG, "attn_select: tensors need 16-byte alignment");

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
   auto ask = [&](Staged<Q8, WAVES>& n, int t) {
     if (t < t1) request<Q8, WAVES, true, true>(n, kc, vc, t * kTileKeys, left_of(t));
   };
-  // tiles on their way beside those in LDS: 8 waves of f16 two (64 tokens, 65536 rows: 221 -> 215 us); q8's arithmetic
+  // tiles on their way beside those in LDS: 8 waves of f16 two (64 tokens, 65536 rows: 227 -> 219 us); q8's arithmetic
   // takes longer than a load, and 4 waves carry twice as much each, whose registers spill: one
   constexpr int kAhead = WAVES == 8 && !Q8 ? 2 : 1;
   Staged<Q8, WAVES> even, odd;
@@ -928,7 +928,7 @@ extern "C" int q27h_attn_blocks(const float* qn, const void* kcache, const void*
                                 size_t ws_bytes, q27h_stream_t s) {
   if (T < 0 || nsel <= 0 || !heads_ok(nqh, nkvh) || nqh / nkvh > 16 || n_ctx <= 0)
     return fail(Q27H_ERR_SHAPE, "attn_blocks: bad shape (at most 16 query heads per kv head)");
-  if (nsel > (1 << 20) || (long long)T * nqh > 0x7fffffffLL / 64) return fail(Q27H_ERR_SHAPE, "attn_blocks: T or nsel too large");
+  if (nsel > (1 << 20) || (long long)T * nqh > 0x7fffffffLL / 128) return fail(Q27H_ERR_SHAPE, "attn_blocks: T or nsel too large");
   if (T == 0) return Q27H_OK;
   if (!qn || !kcache || !vcache || !pos0 || !idx || !o) return fail(Q27H_ERR_ARG, "attn_blocks: null pointer");
   if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
