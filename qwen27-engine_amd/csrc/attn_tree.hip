@@ -488,16 +488,18 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a)
   finish<Q8, 1, kWaves>(st, sh, a, split, a.splits == 1, row(threadIdx.x & 15));
 }
 
-// Joins the splits of one query row: a workgroup takes 64 of the 256 dims (16 lanes of 4), its 16 groups of lanes every
-// 16th split, all requested at once; then the groups' sums are added in order. FIXED: every split was written; else those
-// that split_of used, and nothing is left to do where that is one. (128 splits of 24 rows: 38 us with a thread per dim
-// that walks the splits, 4.7 us so.)
-constexpr int kMaxSplits = 2 * kCUs;
-template <bool FIXED>
+// Joins the splits of one query row: GROUPS groups of lanes take every GROUPS-th split each, all requested at once, a lane 4
+// of the workgroup's 1024 / GROUPS dims; then the groups' sums are added in order. 16 groups where a row has many splits
+// (128 splits of 24 rows: 38 us with a thread per dim that walks the splits, 4.7 us so), 4 where it has up to 32 (12 splits
+// of 1536 rows: a quarter of the workgroups, 38.6 -> 34.9 us with the splits' own kernel).
+// FIXED: every split was written; else those that split_of used, and nothing is left to do where that is one.
+constexpr int kMaxSplits = 2 * kCUs, kFewSplits = 32;
+template <bool FIXED, int GROUPS>
 __global__ void __launch_bounds__(256, 8) attn_join_kernel(AttnArgs a) {
+  constexpr int kLanes = 256 / GROUPS;
   __shared__ float s_f[kMaxSplits], s_red[8];
-  __shared__ f4 s_o[16][16];
-  const int gr = blockIdx.x, tid = threadIdx.x, c = tid & 15, sg = tid >> 4, w = tid >> 6;
+  __shared__ f4 s_o[GROUPS][kLanes];
+  const int gr = blockIdx.x, tid = threadIdx.x, c = tid % kLanes, sg = tid / kLanes, w = tid >> 6;
   int used = a.splits;
   if (!FIXED) {
     const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
@@ -505,12 +507,12 @@ __global__ void __launch_bounds__(256, 8) attn_join_kernel(AttnArgs a) {
     if (used == 1) return;
   }
   const float2* ml = (const float2*)a.ml + (size_t)gr * a.splits;
-  const f4* part = (const f4*)(a.part + (size_t)gr * a.splits * kHD) + blockIdx.y * 16 + c;
+  const f4* part = (const f4*)(a.part + (size_t)gr * a.splits * kHD) + blockIdx.y * kLanes + c;
   constexpr int kBatch = 8;
   f4 x[kBatch];
 #pragma unroll
   for (int k = 0; k < kBatch; k++) {
-    const int s = sg + 16 * k;
+    const int s = sg + GROUPS * k;
     if (s < used) x[k] = part[(size_t)s * (kHD / 4)];
   }
   float2 v[kMaxSplits / 256];
@@ -547,21 +549,27 @@ __global__ void __launch_bounds__(256, 8) attn_join_kernel(AttnArgs a) {
   f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int k = 0; k < kBatch; k++) {
-    const int s = sg + 16 * k;
+    const int s = sg + GROUPS * k;
     if (s < used) o += x[k] * s_f[s];
   }
-  for (int s = sg + 16 * kBatch; s < used; s += 16) o += part[(size_t)s * (kHD / 4)] * s_f[s];
+  for (int s = sg + GROUPS * kBatch; s < used; s += GROUPS) o += part[(size_t)s * (kHD / 4)] * s_f[s];
   s_o[sg][c] = o;
   __syncthreads();
-  if (tid < 16) {
+  if (tid < kLanes) {
     f4 r = s_o[0][tid];
 #pragma unroll
-    for (int k = 1; k < 16; k++) r += s_o[k][tid];
+    for (int k = 1; k < GROUPS; k++) r += s_o[k][tid];
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *((f4*)(a.o + (size_t)gr * kHD) + blockIdx.y * 16 + tid) = r * inv;
+    *((f4*)(a.o + (size_t)gr * kHD) + blockIdx.y * kLanes + tid) = r * inv;
   }
   if (a.lse && tid == 0 && blockIdx.y == 0)
     a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+template <bool FIXED>
+void launch_join(const AttnArgs& a, hipStream_t s) {
+  const bool few = a.splits <= kFewSplits;
+  hipLaunchKernelGGL((few ? attn_join_kernel<FIXED, 4> : attn_join_kernel<FIXED, 16>), dim3((unsigned)(a.T * a.nqh), few ? 1 : 4),
+                     dim3(256), 0, s, a);
 }
 
 // Sums of eight values over the 16 query rows (lanes n) of a lane group: lanes n and n ^ 8 leave with value n & 7 in x[0].
@@ -700,7 +708,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const Vis vis = vis_of(*a.pos0, a.T, a.n_ctx);
   const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
-  const Split sp = split_of(tiles, a.splits, kWaves);
+  const Split sp = split_of(tiles, a.splits, 1);
   if (split >= sp.used) return;
   const int t0 = split * sp.per, t1 = t0 + sp.per < tiles ? t0 + sp.per : tiles;
   if (t0 >= t1) return;
@@ -818,7 +826,9 @@ TreeLayout tree_layout(int T, int nqh, int nkvh, int n_ctx, bool quarter) {
   const int quarters = (t.row_tiles + 3) / 4;
   if (quarter && t.wide && quarters < t.groups * (((t.row_tiles + t.groups - 1) / t.groups + 3) / 4)) t.groups = quarters;
   t.tiles = (t.row_tiles + t.groups - 1) / t.groups;
-  t.waves = 4;
+  // over the cache rows: a split is at least a tile for each (12 tokens of 500 rows: 27.8 us with four tiles to a split of
+  // shared ones, 20 with one)
+  t.waves = t.wide ? 1 : 4;
   // enough workgroups for every compute unit: two of 4 waves on each, or one of 8
   const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + t.waves - 1) / t.waves;
   const bool half = t.wide ? t.tiles <= 4 : t.row_tiles == 1;
@@ -876,7 +886,7 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
     hipLaunchKernelGGL((q8 ? attn_wide_kernel<true, 4> : attn_wide_kernel<false, 4>), grid, dim3(256), 0, stream_of(s), a);
   else
     hipLaunchKernelGGL((q8 ? attn_wide_kernel<true, 8> : attn_wide_kernel<false, 8>), grid, dim3(512), 0, stream_of(s), a);
-  if (lay.splits > 1) hipLaunchKernelGGL(attn_join_kernel<false>, dim3((unsigned)(T * nqh), 4), dim3(256), 0, stream_of(s), a);
+  if (lay.splits > 1) launch_join<false>(a, stream_of(s));
   return check_launch("attn_tree");
 }
 
@@ -898,7 +908,7 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   const bool two = !q8 && lay.tiles > 4 && two_groups * ((two_tiles + 3) / 4) < lay.groups * ((lay.tiles + 3) / 4);
   if (two) lay.groups = two_groups, lay.tiles = two_tiles;
   a.groups = lay.groups, a.tiles = lay.tiles;
-  const int most = ((n_ctx + kTileKeys - 1) / kTileKeys + kWaves - 1) / kWaves;
+  const int waves = lay.wide ? 1 : kWaves, most = ((n_ctx + kTileKeys - 1) / kTileKeys + waves - 1) / waves;
   // narrow: small workgroups, four to a compute unit; wide: as many as are resident
   a.splits = (!lay.wide ? 4 * kCUs : lay.tiles <= 4 ? 2 * kCUs : kCUs) / nkvh;
   a.splits = a.splits > most ? most : a.splits < 1 ? 1 : a.splits;
@@ -943,6 +953,6 @@ extern "C" int q27h_attn_blocks(const float* qn, const void* kcache, const void*
   a.part = (float*)ws, a.ml = a.part + (size_t)T * nqh * a.splits * kHD;
   const auto kern = q8 ? attn_blocks_kernel<true> : attn_blocks_kernel<false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)((long)T * nkvh * a.splits)), dim3(256), 0, stream_of(s), a);
-  if (a.splits > 1) hipLaunchKernelGGL(attn_join_kernel<true>, dim3((unsigned)(T * nqh), 4), dim3(256), 0, stream_of(s), a);
+  if (a.splits > 1) launch_join<true>(a, stream_of(s));
   return check_launch("attn_blocks");
 }
