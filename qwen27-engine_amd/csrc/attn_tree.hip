@@ -1,10 +1,13 @@
 // Attention over the K/V cache that attn_prep writes: a tree of drafted tokens (attn_tree; one token is plain decoding),
 // blocks of 64 rows chosen per token (attn_blocks), and the sums of attention weights per cache row (attn_weights).
 //
-// The rows of the cache are split over workgroups and, in each, over its 4 waves; a wave walks its tiles of 32 rows with
-// the online softmax of attn_core.h, the next tile's loads in flight behind the current one's arithmetic. The query rows
-// of a kv head (tokens x query heads of the group) are 16 or 32 to a wave; more are spread over workgroups that read the
-// same cache rows on the same XCD, so that its L2 serves all but the first. A second launch joins the splits.
+// The rows of the cache are split over workgroups. The query rows of a kv head (tokens x query heads of the group) are taken
+// as row tiles of 16. Up to two: each wave of a workgroup walks tiles of 32 cache rows of its own with the online softmax
+// of attn_core.h, the next tile's loads in flight behind the current one's arithmetic, so that one or two row tiles are
+// bound by HBM (150000 q8_0 rows, one token: 64 us, 5.1 TB/s). More: each wave holds a row tile and the workgroup shares the
+// cache rows (attn_shared.h), bound by the matrix instructions of two f16 terms and, over q8_0, the vector work beside
+// them; more than 8 row tiles are spread over workgroups that read the same cache rows on the same XCD, so that its L2
+// serves all but the first. A second launch joins the splits.
 #include <type_traits>
 
 #include "attn_core.h"
