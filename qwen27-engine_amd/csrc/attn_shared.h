@@ -182,7 +182,6 @@ __device__ __forceinline__ void scores(const SharedTile& t, const QRegs* q, f4 (
         for (int u = 0; u < 2; u++) c[b & 1][rt][u] = mfma16(k[b & 1][u], q[rt].hi[b], c[b & 1][rt][u]);
       if (b) scale(b - 1);
       interleave<2>();
-      if (RT == 2) interleave<2>();
     } else {
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
