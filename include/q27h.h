@@ -175,8 +175,11 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * No counterpart in the reference's launchers (its attn_decode / attn_prefill are other functions). All of them read
  * caches in the layout that attn_prep writes (f16, or q8_0 where q8 != 0), qn [T][nqh][256] as attn_prep leaves it, and
  * the device integer *pos0 = rows of the context before this batch. Rows outside [0, n_ctx) are never read or written.
- * float32 results from the cache's values as they are; one exception: a q8_0 V scale below 2^-14 of the power of two above
- * its row's largest is taken to 2^-24 of that.
+ * The cache's values enter as they are, q and the softmax weights in two f16 terms each, the sums are float32. So, beside
+ * float32's roundings, a value of q is off by less than 2^-21 of itself or, if that is more, 2^-38 of the largest of its
+ * query row; a weight by less than 2^-21 of itself or 2^-36 of the largest of its query row (q8_0: a weight times its V
+ * row's largest scale by less than 2^-33 of the largest weight times the largest scale seen). One value of the cache is
+ * not taken as it is: a q8_0 V scale below 2^-14 of the power of two above its row's largest, to 2^-24 of that.
  * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
  * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
  * at the same time, need one each.

@@ -2,8 +2,10 @@
 //
 // Scores and outputs are float32 results of 16-bit matrix instructions. The cache's values enter them exactly: an f16
 // cache as it is, a q8_0 cache as its codes (|code| <= 127 is exact in f16), with the f16 scales applied outside. The
-// other operand (q, or the weight p times V's scale) is split in two f16 terms, x = hi + lo, each product exact in the
-// instruction's float32 sum, so what is lost is below 2^-21 of a term; one f16 term would lose 2^-12 of it.
+// other operand (q, or the weight p times V's scale) is split in two f16 terms, x = hi + lo, cut off, each product exact
+// in the instruction's float32 sum. So a term loses less than 2^-21 of itself (one f16 term would lose 2^-10 of it) or,
+// where its second part is subnormal, 2^-24 at the scale it is brought to: 2^-38 of the largest value of its query row,
+// 2^-36 of the row's largest weight (see Rows).
 //
 // mfma_f32_16x16x32_f16: lane l holds row (A) or column (B) l & 15 and the eight k = 8 (l >> 4) + e; of the result it
 // holds column l & 15, rows 4 (l >> 4) + i. Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a
@@ -85,8 +87,9 @@ __device__ __forceinline__ KvHead kv_head(const void* cache, int kh, int nkvh, i
 
 // ---------------------------------------------------------------- queries
 // LDS image of 16 query rows: [hi, lo][b = 32-dim block][lane] of 16 bytes, and per row the factor that takes a score from
-// the operands' units to log2 units. A row is scaled by the power of two that brings its largest value into [1, 2) before
-// the split, so neither very large nor very small queries leave f16's range.
+// the operands' units to log2 units. A row is scaled by the power of two that brings its largest value into [2^14, 2^15)
+// before the split: neither very large nor very small queries leave f16's range, and its small values, which large ones
+// of K may meet, have all of it below them.
 struct QTile {
   alignas(16) uint32_t v[2][8][64][4];
   float c[16];
@@ -122,8 +125,8 @@ __device__ __forceinline__ void load_queries(QTile* im, float mult, F row_ptr) {
       a = __builtin_fmaxf(a, lane_xor<8>(a));
       a = __builtin_fmaxf(a, lane_xor<16>(a));
       a = __builtin_fmaxf(a, lane_xor32(a));
-      int e = (int)((__builtin_bit_cast(uint32_t, a) >> 23) & 255) - 127;
-      e = e > 110 ? 110 : e < -110 ? -110 : e;  // a zero row keeps -110 (its scores are 0); inf and NaN stay what they are
+      int e = (int)((__builtin_bit_cast(uint32_t, a) >> 23) & 255) - 127 - 14;
+      e = e < -124 ? -124 : e;  // a zero row keeps that (its scores are 0); inf and NaN stay what they are
       const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < 4; i++) x[i] *= down;
