@@ -178,8 +178,8 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * The cache's values enter as they are, q and the softmax weights in two f16 terms each, the sums are float32. So, beside
  * float32's roundings, a value of q is off by less than 2^-21 of itself or, if that is more, 2^-38 of the largest of its
  * query row; a weight by less than 2^-21 of itself or 2^-36 of the largest of its query row (q8_0: a weight times its V
- * row's largest scale by less than 2^-33 of the largest weight times the largest scale seen). One value of the cache is
- * not taken as it is: a q8_0 V scale below 2^-14 of the power of two above its row's largest, to 2^-24 of that.
+ * row's largest scale by less than 2^-33 of the largest such product of its query row). One value of the cache is not
+ * taken as it is: a q8_0 V scale below 2^-14 of the power of two above its row's largest, to 2^-24 of that.
  * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
  * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
  * at the same time, need one each.

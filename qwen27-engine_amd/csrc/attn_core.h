@@ -192,9 +192,8 @@ __device__ __forceinline__ void put_scales(u2 s, uint8_t* scales) {
   p[96] = (uint16_t)(s.y >> 16);
 }
 // V's: brought to |d / f| <= 1 by the power of two f above the finite scales of the row's 8 blocks, f beside them (0 for
-// a row of zeros, which leaves the others' unit alone). f meets the weight in float32, so a row of large values does not
-// coarsen another, and d / f is a half without loss unless the block's scale is below 2^-14 of f; then it is off by less
-// than 2^-24 of f.
+// a row of zeros, which leaves the others' unit alone). f meets the weight in float32, and d / f is a half without loss
+// unless the block's scale is below 2^-14 of f; then it is off by less than 2^-24 of f.
 __device__ __forceinline__ float exp2i(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 __device__ __forceinline__ void put_value_scales(u2 s, uint8_t* scales, float* factors) {
   const int l = threadIdx.x & 63;
@@ -423,14 +422,16 @@ __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint6
 // State of 16 query rows in a wave: lane (n, g) holds of row n the reference M (the same in its four lanes), its own part
 // of the sum l and 64 outputs. Weights are p = 2^(s - M). M is not the maximum itself: it is only moved when p would leave
 // f16's range, that is when s - M > 15, and then to s - 12, so that the largest weights lie near 2^12, where two f16 terms
-// hold 22 bits, and small ones down to 2^-36 of them are still in range. q8: the outputs are in units of `unit`, the
-// largest row factor f of the V rows seen so far (a power of two), and a row's weight enters the product as p f / unit.
-// O, l and M of different waves and workgroups are joined by M alone.
+// hold 22 bits, and small ones down to 2^-36 of them are still in range. q8: a row's weight enters the product times its
+// V row's factor f, as p f / unit, and the outputs are in units of `unit`, a power of two that is moved as M is: up, when
+// the quotient would pass 2^15, and then to where the largest lies between 2^12 and 2^13. When M moves, the unit goes
+// down with the weights. So neither a row of large values and little weight, nor one whose weight has shrunk since,
+// coarsens the others. O, l and M of different waves and workgroups are joined by M alone.
 struct Rows {
   f4 o[16];
-  float m, l, c, unit;
+  float m, l, c, unit, want;  // want: the unit less what the weights lost since it was set
 };
-constexpr float kLeastUnit = 0x1p-24f;
+constexpr float kLeastUnit = 0x1p-80f;  // f and the quotient by it are in range
 
 template <bool Q8>
 __device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
@@ -439,42 +440,30 @@ __device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
   st.m = -3.0e38f;
   st.l = 0.0f;
   st.c = im.c[threadIdx.x & 15];
-  st.unit = kLeastUnit;
+  st.unit = st.want = kLeastUnit;
 }
 
-// Raises the unit to f where that is larger (powers of two: the quotient's exponent is their difference's).
-__device__ __forceinline__ void raise_unit(Rows& st, float f) {
-  f = __builtin_fmaxf(f, st.unit);
-  const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, f));
-  st.unit = f;
-#pragma unroll
-  for (int i = 0; i < 16; i++) st.o[i] *= a;
+__device__ __forceinline__ float power_below(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0x7f800000u);
 }
-// The row factors of a q8 tile (in LDS) and the unit. HIDDEN: a query row counts those of the rows that it sees, so that
-// what a hidden row holds cannot coarsen its outputs.
-template <bool HIDDEN>
+// Moves the unit where p f of a tile's row would pass 2^15 of it, or where M has moved; factors: the tile's f, in LDS. (The
+// outputs' second scaling stands here, beside the first one's: both in weights() spill 45 registers.)
 __device__ __forceinline__ void widen(Rows& st, const f4 (&p)[2], const float* factors) {
-  if constexpr (HIDDEN) {
-    float f = 0.0f;
+  float mx = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const f4 x = *(const f4*)(factors + 16 * u + 4 * ((threadIdx.x & 63) >> 4));
+  for (int u = 0; u < 2; u++) {
+    const f4 f = *(const f4*)(factors + 16 * u + 4 * ((threadIdx.x & 63) >> 4));
 #pragma unroll
-      for (int i = 0; i < 4; i++) f = p[u][i] != 0.0f ? __builtin_fmaxf(f, x[i]) : f;
-    }
-    if (__any(f > st.unit)) {
-      f = __builtin_fmaxf(f, lane_xor<16>(f));
-      raise_unit(st, __builtin_fmaxf(f, lane_xor32(f)));
-    }
-  } else {
-    float f = factors[threadIdx.x & 31];
-    if (__any(f > st.unit)) {
-      f = __builtin_fmaxf(f, lane_xor<1>(f));
-      f = __builtin_fmaxf(f, lane_xor<2>(f));
-      f = __builtin_fmaxf(f, lane_xor<7>(f));
-      f = __builtin_fmaxf(f, lane_xor<8>(f));
-      raise_unit(st, __builtin_fmaxf(f, lane_xor<16>(f)));
-    }
+    for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, p[u][i] * f[i]);
+  }
+  if (__any((mx > st.unit * 0x1p15f) | (st.want < st.unit))) {
+    mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
+    mx = __builtin_fmaxf(mx, lane_xor32(mx));
+    const float to = power_below(__builtin_fmaxf(__builtin_fmaxf(st.want, kLeastUnit), mx * 0x1p-12f));
+    const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, to));
+    st.unit = st.want = to;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= a;
   }
 }
 // What the outputs have to be multiplied by in the end: the unit, and 2^9 for codes8's 2^-9.
@@ -483,6 +472,7 @@ __device__ __forceinline__ float unit_of(const Rows& st) {
   return Q8 ? st.unit * 512.0f : 1.0f;
 }
 // p[u][i] from the scores (hidden ones are -inf), with the reference moved where it has to be.
+template <bool Q8>
 __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0][0], s[0][1]), __builtin_fmaxf(s[0][2], s[0][3])),
                              __builtin_fmaxf(__builtin_fmaxf(s[1][0], s[1][1]), __builtin_fmaxf(s[1][2], s[1][3])));
@@ -494,6 +484,7 @@ __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
     const float a = __builtin_amdgcn_exp2f(st.m - m1);
     st.m = m1;
     st.l *= a;
+    if (Q8) st.want *= a;
 #pragma unroll
     for (int i = 0; i < 16; i++) st.o[i] *= a;
   }

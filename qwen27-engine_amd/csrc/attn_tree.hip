@@ -124,10 +124,10 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   stage_keys(k, w);
   scores<1>(w, q.im, s);
   hide<1>(s, vis, trees, j0);
-  weights(st, s[0]);
+  weights<true>(st, s[0]);
   __builtin_amdgcn_wave_barrier();
   stage_values(v, w);
-  widen<true>(st, s[0], w.vf);
+  widen(st, s[0], w.vf);
   accumulate<true>(st, s[0], w);
   __builtin_amdgcn_wave_barrier();
 }
@@ -142,7 +142,7 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   scores(w, q.r, s);
   load_rows<true>(v, vc, j0, left);
   hide<1>(s, vis, trees, j0);
-  weights(st, s[0]);
+  weights<false>(st, s[0]);
   accumulate_tail(st, s[0], v, vc, j0, left, (float*)w.k);
 }
 
@@ -175,12 +175,12 @@ struct FullTiles<true> {
       if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
       loads_issued();
       scores<1>(w, q.im, s);
-      weights(st, s[0]);
+      weights<true>(st, s[0]);
       __builtin_amdgcn_wave_barrier();
       stage_values(v, w);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
-      widen<false>(st, s[0], w.vf);
+      widen(st, s[0], w.vf);
       accumulate<false>(st, s[0], w);
       __builtin_amdgcn_wave_barrier();
     } while (j0 >= 0);
@@ -210,7 +210,7 @@ struct FullTiles<false> {
       keys_there<0>();
       if (j0 >= 0) request_keys<false>(w, kc, j0, 0);
       loads_issued();
-      weights(st, s[0]);
+      weights<false>(st, s[0]);
       accumulate(st, s[0], v);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
@@ -403,8 +403,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
       __builtin_amdgcn_s_setprio(1);  // products before the other wave's staging (32 tokens, 65536 q8_0 rows: 171 -> 162 us)
       scores<Q8>(buf[at], &q, s);
       if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
-      weights(st, s[0]);
-      if constexpr (Q8) widen<kPart>(st, s[0], buf[at].vf);
+      weights<Q8>(st, s[0]);
+      if constexpr (Q8) widen(st, s[0], buf[at].vf);
       accumulate<Q8, kPart>(st, s[0], buf[at]);
       if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
     }

@@ -1,5 +1,5 @@
 """Attention over the K/V cache on the GPU where it can go wrong and tests/test_gpu_attn.py does not look, against a plain
-64-bit form: query values far below their row's largest."""
+64-bit form: query values far below their row's largest, V rows of very different size."""
 import numpy as np
 import pytest
 
@@ -28,9 +28,16 @@ def score_bound(q, k, s, scale):
         + np.abs(s) * 2.0 ** -23
 
 
-def attend(q, k, v, vis, scale=SCALE):
+def attend(q, k, v, vis, q8, scale=SCALE):
     """o, lse and the bounds of their errors, as R.attend's, but with each row's weight off by its own score's error.
-    q [T][nqh][256]; k, v [nkvh][n_ctx][256]; vis [T][n_ctx]."""
+    q [T][nqh][256]; k, v [nkvh][n_ctx][256]; vis [T][n_ctx].
+
+    lost: what the weights' two f16 terms lose where the second is subnormal. A weight is cut off to 2^-24 where the largest
+    of its query row lies at 2^12 or above, so it loses 2^-36 of the largest, and at most itself. q8_0: it is cut off as p f
+    in units of which the largest p f holds 2^12 or more, f the power of two above the row's largest scale m (f <= 2 m);
+    the products with the scales round to halves three times more, 2^-25 each where they are subnormal. So a row adds less
+    than 2.5 * 2^-24 * 2^-12 * 127 * 2 max(p m) < 2^-33 * 127 max(p m) wrongly, and at most 127 p m; 127 m is taken as
+    the largest value of the row, which is so where a code of that block is 127 (as here)."""
     T, nqh, _ = q.shape
     nkvh, g, n = k.shape[0], nqh // k.shape[0], vis.shape[1]
     q = q.astype(np.float64).reshape(T, nkvh, g, 256)
@@ -50,7 +57,12 @@ def attend(q, k, v, vis, scale=SCALE):
         common = 2 * np.sqrt(n) * 2.0 ** -23 + 2.0 ** -22
         off, mean = p * e, p @ np.abs(v[kh])
         o[:, kh] = p @ v[kh]
-        bo[:, kh] = off @ np.abs(v[kh]) + (off.sum(-1, keepdims=True) + common) * mean
+        if q8:
+            most = p * np.abs(v[kh]).max(1)
+            lost = np.minimum(most, 2.0 ** -33 * most.max(-1, keepdims=True)).sum(-1, keepdims=True)
+        else:
+            lost = np.minimum(p, 2.0 ** -36 * p.max(-1, keepdims=True)) @ np.abs(v[kh])
+        bo[:, kh] = off @ np.abs(v[kh]) + (off.sum(-1, keepdims=True) + common) * mean + lost
         bl[:, kh] = off.sum(-1) + common + np.abs(np.where(none[:, None], 0, lse[:, kh])) * 2.0 ** -22
     shape = (T, nqh)
     return o.reshape(*shape, 256), lse.reshape(shape), bo.reshape(*shape, 256), bl.reshape(shape)
@@ -75,7 +87,7 @@ def test_query_values_far_below_the_largest(G, T, q8):  # noqa: F811
     bo_, bl_ = G.blocks(dq, dk, dv, pos, G.up(idx), T, 3, nqh, nkvh, n_ctx, q8)
     vis = R.visible(T, pos0, n_ctx, None)
     k, v = R.values(k, nkvh, n_ctx, q8), R.values(v, nkvh, n_ctx, q8)
-    eo, el, bo, bl = attend(q, k, v, vis)
+    eo, el, bo, bl = attend(q, k, v, vis, q8)
     lse = G.down(lse)
     near(G.down(o), eo, bo, "o")
     near(lse, el, bl, "lse")
@@ -90,3 +102,55 @@ def test_query_values_far_below_the_largest(G, T, q8):  # noqa: F811
             want[kh] += p
             off[kh] += p * (score_bound(qd, k[kh], s, SCALE) + (np.abs(s) + abs(lse[t, h])) * 2.0 ** -22 + 2.0 ** -22)
     near(G.down(acc), want, off + want * 2.0 ** -22, "acc")
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("where", ["full", "drafted"])
+@pytest.mark.parametrize("T,nqh", [(1, 24), (4, 24), (8, 24), (12, 24), (20, 24)])
+def test_a_large_row_of_little_weight(G, T, nqh, where, q8):  # noqa: F811
+    """Every token sees one V row 2^26 (f16: 2^20) times as large as the others with 2^-69 of their weight: it gives next
+    to nothing, and the others keep their precision. full: in a tile that all tokens see whole; drafted: the first drafted
+    row, in the tile of the draft."""
+    r = np.random.default_rng(17)
+    pos0, n_ctx, nkvh = 70, 100, 4
+    j = 3 if where == "full" else pos0
+    k, v = r.standard_normal((nkvh, n_ctx, 256)), r.standard_normal((nkvh, n_ctx, 256)) * 2.0 ** -9
+    k[:, :, :32] = 0
+    k[:, j, 0] = -16  # times 48 and the scale: a score of -48
+    v[:, j] *= 2.0 ** (26 if q8 else 20)
+    k, v = cache(k, q8), cache(v, q8)
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    q[:, :, 0] = 48
+    vis = R.visible(T, pos0, n_ctx, None)
+    k64, v64 = R.values(k, nkvh, n_ctx, q8), R.values(v, nkvh, n_ctx, q8)
+    assert np.isfinite(v64).all()
+    eo, el, bo, bl = attend(q, k64, v64, vis, q8)
+    dq, dk, dv, pos = G.up(q), G.up(k), G.up(v), G.i32(pos0)
+    o, lse = G.tree(dq, dk, dv, pos, None, T, nqh, nkvh, n_ctx, q8)
+    near(G.down(o), eo, bo, "o")
+    near(G.down(lse), el, bl, "lse")
+    o, lse = G.blocks(dq, dk, dv, pos, G.up(np.tile(np.arange(2, dtype=np.int32), (T, nkvh, 1))), T, 2, nqh, nkvh, n_ctx, q8)
+    near(G.down(o), eo, bo, "o of blocks")
+    near(G.down(lse), el, bl, "lse of blocks")
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("T,g,nkvh,n", [(1, 6, 4, 20000), (4, 6, 64, 2000), (40, 2, 64, 1500)])
+def test_a_large_row_whose_weight_shrinks(G, T, g, nkvh, n, q8):  # noqa: F811
+    """The scores rise by 60 over the rows that a wave walks, and the first rows' values are the largest: whatever unit they
+    were summed in, the last rows, which have all the weight, keep their precision."""
+    r = np.random.default_rng(29)
+    n_ctx, nqh = n + T, nkvh * g
+    k, v = (r.standard_normal((nkvh, n_ctx, 256), dtype=np.float32) for _ in range(2))
+    k[:, :, :32] = 0
+    step = 20000 / 256 if T == 1 else n / 4  # rows of a split at the most: the scores rise within each
+    at = np.arange(n_ctx) % step / step
+    k[:, :, 0] = 16 * at
+    v *= (2.0 ** np.where(at < 0.1, 12 if q8 else 8, -10))[:, None].astype(np.float32)
+    k, v = cache(k, q8), cache(v, q8)
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    q[:, :, 0] = 60
+    eo, el, bo, bl = attend(q, R.values(k, nkvh, n_ctx, q8), R.values(v, nkvh, n_ctx, q8), R.visible(T, n, n_ctx, None), q8)
+    o, lse = G.tree(G.up(q), G.up(k), G.up(v), G.i32(n), None, T, nqh, nkvh, n_ctx, q8)
+    near(G.down(o), eo, bo, "o")
+    near(G.down(lse), el, bl, "lse")
