@@ -446,26 +446,6 @@ __device__ __forceinline__ void rows_init(Rows& st, const QTile& im) {
 __device__ __forceinline__ float power_below(float x) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0x7f800000u);
 }
-// Moves the unit where p f of a tile's row would pass 2^15 of it, or where M has moved; factors: the tile's f, in LDS. (The
-// outputs' second scaling stands here, beside the first one's: both in weights() spill 45 registers.)
-__device__ __forceinline__ void widen(Rows& st, const f4 (&p)[2], const float* factors) {
-  float mx = 0.0f;
-#pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const f4 f = *(const f4*)(factors + 16 * u + 4 * ((threadIdx.x & 63) >> 4));
-#pragma unroll
-    for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, p[u][i] * f[i]);
-  }
-  if (__any((mx > st.unit * 0x1p15f) | (st.want < st.unit))) {
-    mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
-    mx = __builtin_fmaxf(mx, lane_xor32(mx));
-    const float to = power_below(__builtin_fmaxf(__builtin_fmaxf(st.want, kLeastUnit), mx * 0x1p-12f));
-    const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, to));
-    st.unit = st.want = to;
-#pragma unroll
-    for (int i = 0; i < 16; i++) st.o[i] *= a;
-  }
-}
 // What the outputs have to be multiplied by in the end: the unit, and 2^9 for codes8's 2^-9.
 template <bool Q8>
 __device__ __forceinline__ float unit_of(const Rows& st) {
@@ -509,13 +489,30 @@ __device__ __forceinline__ void split(const f4 (&p)[2], u4& hi, u4& lo) {
   }
 }
 
-// q8: the same of p f / unit, pairs of rows (0, 2), (1, 3) of u = 0, then of u = 1, as codes8 orders them.
-__device__ __forceinline__ void split8(const f4 (&p)[2], const float* factors, float unit, u4& hi, u4& lo) {
-  const int g = (threadIdx.x & 63) >> 4;
-  const float inv = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, unit));  // 1 / unit
+// q8: the same of p f / unit, pairs of rows (0, 2), (1, 3) of u = 0, then of u = 1, as codes8 orders them; factors: the tile's
+// f, in LDS. The unit is moved where p f would pass 2^15 of it, or where M has moved. (The outputs' second scaling stands
+// here, beside the first one's: both in weights() spill 45 registers.)
+__device__ __forceinline__ void split8(Rows& st, const f4 (&p)[2], const float* factors, u4& hi, u4& lo) {
   f4 w[2];
+  float mx = 0.0f;
 #pragma unroll
-  for (int u = 0; u < 2; u++) w[u] = p[u] * (*(const f4*)(factors + 16 * u + 4 * g) * inv);
+  for (int u = 0; u < 2; u++) {
+    w[u] = p[u] * *(const f4*)(factors + 16 * u + 4 * ((threadIdx.x & 63) >> 4));
+#pragma unroll
+    for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, w[u][i]);
+  }
+  if (__any((mx > st.unit * 0x1p15f) | (st.want < st.unit))) {
+    mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
+    mx = __builtin_fmaxf(mx, lane_xor32(mx));
+    const float to = power_below(__builtin_fmaxf(__builtin_fmaxf(st.want, kLeastUnit), mx * 0x1p-12f));
+    const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, to));
+    st.unit = st.want = to;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= a;
+  }
+  const float inv = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, st.unit));  // 1 / unit
+#pragma unroll
+  for (int u = 0; u < 2; u++) w[u] *= inv;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const float w0 = w[e >> 1][e & 1], w1 = w[e >> 1][(e & 1) + 2];
@@ -555,7 +552,7 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
   u2 vs[2][2];
   h8 v[2][2];
   u4 ph, pl, hi[2], lo[2];
-  split8(p, w.vf, st.unit, ph, pl);
+  split8(st, p, w.vf, ph, pl);
   auto ask = [&](int b) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {

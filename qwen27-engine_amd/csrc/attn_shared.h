@@ -204,7 +204,7 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Sha
   u4 ph, pl, hi[2], lo[2];
   h8 v[2][2];
   u2 vs[2][2];
-  if constexpr (Q8) split8(p, t.vf, st.unit, ph, pl);
+  if constexpr (Q8) split8(st, p, t.vf, ph, pl);
   auto ask_v = [&](int b) {
 #pragma unroll
     for (int h = 0; h < 2; h++) v[b & 1][h] = *(const h8*)t.v[2 * b + h][16 * g + (m ^ (2 * b + h))];

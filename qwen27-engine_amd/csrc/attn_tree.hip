@@ -127,7 +127,6 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   weights<true>(st, s[0]);
   __builtin_amdgcn_wave_barrier();
   stage_values(v, w);
-  widen(st, s[0], w.vf);
   accumulate<true>(st, s[0], w);
   __builtin_amdgcn_wave_barrier();
 }
@@ -180,7 +179,6 @@ struct FullTiles<true> {
       stage_values(v, w);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
-      widen(st, s[0], w.vf);
       accumulate<false>(st, s[0], w);
       __builtin_amdgcn_wave_barrier();
     } while (j0 >= 0);
@@ -404,7 +402,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
       scores<Q8>(buf[at], &q, s);
       if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
       weights<Q8>(st, s[0]);
-      if constexpr (Q8) widen(st, s[0], buf[at].vf);
       accumulate<Q8, kPart>(st, s[0], buf[at]);
       if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
     }
