@@ -189,7 +189,9 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * and, usually, itself. tree NULL: a chain (bits 0 .. t); T = 1 with NULL is plain decoding.
  * o [T][nqh][256] = sum_j p_j v_j, p = softmax over the rows seen of scale * q . k_j; lse [T][nqh] (may be NULL) =
  * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. o may not overlap qn. nqh % nkvh == 0:
- * query head h reads kv head h / (nqh / nkvh). Values that are not finite reach the tokens that see their row. Rotary positions of a tree are given to attn_prep through rope3. */
+ * query head h reads kv head h / (nqh / nkvh). A value of V that is not finite makes its channel (a q8_0 scale: its
+ * 32 channels) infinite or NaN for the tokens that see its row, whatever the row's weight, and for no others; a NaN score
+ * makes the token's results NaN. Rotary positions of a tree are given to attn_prep through rope3. */
 size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx);
 int q27h_attn_tree(const float* qn, const void* kcache, const void* vcache, const int* pos0, const uint64_t* tree, int T,
                    float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws, size_t ws_bytes,

@@ -191,28 +191,26 @@ __device__ __forceinline__ void put_scales(u2 s, uint8_t* scales) {
   p[64] = (uint16_t)s.y;
   p[96] = (uint16_t)(s.y >> 16);
 }
-// V's: brought to |d / f| <= 1 by the power of two f above the finite scales of the row's 8 blocks, f beside them (0 for
-// a row of zeros, which leaves the others' unit alone). f meets the weight in float32, and d / f is a half without loss
+// V's: brought to |d / f| <= 1 by the power of two f above the finite scales of the row's 8 blocks, f beside them (0
+// where none is above 0: such a row adds zeros, or NaN, and leaves the unit alone). f meets the weight in float32, and d / f is a half without loss
 // unless the block's scale is below 2^-14 of f; then it is off by less than 2^-24 of f.
 __device__ __forceinline__ float exp2i(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 __device__ __forceinline__ void put_value_scales(u2 s, uint8_t* scales, float* factors) {
   const int l = threadIdx.x & 63;
-  float x[4], m = 0.0f, odd = 0.0f;
+  float x[4], m = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     x[i] = half_of(i < 2 ? s.x : s.y, i & 1);
     const bool finite = __builtin_fabsf(x[i]) < 65536.0f;
     m = finite ? __builtin_fmaxf(m, __builtin_fabsf(x[i])) : m;
-    odd = finite ? odd : 1.0f;
   }
   m = __builtin_fmaxf(m, lane_xor<1>(m));
-  odd = __builtin_fmaxf(odd, lane_xor<1>(odd));
   const uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;  // 2^(e - 127) <= m < 2^(e - 126); 0 for m = 0
   const float down = exp2i(253u - e);
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = e ? x[i] * down : x[i];  // m = 0: zeros, or values that are not finite
   put_scales((u2){pk_rtz(x[0], x[1]), pk_rtz(x[2], x[3])}, scales);
-  if (!(l & 1)) factors[l >> 1] = e ? exp2i(e + 1) : odd;
+  if (!(l & 1)) factors[l >> 1] = e ? exp2i(e + 1) : 0.0f;
 }
 __device__ __forceinline__ void stage_codes(const QRows& t, WaveLds& w) {
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
@@ -400,7 +398,10 @@ struct Vis {
   int n0;   // first drafted row (may lie outside the cache)
   int end;  // one past the last row that exists
 };
-template <int RT>
+// A hidden row's score becomes AS.
+constexpr uint32_t kMinusInf = 0xff800000u;
+constexpr uint32_t kHidden = 0xffffffffu;  // a NaN that no product gives: told from every score, -inf and NaN among them
+template <int RT, uint32_t AS>
 __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint64_t (&tree)[RT], int j0) {
   const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
@@ -413,7 +414,7 @@ __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint6
       for (int rt = 0; rt < RT; rt++) {
         // no branches: eight of them a lane cost more than the shift, and hipcc has lost one's value
         const bool seen = (j < vis.n) | ((j < vis.end) & (d < 64u) & (bool)((tree[rt] >> (d & 63u)) & 1));
-        s[rt][u][i] = seen ? s[rt][u][i] : -__builtin_huge_valf();
+        s[rt][u][i] = seen ? s[rt][u][i] : __builtin_bit_cast(float, AS);
       }
     }
 }
@@ -451,8 +452,9 @@ template <bool Q8>
 __device__ __forceinline__ float unit_of(const Rows& st) {
   return Q8 ? st.unit * 512.0f : 1.0f;
 }
-// p[u][i] from the scores (hidden ones are -inf), with the reference moved where it has to be.
-template <bool Q8>
+// p[u][i] from the scores, with the reference moved where it has to be (maxima pass over NaN). HIDDEN: a hidden row's (kHidden)
+// weight is -0, so that the sign tells it from a row that is seen with a weight of 0, whose infinities make NaN.
+template <bool Q8, bool HIDDEN>
 __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0][0], s[0][1]), __builtin_fmaxf(s[0][2], s[0][3])),
                              __builtin_fmaxf(__builtin_fmaxf(s[1][0], s[1][1]), __builtin_fmaxf(s[1][2], s[1][3])));
@@ -473,7 +475,8 @@ __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   for (int u = 0; u < 2; u++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], st.c, -st.m));
+      const float x = s[u][i], p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, st.c, -st.m));
+      s[u][i] = HIDDEN && __builtin_bit_cast(uint32_t, x) == kHidden ? -0.0f : p;
       sum += s[u][i];
     }
   st.l += sum;
@@ -521,15 +524,14 @@ __device__ __forceinline__ void split8(Rows& st, const f4 (&p)[2], const float* 
   }
 }
 // Times the stored scales d <= 1 of a block of V: hi' = hi d, rounded; the fma gives what that lost, exactly (11 by 11 bits
-// leave at most 11 below the first 11), and lo' = lo d + that. HIDDEN: a row with weight 0 is left out whatever its scale
-// is (0 times infinity is no part of the sum).
+// leave at most 11 below the first 11), and lo' = lo d + that. HIDDEN: a hidden row (weight -0) is left out whatever its
+// scale is (0 times infinity is no part of the sum).
 template <bool HIDDEN>
 __device__ __forceinline__ void weigh(const u4& ph, const u4& pl, const u2 (&vs)[2], u4& hi, u4& lo) {
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     uint32_t x = vs[e >> 1][e & 1];
-    const uint32_t any = ph[e] | pl[e];
-    if (HIDDEN) x &= (any & 0xffffu ? 0xffffu : 0u) | (any >> 16 ? 0xffff0000u : 0u);
+    if (HIDDEN) x &= ~(((ph[e] >> 15) & 0x10001u) * 0xffffu);
     const h2 d = as_h2(x), p = as_h2(ph[e]);
     const h2 h = p * d;
     const h2 lost = __builtin_elementwise_fma(p, d, -h);
@@ -539,8 +541,7 @@ __device__ __forceinline__ void weigh(const u4& ph, const u4& pl, const u2 (&vs)
 }
 
 // O += P V. Output o[i][j]: q8: dim 16 i + 4 g + j; f16: dim 128 (i >> 3) + 8 (4 g + j) + (i & 7).
-// q8: `w` holds the staged codes and scales. TAIL: a hidden row's scale may be anything (a weight of 0 times an infinite
-// scale is no part of the sum).
+// q8: `w` holds the staged codes and scales. TAIL: some rows are hidden, see weigh().
 template <bool TAIL>
 __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const WaveLds& w) {
   const int l = threadIdx.x & 63, j = l & 15, g = l >> 4;
@@ -631,7 +632,7 @@ __device__ __forceinline__ void accumulate_tail(Rows& st, const f4 (&p)[2], HVal
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float f = half_of(x[e >> 1], e & 1);
-        const bool add = (__builtin_bit_cast(uint32_t, f) & 0x7f800000u) == 0x7f800000u && wt != 0.0f;
+        const bool add = (__builtin_bit_cast(uint32_t, f) & 0x7f800000u) == 0x7f800000u && !__builtin_signbit(wt);
         st.o[8 * (q >> 2) + e][q & 3] += add ? wt * f : 0.0f;
       }
     }

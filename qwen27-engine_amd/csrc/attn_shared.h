@@ -259,7 +259,7 @@ __device__ __forceinline__ void add_odd(Rows& st, const f4 (&p)[2], const KvHead
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             const float f = half_of(x[c >> 1], c & 1);
-            const bool add = (__builtin_bit_cast(uint32_t, f) & 0x7f800000u) == 0x7f800000u && wt != 0.0f && j < left;
+            const bool add = (__builtin_bit_cast(uint32_t, f) & 0x7f800000u) == 0x7f800000u && !__builtin_signbit(wt) && j < left;
             const float y = add ? wt * f : 0.0f;
 #pragma unroll
             for (int k = 0; k < 16; k += 4) st.o[k + q][c] += k == i ? y : 0.0f;

@@ -123,8 +123,8 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   load_rows<true>(v, vc, j0, left);
   stage_keys(k, w);
   scores<1>(w, q.im, s);
-  hide<1>(s, vis, trees, j0);
-  weights<true>(st, s[0]);
+  hide<1, kHidden>(s, vis, trees, j0);
+  weights<true, true>(st, s[0]);
   __builtin_amdgcn_wave_barrier();
   stage_values(v, w);
   accumulate<true>(st, s[0], w);
@@ -140,8 +140,8 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   keys_there<0>();
   scores(w, q.r, s);
   load_rows<true>(v, vc, j0, left);
-  hide<1>(s, vis, trees, j0);
-  weights<false>(st, s[0]);
+  hide<1, kHidden>(s, vis, trees, j0);
+  weights<false, true>(st, s[0]);
   accumulate_tail(st, s[0], v, vc, j0, left, (float*)w.k);
 }
 
@@ -174,7 +174,7 @@ struct FullTiles<true> {
       if (j0 >= 0) load_rows<false>(k, kc, j0, 0);
       loads_issued();
       scores<1>(w, q.im, s);
-      weights<true>(st, s[0]);
+      weights<true, false>(st, s[0]);
       __builtin_amdgcn_wave_barrier();
       stage_values(v, w);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
@@ -208,7 +208,7 @@ struct FullTiles<false> {
       keys_there<0>();
       if (j0 >= 0) request_keys<false>(w, kc, j0, 0);
       loads_issued();
-      weights<false>(st, s[0]);
+      weights<false, false>(st, s[0]);
       accumulate(st, s[0], v);
       if (j0 >= 0) load_rows<false>(v, vc, j0, 0);
       loads_issued();
@@ -400,8 +400,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_wide_kernel(AttnArgs a) {
       f4 s[1][2];
       __builtin_amdgcn_s_setprio(1);  // products before the other wave's staging (32 tokens, 65536 q8_0 rows: 171 -> 162 us)
       scores<Q8>(buf[at], &q, s);
-      if (kPart) hide<1>(s, vis, tree, t * kTileKeys);
-      weights<Q8>(st, s[0]);
+      if (kPart) hide<1, kHidden>(s, vis, tree, t * kTileKeys);
+      weights<Q8, kPart>(st, s[0]);
       accumulate<Q8, kPart>(st, s[0], buf[at]);
       if (!Q8 && kPart && s_odd[at]) add_odd(st, s[0], vc, t * kTileKeys, left_of(t));
     }
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs
         keys_there<0>();
         scores(sh.w[w], q, s);
       }
-      if (!full) hide<RT>(s, vis, tree, j0);
+      if (!full) hide<RT, kMinusInf>(s, vis, tree, j0);
       float sum[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_weights_wide_kernel(Weight
           uint64_t bits[kN];
 #pragma unroll
           for (int rt = 0; rt < kN; rt++) bits[rt] = is_row(rt) ? tree_of(a.tree, row(rt) / group, a.T) : 0ull;
-          hide<kN>(s, vis, bits, t * kTileKeys);
+          hide<kN, kMinusInf>(s, vis, bits, t * kTileKeys);
         }
 #pragma unroll
         for (int rt = 0; rt < kN; rt++)

@@ -1,5 +1,5 @@
 """Attention over the K/V cache on the GPU where it can go wrong and tests/test_gpu_attn.py does not look, against a plain
-64-bit form: query values far below their row's largest, V rows of very different size."""
+64-bit form: query values far below their row's largest, V rows of very different size, values that are not finite."""
 import numpy as np
 import pytest
 
@@ -154,3 +154,43 @@ def test_a_large_row_whose_weight_shrinks(G, T, g, nkvh, n, q8):  # noqa: F811
     o, lse = G.tree(G.up(q), G.up(k), G.up(v), G.i32(n), None, T, nqh, nkvh, n_ctx, q8)
     near(G.down(o), eo, bo, "o")
     near(G.down(lse), el, bl, "lse")
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("score", [-48, -192])
+@pytest.mark.parametrize("where", ["full", "beside the draft", "drafted"])
+@pytest.mark.parametrize("T", [1, 4, 8, 12])
+def test_values_that_are_not_finite_reach_all_that_see_them(G, T, where, score, bad, q8):  # noqa: F811
+    """However little the row's weight (2^-69; none in float32), and wherever the row lies: in a tile that all see whole, in
+    the tile of the draft before it, or drafted and seen by every other token."""
+    r = np.random.default_rng(31)
+    pos0, n_ctx, nqh, nkvh = 70, 100, 24, 4
+    j = {"full": 3, "beside the draft": pos0 - 1, "drafted": pos0}[where]
+    k, v = r.standard_normal((nkvh, n_ctx, 256)), r.standard_normal((nkvh, n_ctx, 256))
+    k[:, :, :32] = 0
+    k[:, j, 0] = -16
+    k, v = cache(k, q8), cache(v, q8)
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    q[:, :, 0] = -score
+    tree = np.array([1 << t | (t % 2 == 0) for t in range(T)], np.uint64)
+    vis = R.visible(T, pos0, n_ctx, tree)
+    eo, el, bo, bl = attend(q, R.values(k, nkvh, n_ctx, q8), R.values(v, nkvh, n_ctx, q8), vis, q8)
+    if q8:
+        R.split_q8(v, nkvh, n_ctx)[1][:, j, 3] = bad
+    else:
+        v.view(np.float16).reshape(nkvh, n_ctx, 256)[:, j, 100] = bad
+    dims = np.zeros(256, bool)
+    dims[slice(96, 128) if q8 else 100] = True
+    dq, dk, dv, pos = G.up(q), G.up(k), G.up(v), G.i32(pos0)
+    o, lse = (G.down(x) for x in G.tree(dq, dk, dv, pos, G.u64(tree), T, nqh, nkvh, n_ctx, q8))
+    near(lse, el, bl, "lse")
+    hit = vis[:, j]
+    assert not np.isfinite(o[hit][..., dims]).any()
+    near(o[..., ~dims], eo[..., ~dims], bo[..., ~dims], "o of the other channels")
+    # a channel whose own row is left out differs by next to nothing from one that holds a finite value there
+    near(o[~hit], eo[~hit], bo[~hit], "o of the tokens that do not see the row")
+    if where != "drafted":
+        idx = G.up(np.tile(np.arange(2, dtype=np.int32), (T, nkvh, 1)))
+        o = G.down(G.blocks(dq, dk, dv, pos, idx, T, 2, nqh, nkvh, n_ctx, q8)[0])
+        assert not np.isfinite(o[..., dims]).any() and np.isfinite(o[..., ~dims]).all()
