@@ -207,7 +207,7 @@ int q27h_attn_weights(const float* qn, const float* lse, const void* kcache, con
  * between, the keep - first - last of the largest acc (equal ones: the lower row; NaN below all); all where n <= keep.
  * Kept rows move, in order, to rows 0 .. of kout / vout / acc_out, whose context is n_ctx_out >= keep rows; rows behind
  * them are left as they were. The outputs are the inputs themselves (all three, n_ctx_out = n_ctx: in place) or overlap
- * none of them. kept [nkvh][keep] (may be NULL): the kept rows' numbers, -1 behind the last.
+ * none of them. kept [nkvh][keep] (may be NULL): the kept rows' numbers, -1 behind the last. kept and ws overlap nothing.
  * acc is only read between its ends: attn_weights starts the weights of rows written later. */
 size_t q27h_kv_evict_ws_bytes(int nkvh, int n_ctx, int keep, int q8, int in_place);
 int q27h_kv_evict(const void* kcache, const void* vcache, const float* acc, const int* pos0, int keep, int first, int last,

@@ -440,11 +440,13 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
   const size_t in = cache_bytes(nkvh, n_ctx, q8), out = cache_bytes(nkvh, n_ctx_out, q8);
   const size_t ain = (size_t)nkvh * n_ctx * 4, aout = (size_t)nkvh * n_ctx_out * 4;
   const bool in_place = kout == kcache && vout == vcache && acc_out == acc && n_ctx_out == n_ctx;
-  if (overlaps(kcache, in, vcache, in) || (!in_place && (overlaps(kcache, in, kout, out) || overlaps(kcache, in, vout, out) ||
-      overlaps(vcache, in, kout, out) || overlaps(vcache, in, vout, out) || overlaps(acc, ain, acc_out, aout) ||
-      overlaps(kout, out, vout, out))))
-    return fail(Q27H_ERR_ARG, "kv_evict: the outputs overlap the inputs (all of them in place, or none)");
-  if (ws_bytes < q27h_kv_evict_ws_bytes(nkvh, n_ctx, keep, q8, in_place)) return fail(Q27H_ERR_ARG, "kv_evict: workspace too small");
+  const size_t need = q27h_kv_evict_ws_bytes(nkvh, n_ctx, keep, q8, in_place);
+  const Bytes rows_kept = {kept, (size_t)nkvh * keep * 4}, work = {ws, need}, pos = {pos0, 4};
+  if (overlaps(kcache, in, vcache, in) ||
+      (in_place ? outputs_overlap({{kout, out}, {vout, out}, {acc_out, aout}, rows_kept, work}, {pos})
+                : outputs_overlap({{kout, out}, {vout, out}, {acc_out, aout}, rows_kept, work}, {{kcache, in}, {vcache, in}, {acc, ain}, pos})))
+    return fail(Q27H_ERR_ARG, "kv_evict: the outputs overlap each other or the inputs (all of them in place, or none)");
+  if (ws_bytes < need) return fail(Q27H_ERR_ARG, "kv_evict: workspace too small");
   EvictArgs a = {};
   uint8_t* p = (uint8_t*)ws;
   auto take = [&](size_t n) {

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/q27h.h"
@@ -20,6 +21,22 @@ inline hipStream_t stream_of(q27h_stream_t s) { return (hipStream_t)s; }
 inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return na && nb && x < y + nb && y < x + na;
+}
+
+struct Bytes {
+  const void* p;  // nullptr: none
+  size_t n;
+};
+// True when one of the outputs shares a byte with an input or with another output.
+inline bool outputs_overlap(std::initializer_list<Bytes> out, std::initializer_list<Bytes> in) {
+  for (const Bytes* a = out.begin(); a != out.end(); a++) {
+    if (!a->p) continue;
+    for (const Bytes* b = out.begin(); b != a; b++)
+      if (b->p && overlaps(a->p, a->n, b->p, b->n)) return true;
+    for (const Bytes& b : in)
+      if (b.p && overlaps(a->p, a->n, b.p, b.n)) return true;
+  }
+  return false;
 }
 
 // gdn_rec.hip: whether the process asked for the checker's bits on the GDN prefill path (q27h_gdn_prefill_exact).
