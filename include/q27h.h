@@ -182,13 +182,14 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * taken as it is: a q8_0 V scale below 2^-14 of the power of two above its row's largest, to 2^-24 of that.
  * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
  * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
- * at the same time, need one each.
+ * at the same time, need one each. What a call writes (results, lists, workspace) may share no memory with its other
+ * arguments, but where kv_evict works in place.
  *
  * attn_tree: attention of T <= 64 drafted tokens whose K / V attn_prep wrote to rows *pos0 + t. Token t sees every row
  * before *pos0 and row *pos0 + u where bit u of tree[t] (device, 64-bit; bits >= T are ignored) is set: its ancestors
  * and, usually, itself. tree NULL: a chain (bits 0 .. t); T = 1 with NULL is plain decoding.
  * o [T][nqh][256] = sum_j p_j v_j, p = softmax over the rows seen of scale * q . k_j; lse [T][nqh] (may be NULL) =
- * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. o may not overlap qn. nqh % nkvh == 0:
+ * ln sum_j exp(scale * q . k_j). A token that sees no row gets zeros and -inf. nqh % nkvh == 0:
  * query head h reads kv head h / (nqh / nkvh). A value of V that is not finite makes its channel (a q8_0 scale: its
  * 32 channels) infinite or NaN for the tokens that see its row, whatever the row's weight, and for no others; a NaN score
  * makes the token's results NaN. Rotary positions of a tree are given to attn_prep through rope3. */

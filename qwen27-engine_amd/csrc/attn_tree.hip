@@ -871,6 +871,10 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
   if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_tree: o overlaps qn");
   const size_t need = q27h_attn_tree_ws_bytes(T, nqh, nkvh, n_ctx);
   if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_tree: workspace too small");
+  const size_t qb = (size_t)T * nqh * kHD * 4, cb = q27h_kv_cache_bytes(nkvh, n_ctx, q8);
+  if (outputs_overlap({{o, qb}, {lse, (size_t)T * nqh * 4}, {ws, need}},
+                      {{qn, qb}, {kcache, cb}, {vcache, cb}, {pos0, 4}, {tree, (size_t)T * 8}}))
+    return fail(Q27H_ERR_ARG, "attn_tree: o, lse or ws overlaps another argument");
   AttnArgs a = {};
   a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.tree = tree, a.o = o, a.lse = lse;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
@@ -898,6 +902,10 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   if (T == 0) return Q27H_OK;
   if (!qn || !lse || !kcache || !pos0 || !acc) return fail(Q27H_ERR_ARG, "attn_weights: null pointer");
   if (!aligned16(qn) || !aligned16(kcache)) return fail(Q27H_ERR_ARG, "attn_weights: tensors need 16-byte alignment");
+  const size_t qb = (size_t)T * nqh * kHD * 4, cb = q27h_kv_cache_bytes(nkvh, n_ctx, q8);
+  if (outputs_overlap({{acc, (size_t)nkvh * n_ctx * 4}},
+                      {{qn, qb}, {lse, (size_t)T * nqh * 4}, {kcache, cb}, {pos0, 4}, {tree, (size_t)T * 8}, {rows, 8}}))
+    return fail(Q27H_ERR_ARG, "attn_weights: acc overlaps another argument");
   WeightArgs a = {};
   a.qn = qn, a.lse = lse, a.kcache = kcache, a.pos0 = pos0, a.tree = tree, a.rows = rows, a.acc = acc;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.scale = scale;
@@ -946,6 +954,10 @@ extern "C" int q27h_attn_blocks(const float* qn, const void* kcache, const void*
   if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_blocks: o overlaps qn");
   const size_t need = q27h_attn_blocks_ws_bytes(T, nqh, nkvh, nsel);
   if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_blocks: workspace too small");
+  const size_t qb = (size_t)T * nqh * kHD * 4, cb = q27h_kv_cache_bytes(nkvh, n_ctx, q8);
+  if (outputs_overlap({{o, qb}, {lse, (size_t)T * nqh * 4}, {ws, need}},
+                      {{qn, qb}, {kcache, cb}, {vcache, cb}, {pos0, 4}, {idx, (size_t)T * nkvh * nsel * 4}}))
+    return fail(Q27H_ERR_ARG, "attn_blocks: o, lse or ws overlaps another argument");
   AttnArgs a = {};
   a.qn = qn, a.kcache = kcache, a.vcache = vcache, a.pos0 = pos0, a.idx = idx, a.o = o, a.lse = lse;
   a.T = T, a.nqh = nqh, a.nkvh = nkvh, a.n_ctx = n_ctx, a.nsel = nsel, a.scale = scale;

@@ -490,6 +490,7 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
 extern "C" int q27h_kv_evict_pos(int* pos0, int* rdelta, int keep, q27h_stream_t s) {
   if (keep <= 0) return fail(Q27H_ERR_SHAPE, "kv_evict_pos: keep >= 1");
   if (!pos0) return fail(Q27H_ERR_ARG, "kv_evict_pos: null pointer");
+  if (outputs_overlap({{pos0, 4}, {rdelta, 4}}, {})) return fail(Q27H_ERR_ARG, "kv_evict_pos: pos0 and rdelta overlap");
   hipLaunchKernelGGL(evict_pos_kernel, dim3(1), dim3(1), 0, stream_of(s), pos0, rdelta, keep);
   return check_launch("kv_evict_pos");
 }
@@ -514,7 +515,10 @@ extern "C" int q27h_kv_accept(void* const* caches, int n_caches, float* const* a
     for (int j = 0; j < i; j++) twice |= overlaps(accs[i], ab, accs[j], ab);
     for (int j = 0; j < n_caches; j++) twice |= overlaps(accs[i], ab, caches[j], cb);
   }
-  if (twice) return fail(Q27H_ERR_ARG, "kv_accept: caches or weight arrays overlap");
+  for (int i = 0; i < n_caches + n_accs; i++)
+    twice |= outputs_overlap({i < n_caches ? Bytes{caches[i], cb} : Bytes{accs[i - n_caches], ab}},
+                             {{pos0, 4}, {path, (size_t)T * 4}, {n_path, 4}});
+  if (twice) return fail(Q27H_ERR_ARG, "kv_accept: caches or weight arrays overlap each other or another argument");
   for (int c = 0, w = 0; c < n_caches || w < n_accs;) {
     AcceptArgs a = {};
     a.pos0 = pos0, a.path = path, a.n_path = n_path, a.T = T, a.nkvh = nkvh, a.n_ctx = n_ctx, a.q8 = q8;

@@ -43,3 +43,52 @@ def test_evict_in_place_refuses_lists_and_workspaces_over_the_caches(q27, out, o
 @pytest.mark.parametrize("at", [{"acc": G4 + 1024, "ao": G4 + 1024}, {"acc": 2 * G4, "ao": 2 * G4}])
 def test_evict_in_place_refuses_weights_in_a_cache(q27, at):
     refused(q27, evict, {"ko": G4, "vo": 2 * G4} | at)
+
+
+Q, LSE, TREE = 4 * 24 * 1024, 4 * 24 * 4, 4 * 8
+KB = 4 * 64 * 516
+TREE_ARGS = {"qn": Q, "k": KV, "v": KV, "pos0": 4, "tree": TREE, "o": Q, "lse": LSE, "ws": 1 << 30}
+WEIGHT_ARGS = {"qn": Q, "lse": LSE, "k": KV, "pos0": 4, "tree": TREE, "rows": 8, "acc": ACC}
+BLOCK_ARGS = {"qn": Q, "k": KV, "v": KV, "pos0": 4, "idx": 4 * 4 * 64 * 4, "o": Q, "lse": LSE, "ws": 1 << 30}
+BOUND_ARGS = {"k": KV, "pos0": 4, "kb": KB}
+SELECT_ARGS = {"qn": Q, "kb": KB, "pos0": 4, "idx": 4 * 4 * 64 * 4, "ws": 4 * 4 * 64 * 4}
+ACCEPT_ARGS = {"k": KV, "v": KV, "acc": ACC, "pos0": 4, "path": 4 * 4, "n_path": 4}
+
+
+def tree(ops, **a):
+    ops.attn_tree(a["qn"], a["k"], a["v"], a["pos0"], a["tree"], 4, 0.0625, 24, 4, 4096, True, a["o"], WS(1 << 30, a["ws"]), 0, a["lse"])
+
+
+def weights(ops, **a):
+    ops.attn_weights(a["qn"], a["lse"], a["k"], a["pos0"], a["tree"], 4, 0.0625, 24, 4, 4096, True, a["acc"], 0, a["rows"])
+
+
+def blocks(ops, **a):
+    ops.attn_blocks(a["qn"], a["k"], a["v"], a["pos0"], a["idx"], 4, 64, 0.0625, 24, 4, 4096, True, a["o"], WS(1 << 30, a["ws"]), 0, a["lse"])
+
+
+def bounds(ops, **a):
+    ops.kv_block_bounds(a["k"], a["pos0"], 4, 4, 4096, True, a["kb"], 0)
+
+
+def select(ops, **a):
+    ops.attn_select(a["qn"], a["kb"], a["pos0"], 4, 24, 4, 4096, 64, 1, 2, a["idx"], WS(1 << 30, a["ws"]), 0)
+
+
+def accept(ops, **a):
+    ops.kv_accept([a["k"], a["v"]], [a["acc"]], a["pos0"], a["path"], a["n_path"], 4, 4, 4096, True, 0)
+
+
+@pytest.mark.parametrize("call,args,out,other", [
+    (call, args, a, b) for call, args, outs in ((tree, TREE_ARGS, ("o", "lse", "ws")), (weights, WEIGHT_ARGS, ("acc",)),
+                                                (blocks, BLOCK_ARGS, ("o", "lse", "ws")), (bounds, BOUND_ARGS, ("kb",)),
+                                                (select, SELECT_ARGS, ("idx", "ws")), (accept, ACCEPT_ARGS, ("k", "v", "acc")))
+    for a, b in pairs(outs, args) if b != "ws"])
+def test_outputs_over_other_arguments_are_refused(q27, call, args, out, other):
+    at = {name: (i + 1) * G4 for i, name in enumerate(args)}
+    at[out] = at[other] + (args[other] - 1) // 16 * 16
+    refused(q27, lambda o: call(o, **at))
+
+
+def test_evict_pos_refuses_one_place_for_both(q27):
+    refused(q27, lambda o: o.kv_evict_pos(G4, G4, 4, 0))
