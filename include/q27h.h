@@ -183,7 +183,8 @@ int q27h_attn_prep(const float* qg, const float* k, const float* v, const float*
  * Workspaces (`ws`, 16-byte aligned, at least the bytes that the matching *_ws_bytes gives; NULL where that is 0) hold
  * nothing between calls. One workspace serves one call at a time: calls on different streams, and graphs that may run
  * at the same time, need one each. What a call writes (results, lists, workspace) may share no memory with its other
- * arguments, but where kv_evict works in place.
+ * arguments, but where kv_evict works in place. Caches, qn, o and block bounds need 16-byte alignment, arrays of 64-bit
+ * masks 8-byte, all others 4-byte.
  *
  * attn_tree: attention of T <= 64 drafted tokens whose K / V attn_prep wrote to rows *pos0 + t. Token t sees every row
  * before *pos0 and row *pos0 + u where bit u of tree[t] (device, 64-bit; bits >= T are ignored) is set: its ancestors

@@ -315,6 +315,7 @@ extern "C" int q27h_kv_block_bounds(const void* kcache, const int* pos0, int T, 
   if (T == 0) return Q27H_OK;
   if (!kcache || !pos0 || !kb) return fail(Q27H_ERR_ARG, "kv_block_bounds: null pointer");
   if (!aligned16(kcache) || !aligned16(kb)) return fail(Q27H_ERR_ARG, "kv_block_bounds: tensors need 16-byte alignment");
+  if (!aligned4(pos0)) return fail(Q27H_ERR_ARG, "kv_block_bounds: pos0 needs 4-byte alignment");
   if (outputs_overlap({{kb, q27h_kv_block_bytes(nkvh, n_ctx)}}, {{kcache, q27h_kv_cache_bytes(nkvh, n_ctx, q8)}, {pos0, 4}}))
     return fail(Q27H_ERR_ARG, "kv_block_bounds: kb overlaps another argument");
   const int nblk = blocks_of(n_ctx);
@@ -344,6 +345,7 @@ extern "C" int q27h_attn_select(const float* qn, const void* kb, const int* pos0
   if (T == 0) return Q27H_OK;
   if (!qn || !kb || !pos0 || !idx || !ws) return fail(Q27H_ERR_ARG, "attn_select: null pointer");
   if (!aligned16(qn) || !aligned16(kb) || !aligned4(ws)) return fail(Q27H_ERR_ARG, "attn_select: tensors need 16-byte alignment");
+  if (!aligned4(idx) || !aligned4(pos0)) return fail(Q27H_ERR_ARG, "attn_select: idx and pos0 need 4-byte alignment");
   const size_t need = q27h_attn_select_ws_bytes(T, nkvh, n_ctx);
   if (ws_bytes < need) return fail(Q27H_ERR_ARG, "attn_select: workspace too small");
   if (outputs_overlap({{idx, (size_t)T * nkvh * nsel * 4}, {ws, need}},

@@ -868,6 +868,8 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
   if (!qn || !kcache || !vcache || !pos0 || !o) return fail(Q27H_ERR_ARG, "attn_tree: null pointer");
   if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
     return fail(Q27H_ERR_ARG, "attn_tree: tensors need 16-byte alignment");
+  if (!aligned8(tree) || !aligned4(lse) || !aligned4(pos0))
+    return fail(Q27H_ERR_ARG, "attn_tree: tree needs 8-byte alignment, lse and pos0 4-byte");
   if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_tree: o overlaps qn");
   const size_t need = q27h_attn_tree_ws_bytes(T, nqh, nkvh, n_ctx);
   if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_tree: workspace too small");
@@ -902,6 +904,8 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   if (T == 0) return Q27H_OK;
   if (!qn || !lse || !kcache || !pos0 || !acc) return fail(Q27H_ERR_ARG, "attn_weights: null pointer");
   if (!aligned16(qn) || !aligned16(kcache)) return fail(Q27H_ERR_ARG, "attn_weights: tensors need 16-byte alignment");
+  if (!aligned8(tree) || !aligned8(rows) || !aligned4(lse) || !aligned4(acc) || !aligned4(pos0))
+    return fail(Q27H_ERR_ARG, "attn_weights: tree and rows need 8-byte alignment, lse, acc and pos0 4-byte");
   const size_t qb = (size_t)T * nqh * kHD * 4, cb = q27h_kv_cache_bytes(nkvh, n_ctx, q8);
   if (outputs_overlap({{acc, (size_t)nkvh * n_ctx * 4}},
                       {{qn, qb}, {lse, (size_t)T * nqh * 4}, {kcache, cb}, {pos0, 4}, {tree, (size_t)T * 8}, {rows, 8}}))
@@ -951,6 +955,8 @@ extern "C" int q27h_attn_blocks(const float* qn, const void* kcache, const void*
   if (!qn || !kcache || !vcache || !pos0 || !idx || !o) return fail(Q27H_ERR_ARG, "attn_blocks: null pointer");
   if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
     return fail(Q27H_ERR_ARG, "attn_blocks: tensors need 16-byte alignment");
+  if (!aligned4(idx) || !aligned4(lse) || !aligned4(pos0))
+    return fail(Q27H_ERR_ARG, "attn_blocks: idx, lse and pos0 need 4-byte alignment");
   if (overlaps(qn, (size_t)T * nqh * kHD * 4, o, (size_t)T * nqh * kHD * 4)) return fail(Q27H_ERR_ARG, "attn_blocks: o overlaps qn");
   const size_t need = q27h_attn_blocks_ws_bytes(T, nqh, nkvh, nsel);
   if (ws_bytes < need || (need && !ws)) return fail(Q27H_ERR_ARG, "attn_blocks: workspace too small");

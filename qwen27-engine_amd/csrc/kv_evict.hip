@@ -437,6 +437,8 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
     return fail(Q27H_ERR_ARG, "kv_evict: null pointer");
   if (!aligned16(kcache) || !aligned16(vcache) || !aligned16(kout) || !aligned16(vout) || !aligned16(ws))
     return fail(Q27H_ERR_ARG, "kv_evict: tensors need 16-byte alignment");
+  if (!aligned4(acc) || !aligned4(acc_out) || !aligned4(kept) || !aligned4(pos0))
+    return fail(Q27H_ERR_ARG, "kv_evict: acc, acc_out, kept and pos0 need 4-byte alignment");
   const size_t in = cache_bytes(nkvh, n_ctx, q8), out = cache_bytes(nkvh, n_ctx_out, q8);
   const size_t ain = (size_t)nkvh * n_ctx * 4, aout = (size_t)nkvh * n_ctx_out * 4;
   const bool in_place = kout == kcache && vout == vcache && acc_out == acc && n_ctx_out == n_ctx;
@@ -490,6 +492,7 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
 extern "C" int q27h_kv_evict_pos(int* pos0, int* rdelta, int keep, q27h_stream_t s) {
   if (keep <= 0) return fail(Q27H_ERR_SHAPE, "kv_evict_pos: keep >= 1");
   if (!pos0) return fail(Q27H_ERR_ARG, "kv_evict_pos: null pointer");
+  if (!aligned4(pos0) || !aligned4(rdelta)) return fail(Q27H_ERR_ARG, "kv_evict_pos: pos0 and rdelta need 4-byte alignment");
   if (outputs_overlap({{pos0, 4}, {rdelta, 4}}, {})) return fail(Q27H_ERR_ARG, "kv_evict_pos: pos0 and rdelta overlap");
   hipLaunchKernelGGL(evict_pos_kernel, dim3(1), dim3(1), 0, stream_of(s), pos0, rdelta, keep);
   return check_launch("kv_evict_pos");
@@ -507,6 +510,9 @@ extern "C" int q27h_kv_accept(void* const* caches, int n_caches, float* const* a
   }
   for (int i = 0; i < n_accs; i++)
     if (!accs[i]) return fail(Q27H_ERR_ARG, "kv_accept: null pointer");
+  bool odd = !aligned4(pos0) || !aligned4(path) || !aligned4(n_path);
+  for (int i = 0; i < n_accs; i++) odd |= !aligned4(accs[i]);
+  if (odd) return fail(Q27H_ERR_ARG, "kv_accept: weight arrays, pos0, path and n_path need 4-byte alignment");
   const size_t cb = cache_bytes(nkvh, n_ctx, q8), ab = (size_t)nkvh * n_ctx * 4;
   bool twice = false;  // a row moved twice, by workgroups that run at once
   for (int i = 0; i < n_caches; i++)
@@ -517,7 +523,7 @@ extern "C" int q27h_kv_accept(void* const* caches, int n_caches, float* const* a
   }
   for (int i = 0; i < n_caches + n_accs; i++)
     twice |= outputs_overlap({i < n_caches ? Bytes{caches[i], cb} : Bytes{accs[i - n_caches], ab}},
-                             {{pos0, 4}, {path, (size_t)T * 4}, {n_path, 4}});
+                             {{pos0, 4}, {path, 4}, {n_path, 4}});  // path: *n_path entries, which may be one
   if (twice) return fail(Q27H_ERR_ARG, "kv_accept: caches or weight arrays overlap each other or another argument");
   for (int c = 0, w = 0; c < n_caches || w < n_accs;) {
     AcceptArgs a = {};

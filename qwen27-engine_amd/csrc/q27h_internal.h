@@ -15,6 +15,7 @@ int fail(int code, const std::string& msg);
 // Checks the launch that was just enqueued; returns Q27H_OK or Q27H_ERR_HIP with the HIP error text.
 int check_launch(const char* what);
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool aligned8(const void* p) { return ((uintptr_t)p & 7u) == 0; }
 inline bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
 inline hipStream_t stream_of(q27h_stream_t s) { return (hipStream_t)s; }
 // True when the byte ranges [a, a + na) and [b, b + nb) share a byte.

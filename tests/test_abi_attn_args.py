@@ -1,5 +1,5 @@
-"""Refusals of the operators over the K/V cache that depend on two arguments at once: memory that is written and shared with
-another argument (no GPU needed; nothing is enqueued)."""
+"""Refusals of the operators over the K/V cache (no GPU needed; nothing is enqueued): memory that is written and shared with
+another argument, small arrays out of alignment."""
 import pytest
 
 from test_abi_attn import WS
@@ -92,3 +92,20 @@ def test_outputs_over_other_arguments_are_refused(q27, call, args, out, other):
 
 def test_evict_pos_refuses_one_place_for_both(q27):
     refused(q27, lambda o: o.kv_evict_pos(G4, G4, 4, 0))
+
+
+@pytest.mark.parametrize("call,args,name,by", [
+    (call, args, name, by) for call, args, names in (
+        (tree, TREE_ARGS, {"tree": 4, "lse": 2, "pos0": 1}), (weights, WEIGHT_ARGS, {"tree": 4, "rows": 4, "lse": 2, "acc": 1, "pos0": 2}),
+        (blocks, BLOCK_ARGS, {"idx": 2, "lse": 1, "pos0": 2}), (bounds, BOUND_ARGS, {"pos0": 2}), (select, SELECT_ARGS, {"idx": 1, "pos0": 2}),
+        (accept, ACCEPT_ARGS, {"acc": 2, "pos0": 1, "path": 2, "n_path": 3})) for name, by in names.items()])
+def test_arrays_out_of_alignment_are_refused(q27, call, args, name, by):
+    at = {n: (i + 1) * G4 for i, n in enumerate(args)}
+    at[name] += by
+    refused(q27, lambda o: call(o, **at), needle="alignment")
+
+
+@pytest.mark.parametrize("name,by", [("acc", 2), ("ao", 1), ("kept", 2), ("pos0", 1)])
+def test_evict_arrays_out_of_alignment_are_refused(q27, name, by):
+    refused(q27, evict, {name: EVICT[name] * G4 + by}, needle="alignment")
+    refused(q27, lambda o: o.kv_evict_pos(G4, 2 * G4 + by, 4, 0), needle="alignment")
