@@ -847,6 +847,9 @@ int blocks_splits(int T, int nkvh, int nsel) {
 size_t part_bytes(size_t rows, int splits) { return splits <= 1 ? 0 : rows * splits * (kHD + 2) * sizeof(float); }
 
 bool heads_ok(int nqh, int nkvh) { return nkvh > 0 && nqh > 0 && nqh % nkvh == 0; }
+// A grid holds less than 2^32 threads, and the grids below no more than a workgroup of 256 for each query row (the kernels
+// with larger ones have 16 and more rows for each) and 7 beside.
+bool rows_ok(int T, int nqh) { return (long long)T * nqh <= 0x7fffffffLL / 256; }
 
 }  // namespace
 }  // namespace q27h
@@ -854,7 +857,7 @@ bool heads_ok(int nqh, int nkvh) { return nkvh > 0 && nqh > 0 && nqh % nkvh == 0
 using namespace q27h;
 
 extern "C" size_t q27h_attn_tree_ws_bytes(int T, int nqh, int nkvh, int n_ctx) {
-  if (T <= 0 || T > kMaxTree || !heads_ok(nqh, nkvh) || n_ctx <= 0) return 0;
+  if (T <= 0 || T > kMaxTree || !heads_ok(nqh, nkvh) || n_ctx <= 0 || !rows_ok(T, nqh)) return 0;
   const int s0 = tree_layout(T, nqh, nkvh, n_ctx, false).splits, s1 = tree_layout(T, nqh, nkvh, n_ctx, true).splits;
   return part_bytes((size_t)T * nqh, s0 > s1 ? s0 : s1);
 }
@@ -864,6 +867,7 @@ extern "C" int q27h_attn_tree(const float* qn, const void* kcache, const void* v
                               size_t ws_bytes, q27h_stream_t s) {
   if (T < 0 || T > kMaxTree) return fail(Q27H_ERR_SHAPE, "attn_tree: T must be 0..64");
   if (!heads_ok(nqh, nkvh) || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "attn_tree: bad shape");
+  if (!rows_ok(T, nqh)) return fail(Q27H_ERR_SHAPE, "attn_tree: too many query rows (T * nqh)");
   if (T == 0) return Q27H_OK;
   if (!qn || !kcache || !vcache || !pos0 || !o) return fail(Q27H_ERR_ARG, "attn_tree: null pointer");
   if (!aligned16(qn) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(o) || !aligned16(ws))
@@ -901,6 +905,7 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
                                  q27h_stream_t s) {
   if (T < 0 || T > kMaxTree) return fail(Q27H_ERR_SHAPE, "attn_weights: T must be 0..64");
   if (!heads_ok(nqh, nkvh) || n_ctx <= 0) return fail(Q27H_ERR_SHAPE, "attn_weights: bad shape");
+  if (!rows_ok(T, nqh)) return fail(Q27H_ERR_SHAPE, "attn_weights: too many query rows (T * nqh)");
   if (T == 0) return Q27H_OK;
   if (!qn || !lse || !kcache || !pos0 || !acc) return fail(Q27H_ERR_ARG, "attn_weights: null pointer");
   if (!aligned16(qn) || !aligned16(kcache)) return fail(Q27H_ERR_ARG, "attn_weights: tensors need 16-byte alignment");

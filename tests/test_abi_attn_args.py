@@ -1,5 +1,5 @@
 """Refusals of the operators over the K/V cache (no GPU needed; nothing is enqueued): memory that is written and shared with
-another argument, small arrays out of alignment."""
+another argument, small arrays out of alignment, more query rows than a grid holds."""
 import pytest
 
 from test_abi_attn import WS
@@ -109,3 +109,13 @@ def test_arrays_out_of_alignment_are_refused(q27, call, args, name, by):
 def test_evict_arrays_out_of_alignment_are_refused(q27, name, by):
     refused(q27, evict, {name: EVICT[name] * G4 + by}, needle="alignment")
     refused(q27, lambda o: o.kv_evict_pos(G4, 2 * G4 + by, 4, 0), needle="alignment")
+
+
+@pytest.mark.parametrize("T,nqh,nkvh", [(1, 1 << 24, 1 << 24), (1, 1 << 24, 1), (64, 1 << 18, 4), (64, 1 << 30, 1 << 10), (17, 1 << 29, 1)])
+def test_more_query_rows_than_a_grid_holds_are_refused(q27, T, nqh, nkvh):
+    a = {n: (i + 1) << 50 for i, n in enumerate(TREE_ARGS)}
+    assert q27.ops.attn_tree_ws_bytes(T, nqh, nkvh, 4096) == 0
+    refused(q27, lambda o: o.attn_tree(a["qn"], a["k"], a["v"], a["pos0"], None, T, 0.0625, nqh, nkvh, 4096, True, a["o"],
+                                       WS(1 << 60, a["ws"]), 0), needle="too many", code=-1)
+    refused(q27, lambda o: o.attn_weights(a["qn"], a["lse"], a["k"], a["pos0"], None, T, 0.0625, nqh, nkvh, 4096, True, a["o"], 0),
+            needle="too many", code=-1)
