@@ -456,8 +456,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_blocks_kernel(AttnArgs a)
   auto tile = [&](int i, bool part) {
     // a scalar load: a vector load's wait would be for the tiles on their way as well
     const int b = *(const __attribute__((address_space(4))) int*)(list + (i >> 1));
-    const int j0 = b * kBlockRows + (i & 1) * kTileKeys;
-    return b >= 0 && b < nb && j0 < vis.n && (j0 + kTileKeys > vis.n) == part ? j0 : -1;
+    // the entry is any number: the product is formed of one that is a block
+    const bool is = (unsigned)b < (unsigned)nb;
+    const int j0 = (is ? b : 0) * kBlockRows + (i & 1) * kTileKeys;
+    return is && j0 < vis.n && (j0 + kTileKeys > vis.n) == part ? j0 : -1;
   };
   int i = split * per + w;
   auto next = [&] {

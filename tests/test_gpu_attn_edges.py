@@ -194,3 +194,20 @@ def test_values_that_are_not_finite_reach_all_that_see_them(G, T, where, score, 
         idx = G.up(np.tile(np.arange(2, dtype=np.int32), (T, nkvh, 1)))
         o = G.down(G.blocks(dq, dk, dv, pos, idx, T, 2, nqh, nkvh, n_ctx, q8)[0])
         assert not np.isfinite(o[..., dims]).any() and np.isfinite(o[..., ~dims]).all()
+
+
+@pytest.mark.parametrize("q8", [True, False])
+def test_entries_that_are_no_block_whatever_their_number(G, q8):  # noqa: F811
+    """Among them numbers whose product with the block's 64 rows is a row of the context again in 32 bits."""
+    r = np.random.default_rng(37)
+    pos0, n_ctx, nqh, nkvh = 200, 260, 24, 4
+    k, v = (R.make_cache(r, nkvh, n_ctx, q8, garbage_from=pos0 + 1) for _ in range(2))
+    q = r.standard_normal((1, nqh, 256)).astype(np.float32)
+    odd = [2 ** 25, 2 ** 25 + 1, 2 ** 26, 2 ** 26 + 1, 2 ** 26 + 3, 2 ** 31 - 1, -2 ** 31, -2 ** 31 + 1, -2 ** 26, -2 ** 26 + 2, -1, 4, 5]
+    idx = np.array(odd + [1] + odd + [3], np.int32)
+    vis = np.zeros((1, n_ctx), bool)
+    vis[:, 64:128] = vis[:, 192:pos0 + 1] = True
+    eo, el, bo, bl = attend(q, *(np.nan_to_num(R.values(x, nkvh, n_ctx, q8)) for x in (k, v)), vis, q8)
+    o, lse = G.blocks(G.up(q), G.up(k), G.up(v), G.i32(pos0), G.up(np.tile(idx, (1, nkvh, 1))), 1, len(idx), nqh, nkvh, n_ctx, q8)
+    near(G.down(o), eo, bo, "o")
+    near(G.down(lse), el, bl, "lse")
