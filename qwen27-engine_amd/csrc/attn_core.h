@@ -462,7 +462,7 @@ __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   if (__any(mx - st.m > 15.0f)) {
     mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
     mx = __builtin_fmaxf(mx, lane_xor32(mx));
-    const float m1 = __builtin_fmaxf(st.m, mx - 12.0f);
+    const float m1 = mx - st.m > 15.0f ? mx - 12.0f : st.m;  // by its own row alone: its bits are the same beside any others
     const float a = __builtin_amdgcn_exp2f(st.m - m1);
     st.m = m1;
     st.l *= a;
@@ -507,7 +507,8 @@ __device__ __forceinline__ void split8(Rows& st, const f4 (&p)[2], const float* 
   if (__any((mx > st.unit * 0x1p15f) | (st.want < st.unit))) {
     mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
     mx = __builtin_fmaxf(mx, lane_xor32(mx));
-    const float to = power_below(__builtin_fmaxf(__builtin_fmaxf(st.want, kLeastUnit), mx * 0x1p-12f));
+    const bool move = (mx > st.unit * 0x1p15f) | (st.want < st.unit);
+    const float to = move ? power_below(__builtin_fmaxf(__builtin_fmaxf(st.want, kLeastUnit), mx * 0x1p-12f)) : st.unit;
     const float a = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, st.unit) + (127u << 23) - __builtin_bit_cast(uint32_t, to));
     st.unit = st.want = to;
 #pragma unroll
