@@ -412,7 +412,9 @@ __device__ __forceinline__ void hide(f4 (&s)[RT][2], const Vis& vis, const uint6
       const unsigned d = (unsigned)(j - vis.n0);
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
-        // no branches: eight of them a lane cost more than the shift, and hipcc has lost one's value
+        // | and not ||: eight branches a lane cost more than the shift. And hipcc (clang 22) lost the score of the first of
+        // them in attn_weights' kernels: it keeps the score's register for the result, sets it to -inf where the first
+        // condition is false, and emits nothing under the mask of the lanes where the second is true.
         const bool seen = (j < vis.n) | ((j < vis.end) & (d < 64u) & (bool)((tree[rt] >> (d & 63u)) & 1));
         s[rt][u][i] = seen ? s[rt][u][i] : __builtin_bit_cast(float, AS);
       }
