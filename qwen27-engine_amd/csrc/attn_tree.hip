@@ -603,9 +603,9 @@ struct WeightArgs {
   float scale;
 };
 
-// attn_weights: a workgroup takes a split of the cache rows of one kv head, walks the query rows in groups of 16 RT and,
-// for each, its tiles; the sum over the 16 query rows of a tile is a lane reduction, that over row tiles and groups is
-// taken in order, and a row of the cache belongs to one wave: the same bits always.
+// attn_weights of up to 16 RT query rows: a workgroup takes a split of the cache rows of one kv head; the sum over the 16
+// query rows of a tile is a lane reduction, that over row tiles is taken in order, and a row of the cache belongs to one
+// wave: the same bits always.
 template <bool Q8, int RT>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs a) {
   __shared__ union {
@@ -626,73 +626,69 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_weights_kernel(WeightArgs
   const uint64_t used = a.rows ? *a.rows : ~0ull;
   const KvHead kc = kv_head<Q8>(a.kcache, kh, a.nkvh, a.n_ctx);
   float* acc = a.acc + (size_t)kh * a.n_ctx;
-  for (int rg = 0; rg < a.groups; rg++) {
+  load_queries<Q8, kWaves, RT>(im, a.scale * kLog2e, [&](int r) {
+    return r < rows ? a.qn + ((size_t)(r / group) * a.nqh + kh * group + r % group) * kHD : nullptr;
+  });
+  if (threadIdx.x < RT * 16) {
+    const int r = threadIdx.x;
+    const bool on = r < rows && ((used >> (r / group)) & 1);
+    s_lse[threadIdx.x] = on ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : __builtin_huge_valf();
+  }
+  __syncthreads();
+  uint64_t tree[RT];
+  float c[RT], lse[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) {
+    const int r = rt * 16 + n;
+    tree[rt] = r < rows ? tree_of(a.tree, r / group, a.T) : 0ull;
+    c[rt] = im[rt].c[n];
+    lse[rt] = s_lse[rt * 16 + n];
+  }
+  QRegs q[RT];
+  if constexpr (!Q8) {
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) take_queries(q[rt], im[rt]);
     __syncthreads();
-    load_queries<Q8, kWaves, RT>(im, a.scale * kLog2e, [&](int r) {
-      r += rg * RT * 16;
-      return r < rows ? a.qn + ((size_t)(r / group) * a.nqh + kh * group + r % group) * kHD : nullptr;
-    });
-    if (threadIdx.x < RT * 16) {
-      const int r = rg * RT * 16 + threadIdx.x;
-      const bool on = r < rows && ((used >> (r / group)) & 1);
-      s_lse[threadIdx.x] = on ? a.lse[(size_t)(r / group) * a.nqh + kh * group + r % group] * kLog2e : __builtin_huge_valf();
+  }
+  for (int t = split * sp.per + w; t < t1; t += kWaves) {
+    const int j0 = t * kTileKeys;
+    const bool full = j0 + kTileKeys <= vis.n;
+    QRows k;
+    f4 s[RT][2];
+    if constexpr (Q8) {
+      if (full) load_rows<false>(k, kc, j0, 0);
+      else load_rows<true>(k, kc, j0, vis.end - j0);
+    } else {
+      if (full) request_keys<false>(sh.w[w], kc, j0, 0);
+      else request_keys<true>(sh.w[w], kc, j0, vis.end - j0);
     }
-    __syncthreads();
-    uint64_t tree[RT];
-    float c[RT], lse[RT];
+    const int j = j0 + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);  // the row this lane stores (n < 8)
+    const bool mine = n < 8 && j < vis.end;
+    const float old = mine && j < vis.n ? acc[j] : 0.0f;  // the weights of a drafted row begin here
+    asm volatile("" ::: "memory");
+    if constexpr (Q8) {
+      __builtin_amdgcn_wave_barrier();
+      stage_keys(k, s_w[w]);
+      scores<RT>(s_w[w], im, s);
+    } else {
+      keys_there<0>();
+      scores(sh.w[w], q, s);
+    }
+    if (!full) hide<RT, kMinusInf>(s, vis, tree, j0);
+    float sum[8];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-      const int r = rg * RT * 16 + rt * 16 + n;
-      tree[rt] = r < rows ? tree_of(a.tree, r / group, a.T) : 0ull;
-      c[rt] = im[rt].c[n];
-      lse[rt] = s_lse[rt * 16 + n];
-    }
-    QRegs q[RT];
-    if constexpr (!Q8) {
+    for (int e = 0; e < 8; e++) {
+      sum[e] = 0.0f;
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++) take_queries(q[rt], im[rt]);
-      __syncthreads();
-    }
-    for (int t = split * sp.per + w; t < t1; t += kWaves) {
-      const int j0 = t * kTileKeys;
-      const bool full = j0 + kTileKeys <= vis.n;
-      QRows k;
-      f4 s[RT][2];
-      if constexpr (Q8) {
-        if (full) load_rows<false>(k, kc, j0, 0);
-        else load_rows<true>(k, kc, j0, vis.end - j0);
-      } else {
-        if (full) request_keys<false>(sh.w[w], kc, j0, 0);
-        else request_keys<true>(sh.w[w], kc, j0, vis.end - j0);
+      for (int rt = 0; rt < RT; rt++) {
+        const float x = s[rt][e >> 2][e & 3];
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[rt], -lse[rt]));
+        // rows not asked for, and hidden cache rows (of a query row that sees none lse is -inf too)
+        sum[e] += lse[rt] == __builtin_huge_valf() || x == -__builtin_huge_valf() ? 0.0f : p;
       }
-      const int j = j0 + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);  // the row this lane stores (n < 8)
-      const bool mine = n < 8 && j < vis.end;
-      const float old = mine && (j < vis.n || rg) ? acc[j] : 0.0f;  // the weights of a drafted row begin here
-      asm volatile("" ::: "memory");
-      if constexpr (Q8) {
-        __builtin_amdgcn_wave_barrier();
-        stage_keys(k, s_w[w]);
-        scores<RT>(s_w[w], im, s);
-      } else {
-        keys_there<0>();
-        scores(sh.w[w], q, s);
-      }
-      if (!full) hide<RT, kMinusInf>(s, vis, tree, j0);
-      float sum[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        sum[e] = 0.0f;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-          const float x = s[rt][e >> 2][e & 3];
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[rt], -lse[rt]));
-          // rows not asked for, and hidden cache rows (of a query row that sees none lse is -inf too)
-          sum[e] += lse[rt] == __builtin_huge_valf() || x == -__builtin_huge_valf() ? 0.0f : p;
-        }
-      }
-      sum_rows(sum);
-      if (mine) acc[j] = old + sum[0];
     }
+    sum_rows(sum);
+    if (mine) acc[j] = old + sum[0];
   }
 }
 
@@ -928,7 +924,7 @@ extern "C" int q27h_attn_weights(const float* qn, const float* lse, const void* 
   if (two) lay.groups = two_groups, lay.tiles = two_tiles;
   a.groups = lay.groups, a.tiles = lay.tiles;
   const int waves = lay.wide ? 1 : kWaves, most = ((n_ctx + kTileKeys - 1) / kTileKeys + waves - 1) / waves;
-  // narrow: small workgroups, four to a compute unit; wide: as many as are resident
+  // narrow: two rounds of workgroups (two are resident on a compute unit, by their LDS); wide: as many as are resident
   a.splits = (!lay.wide ? 4 * kCUs : lay.tiles <= 4 ? 2 * kCUs : kCUs) / nkvh;
   a.splits = a.splits > most ? most : a.splits < 1 ? 1 : a.splits;
   const dim3 grid((unsigned)(nkvh * a.splits));
