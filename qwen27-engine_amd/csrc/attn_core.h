@@ -192,8 +192,8 @@ __device__ __forceinline__ void put_scales(u2 s, uint8_t* scales) {
   p[96] = (uint16_t)(s.y >> 16);
 }
 // V's: brought to |d / f| <= 1 by the power of two f above the finite scales of the row's 8 blocks, f beside them (0
-// where none is above 0: such a row adds zeros, or NaN, and leaves the unit alone). f meets the weight in float32, and d / f is a half without loss
-// unless the block's scale is below 2^-14 of f; then it is off by less than 2^-24 of f.
+// where none is above 0: such a row adds zeros, or NaN, and leaves the unit alone). f meets the weight in float32, and
+// d / f is a half without loss unless the block's scale is below 2^-14 of f; then it is off by less than 2^-24 of f.
 __device__ __forceinline__ float exp2i(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 __device__ __forceinline__ void put_value_scales(u2 s, uint8_t* scales, float* factors) {
   const int l = threadIdx.x & 63;
@@ -454,8 +454,8 @@ template <bool Q8>
 __device__ __forceinline__ float unit_of(const Rows& st) {
   return Q8 ? st.unit * 512.0f : 1.0f;
 }
-// p[u][i] from the scores, with the reference moved where it has to be (maxima pass over NaN). HIDDEN: a hidden row's (kHidden)
-// weight is -0, so that the sign tells it from a row that is seen with a weight of 0, whose infinities make NaN.
+// p[u][i] from the scores, with the reference moved where it has to be (maxima pass over NaN). HIDDEN: the weight of a
+// hidden row (kHidden) is -0: the sign tells it from a row that is seen with a weight of 0, whose infinities make NaN.
 template <bool Q8, bool HIDDEN>
 __device__ __forceinline__ void weights(Rows& st, f4 (&s)[2]) {
   float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(s[0][0], s[0][1]), __builtin_fmaxf(s[0][2], s[0][3])),

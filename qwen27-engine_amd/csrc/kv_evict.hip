@@ -443,10 +443,9 @@ extern "C" int q27h_kv_evict(const void* kcache, const void* vcache, const float
   const size_t ain = (size_t)nkvh * n_ctx * 4, aout = (size_t)nkvh * n_ctx_out * 4;
   const bool in_place = kout == kcache && vout == vcache && acc_out == acc && n_ctx_out == n_ctx;
   const size_t need = q27h_kv_evict_ws_bytes(nkvh, n_ctx, keep, q8, in_place);
-  const Bytes rows_kept = {kept, (size_t)nkvh * keep * 4}, work = {ws, need}, pos = {pos0, 4};
-  if (overlaps(kcache, in, vcache, in) ||
-      (in_place ? outputs_overlap({{kout, out}, {vout, out}, {acc_out, aout}, rows_kept, work}, {pos})
-                : outputs_overlap({{kout, out}, {vout, out}, {acc_out, aout}, rows_kept, work}, {{kcache, in}, {vcache, in}, {acc, ain}, pos})))
+  const Bytes k = {kout, out}, v = {vout, out}, w = {acc_out, aout}, l = {kept, (size_t)nkvh * keep * 4}, work = {ws, need};
+  if (overlaps(kcache, in, vcache, in) || outputs_overlap({k, v, w, l, work}, {{pos0, 4}}) ||
+      (!in_place && outputs_overlap({k, v, w, l, work}, {{kcache, in}, {vcache, in}, {acc, ain}})))
     return fail(Q27H_ERR_ARG, "kv_evict: the outputs overlap each other or the inputs (all of them in place, or none)");
   if (ws_bytes < need) return fail(Q27H_ERR_ARG, "kv_evict: workspace too small");
   EvictArgs a = {};

@@ -1,5 +1,6 @@
 """Attention over the K/V cache on the GPU where it can go wrong and tests/test_gpu_attn.py does not look, against a plain
-64-bit form: query values far below their row's largest, V rows of very different size, values that are not finite."""
+64-bit form: query values far below their row's largest, V rows of very different size, values that are not finite, lists
+of any numbers."""
 import numpy as np
 import pytest
 
@@ -211,3 +212,43 @@ def test_entries_that_are_no_block_whatever_their_number(G, q8):  # noqa: F811
     o, lse = G.blocks(G.up(q), G.up(k), G.up(v), G.i32(pos0), G.up(np.tile(idx, (1, nkvh, 1))), 1, len(idx), nqh, nkvh, n_ctx, q8)
     near(G.down(o), eo, bo, "o")
     near(G.down(lse), el, bl, "lse")
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("j", [3, 69, 70])
+@pytest.mark.parametrize("T", [1, 4, 8, 12])
+def test_a_row_without_a_finite_scale(G, T, j, bad):  # noqa: F811
+    """q8_0: none of a V row's scales is finite. Row 70 is drafted and seen by every other token, the others by all."""
+    r = np.random.default_rng(47)
+    pos0, n_ctx, nqh, nkvh = 70, 100, 24, 4
+    k, v = (R.make_cache(r, nkvh, n_ctx, True) for _ in range(2))
+    R.split_q8(v, nkvh, n_ctx)[0][:, :, ::32] = 127
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    tree = np.array([1 << t | (t % 2 == 0) for t in range(T)], np.uint64)
+    vis = R.visible(T, pos0, n_ctx, tree)
+    eo, el, bo, bl = attend(q, R.values(k, nkvh, n_ctx, True), R.values(v, nkvh, n_ctx, True), vis, True)
+    R.split_q8(v, nkvh, n_ctx)[1][:, j] = bad
+    o, lse = (G.down(x) for x in G.tree(G.up(q), G.up(k), G.up(v), G.i32(pos0), G.u64(tree), T, nqh, nkvh, n_ctx, True))
+    hit = vis[:, j]
+    near(lse, el, bl, "lse")
+    assert not np.isfinite(o[hit]).any()
+    near(o[~hit], eo[~hit], bo[~hit], "o")
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("T", [2, 4, 8, 12])
+def test_a_query_that_is_not_finite(G, T, bad, q8):  # noqa: F811
+    """One head of one token: its results are NaN, all others keep their bits."""
+    r = np.random.default_rng(53)
+    pos0, n_ctx, nqh, nkvh = 70, 100, 24, 4
+    k, v = (G.up(R.make_cache(r, nkvh, n_ctx, q8)) for _ in range(2))
+    q = r.standard_normal((T, nqh, 256)).astype(np.float32)
+    run = lambda q: [G.down(x) for x in G.tree(G.up(q), k, v, G.i32(pos0), None, T, nqh, nkvh, n_ctx, q8)]  # noqa: E731
+    want = run(q)
+    q[1, 7, 100] = bad
+    got = run(q)
+    for x, y in zip(got, want):
+        assert np.isnan(x[1, 7]).all()
+        x[1, 7] = y[1, 7]
+        assert (x.view(np.int32) == y.view(np.int32)).all()
