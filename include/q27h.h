@@ -248,6 +248,77 @@ int q27h_attn_blocks(const float* qn, const void* kcache, const void* vcache, co
                      float scale, int nqh, int nkvh, int n_ctx, int q8, float* o, float* lse, void* ws, size_t ws_bytes,
                      q27h_stream_t s);
 
+/* ---------------------------------------------------------------- a batch of sequences over a K/V cache in pages
+ * No counterpart in the reference, which serves one sequence. A page of K or V (q27h_kv_page_bytes) is a cache of page_rows
+ * rows in attn_prep's layout: f16 [nkvh][page_rows][256], or int8 codes [nkvh][page_rows][256] followed by f16 scales
+ * [nkvh][page_rows][8]; V in 4 bits: [nkvh][page_rows][128], then the scales, byte j of a block's 16 holding the code, 0 .. 15,
+ * of value j in its low half and of value j + 16 in its high half, value = (code - 8) * scale. Row i of sequence b lies in row
+ * i % page_rows of page table[b][i / page_rows]. Rows whose page is outside [0, n_pages), or that lie outside
+ * [0, max_pages * page_rows), do not exist: they are not written, not seen, and read as zeros. Sequences may share pages
+ * that nothing writes.
+ *
+ * A batch: tokens cu[b] .. cu[b + 1] - 1 of T are the new ones of sequence b (cu [n_seqs + 1], rising, within 0 .. T; a
+ * sequence may have none; NULL: one token each, T = n_seqs), and pos[b] its rows before the batch; token t of them has row
+ * pos[b] + t. pos, cu and the table are device memory, read by the kernels; the handle is read during the call. What a call
+ * writes may share no memory with its other arguments. Rows of results that belong to no sequence are left as they were.
+ * Pages, tensors and workspaces need 16-byte alignment, all other arrays 4-byte. A workspace holds nothing between calls and
+ * serves one call at a time: calls on different streams, and graphs that may run at the same time, need one each. */
+#define Q27H_KV_F16 0   /* K and V as f16 */
+#define Q27H_KV_Q8 1    /* K and V as q8_0 */
+#define Q27H_KV_Q8_Q4 2 /* K as q8_0, V in 4 bits */
+#define Q27H_F32 0
+#define Q27H_F16 1
+#define Q27H_BF16 2
+typedef struct {
+  void *k, *v;      /* n_pages pages each, one behind the other */
+  const int* table; /* device, [n_seqs][max_pages] */
+  int n_seqs, max_pages, n_pages;
+  int nkvh, page_rows; /* page_rows: a power of two, 32 to 65536; max_pages * page_rows <= 2^30 */
+  int type;            /* Q27H_KV_* */
+} q27h_kv_pages;
+/* Bytes of a page of K (v = 0) or V (v = 1); 0 for a bad argument. */
+size_t q27h_kv_page_bytes(int nkvh, int page_rows, int type, int v);
+/* attn_prep_paged: attn_prep for a ragged batch over pages: the same norms, rotation and q8_0 / f16 rows, bit for bit. The
+ * rotary position of a token is rope3[token][j % 3] (may be NULL) or its row less rdelta[b] (rdelta [n_seqs], may be NULL).
+ * 4 bits, per 32 values: d = e / -8 for the value e of largest magnitude (of +e and -e the negative one), code = min(15,
+ * trunc(x * (1 / d) + 8.5)), or of x * 0 for d = 0, scale = f16(d). */
+int q27h_attn_prep_paged(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm, float* qn,
+                         const q27h_kv_pages* kv, const int* pos, const int* cu, int T, float eps, float theta_scale, int nqh,
+                         q27h_stream_t s, const int* rope3, const int* rdelta);
+/* attn_paged: o [T][nqh][256] and lse [T][nqh] (may be NULL), as attn_tree's, of every token over the rows of its sequence up
+ * to its own; with attn_tree's arithmetic and bounds, 4-bit codes entering exactly as q8_0's do. At most max_tokens (1 to 64)
+ * tokens of a sequence are taken; those behind them are left out. A token that sees no row gets zeros and -inf. The same call
+ * gives the same bits; how a sequence's rows are split, and so the order of its sums, hangs on the lengths of all sequences.
+ * ws: q27h_attn_paged_ws_bytes of the same handle's sizes, T, max_tokens and nqh. */
+size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int max_tokens, int nqh);
+int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens, float scale,
+                    int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s);
+/* kv_pages_read: rows from[b] .. from[b] + count[b] - 1 (from NULL: 0; count cut to 0 .. n_out; both device, [n_seqs]) as
+ * values in kout and vout [n_seqs][nkvh][n_out][256] (either may be NULL), Q27H_F32, Q27H_F16 or Q27H_BF16 (rounded to the
+ * nearest once), from row 0 on; rows behind them are left as they were. The f16 form of one sequence is an f16 cache of
+ * n_ctx = n_out rows for attn_tree, attn_weights and attn_blocks. */
+int q27h_kv_pages_read(const q27h_kv_pages* kv, const int* from, const int* count, int n_out, int out_type, void* kout,
+                       void* vout, q27h_stream_t s);
+/* draft_verify: which drafted tokens stand, and the token after them, by given random numbers. Row t of a sequence's tokens
+ * (cu as above, not NULL; at most 64 tokens of a sequence are taken) is token t's: ids its number in the vocabulary, p (rows
+ * of V floats, ldp apart) the target's distribution behind it. Token 0 is the sequence's last one and stands. u [T] and u_last
+ * [n_seqs] are uniform in [0, 1).
+ * With q (rows ldq apart): token t >= 1 of a chain was drawn from q[t]; it stands if those before it do and
+ *   u[t] * q[t][id] < p[t - 1][id]. Behind the last one that stands, the next token is drawn from max(p - q, 0), q the row of
+ *   the refused token (from p where that is 0 everywhere), or from p where none was refused.
+ * Without q: the drafts are a tree, parent[t] < t (NULL: t - 1; a token whose parent is none of them is left out). From token
+ *   0 on, the children of the last one that stands are tried in order: a child stands if u * rest < p[id], p the parent's, rest = 1 -
+ *   the p[id] of those refused before it (in 64 bits); one that repeats a refused id is refused. The next token is drawn from p
+ *   without the refused ids.
+ * A draw: the least x with sum of w over 0 .. x > u_last * S, S the sum over all, w clamped to [0, 1] (NaN: 0) and rounded to
+ * multiples of 2^-40: exact, the same in any order. No weight at all: -1. An id outside [0, V) is refused.
+ * out [T]: the tokens that stand behind token 0, then the next one, -1 behind it; path [T]: the rows t that stand (0 first),
+ * -1 behind them; n_path [n_seqs]: how many (path and n_path are kv_accept's); pos [n_seqs] (may be NULL) grows by n_path. */
+size_t q27h_draft_verify_ws_bytes(int n_seqs, int V);
+int q27h_draft_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, const int* ids, const int* parent, const float* u,
+                      const float* u_last, const int* cu, int n_seqs, int T, int V, int* out, int* path, int* n_path, int* pos,
+                      void* ws, size_t ws_bytes, q27h_stream_t s);
+
 /* ---------------------------------------------------------------- quantized embedding gather */
 /* get_rows_iq2_s (src/ops.h:22-23, src/ops.cu:756-766): rows ids[t] (device) of an IQ2_S table (82-byte
  * super-blocks, row_bytes apart) -> f32 y [T][n], n % 256 == 0; id < 0 copies row (-id - 1) of img [..][n]

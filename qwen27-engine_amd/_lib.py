@@ -32,6 +32,12 @@ class GValueC(C.Structure):
                 ("n", C.c_uint64), ("ai", C.POINTER(C.c_int64)), ("af", C.POINTER(C.c_double))]
 
 
+class KvPagesC(C.Structure):
+    """q27h_kv_pages"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("n_seqs", C.c_int), ("max_pages", C.c_int),
+                ("n_pages", C.c_int), ("nkvh", C.c_int), ("page_rows", C.c_int), ("type", C.c_int)]
+
+
 # name -> argument types (all return int status unless listed in _RESTYPE)
 SIGNATURES = {
     "q27h_rmsnorm": [_p, _p, _p, _i, _i, _f, _p, _i],
@@ -75,6 +81,13 @@ SIGNATURES = {
     "q27h_attn_select": [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _sz, _p],
     "q27h_attn_blocks_ws_bytes": [_i, _i, _i, _i],
     "q27h_attn_blocks": [_p, _p, _p, _p, _p, _i, _i, _f, _i, _i, _i, _i, _p, _p, _p, _sz, _p],
+    "q27h_kv_page_bytes": [_i, _i, _i, _i],
+    "q27h_attn_prep_paged": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _f, _i, _p, _p, _p],
+    "q27h_attn_paged_ws_bytes": [_p, _i, _i, _i],
+    "q27h_attn_paged": [_p, _p, _p, _p, _i, _i, _f, _i, _p, _p, _p, _sz, _p],
+    "q27h_kv_pages_read": [_p, _p, _p, _i, _i, _p, _p, _p],
+    "q27h_draft_verify_ws_bytes": [_i, _i],
+    "q27h_draft_verify": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _p, _p, _sz, _p],
     "q27h_get_rows_iq2_s": [_p, _i64, _p, _i, _p, _i, _p, _p],
     "q27h_get_rows_q4_k": [_p, _i64, _p, _i, _p, _i, _p, _p],
     "q27h_get_rows_q6_k": [_p, _i64, _p, _i, _p, _i, _p, _p],
@@ -104,6 +117,7 @@ SIGNATURES = {
 }
 _RESTYPE = {"q27h_kv_cache_bytes": _sz, "q27h_attn_tree_ws_bytes": _sz, "q27h_kv_evict_ws_bytes": _sz,
             "q27h_kv_block_bytes": _sz, "q27h_attn_select_ws_bytes": _sz, "q27h_attn_blocks_ws_bytes": _sz,
+            "q27h_kv_page_bytes": _sz, "q27h_attn_paged_ws_bytes": _sz, "q27h_draft_verify_ws_bytes": _sz,
             "q27h_qmat_bytes": _sz, "q27h_last_error": C.c_char_p,
             "q27h_gtype_name": C.c_char_p, "q27h_gguf_close": None, "q27h_gguf_n_tensors": _i64, "q27h_gguf_find": _i64,
             "q27h_gguf_n_kv": _i64}

@@ -1,0 +1,248 @@
+// A K/V cache in pages: its handle's checks, and its rows read back as values (kv_pages_read).
+//
+// Reading back is a copy that widens: rows x nkvh x (144 to 512 bytes in, 512 or 1024 out) for each of K and V, no arithmetic
+// but one product a value, so it is bound by HBM. A piece of work is kChunk rows of one head; the sequences' pieces are laid
+// end to end and cut in equal parts (share_of), since sequences are of any length.
+#include <hip/hip_bfloat16.h>
+
+#include <type_traits>
+
+#include "paged.h"
+
+namespace q27h {
+
+int check_pages(const q27h_kv_pages* kv, const char* what) {
+  const std::string w = what;
+  if (!kv) return fail(Q27H_ERR_ARG, w + ": null handle of pages");
+  if (kv->type != Q27H_KV_F16 && kv->type != Q27H_KV_Q8 && kv->type != Q27H_KV_Q8_Q4)
+    return fail(Q27H_ERR_SHAPE, w + ": unknown type of cache");
+  if (kv->page_rows < 32 || kv->page_rows > 65536 || (kv->page_rows & (kv->page_rows - 1)))
+    return fail(Q27H_ERR_SHAPE, w + ": the rows of a page must be a power of two, 32 to 65536");
+  if (kv->nkvh <= 0 || kv->nkvh > 4096 || kv->n_seqs < 0 || kv->n_pages < 0 || kv->max_pages < 0 ||
+      (long long)kv->max_pages * kv->page_rows > 1 << 30)
+    return fail(Q27H_ERR_SHAPE, w + ": bad sizes of the paged cache (at most 2^30 rows a sequence)");
+  if ((kv->n_pages && (!kv->k || !kv->v)) || (kv->n_seqs && kv->max_pages && !kv->table))
+    return fail(Q27H_ERR_ARG, w + ": null pointer in the handle of pages");
+  if (!aligned16(kv->k) || !aligned16(kv->v) || !aligned4(kv->table))
+    return fail(Q27H_ERR_ARG, w + ": pages need 16-byte alignment, their table 4-byte");
+  return Q27H_OK;
+}
+
+Pages pages_of(const q27h_kv_pages* kv) {
+  Pages p;
+  p.k = (uint8_t*)kv->k, p.v = (uint8_t*)kv->v, p.table = kv->table;
+  p.kb = q27h_kv_page_bytes(kv->nkvh, kv->page_rows, kv->type, 0), p.vb = q27h_kv_page_bytes(kv->nkvh, kv->page_rows, kv->type, 1);
+  p.n_seqs = kv->n_seqs, p.max_pages = kv->max_pages, p.n_pages = kv->n_pages, p.nkvh = kv->nkvh, p.type = kv->type;
+  p.shift = __builtin_ctz((unsigned)kv->page_rows);
+  return p;
+}
+
+namespace {
+
+constexpr int kChunk = 32;    // rows of a piece
+constexpr int kBlocks = 8 * kCUs;
+
+struct ReadArgs {
+  Pages pg;
+  const int *from, *count;
+  void *kout, *vout;
+  int n_out;
+};
+
+typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+typedef uint32_t w2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// Eight neighbouring values to their place.
+__device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) __builtin_nontemporal_store((f4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}, (f4*)p + i);
+}
+__device__ __forceinline__ void put8(uint16_t* p, const uint32_t (&h)[8]) {
+  __builtin_nontemporal_store((w4){h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16}, (w4*)p);
+}
+struct AsF32 {
+  typedef float type;
+  static __device__ __forceinline__ void put(float* p, const float (&x)[8]) { put8(p, x); }
+};
+struct AsF16 {
+  typedef uint16_t type;
+  static __device__ __forceinline__ void put(uint16_t* p, const float (&x)[8]) {
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[i] = f2h_bits(x[i]);
+    put8(p, h);
+  }
+};
+struct AsBf16 {
+  typedef uint16_t type;
+  static __device__ __forceinline__ void put(uint16_t* p, const float (&x)[8]) {
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {  // to the nearest, ties to even; NaN stays one
+      const uint32_t b = __builtin_bit_cast(uint32_t, x[i]);
+      h[i] = x[i] != x[i] ? (b >> 16) | 0x40 : (b + 0x7fff + (b >> 16 & 1)) >> 16;
+    }
+    put8(p, h);
+  }
+};
+
+// What a lane has of a row: 16 values, at dims d and d + off. 16 lanes to a row.
+template <int BITS>
+struct Piece;
+template <>
+struct Piece<16> {
+  w4 x[2];
+  __device__ __forceinline__ void load(const uint8_t* head, int n, int row, int l) {
+    const uint8_t* p = head + (size_t)row * kRowF16 + 16 * l;
+    x[0] = *(const w4*)p, x[1] = *(const w4*)(p + 256);
+  }
+  static __device__ __forceinline__ int dim(int l, int i) { return 8 * l + 128 * i; }
+  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = h2f_bits((uint16_t)(x[i][e >> 1] >> 16 * (e & 1)));
+  }
+};
+template <>
+struct Piece<8> {
+  w2 x[2];
+  uint16_t d[2];
+  __device__ __forceinline__ void load(const uint8_t* head, const uint8_t* scales, int row, int l) {
+    const uint8_t* p = head + (size_t)row * 256 + 8 * l;
+    x[0] = *(const w2*)p, x[1] = *(const w2*)(p + 128);
+    const uint16_t* s = (const uint16_t*)scales + (size_t)row * 8 + (l >> 2);
+    d[0] = s[0], d[1] = s[4];
+  }
+  static __device__ __forceinline__ int dim(int l, int i) { return 8 * l + 128 * i; }
+  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
+    const float s = h2f_bits(d[i]);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = (float)(int8_t)(x[i][e >> 2] >> 8 * (e & 3)) * s;
+  }
+};
+template <>
+struct Piece<4> {
+  w2 x;
+  uint16_t d;
+  __device__ __forceinline__ void load(const uint8_t* head, const uint8_t* scales, int row, int l) {
+    x = *(const w2*)(head + (size_t)row * 128 + 8 * l);
+    d = *((const uint16_t*)scales + (size_t)row * 8 + (l >> 1));
+  }
+  static __device__ __forceinline__ int dim(int l, int i) { return 32 * (l >> 1) + 8 * (l & 1) + 16 * i; }
+  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
+    const float s = h2f_bits(d);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = (float)((int)(x[e >> 2] >> (8 * (e & 3) + 4 * i) & 15u) - 8) * s;
+  }
+};
+
+// A workgroup takes a chunk of 32 rows in two steps of 16, K and V of a step requested together. Rows of a page that is none
+// of the cache's are zeros.
+template <int KB, int VB, typename OUT>
+__global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
+  typedef typename OUT::type O;
+  const int l = threadIdx.x & 15, r = threadIdx.x >> 4;
+  auto rows_of = [&](int b) {
+    const int n = a.count[b];
+    return n < 0 ? 0 : n < a.n_out ? n : a.n_out;
+  };
+  Share sp = share_of<256>(a.pg.n_seqs, 1, nullptr, [&](int b) { return a.pg.nkvh * ((rows_of(b) + kChunk - 1) / kChunk); });
+  const int n = 1 << a.pg.shift;
+  while (sp.x < sp.end) {
+    const int b = sp.seq, count = rows_of(b), chunks = (count + kChunk - 1) / kChunk;
+    if (sp.x >= sp.start + a.pg.nkvh * chunks) {
+      sp.start += a.pg.nkvh * chunks;
+      sp.seq++;
+      continue;
+    }
+    const int at = sp.x - sp.start, kh = at / chunks, i0 = (at - kh * chunks) * kChunk;
+    sp.x++;
+    const long long from = a.from ? a.from[b] : 0;
+    Piece<KB> k[2];
+    Piece<VB> v[2];
+    bool is[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int i = i0 + 16 * s + r;
+      const long long j = from + i;
+      const long long pi = j >> a.pg.shift;
+      int page = -1;
+      if (i < count && pi >= 0 && pi < a.pg.max_pages) page = a.pg.table[(size_t)b * a.pg.max_pages + pi];
+      is[s] = (unsigned)page < (unsigned)a.pg.n_pages;
+      if (!is[s]) continue;
+      const int row = kh * n + (int)(j & (n - 1));
+      const uint8_t *kp = a.pg.k + (size_t)page * a.pg.kb, *vp = a.pg.v + (size_t)page * a.pg.vb;
+      const size_t codes = (size_t)a.pg.nkvh * n;
+      if constexpr (KB == 16) {
+        if (a.kout) k[s].load(kp, 0, row, l);
+        if (a.vout) v[s].load(vp, 0, row, l);
+      } else {
+        if (a.kout) k[s].load(kp, kp + codes * (32 * KB), row, l);
+        if (a.vout) v[s].load(vp, vp + codes * (32 * VB), row, l);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int i = i0 + 16 * s + r;
+      if (i >= count) continue;
+      const size_t o = (((size_t)b * a.pg.nkvh + kh) * a.n_out + i) * kHeadDim;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float y[8];
+        if (a.kout) {
+          k[s].values(h, y);
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = is[s] ? y[e] : 0.0f;
+          OUT::put((O*)a.kout + o + Piece<KB>::dim(l, h), y);
+        }
+        if (a.vout) {
+          v[s].values(h, y);
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = is[s] ? y[e] : 0.0f;
+          OUT::put((O*)a.vout + o + Piece<VB>::dim(l, h), y);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace q27h
+
+using namespace q27h;
+
+extern "C" size_t q27h_kv_page_bytes(int nkvh, int page_rows, int type, int v) {
+  if (nkvh <= 0 || page_rows <= 0 || type < Q27H_KV_F16 || type > Q27H_KV_Q8_Q4) return 0;
+  return (size_t)nkvh * page_rows * kv_row_bytes(type, v != 0);
+}
+
+extern "C" int q27h_kv_pages_read(const q27h_kv_pages* kv, const int* from, const int* count, int n_out, int out_type, void* kout,
+                                  void* vout, q27h_stream_t s) {
+  if (const int bad = check_pages(kv, "kv_pages_read")) return bad;
+  if (n_out < 0 || n_out > 1 << 30 || out_type < Q27H_F32 || out_type > Q27H_BF16)
+    return fail(Q27H_ERR_SHAPE, "kv_pages_read: bad n_out or type of the values");
+  if ((double)kv->n_seqs * kv->nkvh * ((n_out + kChunk - 1) / kChunk) > 2.0e9)
+    return fail(Q27H_ERR_SHAPE, "kv_pages_read: too many rows in all");
+  if (kv->n_seqs == 0 || n_out == 0 || (!kout && !vout)) return Q27H_OK;
+  if (!count) return fail(Q27H_ERR_ARG, "kv_pages_read: null pointer");
+  if (!aligned16(kout) || !aligned16(vout)) return fail(Q27H_ERR_ARG, "kv_pages_read: results need 16-byte alignment");
+  if (!aligned4(from) || !aligned4(count)) return fail(Q27H_ERR_ARG, "kv_pages_read: from and count need 4-byte alignment");
+  ReadArgs a = {pages_of(kv), from, count, kout, vout, n_out};
+  const size_t B = (size_t)kv->n_seqs, ob = B * kv->nkvh * n_out * kHeadDim * (out_type == Q27H_F32 ? 4 : 2);
+  if (outputs_overlap({{kout, ob}, {vout, ob}}, {{a.pg.k, a.pg.kb * kv->n_pages}, {a.pg.v, a.pg.vb * kv->n_pages},
+                                                 {a.pg.table, B * kv->max_pages * 4}, {from, B * 4}, {count, B * 4}}))
+    return fail(Q27H_ERR_ARG, "kv_pages_read: a result overlaps another argument");
+  // never more workgroups than there can be pieces
+  const double pieces = (double)B * kv->nkvh * ((n_out + kChunk - 1) / kChunk);
+  const dim3 grid((unsigned)(pieces < kBlocks ? pieces : kBlocks)), block(256);
+  auto launch = [&](auto f32, auto f16, auto bf16) {
+    hipLaunchKernelGGL((out_type == Q27H_F32 ? f32 : out_type == Q27H_F16 ? f16 : bf16), grid, block, 0, stream_of(s), a);
+  };
+  if (kv->type == Q27H_KV_F16)
+    launch(kv_pages_read_kernel<16, 16, AsF32>, kv_pages_read_kernel<16, 16, AsF16>, kv_pages_read_kernel<16, 16, AsBf16>);
+  else if (kv->type == Q27H_KV_Q8)
+    launch(kv_pages_read_kernel<8, 8, AsF32>, kv_pages_read_kernel<8, 8, AsF16>, kv_pages_read_kernel<8, 8, AsBf16>);
+  else
+    launch(kv_pages_read_kernel<8, 4, AsF32>, kv_pages_read_kernel<8, 4, AsF16>, kv_pages_read_kernel<8, 4, AsBf16>);
+  return check_launch("kv_pages_read");
+}

@@ -201,6 +201,79 @@ def attn_blocks(qn, kcache, vcache, pos0, idx, T, nsel, scale, nqh, nkvh, n_ctx,
                                  int(q8), _ptr(o), _ptr(lse), _ptr(ws), _bytes(ws), _stream(s)))
 
 
+# ---------------------------------------------------------------- a batch of sequences over a K/V cache in pages
+KV_F16, KV_Q8, KV_Q8_Q4 = 0, 1, 2  # K and V as f16; both as q8_0; K as q8_0, V in 4 bits
+
+
+def kv_page_bytes(nkvh, page_rows, type, v):
+    """Bytes of a page of K (v False) or of V."""
+    return int(lib().q27h_kv_page_bytes(nkvh, page_rows, type, int(v)))
+
+
+class KvPages:
+    """A layer's K and V pages (tensors of whole pages) with the sequences' table (int32 [n_seqs][max_pages], contiguous); holds
+    the tensors. The table's values may change between calls, its shape may not."""
+
+    def __init__(self, k, v, table, nkvh, page_rows, type):
+        import ctypes
+
+        from ._lib import KvPagesC
+
+        kb, vb = kv_page_bytes(nkvh, page_rows, type, False), kv_page_bytes(nkvh, page_rows, type, True)
+        n = min(_bytes(k) // kb, _bytes(v) // vb) if kb else 0
+        if not table.is_contiguous() or table.dim() != 2 or table.element_size() != 4:
+            raise ValueError("KvPages: the table is a contiguous int32 tensor [n_seqs][max_pages]")
+        self.k, self.v, self.table = k, v, table
+        self.c = KvPagesC(_ptr(k), _ptr(v), _ptr(table), table.shape[0], table.shape[1], n, nkvh, page_rows, type)
+        self.ref = ctypes.addressof(self.c)
+
+
+def attn_prep_paged(qg, k, v, q_norm, k_norm, qn, kv, pos, cu, T, eps, theta_scale, nqh, s=None, rope3=None, rdelta=None):
+    """attn_prep for the new tokens of kv's sequences (tokens cu[b] .. cu[b + 1] - 1, rows pos[b] + t; cu None: one each)."""
+    check(lib().q27h_attn_prep_paged(_ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(qn), kv.ref, _ptr(pos), _ptr(cu), T,
+                                     eps, theta_scale, nqh, _stream(s), _ptr(rope3), _ptr(rdelta)))
+
+
+def attn_paged_ws_bytes(kv, T, max_tokens, nqh):
+    return int(lib().q27h_attn_paged_ws_bytes(kv.ref, T, max_tokens, nqh))
+
+
+def attn_paged(qn, kv, pos, cu, T, max_tokens, scale, nqh, o, ws, s=None, lse=None):
+    """Attention of each sequence's new tokens (at most max_tokens <= 64 each) over its rows in the pages: o f32 [T][nqh][256],
+    lse f32 [T][nqh]; ws: a tensor of attn_paged_ws_bytes() bytes, one per call that may run at a time."""
+    check(lib().q27h_attn_paged(_ptr(qn), kv.ref, _ptr(pos), _ptr(cu), T, max_tokens, scale, nqh, _ptr(o), _ptr(lse), _ptr(ws),
+                                _bytes(ws), _stream(s)))
+
+
+def kv_pages_read(kv, start, count, n_out, kout, vout, s=None):
+    """Rows start[b] .. start[b] + count[b] - 1 (start None: 0) of each sequence as values in kout and vout, float32, float16 or
+    bfloat16 [n_seqs][nkvh][n_out][256] (either may be None)."""
+    import torch
+
+    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    kinds = {types.get(t.dtype, -1) for t in (kout, vout) if t is not None} or {0}
+    if len(kinds) != 1:
+        raise ValueError("kv_pages_read: kout and vout have one type")
+    check(lib().q27h_kv_pages_read(kv.ref, _ptr(start), _ptr(count), n_out, kinds.pop(), _ptr(kout), _ptr(vout), _stream(s)))
+
+
+def draft_verify_ws_bytes(n_seqs, V):
+    return int(lib().q27h_draft_verify_ws_bytes(n_seqs, V))
+
+
+def draft_verify(p, q, ids, parent, u, u_last, cu, n_seqs, V, out, path, n_path, ws, s=None, pos=None):
+    """Which drafted tokens stand and the token after them (out), their rows (path, n_path: kv_accept's), by the uniform numbers u
+    and u_last. p, q: f32 rows of V values, one per token; q None: drafts without probabilities, a tree by parent (None: a
+    chain). pos int32 [n_seqs] (may be None) grows by n_path."""
+    for x in (p, q):
+        if x is not None and x.dim() == 2 and x.stride(1) != 1:
+            raise ValueError("draft_verify: rows of p and q are contiguous")
+    T = ids.numel()
+    ld = lambda x: x.stride(0) if x is not None and x.dim() == 2 and T > 1 else V  # noqa: E731
+    check(lib().q27h_draft_verify(_ptr(p), ld(p), _ptr(q), ld(q), _ptr(ids), _ptr(parent), _ptr(u), _ptr(u_last), _ptr(cu), n_seqs, T, V,
+                                  _ptr(out), _ptr(path), _ptr(n_path), _ptr(pos), _ptr(ws), _bytes(ws), _stream(s)))
+
+
 def rmsnorm_q8(x, w, h, xq, xd, n, rows, eps, s=None, xs=None):
     check(lib().q27h_rmsnorm_q8(_ptr(x), _ptr(w), _ptr(h), _ptr(xq), _ptr(xd), n, rows, eps, _stream(s), _ptr(xs)))
 
