@@ -46,19 +46,23 @@ __device__ __forceinline__ float half_of(uint32_t pair, int hi) {
 }
 // Four int8 codes -> four halves of value code * 2^-9: byte ^ 0x80 = code + 128 = u, which as the low byte of a half is
 // the subnormal u 2^-24; fma(u 2^-24, 2^15, -2^-2) = (u - 128) 2^-9, exact. ev = codes 0, 2; od = codes 1, 3.
+// BIAS 8: bytes of codes 0 .. 15 of (code - 8), the same without the sign's turn.
+template <int BIAS = 128>
 __device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& ev, uint32_t& od) {
-  const h2 k = {(_Float16)32768.0f, (_Float16)32768.0f}, m = {(_Float16)-0.25f, (_Float16)-0.25f};
-  x ^= 0x80808080u;
+  constexpr _Float16 kM = (_Float16)(-0x1p-9f * BIAS);
+  const h2 k = {(_Float16)32768.0f, (_Float16)32768.0f}, m = {kM, kM};
+  if (BIAS == 128) x ^= 0x80808080u;
   const h2 a = __builtin_bit_cast(h2, x & 0x00ff00ffu);
   const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, x, 0x0c030c01u));
   ev = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(a, k, m));
   od = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, k, m));
 }
 // Eight codes in two dwords -> the operand of eight halves; the order of the eight is 0, 2, 1, 3, 4, 6, 5, 7.
+template <int BIAS = 128>
 __device__ __forceinline__ h8 codes8(uint32_t x, uint32_t y) {
   uint32_t r[4];
-  codes_to_half(x, r[0], r[1]);
-  codes_to_half(y, r[2], r[3]);
+  codes_to_half<BIAS>(x, r[0], r[1]);
+  codes_to_half<BIAS>(y, r[2], r[3]);
   return __builtin_bit_cast(h8, (u4){r[0], r[1], r[2], r[3]});
 }
 
@@ -547,8 +551,8 @@ __device__ __forceinline__ void weigh(const u4& ph, const u4& pl, const u2 (&vs)
 }
 
 // O += P V. Output o[i][j]: q8: dim 16 i + 4 g + j; f16: dim 128 (i >> 3) + 8 (4 g + j) + (i & 7).
-// q8: `w` holds the staged codes and scales. TAIL: some rows are hidden, see weigh().
-template <bool TAIL>
+// q8: `w` holds the staged codes and scales. TAIL: some rows are hidden, see weigh(). BIAS: the codes', see codes_to_half.
+template <bool TAIL, int BIAS = 128>
 __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const WaveLds& w) {
   const int l = threadIdx.x & 63, j = l & 15, g = l >> 4;
   // the transposing read: in a group of 16 lanes, lane j gives the address of 8 bytes of row j >> 1 and gets column j of
@@ -569,7 +573,7 @@ __device__ __forceinline__ void accumulate(Rows& st, const f4 (&p)[2], const Wav
   };
   auto turn = [&](int b) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) v[b & 1][h] = codes8((uint32_t)c[b & 1][h].x, (uint32_t)c[b & 1][h].y);
+    for (int h = 0; h < 2; h++) v[b & 1][h] = codes8<BIAS>((uint32_t)c[b & 1][h].x, (uint32_t)c[b & 1][h].y);
     weigh<TAIL>(ph, pl, vs[b & 1], hi[b & 1], lo[b & 1]);
   };
   ask(0);

@@ -43,17 +43,14 @@ __device__ __forceinline__ void load_rows(QRows4& t, const KvHead& h, int j0, in
   t.s = *(const u2*)(h.scale + (ptrdiff_t)j0 * 16 + (unsigned)(tile_row<TAIL>(l >> 1, left) * 16 + 8 * (l & 1)));
   if (TAIL && (l >> 1) >= left) t.s = (u2){0u, 0u};
 }
-// To bytes of code - 8 in LDS, where the 8-bit form has its codes: u + 0x78 = (u - 8) + 0x80 in each byte, without a carry.
+// To bytes in LDS, where the 8-bit form has its codes: the signs are turned and 8 is taken off with the turn to halves.
 __device__ __forceinline__ void stage_values(const QRows4& t, WaveLds& w) {
   const int l = threadIdx.x & 63;
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     u4 lo, hi;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      lo[i] = ((t.x[r][i] & 0x0f0f0f0fu) + 0x78787878u) ^ 0x80808080u;
-      hi[i] = ((t.x[r][i] >> 4 & 0x0f0f0f0fu) + 0x78787878u) ^ 0x80808080u;
-    }
+    for (int i = 0; i < 4; i++) lo[i] = t.x[r][i] & 0x0f0f0f0fu, hi[i] = t.x[r][i] >> 4 & 0x0f0f0f0fu;
     uint8_t* p = w.codes + (r >= 2 ? kUpper + (8 * (r - 2) + (l >> 3)) * kRow : (8 * r + (l >> 3)) * kRow) + 32 * (l & 7);
     *(u4*)p = lo;
     *(u4*)(p + 16) = hi;
@@ -61,6 +58,11 @@ __device__ __forceinline__ void stage_values(const QRows4& t, WaveLds& w) {
   put_value_scales(t.s, w.vs, w.vf);
   __builtin_amdgcn_wave_barrier();
 }
+
+}  // namespace
+template <>
+constexpr int bias_of<QRows4> = 8;
+namespace {
 
 // A tile's place: K and V of its page and head, such that the sequence's row j lies at rows + j * (bytes of a row).
 struct TileAt {
@@ -132,7 +134,7 @@ struct PagedTiles {
       stage_values(v, w);
       if (at.j0 >= 0) load_rows<false>(v, at.v, at.j0, 0);
       loads_issued();
-      accumulate<false>(st, s[0], w);
+      accumulate<false, bias_of<decltype(v)>>(st, s[0], w);
       __builtin_amdgcn_wave_barrier();
     } while (at.j0 >= 0);
   }
@@ -325,29 +327,29 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   });
 }
 
-// Joins the parts of one query row (token t of sequence b, query head h), in order: wave w takes every fourth part, a lane
-// four dims; then the waves' sums are added in order.
-__global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedArgs a, int rows) {
-  __shared__ f4 s_o[kWaves][64];
+// Joins the parts of one query row (token t of sequence b, query head h), in order: wave w of WAVES takes every WAVES-th
+// part, a lane four dims; then the waves' sums are added in order. 16 waves where there are few rows, which may have many
+// parts; 4 where there are many.
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArgs a, int rows) {
+  __shared__ f4 s_o[WAVES][64];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   const int h = blockIdx.x % a.nqh, t = (int)(blockIdx.x / a.nqh) % a.most, b = (int)(blockIdx.x / a.nqh) / a.most;
-  const int start = uniform_load(a.starts + b), total = uniform_load(a.starts + a.pg.n_seqs);
+  const int start = uniform_load(a.starts + b), total = uniform_load(a.starts + a.pg.n_seqs), pos = uniform_load(a.pos + b);
   const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
   if (t >= tk.nt) return;
-  const Vis vis = vis_of(uniform_load(a.pos + b), tk.nt, a.pg.max_pages << a.pg.shift);
-  const Cut cut = cut_of(demand_of(a, tk.nt, vis, rows).span, total);
-  const int n = cut.parts;
+  const Vis vis = vis_of(pos, tk.nt, a.pg.max_pages << a.pg.shift);
+  const int n = cut_of(demand_of(a, tk.nt, vis, rows).span, total).parts;
   if (n == 1) return;
   const int group = a.nqh / a.pg.nkvh, r = t * group + h % group, groups = (tk.nt * group + rows - 1) / rows;
   const size_t place = ((size_t)start + (size_t)(h / group * groups + r / rows) * n) * rows + r % rows;
   const f4* part = (const f4*)(a.part + place * kHD) + l;  // part k: k * rows rows on
   const float2* ml = (const float2*)a.ml + place;
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 4;
   f4 x[kBatch];
-  float2 y[kBatch];
 #pragma unroll
   for (int k = 0; k < kBatch; k++)
-    if (w + kWaves * k < n) x[k] = part[(size_t)(w + kWaves * k) * rows * 64], y[k] = ml[(w + kWaves * k) * rows];
+    if (w + WAVES * k < n) x[k] = part[(size_t)(w + WAVES * k) * rows * 64];
   auto all = [&](float y, auto op) {
     y = op(y, lane_xor<1>(y));
     y = op(y, lane_xor<2>(y));
@@ -356,20 +358,37 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedArgs a, int r
     y = op(y, lane_xor<16>(y));
     return op(y, lane_xor32(y));
   };
-  float m = -3.0e38f, sum = 0.0f;
-  for (int k = l; k < n; k += 64) m = __builtin_fmaxf(m, ml[k * rows].x);  // every wave for itself
+  // every wave for itself, lane l parts l, l + 64, ..
+  float2 v = l < n ? ml[l * rows] : make_float2(-3.0e38f, 0.0f);
+  float m = v.x;
+  for (int k = l + 64; k < n; k += 64) m = __builtin_fmaxf(m, ml[k * rows].x);
   m = all(m, [](float p, float q) { return __builtin_fmaxf(p, q); });
-  for (int k = l; k < n; k += 64) sum += ml[k * rows].y * __builtin_amdgcn_exp2f(ml[k * rows].x - m);
+  const float f = __builtin_amdgcn_exp2f(v.x - m);
+  float sum = v.y * f;
+  for (int k = l + 64; k < n; k += 64) sum += ml[k * rows].y * __builtin_amdgcn_exp2f(ml[k * rows].x - m);
   sum = all(sum, [](float p, float q) { return p + q; });
+  auto factor = [&](int k) {  // of part k, the same in the whole wave
+    return k < 64 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k))
+                  : __builtin_amdgcn_exp2f(ml[k * rows].x - m);
+  };
   f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int w0 = __builtin_amdgcn_readfirstlane(w);
 #pragma unroll
   for (int k = 0; k < kBatch; k++)
-    if (w + kWaves * k < n) o += x[k] * __builtin_amdgcn_exp2f(y[k].x - m);
-  for (int k = w + kWaves * kBatch; k < n; k += kWaves) o += part[(size_t)k * rows * 64] * __builtin_amdgcn_exp2f(ml[k * rows].x - m);
+    if (w0 + WAVES * k < n) o += x[k] * factor(w0 + WAVES * k);
+  for (int k0 = w0 + WAVES * kBatch; k0 < n; k0 += WAVES * kBatch) {
+#pragma unroll
+    for (int k = 0; k < kBatch; k++)
+      if (k0 + WAVES * k < n) x[k] = part[(size_t)(k0 + WAVES * k) * rows * 64];
+#pragma unroll
+    for (int k = 0; k < kBatch; k++)
+      if (k0 + WAVES * k < n) o += x[k] * factor(k0 + WAVES * k);
+  }
   s_o[w][l] = o;
   __syncthreads();
   if (w) return;
-  o = (s_o[0][l] + s_o[1][l]) + (s_o[2][l] + s_o[3][l]);
+#pragma unroll
+  for (int k = 1; k < WAVES; k++) o += s_o[k][l];
   const size_t gr = (size_t)(tk.t0 + t) * a.nqh + h;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   *((f4*)(a.o + gr * kHD) + l) = o * inv;
@@ -439,7 +458,10 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
   if (kv->type == Q27H_KV_F16) launch(attn_paged_kernel<Q27H_KV_F16, 1>, attn_paged_kernel<Q27H_KV_F16, 2>);
   else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_kernel<Q27H_KV_Q8, 2>);
   else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_kernel<Q27H_KV_Q8_Q4, 2>);
-  hipLaunchKernelGGL(attn_paged_join_kernel, dim3((unsigned)(kv->n_seqs * max_tokens * nqh)), dim3(256), 0, stream_of(s), a,
-                     16 * y.wr);
+  const int qrows = kv->n_seqs * max_tokens * nqh;
+  if (qrows <= 2 * kCUs)
+    hipLaunchKernelGGL(attn_paged_join_kernel<16>, dim3((unsigned)qrows), dim3(1024), 0, stream_of(s), a, 16 * y.wr);
+  else
+    hipLaunchKernelGGL(attn_paged_join_kernel<4>, dim3((unsigned)qrows), dim3(256), 0, stream_of(s), a, 16 * y.wr);
   return check_launch("attn_paged");
 }

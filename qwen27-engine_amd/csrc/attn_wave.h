@@ -69,6 +69,9 @@ __device__ __forceinline__ void begin_rows(Rows& st, Queries<false>& q, AttnShar
 }
 
 // A wave's tile of which some rows are hidden or do not exist.
+// VRows: V's form on its way to LDS, bias_of<VRows> that of its codes there.
+template <typename VRows>
+constexpr int bias_of = 128;
 template <typename VRows = QRows>
 __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<true>& q, WaveLds& w,
                                           const Vis& vis, uint64_t tree, int j0) {
@@ -85,7 +88,7 @@ __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHe
   weights<true, true>(st, s[0]);
   __builtin_amdgcn_wave_barrier();
   stage_values(v, w);
-  accumulate<true>(st, s[0], w);
+  accumulate<true, bias_of<VRows>>(st, s[0], w);
   __builtin_amdgcn_wave_barrier();
 }
 __device__ __forceinline__ void tail_tile(Rows& st, const KvHead& kc, const KvHead& vc, const Queries<false>& q, HKeysLds& w,

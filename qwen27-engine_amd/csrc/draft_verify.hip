@@ -73,13 +73,16 @@ __device__ __forceinline__ Walk walk_of(const VerifyArgs& a, int b) {
     return w;
   }
   double rest = 1.0;  // 1 - the probabilities of the refused children
-  for (int t = 1; t < w.nt; t++) {
-    if (__builtin_amdgcn_readlane(parent, t) != w.node) continue;
+  const uint64_t drafts = w.nt > 1 ? (w.nt < 64 ? 1ull << w.nt : 0ull) - 2 : 0ull;  // tokens 1 .. nt - 1
+  for (uint64_t todo = drafts & __ballot(parent == 0); todo;) {
+    const int t = __builtin_ctzll(todo);
+    todo &= todo - 1;
     const int id = __builtin_amdgcn_readlane(w.id, t);
     const bool again = (__ballot(w.id == id) & w.tried) != 0;  // a token that was refused already
     const double x = again ? 0.0 : (double)read_lane(p, t);
     if ((double)read_lane(u, t) * rest < x) {
       w.node = t, w.path |= 1ull << t, w.tried = 0, rest = 1.0;
+      todo = drafts & __ballot(parent == t) & ~((2ull << t) - 1);  // a child lies behind its parent
     } else {
       rest -= x, w.tried |= 1ull << t;
     }
@@ -167,37 +170,44 @@ __device__ __forceinline__ double before_of(double x, double* red, double& total
 
 __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   __shared__ double s_red[kThreads / 64], s_before;
-  __shared__ int s_chunk, s_token;
+  __shared__ int s_chunk, s_token, s_n;
   __shared__ int s_bad[kMostTokens];
+  __shared__ double s_takes[kMostTokens];
   const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63;
   const Walk k = walk_of(a, b);
   if (!k.nt) {
     if (tid == 0) a.n_path[b] = 0;
     return;
   }
-  if (tid == 0) s_chunk = s_token = -1;
-  // the refused children: they weigh nothing. Their ids, each once, in lanes' order.
-  const uint64_t tried = k.tried;
-  if (tid < kMostTokens) s_bad[tid] = (tried >> tid & 1) ? k.id : -1;
-  __syncthreads();
   const float* prow = a.p + (size_t)(k.t0 + k.node) * a.ldp;
   const float* qrow = a.q ? a.q + (size_t)(k.t0 + k.node + 1) * a.ldq : nullptr;
+  // the refused children weigh nothing: their ids, each once, and what they take from their chunks' sums, exactly
+  if (tid < 64) {
+    const bool bad = k.tried >> l & 1;
+    bool first = bad && (unsigned)k.id < (unsigned)a.V;
+    for (uint64_t m = k.tried; m; m &= m - 1) {
+      const int t = __builtin_ctzll(m);
+      if (__builtin_amdgcn_readlane(k.id, t) == k.id && t < l) first = false;
+    }
+    const uint64_t each = __ballot(first);
+    if (first) {
+      const int at = __builtin_popcountll(each & ((1ull << l) - 1));
+      s_bad[at] = k.id;
+      s_takes[at] = weight_of(prow[k.id]);
+    }
+    if (l == 0) s_n = __builtin_popcountll(each), s_chunk = s_token = -1;
+  }
+  __syncthreads();
+  const int n_bad = s_n;
   auto is_bad = [&](int i) {
     bool bad = false;
-    for (uint64_t m = tried; m; m &= m - 1) bad |= s_bad[__builtin_ctzll(m)] == i;
+    for (int j = 0; j < n_bad; j++) bad |= s_bad[j] == i;
     return bad;
   };
   const double2* sums = a.sums + (size_t)b * a.chunks;
-  // what the refused children take from a chunk's sum, exactly: each id once
   auto taken = [&](int chunk) {
     double t = 0.0;
-    for (uint64_t m = tried; m; m &= m - 1) {
-      const int j = __builtin_ctzll(m), id = s_bad[j];
-      if ((unsigned)id >= (unsigned)a.V || id / kChunk != chunk) continue;
-      bool again = false;
-      for (uint64_t e = tried & ((1ull << j) - 1); e; e &= e - 1) again |= s_bad[__builtin_ctzll(e)] == id;
-      if (!again) t += weight_of(prow[id]);
-    }
+    for (int j = 0; j < n_bad; j++) t += s_bad[j] / kChunk == chunk ? s_takes[j] : 0.0;
     return t;
   };
   // the chunk: 256 of them at a time, first their whole sum
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
       for (int i = 0; i < kPerThread; i++)
         wt[i] = i0 + i < a.V ? weight_of(use_q ? (double)prow[i0 + i] - qrow[i0 + i] : (double)prow[i0 + i]) : 0.0;
     }
-    if (tried) {
+    if (n_bad) {
 #pragma unroll
       for (int i = 0; i < kPerThread; i++) wt[i] = is_bad(i0 + i) ? 0.0 : wt[i];
     }

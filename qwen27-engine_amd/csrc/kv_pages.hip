@@ -53,86 +53,69 @@ typedef uint32_t w4 __attribute__((ext_vector_type(4)));
 typedef uint32_t w2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-// Eight neighbouring values to their place.
-__device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 2; i++) __builtin_nontemporal_store((f4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}, (f4*)p + i);
-}
-__device__ __forceinline__ void put8(uint16_t* p, const uint32_t (&h)[8]) {
-  __builtin_nontemporal_store((w4){h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16}, (w4*)p);
-}
+// Values as they are stored: 16 bytes a lane and store, so that the 16 lanes of a row write 256 bytes that lie together (a
+// lane's values one behind the other in several stores would leave every cache line to be written in pieces: 8 sequences
+// of 81250 rows, K in 8 bits and V in 4, to f16: 167 us, @@ so).
 struct AsF32 {
   typedef float type;
-  static __device__ __forceinline__ void put(float* p, const float (&x)[8]) { put8(p, x); }
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ void put(float* p, const float (&x)[kN]) {
+    __builtin_nontemporal_store((f4){x[0], x[1], x[2], x[3]}, (f4*)p);
+  }
 };
 struct AsF16 {
   typedef uint16_t type;
-  static __device__ __forceinline__ void put(uint16_t* p, const float (&x)[8]) {
-    uint32_t h[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = f2h_bits(x[i]);
-    put8(p, h);
-  }
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ uint32_t bits(float x) { return f2h_bits(x); }
 };
 struct AsBf16 {
   typedef uint16_t type;
-  static __device__ __forceinline__ void put(uint16_t* p, const float (&x)[8]) {
-    uint32_t h[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {  // to the nearest, ties to even; NaN stays one
-      const uint32_t b = __builtin_bit_cast(uint32_t, x[i]);
-      h[i] = x[i] != x[i] ? (b >> 16) | 0x40 : (b + 0x7fff + (b >> 16 & 1)) >> 16;
-    }
-    put8(p, h);
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ uint32_t bits(float x) {  // to the nearest, ties to even; NaN stays one
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return x != x ? (b >> 16) | 0x40 : (b + 0x7fff + (b >> 16 & 1)) >> 16;
   }
 };
+template <typename OUT>
+__device__ __forceinline__ void put(typename OUT::type* p, const float (&x)[OUT::kN]) {
+  if constexpr (OUT::kN == 4) {
+    OUT::put(p, x);
+  } else {
+    w4 y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = OUT::bits(x[2 * i]) | OUT::bits(x[2 * i + 1]) << 16;
+    __builtin_nontemporal_store(y, (w4*)p);
+  }
+}
 
-// What a lane has of a row: 16 values, at dims d and d + off. 16 lanes to a row.
-template <int BITS>
-struct Piece;
-template <>
-struct Piece<16> {
-  w4 x[2];
-  __device__ __forceinline__ void load(const uint8_t* head, int n, int row, int l) {
-    const uint8_t* p = head + (size_t)row * kRowF16 + 16 * l;
-    x[0] = *(const w4*)p, x[1] = *(const w4*)(p + 256);
-  }
-  static __device__ __forceinline__ int dim(int l, int i) { return 8 * l + 128 * i; }
-  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
+// What a lane has of a row: N values from dim N l + 16 N i on, i < 16 / N. 16 lanes to a row.
+template <int BITS, int N>
+struct Piece {
+  static constexpr int kStores = 16 / N, kWords = BITS == 4 ? N / 4 : N * BITS / 32;
+  uint32_t x[kStores][kWords];
+  uint16_t d[kStores];
+  __device__ __forceinline__ void load(const uint8_t* page, size_t rows, size_t row, int l) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = h2f_bits((uint16_t)(x[i][e >> 1] >> 16 * (e & 1)));
+    for (int i = 0; i < kStores; i++) {
+      const int dim = N * l + 16 * N * i;
+      // 4 bits: the low halves of bytes e .. of the block, or the high ones
+      const uint8_t* p = page + row * (32 * BITS) + (BITS == 4 ? dim / 32 * 16 + (dim & 15) : dim * (BITS / 8));
+      if constexpr (kWords == 1) x[i][0] = *(const uint32_t*)p;
+      else if constexpr (kWords == 2) *(w2*)x[i] = *(const w2*)p;
+      else *(w4*)x[i] = *(const w4*)p;
+      if constexpr (BITS != 16) d[i] = *((const uint16_t*)(page + rows * (32 * BITS)) + row * 8 + dim / 32);
+    }
   }
-};
-template <>
-struct Piece<8> {
-  w2 x[2];
-  uint16_t d[2];
-  __device__ __forceinline__ void load(const uint8_t* head, const uint8_t* scales, int row, int l) {
-    const uint8_t* p = head + (size_t)row * 256 + 8 * l;
-    x[0] = *(const w2*)p, x[1] = *(const w2*)(p + 128);
-    const uint16_t* s = (const uint16_t*)scales + (size_t)row * 8 + (l >> 2);
-    d[0] = s[0], d[1] = s[4];
-  }
-  static __device__ __forceinline__ int dim(int l, int i) { return 8 * l + 128 * i; }
-  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
-    const float s = h2f_bits(d[i]);
+  __device__ __forceinline__ void values(int i, int l, float (&y)[N]) const {
+    const int high = BITS == 4 ? (N * l + 16 * N * i) & 16 ? 4 : 0 : 0;
+    float s = 0.0f;
+    if constexpr (BITS != 16) s = h2f_bits(d[i]);
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = (float)(int8_t)(x[i][e >> 2] >> 8 * (e & 3)) * s;
-  }
-};
-template <>
-struct Piece<4> {
-  w2 x;
-  uint16_t d;
-  __device__ __forceinline__ void load(const uint8_t* head, const uint8_t* scales, int row, int l) {
-    x = *(const w2*)(head + (size_t)row * 128 + 8 * l);
-    d = *((const uint16_t*)scales + (size_t)row * 8 + (l >> 1));
-  }
-  static __device__ __forceinline__ int dim(int l, int i) { return 32 * (l >> 1) + 8 * (l & 1) + 16 * i; }
-  __device__ __forceinline__ void values(int i, float (&y)[8]) const {
-    const float s = h2f_bits(d);
-#pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = (float)((int)(x[e >> 2] >> (8 * (e & 3) + 4 * i) & 15u) - 8) * s;
+    for (int e = 0; e < N; e++) {
+      if constexpr (BITS == 16) y[e] = h2f_bits((uint16_t)(x[i][e >> 1] >> 16 * (e & 1)));
+      else if constexpr (BITS == 8) y[e] = (float)(int8_t)(x[i][e >> 2] >> 8 * (e & 3)) * s;
+      else y[e] = (float)((int)((x[i][e >> 2] >> high) >> 8 * (e & 3) & 15u) - 8) * s;
+    }
   }
 };
 
@@ -158,8 +141,9 @@ __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
     const int at = sp.x - sp.start, kh = at / chunks, i0 = (at - kh * chunks) * kChunk;
     sp.x++;
     const long long from = a.from ? a.from[b] : 0;
-    Piece<KB> k[2];
-    Piece<VB> v[2];
+    constexpr int N = OUT::kN;
+    Piece<KB, N> k[2];
+    Piece<VB, N> v[2];
     bool is[2];
 #pragma unroll
     for (int s = 0; s < 2; s++) {
@@ -170,36 +154,29 @@ __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
       if (i < count && pi >= 0 && pi < a.pg.max_pages) page = a.pg.table[(size_t)b * a.pg.max_pages + pi];
       is[s] = (unsigned)page < (unsigned)a.pg.n_pages;
       if (!is[s]) continue;
-      const int row = kh * n + (int)(j & (n - 1));
-      const uint8_t *kp = a.pg.k + (size_t)page * a.pg.kb, *vp = a.pg.v + (size_t)page * a.pg.vb;
-      const size_t codes = (size_t)a.pg.nkvh * n;
-      if constexpr (KB == 16) {
-        if (a.kout) k[s].load(kp, 0, row, l);
-        if (a.vout) v[s].load(vp, 0, row, l);
-      } else {
-        if (a.kout) k[s].load(kp, kp + codes * (32 * KB), row, l);
-        if (a.vout) v[s].load(vp, vp + codes * (32 * VB), row, l);
-      }
+      const size_t rows = (size_t)a.pg.nkvh * n, row = (size_t)kh * n + (size_t)(j & (n - 1));
+      if (a.kout) k[s].load(a.pg.k + (size_t)page * a.pg.kb, rows, row, l);
+      if (a.vout) v[s].load(a.pg.v + (size_t)page * a.pg.vb, rows, row, l);
     }
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       const int i = i0 + 16 * s + r;
       if (i >= count) continue;
-      const size_t o = (((size_t)b * a.pg.nkvh + kh) * a.n_out + i) * kHeadDim;
+      const size_t o = (((size_t)b * a.pg.nkvh + kh) * a.n_out + i) * kHeadDim + N * l;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float y[8];
+      for (int h = 0; h < 16 / N; h++) {
+        float y[N];
         if (a.kout) {
-          k[s].values(h, y);
+          k[s].values(h, l, y);
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = is[s] ? y[e] : 0.0f;
-          OUT::put((O*)a.kout + o + Piece<KB>::dim(l, h), y);
+          for (int e = 0; e < N; e++) y[e] = is[s] ? y[e] : 0.0f;
+          put<OUT>((O*)a.kout + o + 16 * N * h, y);
         }
         if (a.vout) {
-          v[s].values(h, y);
+          v[s].values(h, l, y);
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = is[s] ? y[e] : 0.0f;
-          OUT::put((O*)a.vout + o + Piece<VB>::dim(l, h), y);
+          for (int e = 0; e < N; e++) y[e] = is[s] ? y[e] : 0.0f;
+          put<OUT>((O*)a.vout + o + 16 * N * h, y);
         }
       }
     }

@@ -17,12 +17,21 @@ def _ptr(t):
     return t.data_ptr()
 
 
+_raw_stream = None
+
+
 def _stream(s):
     if s is not None:
         return s
-    import torch
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
 
-    return torch.cuda.current_stream().cuda_stream
+        # the handle alone, where this torch gives it: a Stream object takes longer than a launch
+        raw, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+        torch.cuda.init()
+        _raw_stream = (lambda: raw(device())) if raw and device else lambda: torch.cuda.current_stream().cuda_stream
+    return _raw_stream()
 
 
 # ---------------------------------------------------------------- ops.h
