@@ -15,7 +15,6 @@ namespace q27h {
 namespace {
 
 constexpr int kWaves = 4;          // waves that share a segment's tiles
-constexpr int kParts = 2 * kCUs;   // shares of the whole work, see cut_of
 constexpr int kMostTokens = 64;    // tokens of one sequence: hide()'s 64-bit masks
 
 struct PagedArgs {
@@ -24,8 +23,8 @@ struct PagedArgs {
   const int *pos, *cu;
   float *o, *lse;        // lse may be null
   float *part, *ml;      // [place][row of its unit][256], [..][2]
-  int* starts;           // [n_seqs + 1]: each sequence's first place; the total of tiles
-  int T, most, nqh;
+  int* starts;           // [n_seqs + 1]: each sequence's first place; the size of a part
+  int T, most, nqh, slots;  // slots: workgroups that run at a time
   float scale;
 };
 
@@ -179,31 +178,28 @@ __device__ __forceinline__ Demand demand_of(const PagedArgs& a, int nt, const Vi
   const int tiles = vis.end > 0 ? (vis.end + kTileKeys - 1) / kTileKeys : 1;
   return {a.pg.nkvh * ((nt * (a.nqh / a.pg.nkvh) + rows - 1) / rows), (tiles + kWaves - 1) / kWaves * kWaves};
 }
-// A unit of `span` tiles, `total` of them in all, is cut in `parts` of `size`: none is longer than a kParts-th of the total.
-struct Cut {
-  int parts, size;
-};
-__device__ __forceinline__ Cut cut_of(int span, int total) {
-  const int most = ((total + kParts - 1) / kParts + kWaves - 1) / kWaves * kWaves;
-  Cut c;
-  c.parts = (span + most - 1) / most;
-  c.size = ((span + c.parts - 1) / c.parts + kWaves - 1) / kWaves * kWaves;
-  c.parts = (span + c.size - 1) / c.size;  // rounding up to a step may leave the last one nothing
-  return c;
+// Every unit is cut in parts of one size, its last one what is left: the total by the workgroups that run at a time.
+__device__ __forceinline__ int size_of(int total, int slots) {
+  const int each = (total + slots - 1) / slots;
+  return each ? (each + kWaves - 1) / kWaves * kWaves : kWaves;
 }
 
-// The part that a workgroup has: sequence, unit of it, the part's number in the unit and the unit's cut, its total of tiles,
-// and the part's place in the workspace. seq < 0: none. The first workgroup leaves for the join where the places of each
-// sequence begin, and the total behind them.
+// The part that a workgroup has: sequence, unit of it, the part's number in the unit and how many it has, their size, and
+// the part's place in the workspace. seq < 0: none. Whole parts come before those that are left over, and of these the ones
+// over half the size before the others: workgroups start in this order as others end, so that the last to end are short (48
+// sequences of 500 to 32768 rows, 704 parts in any order: @@, so @@). The first workgroup leaves for the join where the
+// places of each sequence begin, and the size behind them.
 struct Part {
-  int seq, unit, k, place;
-  Cut cut;
+  int seq, unit, k, parts, size, place;
+};
+struct Counts {
+  uint64_t a, b;  // whole parts, and above them places of parts that are joined; large rests, and above them small ones
 };
 template <int THREADS>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   constexpr int kW = THREADS / 64;
   __shared__ int s_total[kW], s_part[3];
-  __shared__ uint64_t s_count[kW];
+  __shared__ Counts s_count[kW];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, cap = a.pg.max_pages << a.pg.shift;
   const int each = (a.pg.n_seqs + THREADS - 1) / THREADS, b0 = tid * each;
   const int b1 = b0 + each < a.pg.n_seqs ? b0 + each : a.pg.n_seqs;
@@ -225,46 +221,63 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   int total = 0;
 #pragma unroll
   for (int k = 0; k < kW; k++) total += s_total[k];
-  // workgroups below, and above them the places of the parts that are joined
+  Part p;
+  p.size = size_of(total, a.slots);
   auto count = [&](const Demand& d) {
-    const int parts = cut_of(d.span, total).parts;
-    const uint64_t n = (uint64_t)d.units * parts;
-    return d.units == 0 ? 0ull : parts > 1 ? n << 32 | n : n;
+    const int whole = d.span / p.size, rest = d.span - whole * p.size;
+    const uint32_t u = (uint32_t)d.units, parts = whole + (rest > 0);
+    return Counts{(uint64_t)(parts > 1 ? u * parts : 0) << 32 | u * whole,
+                  rest == 0 ? 0ull : 2 * rest > p.size ? (uint64_t)u : (uint64_t)u << 32};
   };
-  uint64_t mine = count(first);
-  for (int b = b0 + 1; b < b1; b++) mine += count(demand(b));
-  uint64_t before = mine;
+  Counts mine = count(first);
+  for (int b = b0 + 1; b < b1; b++) {
+    const Counts c = count(demand(b));
+    mine.a += c.a, mine.b += c.b;
+  }
+  Counts at = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint64_t y = __shfl_up(before, d);
-    before += l >= d ? y : 0;
+    const uint64_t x = __shfl_up(at.a, d), y = __shfl_up(at.b, d);
+    at.a += l >= d ? x : 0, at.b += l >= d ? y : 0;
   }
-  if (l == 63) s_count[w] = before;
+  if (l == 63) s_count[w] = at;
   __syncthreads();
-  before -= mine;
+  at.a -= mine.a, at.b -= mine.b;
+  Counts all = {0, 0};
 #pragma unroll
-  for (int k = 0; k < kW; k++) before += k < w ? s_count[k] : 0;
-  const int me = (int)blockIdx.x;
-  const bool here = (int)before <= me && me < (int)(before + mine);
-  if (me == 0 && tid == 0) a.starts[a.pg.n_seqs] = total;
-  if (me == 0 || here) {
-    uint64_t at = before;
+  for (int k = 0; k < kW; k++) {
+    if (k < w) at.a += s_count[k].a, at.b += s_count[k].b;
+    all.a += s_count[k].a, all.b += s_count[k].b;
+  }
+  // the workgroup's number among the whole parts, the large rests or the small ones
+  int me = (int)blockIdx.x, kind = 0;
+  if (me >= (int)all.a) me -= (int)all.a, kind = 1;
+  if (kind == 1 && me >= (int)all.b) me -= (int)all.b, kind = 2;
+  auto of_kind = [&](const Counts& c) { return kind == 0 ? (int)c.a : kind == 1 ? (int)c.b : (int)(c.b >> 32); };
+  const int lo = of_kind(at);
+  const bool lead = blockIdx.x == 0, here = lo <= me && me < lo + of_kind(mine);
+  if (lead && tid == 0) a.starts[a.pg.n_seqs] = p.size;
+  if (lead || here) {
     for (int b = b0; b < b1; b++) {
-      const uint64_t n = count(b == b0 ? first : demand(b));
-      if (me == 0) a.starts[b] = (int)(at >> 32);
-      if ((int)at <= me && me < (int)(at + n)) s_part[0] = b, s_part[1] = me - (int)at, s_part[2] = (int)(at >> 32);
-      at += n;
+      const Counts c = count(b == b0 ? first : demand(b));
+      const int x = of_kind(at);
+      if (lead) a.starts[b] = (int)(at.a >> 32);
+      if (x <= me && me < x + of_kind(c)) s_part[0] = b, s_part[1] = me - x, s_part[2] = (int)(at.a >> 32);
+      at.a += c.a, at.b += c.b;
     }
   }
   __syncthreads();
-  Part p;
+  p.size = __builtin_amdgcn_readfirstlane(p.size);
   p.seq = __builtin_amdgcn_readfirstlane(s_part[0]);
   if (p.seq < 0) return p;
   const int i = __builtin_amdgcn_readfirstlane(s_part[1]);
+  kind = __builtin_amdgcn_readfirstlane(kind);
   const Tokens tk = tokens_of(a.cu, p.seq, a.T, a.most);
-  p.cut = cut_of(demand_of(a, tk.nt, vis_of(uniform_load(a.pos + p.seq), tk.nt, cap), rows).span, __builtin_amdgcn_readfirstlane(total));
-  p.unit = i / p.cut.parts, p.k = i - p.unit * p.cut.parts;
-  p.place = __builtin_amdgcn_readfirstlane(s_part[2]) + i;
+  const int span = demand_of(a, tk.nt, vis_of(uniform_load(a.pos + p.seq), tk.nt, cap), rows).span, whole = span / p.size;
+  p.parts = (span + p.size - 1) / p.size;
+  p.unit = kind == 0 ? i / whole : i;
+  p.k = kind == 0 ? i - p.unit * whole : whole;
+  p.place = __builtin_amdgcn_readfirstlane(s_part[2]) + p.unit * p.parts + p.k;
   return p;
 }
 
@@ -281,7 +294,7 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   const Vis vis = vis_of(uniform_load(a.pos + pt.seq), tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
   const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
-  const int t0 = pt.k * pt.cut.size, t1 = t0 + pt.cut.size < tiles ? t0 + pt.cut.size : tiles;
+  const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
   const int full = vis.n / kTileKeys < t1 ? vis.n / kTileKeys : t1;
   auto row = [&](int r) {  // the global row (token * nqh + head) of the unit's query row r, or -1
     r += first;
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
     if constexpr (TYPE == Q27H_KV_Q8_Q4) tail_tile<QRows4>(st, at.k, at.v, q, sh.w[w], vis, chain, at.j0);
     else tail_tile(st, at.k, at.v, q, sh.w[w], vis, chain, at.j0);
   }
-  const bool whole = pt.cut.parts == 1;
+  const bool whole = pt.parts == 1;
   const size_t place = (size_t)pt.place * kRows + mine;
   finish<Q8, WR, kWaves>(st, sh, [&a, gr, whole, place](Rows& st, float m, float sum) {
     if (gr < 0) return;
@@ -327,6 +340,377 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   });
 }
 
+// ---------------------------------------------------------------- more than 16 query rows
+// A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
+// of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
+// query rows, and a wave holds a quarter of the outputs. The weights go from the one to the other through LDS. K is loaded
+// as the matrix operand it becomes; V's slice of 64 dims goes through the wave's own LDS, to be read transposed.
+//
+// One reference E for each query row, the same in all waves: a row's product of weight and V scale is 2^(s - E) f d, f the
+// power of two above the V row's scales and d what is left of each (at most 1). E moves when a row's s + log2 f passes
+// E + 15, to 12 below it, so that what enters the product as two f16 terms is in their range, as in attn_core.h; the sum of
+// the weights is kept in units of 2^E as well. Rows whose V scales are all 0 count as f = 2^-25.
+constexpr int kWideTile = kWaves * kTileKeys;
+template <int QT>
+struct WideLds {
+  union {
+    QTile q[QT];
+    alignas(16) uint8_t v[kWaves][kWideTile * 64];  // row r's 16-byte piece c at c ^ (r >> 2 & 1 | r >> 3 & 2)
+  };
+  alignas(16) uint32_t lo[QT][8][64][4];          // the queries' second terms
+  alignas(16) uint32_t p[QT][kWaves][2][64][4];  // weights as operands: two terms of 32 rows
+  alignas(16) uint8_t ks[kWaves][kScales], vs[kWaves][kScales];
+  alignas(16) float f[kWaves][kTileKeys], lf[kWaves][kTileKeys];  // f and its logarithm
+  float mx[kWaves][QT][16], l[kWaves][QT][16];
+};
+
+// The tile's groups of 32 rows, one behind the other in the sequence; where the page of one lies, or null.
+struct WideTile {
+  const uint8_t *k, *ks, *vs;  // of the wave's own group
+  int page[kWaves], left[kWaves], mine;  // rows that exist; those of the wave's own group
+  int j0;
+};
+
+template <int TYPE>
+struct WideRegs {
+  u2 k[2][8];  // operand of block b, rows 16 u + n: dims 32 b + 8 g ..
+  u4 v[TYPE == Q27H_KV_Q8_Q4 ? 4 : 8];
+  u2 ks, vs;
+};
+
+// Rows behind the last one that exists are read from it, a group of which none does from row 0 of a page; their scales are 0.
+template <int TYPE>
+__device__ __forceinline__ void wide_load_k(WideRegs<TYPE>& r, const WideTile& t, int l) {
+  const int n = l & 15, g = l >> 4, last = t.mine > 0 ? t.mine - 1 : 0;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int row = 16 * u + n < last ? 16 * u + n : last;
+#pragma unroll
+    for (int b = 0; b < 8; b++) r.k[u][b] = *(const u2*)(t.k + (unsigned)(row * kHD + 8 * g) + 32 * b);
+  }
+  const unsigned at = ((l >> 1) < last ? (l >> 1) : last) * 16 + 8 * (l & 1);
+  r.ks = *(const u2*)(t.ks + at);
+  r.vs = *(const u2*)(t.vs + at);
+}
+template <int TYPE>
+__device__ __forceinline__ void wide_load_v(WideRegs<TYPE>& r, const WideTile& t, const Pages& pg, int kh, int w, int l) {
+#pragma unroll
+  for (int k = 0; k < kWaves; k++) {
+    const int last = t.left[k] > 0 ? t.left[k] - 1 : 0, n = 1 << pg.shift;
+    const uint8_t* v = pg.v + (size_t)t.page[k] * pg.vb + ((size_t)kh * n + ((t.j0 + kTileKeys * k) & (n - 1))) * (TYPE == Q27H_KV_Q8_Q4 ? kHD / 2 : kHD);
+    if constexpr (TYPE == Q27H_KV_Q8_Q4) {
+      r.v[k] = *(const u4*)(v + (unsigned)(((l >> 1) < last ? (l >> 1) : last) * (kHD / 2) + 32 * w + 16 * (l & 1)));
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int row = 16 * h + (l >> 2) < last ? 16 * h + (l >> 2) : last;
+        r.v[2 * k + h] = *(const u4*)(v + (unsigned)(row * kHD + 64 * w + 16 * (l & 3)));
+      }
+    }
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* lds, int l) {
+  auto at = [&](int row, int c) { return (u4*)(lds + row * 64 + ((c ^ ((row >> 2 & 1) | (row >> 3 & 2))) * 16)); };
+#pragma unroll
+  for (int k = 0; k < kWaves; k++) {
+    if constexpr (TYPE == Q27H_KV_Q8_Q4) {
+      u4 lo, hi;
+#pragma unroll
+      for (int i = 0; i < 4; i++) lo[i] = r.v[k][i] & 0x0f0f0f0fu, hi[i] = r.v[k][i] >> 4 & 0x0f0f0f0fu;
+      *at(32 * k + (l >> 1), 2 * (l & 1)) = lo;
+      *at(32 * k + (l >> 1), 2 * (l & 1) + 1) = hi;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++) *at(32 * k + 16 * h + (l >> 2), l & 3) = r.v[2 * k + h];
+    }
+  }
+}
+
+// Scores of the wave's 32 rows and QT row tiles: as attn_core.h's, K's codes from registers.
+template <int QT>
+__device__ __forceinline__ void wide_scores(const u2 (&k)[2][8], const uint8_t* ks, const h8 (&hi)[QT][8],
+                                            const uint32_t (*lo)[8][64][4], f4 (&s)[QT][2]) {
+  const int l = threadIdx.x & 63;
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < QT; q++) s[q][0] = s[q][1] = zero;
+  h8 ql[QT], x[2];
+  u2 sc[2][2];
+  f4 c[QT][2];
+  auto ask = [&](int b) {
+#pragma unroll
+    for (int q = 0; q < QT; q++) ql[q] = *(const h8*)lo[q][b][l];
+#pragma unroll
+    for (int u = 0; u < 2; u++) sc[b & 1][u] = scales_of(ks, b, u);
+  };
+  auto turn = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) x[u] = codes8(k[u][b].x, k[u][b].y);
+  };
+  ask(0);
+  turn(0);
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < QT; q++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[q][u] = mfma16(x[u], ql[q], zero);
+    if (b < 7) ask(b + 1);
+#pragma unroll
+    for (int q = 0; q < QT; q++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) c[q][u] = mfma16(x[u], hi[q][b], c[q][u]);
+    if (b < 7) turn(b + 1);  // while the products are on their way
+#pragma unroll
+    for (int q = 0; q < QT; q++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          s[q][u][i] = __builtin_fmaf(half_of(sc[b & 1][u][i & 1], i >> 1), c[q][u][i], s[q][u][i]);
+        asm("" : "+v"(s[q][u]));
+      }
+  }
+}
+
+template <int TYPE, int QT>
+__global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedArgs a) {
+  constexpr int kRows = 16 * QT, kV = TYPE == Q27H_KV_Q8_Q4 ? kHD / 2 : kHD, kBias = TYPE == Q27H_KV_Q8_Q4 ? 8 : 128;
+  __shared__ WideLds<QT> sh;
+  const Part pt = part_of<kWaves * 64>(a, kRows);
+  if (pt.seq < 0) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const int group = a.nqh / a.pg.nkvh;
+  const Tokens tk = tokens_of(a.cu, pt.seq, a.T, a.most);
+  const Vis vis = vis_of(uniform_load(a.pos + pt.seq), tk.nt, a.pg.max_pages << a.pg.shift);
+  const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
+  const int tiles = a.pg.n_pages ? (vis.end + kTileKeys - 1) / kTileKeys : 0;  // without a page there is nothing to read
+  const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
+  auto row = [&](int r) {  // the global row (token * nqh + head) of the unit's query row r, or -1
+    r += first;
+    return r < rows ? (tk.t0 + r / group) * a.nqh + kh * group + r % group : -1;
+  };
+  const int* table = a.pg.table + (size_t)pt.seq * a.pg.max_pages;
+  const int prow = 1 << a.pg.shift;
+  int page[kWaves];
+  auto ask_pages = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < kWaves; k++) page[k] = t + k < t1 ? uniform_load(table + ((t + k) >> (a.pg.shift - 5))) : -1;
+  };
+  WideTile wt;
+  bool whole;  // every row of the tile is seen by every query
+  auto place = [&](int t) {
+    whole = (t + kWaves) * kTileKeys <= vis.n && t + kWaves <= t1;
+    wt.j0 = t * kTileKeys;
+#pragma unroll
+    for (int k = 0; k < kWaves; k++) {
+      const int j0 = (t + k) * kTileKeys;
+      const bool is = (unsigned)page[k] < (unsigned)a.pg.n_pages;
+      whole = whole && is;
+      wt.left[k] = is ? (vis.end - j0 < kTileKeys ? vis.end - j0 : kTileKeys) : 0;
+      wt.page[k] = is ? page[k] : 0;
+      if (k != w) continue;
+      const size_t at = (size_t)kh * prow + (j0 & (prow - 1)), p = wt.page[k];
+      wt.mine = wt.left[k];
+      wt.k = a.pg.k + p * a.pg.kb + at * kHD;
+      wt.ks = a.pg.k + p * a.pg.kb + (size_t)a.pg.nkvh * prow * kHD + at * 16;
+      wt.vs = a.pg.v + p * a.pg.vb + (size_t)a.pg.nkvh * prow * kV + at * 16;
+    }
+  };
+  WideRegs<TYPE> r;
+  if (t0 < t1) {
+    ask_pages(t0);
+    place(t0);
+    wide_load_k(r, wt, l);
+    wide_load_v(r, wt, a.pg, kh, w, l);
+    ask_pages(t0 + kWaves);
+  }
+  load_queries<true, kWaves, QT>(sh.q, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
+  });
+  __syncthreads();
+  h8 hi[QT][8];
+  float c[QT], e[QT], sum[QT];
+  f4 o[QT][4];
+#pragma unroll
+  for (int q = 0; q < QT; q++) {
+    c[q] = sh.q[q].c[n];
+    e[q] = -3.0e38f, sum[q] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 8; b++) hi[q][b] = *(const h8*)sh.q[q].v[0][b][l];
+#pragma unroll
+    for (int b = 0; b < 8; b += kWaves) *(h8*)sh.lo[q][b + w][l] = *(const h8*)sh.q[q].v[1][b + w][l];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[q][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __syncthreads();
+
+  int t = t0;
+  auto step = [&](auto hidden) __attribute__((always_inline)) {
+    constexpr bool kPart = decltype(hidden)::value;
+    const int left = wt.mine;
+    f4 s[QT][2];
+    int lane = l;
+    asm volatile("" : "+v"(lane));  // addresses are formed for each tile: kept over the loop they would spill
+    const int n = lane & 15, g = lane >> 4;
+    if (kPart && (lane >> 1) >= left) r.ks = r.vs = (u2){0u, 0u};
+    put_scales(r.ks, sh.ks[w]);
+    // V's scales: f, and what is left of them
+    u2 vs;
+    {
+      float x[4], m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[i] = half_of(i < 2 ? r.vs.x : r.vs.y, i & 1);
+        m = __builtin_fabsf(x[i]) < 65536.0f ? __builtin_fmaxf(m, __builtin_fabsf(x[i])) : m;
+      }
+      m = __builtin_fmaxf(m, lane_xor<1>(m));
+      const int ex = (int)(__builtin_bit_cast(uint32_t, m) >> 23) - 126;  // 2^(ex - 1) <= m < 2^ex
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = m > 0.0f ? __builtin_amdgcn_ldexpf(x[i], -ex) : x[i];
+      vs = (u2){pk_rtz(x[0], x[1]), pk_rtz(x[2], x[3])};
+      const int lf = m > 0.0f ? ex : -25;
+      if (!(lane & 1)) sh.lf[w][lane >> 1] = (float)lf, sh.f[w][lane >> 1] = exp2i((uint32_t)(127 + lf));
+    }
+    __builtin_amdgcn_wave_barrier();
+    wide_scores<QT>(r.k, sh.ks[w], hi, sh.lo, s);
+    t += kWaves;
+    if (t < t1) {
+      place(t);
+      wide_load_k(r, wt, lane);
+      ask_pages(t + kWaves);
+    }
+    loads_issued();
+    if (kPart) {
+      Vis mine = vis;
+      int m = n;
+      asm volatile("" : "+v"(m));
+      uint64_t chain[QT];
+#pragma unroll
+      for (int q = 0; q < QT; q++) chain[q] = row(16 * q + m) >= 0 ? ~0ull >> (63 - (first + 16 * q + m) / group) : 0ull;
+      if (left <= 0) mine.n = mine.end = 0;
+      hide<QT, kHidden>(s, mine, chain, (t - kWaves + w) * kTileKeys);
+    }
+    const f4 lf[2] = {*(const f4*)&sh.lf[w][4 * g], *(const f4*)&sh.lf[w][16 + 4 * g]};
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+      float mx = -3.0e38f;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, __builtin_fmaf(s[q][u][i], c[q], lf[u][i]));
+      mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
+      mx = __builtin_fmaxf(mx, lane_xor32(mx));
+      if (g == 0) sh.mx[w][q][n] = mx;
+    }
+    __syncthreads();  // the outputs of the tile before are formed: what the waves share is free
+    const f4 f[2] = {*(const f4*)&sh.f[w][4 * g], *(const f4*)&sh.f[w][16 + 4 * g]};
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+      const float mx = __builtin_fmaxf(__builtin_fmaxf(sh.mx[0][q][n], sh.mx[1][q][n]), __builtin_fmaxf(sh.mx[2][q][n], sh.mx[3][q][n]));
+      if (__any(mx - e[q] > 15.0f)) {
+        const float to = mx - e[q] > 15.0f ? mx - 12.0f : e[q];  // by its own row alone
+        const float x = __builtin_amdgcn_exp2f(e[q] - to);
+        e[q] = to;
+        sum[q] *= x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[q][i] *= x;
+      }
+      f4 p[2];
+      float add = 0.0f;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float x = s[q][u][i], y = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[q], -e[q]));
+          const float z = kPart && __builtin_bit_cast(uint32_t, x) == kHidden ? -0.0f : y;
+          add += z;
+          p[u][i] = z * f[u][i];
+        }
+      sum[q] += add;
+      u4 ph, pl;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {  // pairs of rows (0, 2), (1, 3), as codes8 orders them
+        const float w0 = p[k >> 1][k & 1], w1 = p[k >> 1][(k & 1) + 2];
+        ph[k] = pk_rtz(w0, w1);
+        pl[k] = pk_rtz(minus_half(w0, ph[k], 0), minus_half(w1, ph[k], 1));
+      }
+      *(u4*)sh.p[q][w][0][lane] = ph;
+      *(u4*)sh.p[q][w][1][lane] = pl;
+    }
+    put_scales(vs, sh.vs[w]);
+    wide_stage_v(r, sh.v[w], lane);
+    if (t < t1) wide_load_v(r, wt, a.pg, kh, w, lane);
+    loads_issued();
+    __syncthreads();
+    // O += P V: the wave's two blocks of 32 dims
+    const int vrow = (n >> 1) >= 4 ? 12 + 4 * g + (n >> 1) : 4 * g + (n >> 1);  // the transposing read, see attn_core.h
+    const uint8_t* vbase = sh.v[w] + vrow * 64 + 8 * (n & 1);
+    const int vx = (vrow >> 2 & 1) | (vrow >> 3 & 2);
+#pragma unroll
+    for (int k = 0; k < kWaves; k++) {
+      __builtin_amdgcn_sched_barrier(0);
+      u4 ph[QT], pl[QT];
+#pragma unroll
+      for (int q = 0; q < QT; q++) ph[q] = *(const u4*)sh.p[q][k][0][lane], pl[q] = *(const u4*)sh.p[q][k][1][lane];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        u2 d[2];
+        u4 wh[QT], wl[QT];
+#pragma unroll
+        for (int u = 0; u < 2; u++) d[u] = scales_of(sh.vs[k], 2 * w + b, u);
+#pragma unroll
+        for (int q = 0; q < QT; q++) weigh<kPart>(ph[q], pl[q], d, wh[q], wl[q]);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          typedef int v2i __attribute__((ext_vector_type(2)));
+          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) v2i*)(vbase + 2048 * k + ((2 * b + h) ^ vx) * 16));
+          const h8 v = codes8<kBias>((uint32_t)x.x, (uint32_t)x.y);
+#pragma unroll
+          for (int q = 0; q < QT; q++) o[q][2 * b + h] = mfma16(v, __builtin_bit_cast(h8, wl[q]), o[q][2 * b + h]);
+#pragma unroll
+          for (int q = 0; q < QT; q++) o[q][2 * b + h] = mfma16(v, __builtin_bit_cast(h8, wh[q]), o[q][2 * b + h]);
+        }
+      }
+    }
+  };
+  while (t < t1) {
+    while (t < t1 && whole) step(std::false_type());
+    if (t < t1) step(std::true_type());
+  }
+#pragma unroll
+  for (int q = 0; q < QT; q++) {
+    sum[q] += lane_xor<16>(sum[q]);
+    sum[q] += lane_xor32(sum[q]);
+    if (g == 0) sh.l[w][q][n] = sum[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < QT; q++) {
+    const int gr = row(16 * q + n);
+    if (gr < 0) continue;
+    const float total = (sh.l[0][q][n] + sh.l[1][q][n]) + (sh.l[2][q][n] + sh.l[3][q][n]);
+    const bool lead = w == 0 && g == 0;
+    float x = 512.0f;  // codes8's 2^-9
+    float* dst;
+    if (pt.parts == 1) {
+      x = total == 0.0f ? 0.0f : x / total;
+      dst = a.o + (size_t)gr * kHD;
+      if (a.lse && lead) a.lse[gr] = total == 0.0f ? -__builtin_huge_valf() : (e[q] + __builtin_amdgcn_logf(total)) * kLn2;
+    } else {
+      const size_t at = (size_t)pt.place * kRows + 16 * q + n;
+      dst = a.part + at * kHD;
+      if (lead) *(float2*)(a.ml + at * 2) = make_float2(e[q], total);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) *(f4*)(dst + 64 * w + 16 * i + 4 * g) = o[q][i] * x;
+  }
+}
+
 // Joins the parts of one query row (token t of sequence b, query head h), in order: wave w of WAVES takes every WAVES-th
 // part, a lane four dims; then the waves' sums are added in order. 16 waves where there are few rows, which may have many
 // parts; 4 where there are many.
@@ -335,11 +719,11 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
   __shared__ f4 s_o[WAVES][64];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   const int h = blockIdx.x % a.nqh, t = (int)(blockIdx.x / a.nqh) % a.most, b = (int)(blockIdx.x / a.nqh) / a.most;
-  const int start = uniform_load(a.starts + b), total = uniform_load(a.starts + a.pg.n_seqs), pos = uniform_load(a.pos + b);
+  const int start = uniform_load(a.starts + b), size = uniform_load(a.starts + a.pg.n_seqs), pos = uniform_load(a.pos + b);
   const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
   if (t >= tk.nt) return;
   const Vis vis = vis_of(pos, tk.nt, a.pg.max_pages << a.pg.shift);
-  const int n = cut_of(demand_of(a, tk.nt, vis, rows).span, total).parts;
+  const int n = (demand_of(a, tk.nt, vis, rows).span + size - 1) / size;
   if (n == 1) return;
   const int group = a.nqh / a.pg.nkvh, r = t * group + h % group, groups = (tk.nt * group + rows - 1) / rows;
   const size_t place = ((size_t)start + (size_t)(h / group * groups + r / rows) * n) * rows + r % rows;
@@ -396,19 +780,22 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
 }
 
 struct Layout {
-  int wr, grid;
+  int wr, threads, slots, grid;
   size_t places, bytes;
 };
-// Up to 16 query rows a kv head: one row tile, two workgroups of four waves a compute unit; more: two row tiles, whose waves
-// read the same cache rows, one workgroup of eight.
-Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh) {
+// Up to 16 query rows a kv head: one row tile. Two workgroups of four waves run on a compute unit, or one of eight (f16,
+// two row tiles, whose waves read the same cache rows).
+Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   Layout y;
   const int rows = max_tokens * (nqh / nkvh);
   y.wr = rows <= 16 ? 1 : 2;
-  // cut_of gives a unit at most one part more than its share of kParts, and two at least where it is cut at all
+  y.threads = y.wr == 2 && type == Q27H_KV_F16 ? 512 : 256;
+  y.slots = 2 * kCUs * 256 / y.threads;
+  // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has two
+  // parts at least and not two more than its share
   const int units = n_seqs * nkvh * ((rows + 16 * y.wr - 1) / (16 * y.wr));
-  y.grid = units + kParts;
-  y.places = (size_t)(y.grid < 2 * kParts ? y.grid : 2 * kParts) * 16 * y.wr;
+  y.grid = units + y.slots;
+  y.places = (size_t)(y.grid < 2 * y.slots ? y.grid : 2 * y.slots) * 16 * y.wr;
   y.bytes = y.places * (kHD + 2) * sizeof(float) + ((size_t)n_seqs + 1) * sizeof(int);
   return y;
 }
@@ -423,7 +810,7 @@ using namespace q27h;
 
 extern "C" size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int max_tokens, int nqh) {
   if (check_pages(kv, "attn_paged") != Q27H_OK || T <= 0 || !shape_ok(kv, max_tokens, nqh)) return 0;
-  return layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh).bytes;
+  return layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh, kv->type).bytes;
 }
 
 extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens,
@@ -442,7 +829,7 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
   if (!qn || !pos || !o) return fail(Q27H_ERR_ARG, "attn_paged: null pointer");
   if (!aligned16(qn) || !aligned16(o) || !aligned16(ws)) return fail(Q27H_ERR_ARG, "attn_paged: tensors need 16-byte alignment");
   if (!aligned4(pos) || !aligned4(cu) || !aligned4(lse)) return fail(Q27H_ERR_ARG, "attn_paged: pos, cu and lse need 4-byte alignment");
-  const Layout y = layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh);
+  const Layout y = layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh, kv->type);
   if (ws_bytes < y.bytes || !ws) return fail(Q27H_ERR_ARG, "attn_paged: workspace too small");
   const Pages pg = pages_of(kv);
   const size_t qb = (size_t)T * nqh * kHD * 4, B = (size_t)kv->n_seqs;
@@ -452,12 +839,13 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
     return fail(Q27H_ERR_ARG, "attn_paged: o, lse or ws overlaps another argument");
   PagedArgs a = {};
   a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
+  a.slots = y.slots;
   a.part = (float*)ws, a.ml = a.part + y.places * kHD, a.starts = (int*)(a.ml + y.places * 2);
-  const dim3 grid((unsigned)y.grid), block(256 * y.wr);
+  const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);
   auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.wr == 1 ? one : two), grid, block, 0, stream_of(s), a); };
   if (kv->type == Q27H_KV_F16) launch(attn_paged_kernel<Q27H_KV_F16, 1>, attn_paged_kernel<Q27H_KV_F16, 2>);
-  else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_kernel<Q27H_KV_Q8, 2>);
-  else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_kernel<Q27H_KV_Q8_Q4, 2>);
+  else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_wide_kernel<Q27H_KV_Q8, 2>);
+  else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_wide_kernel<Q27H_KV_Q8_Q4, 2>);
   const int qrows = kv->n_seqs * max_tokens * nqh;
   if (qrows <= 2 * kCUs)
     hipLaunchKernelGGL(attn_paged_join_kernel<16>, dim3((unsigned)qrows), dim3(1024), 0, stream_of(s), a, 16 * y.wr);
