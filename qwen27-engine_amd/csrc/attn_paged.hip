@@ -191,12 +191,64 @@ __device__ __forceinline__ int size_of(int total, int slots) {
 // places of each sequence begin, and the size behind them.
 struct Part {
   int seq, unit, k, parts, size, place;
+  Tokens tk;
+  int pos;
 };
 struct Counts {
   uint64_t a, b;  // whole parts, and above them places of parts that are joined; large rests, and above them small ones
 };
+// Sums over the lanes up to each one.
+__device__ __forceinline__ int lanes_before(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31: the rows before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+// Up to 64 sequences: every wave finds the part by itself, a sequence in each lane, without a barrier.
+__device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
+  const int l = threadIdx.x & 63, cap = a.pg.max_pages << a.pg.shift;
+  const bool is = l < a.pg.n_seqs;
+  int c0 = l, c1 = l + 1, pos = 0;
+  if (is) {
+    pos = a.pos[l];
+    if (a.cu) c0 = a.cu[l], c1 = a.cu[l + 1];
+  }
+  const Tokens tk = tokens_of(c0, c1, a.T, a.most);
+  const Demand d = is ? demand_of(a, tk.nt, vis_of(pos, tk.nt, cap), rows) : Demand{0, kWaves};
+  Part p;
+  p.size = size_of(__builtin_amdgcn_readlane(lanes_before(d.units * d.span), 63), a.slots);
+  const int whole = d.span / p.size, rest = d.span - whole * p.size, parts = whole + (rest > 0);
+  const int n0 = d.units * whole, n1 = 2 * rest > p.size ? d.units : 0, n2 = rest && !n1 ? d.units : 0, np = parts > 1 ? d.units * parts : 0;
+  const int s0 = lanes_before(n0), s1 = lanes_before(n1), s2 = lanes_before(n2), sp = lanes_before(np);
+  const int all0 = __builtin_amdgcn_readlane(s0, 63), all1 = __builtin_amdgcn_readlane(s1, 63);
+  if (blockIdx.x == 0 && threadIdx.x < 64) {
+    if (is) a.starts[l] = sp - np;
+    if (l == 0) a.starts[a.pg.n_seqs] = p.size;
+  }
+  int me = (int)blockIdx.x, kind = 0;
+  if (me >= all0) me -= all0, kind = 1;
+  if (kind == 1 && me >= all1) me -= all1, kind = 2;
+  const int n = kind == 0 ? n0 : kind == 1 ? n1 : n2, x = (kind == 0 ? s0 : kind == 1 ? s1 : s2) - n;
+  const uint64_t here = __ballot(x <= me && me < x + n);
+  p.seq = -1;
+  if (!here) return p;
+  p.seq = __builtin_ctzll(here);
+  auto of = [&](int y) { return __builtin_amdgcn_readlane(y, p.seq); };
+  const int i = me - of(x), w = of(whole);
+  p.parts = of(parts);
+  p.unit = kind == 0 ? i / w : i;
+  p.k = kind == 0 ? i - p.unit * w : w;
+  p.place = of(sp - np) + p.unit * p.parts + p.k;
+  p.tk = {of(tk.t0), of(tk.nt)};
+  p.pos = of(pos);
+  return p;
+}
 template <int THREADS>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
+  if (a.pg.n_seqs <= 64) return part_of_64(a, rows);
   constexpr int kW = THREADS / 64;
   __shared__ int s_total[kW], s_part[3];
   __shared__ Counts s_count[kW];
@@ -272,8 +324,9 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   if (p.seq < 0) return p;
   const int i = __builtin_amdgcn_readfirstlane(s_part[1]);
   kind = __builtin_amdgcn_readfirstlane(kind);
-  const Tokens tk = tokens_of(a.cu, p.seq, a.T, a.most);
-  const int span = demand_of(a, tk.nt, vis_of(uniform_load(a.pos + p.seq), tk.nt, cap), rows).span, whole = span / p.size;
+  p.tk = tokens_of(a.cu, p.seq, a.T, a.most);
+  p.pos = uniform_load(a.pos + p.seq);
+  const int span = demand_of(a, p.tk.nt, vis_of(p.pos, p.tk.nt, cap), rows).span, whole = span / p.size;
   p.parts = (span + p.size - 1) / p.size;
   p.unit = kind == 0 ? i / whole : i;
   p.k = kind == 0 ? i - p.unit * whole : whole;
@@ -290,8 +343,8 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = w % WR, wk = w / WR;
   const int group = a.nqh / a.pg.nkvh;
-  const Tokens tk = tokens_of(a.cu, pt.seq, a.T, a.most);
-  const Vis vis = vis_of(uniform_load(a.pos + pt.seq), tk.nt, a.pg.max_pages << a.pg.shift);
+  const Tokens tk = pt.tk;
+  const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
   const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
   const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
@@ -427,7 +480,9 @@ __device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* l
   }
 }
 
-// Scores of the wave's 32 rows and QT row tiles: as attn_core.h's, K's codes from registers.
+// Scores of the wave's 32 rows and QT row tiles: as attn_core.h's, K's codes from registers. A step is (block, row tile): its
+// four matrix instructions, and between them the scaling of the step before and a share of the next block's codes, since a
+// wave issues in order and a matrix instruction takes four times a vector one.
 template <int QT>
 __device__ __forceinline__ void wide_scores(const u2 (&k)[2][8], const uint8_t* ks, const h8 (&hi)[QT][8],
                                             const uint32_t (*lo)[8][64][4], f4 (&s)[QT][2]) {
@@ -435,44 +490,47 @@ __device__ __forceinline__ void wide_scores(const u2 (&k)[2][8], const uint8_t* 
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int q = 0; q < QT; q++) s[q][0] = s[q][1] = zero;
-  h8 ql[QT], x[2];
+  h8 ql[2], x[2][2];
   u2 sc[2][2];
-  f4 c[QT][2];
-  auto ask = [&](int b) {
-#pragma unroll
-    for (int q = 0; q < QT; q++) ql[q] = *(const h8*)lo[q][b][l];
+  f4 c[2][2];  // of this step and the one before
+  auto ask_q = [&](int i) { ql[i & 1] = *(const h8*)lo[i % QT][i / QT][l]; };
+  auto ask_s = [&](int b) {
 #pragma unroll
     for (int u = 0; u < 2; u++) sc[b & 1][u] = scales_of(ks, b, u);
   };
-  auto turn = [&](int b) {
+  auto turn = [&](int b, int u) { x[b & 1][u] = codes8(k[u][b].x, k[u][b].y); };
+  auto scale = [&](int i) {
+    const int b = i / QT, q = i % QT;
 #pragma unroll
-    for (int u = 0; u < 2; u++) x[u] = codes8(k[u][b].x, k[u][b].y);
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[q][u][e] = __builtin_fmaf(half_of(sc[b & 1][u][e & 1], e >> 1), c[i & 1][u][e], s[q][u][e]);
+      asm("" : "+v"(s[q][u]));
+    }
   };
-  ask(0);
-  turn(0);
+  ask_q(0);
+  ask_s(0);
+  turn(0, 0);
+  turn(0, 1);
 #pragma unroll
-  for (int b = 0; b < 8; b++) {
+  for (int i = 0; i < 8 * QT; i++) {
+    const int b = i / QT, q = i % QT;
     __builtin_amdgcn_sched_barrier(0);
+    if (i + 1 < 8 * QT) ask_q(i + 1);
+    if (q == 0 && b < 7 && QT == 1) ask_s(b + 1);
 #pragma unroll
-    for (int q = 0; q < QT; q++)
+    for (int u = 0; u < 2; u++) c[i & 1][u] = mfma16(x[b & 1][u], ql[i & 1], zero);
 #pragma unroll
-      for (int u = 0; u < 2; u++) c[q][u] = mfma16(x[u], ql[q], zero);
-    if (b < 7) ask(b + 1);
-#pragma unroll
-    for (int q = 0; q < QT; q++)
-#pragma unroll
-      for (int u = 0; u < 2; u++) c[q][u] = mfma16(x[u], hi[q][b], c[q][u]);
-    if (b < 7) turn(b + 1);  // while the products are on their way
-#pragma unroll
-    for (int q = 0; q < QT; q++)
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          s[q][u][i] = __builtin_fmaf(half_of(sc[b & 1][u][i & 1], i >> 1), c[q][u][i], s[q][u][i]);
-        asm("" : "+v"(s[q][u]));
-      }
+    for (int u = 0; u < 2; u++) c[i & 1][u] = mfma16(x[b & 1][u], hi[q][b], c[i & 1][u]);
+    if (i) scale(i - 1);
+    if (q == QT - 1 && b < 7 && QT > 1) ask_s(b + 1);  // behind the last use of the block's before
+    if (b < 7) {
+      if (QT == 1 || q == 0) turn(b + 1, 0);
+      if (QT == 1 || q == 1) turn(b + 1, 1);
+    }
+    interleave<QT == 1 ? 7 : 4>();
   }
+  scale(8 * QT - 1);
 }
 
 template <int TYPE, int QT>
@@ -483,8 +541,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const int group = a.nqh / a.pg.nkvh;
-  const Tokens tk = tokens_of(a.cu, pt.seq, a.T, a.most);
-  const Vis vis = vis_of(uniform_load(a.pos + pt.seq), tk.nt, a.pg.max_pages << a.pg.shift);
+  const Tokens tk = pt.tk;
+  const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
   const int tiles = a.pg.n_pages ? (vis.end + kTileKeys - 1) / kTileKeys : 0;  // without a page there is nothing to read
   const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
@@ -556,6 +614,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
     int lane = l;
     asm volatile("" : "+v"(lane));  // addresses are formed for each tile: kept over the loop they would spill
     const int n = lane & 15, g = lane >> 4;
+    wide_stage_v(r, sh.v[w], lane);
     if (kPart && (lane >> 1) >= left) r.ks = r.vs = (u2){0u, 0u};
     put_scales(r.ks, sh.ks[w]);
     // V's scales: f, and what is left of them
@@ -575,14 +634,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       const int lf = m > 0.0f ? ex : -25;
       if (!(lane & 1)) sh.lf[w][lane >> 1] = (float)lf, sh.f[w][lane >> 1] = exp2i((uint32_t)(127 + lf));
     }
-    __builtin_amdgcn_wave_barrier();
-    wide_scores<QT>(r.k, sh.ks[w], hi, sh.lo, s);
     t += kWaves;
     if (t < t1) {
       place(t);
-      wide_load_k(r, wt, lane);
+      wide_load_v(r, wt, a.pg, kh, w, lane);
       ask_pages(t + kWaves);
     }
+    loads_issued();
+    wide_scores<QT>(r.k, sh.ks[w], hi, sh.lo, s);
+    if (t < t1) wide_load_k(r, wt, lane);
     loads_issued();
     if (kPart) {
       Vis mine = vis;
@@ -642,39 +702,60 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       *(u4*)sh.p[q][w][1][lane] = pl;
     }
     put_scales(vs, sh.vs[w]);
-    wide_stage_v(r, sh.v[w], lane);
-    if (t < t1) wide_load_v(r, wt, a.pg, kh, w, lane);
-    loads_issued();
     __syncthreads();
     // O += P V: the wave's two blocks of 32 dims
     const int vrow = (n >> 1) >= 4 ? 12 + 4 * g + (n >> 1) : 4 * g + (n >> 1);  // the transposing read, see attn_core.h
     const uint8_t* vbase = sh.v[w] + vrow * 64 + 8 * (n & 1);
     const int vx = (vrow >> 2 & 1) | (vrow >> 3 & 2);
-#pragma unroll
-    for (int k = 0; k < kWaves; k++) {
-      __builtin_amdgcn_sched_barrier(0);
-      u4 ph[QT], pl[QT];
+    // a step per (group, block): its products, the next step's weights and codes between them
+    u4 ph[QT], pl[QT], wh[2][QT], wl[2][QT];
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i x[2];
+    u2 d[2];
+    h8 v[2][2];
+    auto ask_p = [&](int k) {
 #pragma unroll
       for (int q = 0; q < QT; q++) ph[q] = *(const u4*)sh.p[q][k][0][lane], pl[q] = *(const u4*)sh.p[q][k][1][lane];
+    };
+    auto ask = [&](int i) {
+      const int k = i >> 1, b = i & 1;
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        u2 d[2];
-        u4 wh[QT], wl[QT];
+      for (int u = 0; u < 2; u++) d[u] = scales_of(sh.vs[k], 2 * w + b, u);
 #pragma unroll
-        for (int u = 0; u < 2; u++) d[u] = scales_of(sh.vs[k], 2 * w + b, u);
+      for (int h = 0; h < 2; h++)
+        x[h] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) v2i*)(vbase + 2048 * k + ((2 * b + h) ^ vx) * 16));
+    };
+    auto turn = [&](int i) {
 #pragma unroll
-        for (int q = 0; q < QT; q++) weigh<kPart>(ph[q], pl[q], d, wh[q], wl[q]);
+      for (int q = 0; q < QT; q++) weigh<kPart>(ph[q], pl[q], d, wh[i & 1][q], wl[i & 1][q]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          typedef int v2i __attribute__((ext_vector_type(2)));
-          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) v2i*)(vbase + 2048 * k + ((2 * b + h) ^ vx) * 16));
-          const h8 v = codes8<kBias>((uint32_t)x.x, (uint32_t)x.y);
+      for (int h = 0; h < 2; h++) v[i & 1][h] = codes8<kBias>((uint32_t)x[h].x, (uint32_t)x[h].y);
+    };
+    ask_p(0);
+    ask(0);
+    turn(0);
+    ask(1);
 #pragma unroll
-          for (int q = 0; q < QT; q++) o[q][2 * b + h] = mfma16(v, __builtin_bit_cast(h8, wl[q]), o[q][2 * b + h]);
+    for (int i = 0; i < 2 * kWaves; i++) {
+      const int b = i & 1;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int q = 0; q < QT; q++) o[q][2 * b + h] = mfma16(v, __builtin_bit_cast(h8, wh[q]), o[q][2 * b + h]);
+      for (int q = 0; q < QT; q++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) o[q][2 * b + h] = mfma16(v[b][h], __builtin_bit_cast(h8, wl[b][q]), o[q][2 * b + h]);
+#pragma unroll
+      for (int q = 0; q < QT; q++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) o[q][2 * b + h] = mfma16(v[b][h], __builtin_bit_cast(h8, wh[b][q]), o[q][2 * b + h]);
+      if (i + 1 < 2 * kWaves) {
+        turn(i + 1);
+        if (i + 2 < 2 * kWaves) {
+          if (!b) ask_p((i + 2) >> 1);
+          ask(i + 2);
         }
+        interleave<5>();
+        if (QT == 2) interleave<5>();
       }
     }
   };
