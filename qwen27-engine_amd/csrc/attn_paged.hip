@@ -24,7 +24,7 @@ struct PagedArgs {
   float *o, *lse;        // lse may be null
   float *part, *ml;      // [place][row of its unit][256], [..][2]
   int* starts;           // [n_seqs + 1]: each sequence's first place; the size of a part
-  int T, most, nqh, slots;  // slots: workgroups that run at a time
+  int T, most, nqh, slots;  // slots: shares of the whole work, see Part
   float scale;
 };
 
@@ -396,109 +396,102 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
 // ---------------------------------------------------------------- more than 16 query rows
 // A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
 // of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
-// query rows, and a wave holds a quarter of the outputs. The weights go from the one to the other through LDS. K is loaded
-// as the matrix operand it becomes; V's slice of 64 dims goes through the wave's own LDS, to be read transposed.
+// query rows, and a wave holds a quarter of the outputs. The weights and the V rows go from the one to the other through LDS.
 //
 // One reference E for each query row, the same in all waves: a row's product of weight and V scale is 2^(s - E) f d, f the
 // power of two above the V row's scales and d what is left of each (at most 1). E moves when a row's s + log2 f passes
 // E + 15, to 12 below it, so that what enters the product as two f16 terms is in their range, as in attn_core.h; the sum of
 // the weights is kept in units of 2^E as well. Rows whose V scales are all 0 count as f = 2^-25.
-constexpr int kWideTile = kWaves * kTileKeys;
 template <int QT>
 struct WideLds {
   union {
     QTile q[QT];
-    alignas(16) uint8_t v[kWaves][kWideTile * 64];  // row r's 16-byte piece c at c ^ (r >> 2 & 1 | r >> 3 & 2)
+    alignas(16) uint8_t codes[kWaves][kCodes];  // a wave's rows of K, then of V, as WaveLds has them
   };
   alignas(16) uint32_t lo[QT][8][64][4];          // the queries' second terms
   alignas(16) uint32_t p[QT][kWaves][2][64][4];  // weights as operands: two terms of 32 rows
   alignas(16) uint8_t ks[kWaves][kScales], vs[kWaves][kScales];
-  alignas(16) float f[kWaves][kTileKeys], lf[kWaves][kTileKeys];  // f and its logarithm
-  float mx[kWaves][QT][16], l[kWaves][QT][16];
+  alignas(16) int lf[kWaves][kTileKeys];  // the logarithms of f
+  float mx[kWaves][QT][16];               // of the scores; in the end the sums of the weights
 };
 
-// The tile's groups of 32 rows, one behind the other in the sequence; where the page of one lies, or null.
-struct WideTile {
-  const uint8_t *k, *ks, *vs;  // of the wave's own group
-  int page[kWaves], left[kWaves], mine;  // rows that exist; those of the wave's own group
-  int j0;
-};
-
+// A wave's rows on their way. Rows behind the last one that exists are read from it, those of a group without any from row 0
+// of a page; their scales are taken as 0.
 template <int TYPE>
 struct WideRegs {
-  u2 k[2][8];  // operand of block b, rows 16 u + n: dims 32 b + 8 g ..
-  u4 v[TYPE == Q27H_KV_Q8_Q4 ? 4 : 8];
+  u4 k[8], v[TYPE == Q27H_KV_Q8_Q4 ? 4 : 8];
   u2 ks, vs;
 };
-
-// Rows behind the last one that exists are read from it, a group of which none does from row 0 of a page; their scales are 0.
+struct WideTile {
+  const uint8_t *k, *v, *ks, *vs;
+  int left;  // of the wave's 32 rows, those that exist
+};
 template <int TYPE>
 __device__ __forceinline__ void wide_load_k(WideRegs<TYPE>& r, const WideTile& t, int l) {
-  const int n = l & 15, g = l >> 4, last = t.mine > 0 ? t.mine - 1 : 0;
+  const int last = t.left > 0 ? t.left - 1 : 0;
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int row = 16 * u + n < last ? 16 * u + n : last;
-#pragma unroll
-    for (int b = 0; b < 8; b++) r.k[u][b] = *(const u2*)(t.k + (unsigned)(row * kHD + 8 * g) + 32 * b);
+  for (int i = 0; i < 8; i++) {
+    const int row = 4 * i + (l >> 4);
+    r.k[i] = *(const u4*)(t.k + (unsigned)((row < last ? row : last) * kHD + 16 * (l & 15)));
   }
   const unsigned at = ((l >> 1) < last ? (l >> 1) : last) * 16 + 8 * (l & 1);
   r.ks = *(const u2*)(t.ks + at);
   r.vs = *(const u2*)(t.vs + at);
 }
 template <int TYPE>
-__device__ __forceinline__ void wide_load_v(WideRegs<TYPE>& r, const WideTile& t, const Pages& pg, int kh, int w, int l) {
+__device__ __forceinline__ void wide_load_v(WideRegs<TYPE>& r, const WideTile& t, int l) {
+  const int last = t.left > 0 ? t.left - 1 : 0;
+  constexpr bool k4 = TYPE == Q27H_KV_Q8_Q4;
 #pragma unroll
-  for (int k = 0; k < kWaves; k++) {
-    const int last = t.left[k] > 0 ? t.left[k] - 1 : 0, n = 1 << pg.shift;
-    const uint8_t* v = pg.v + (size_t)t.page[k] * pg.vb + ((size_t)kh * n + ((t.j0 + kTileKeys * k) & (n - 1))) * (TYPE == Q27H_KV_Q8_Q4 ? kHD / 2 : kHD);
-    if constexpr (TYPE == Q27H_KV_Q8_Q4) {
-      r.v[k] = *(const u4*)(v + (unsigned)(((l >> 1) < last ? (l >> 1) : last) * (kHD / 2) + 32 * w + 16 * (l & 1)));
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int row = 16 * h + (l >> 2) < last ? 16 * h + (l >> 2) : last;
-        r.v[2 * k + h] = *(const u4*)(v + (unsigned)(row * kHD + 64 * w + 16 * (l & 3)));
-      }
-    }
+  for (int i = 0; i < (k4 ? 4 : 8); i++) {
+    const int row = k4 ? 8 * i + (l >> 3) : 4 * i + (l >> 4);
+    r.v[i] = *(const u4*)(t.v + (unsigned)((row < last ? row : last) * (k4 ? kHD / 2 : kHD) + 16 * (l & (k4 ? 7 : 15))));
   }
 }
 template <int TYPE>
-__device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* lds, int l) {
-  auto at = [&](int row, int c) { return (u4*)(lds + row * 64 + ((c ^ ((row >> 2 & 1) | (row >> 3 & 2))) * 16)); };
+__device__ __forceinline__ void wide_stage_k(const WideRegs<TYPE>& r, uint8_t* codes, int l) {
 #pragma unroll
-  for (int k = 0; k < kWaves; k++) {
-    if constexpr (TYPE == Q27H_KV_Q8_Q4) {
+  for (int i = 0; i < 8; i++) *(u4*)(codes + (i >= 4 ? kUpper - 16 * kRow : 0) + 4 * i * kRow + (l >> 4) * kRow + 16 * (l & 15)) = r.k[i];
+}
+template <int TYPE>
+__device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* codes, int l) {
+  if constexpr (TYPE == Q27H_KV_Q8_Q4) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
       u4 lo, hi;
 #pragma unroll
-      for (int i = 0; i < 4; i++) lo[i] = r.v[k][i] & 0x0f0f0f0fu, hi[i] = r.v[k][i] >> 4 & 0x0f0f0f0fu;
-      *at(32 * k + (l >> 1), 2 * (l & 1)) = lo;
-      *at(32 * k + (l >> 1), 2 * (l & 1) + 1) = hi;
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; h++) *at(32 * k + 16 * h + (l >> 2), l & 3) = r.v[2 * k + h];
+      for (int e = 0; e < 4; e++) lo[e] = r.v[i][e] & 0x0f0f0f0fu, hi[e] = r.v[i][e] >> 4 & 0x0f0f0f0fu;
+      uint8_t* p = codes + (i >= 2 ? kUpper - 16 * kRow : 0) + 8 * i * kRow + (l >> 3) * kRow + 32 * (l & 7);
+      *(u4*)p = lo;
+      *(u4*)(p + 16) = hi;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) *(u4*)(codes + (i >= 4 ? kUpper - 16 * kRow : 0) + 4 * i * kRow + (l >> 4) * kRow + 16 * (l & 15)) = r.v[i];
   }
 }
 
-// Scores of the wave's 32 rows and QT row tiles: as attn_core.h's, K's codes from registers. A step is (block, row tile): its
-// four matrix instructions, and between them the scaling of the step before and a share of the next block's codes, since a
-// wave issues in order and a matrix instruction takes four times a vector one.
+// Scores of the wave's 32 rows and QT row tiles, as attn_core.h's. A step is (block, row tile): its four matrix
+// instructions, and between them the scaling of the step before and a share of the next block's codes, since a wave
+// issues in order and a matrix instruction takes four times a vector one.
 template <int QT>
-__device__ __forceinline__ void wide_scores(const u2 (&k)[2][8], const uint8_t* ks, const h8 (&hi)[QT][8],
+__device__ __forceinline__ void wide_scores(const uint8_t* codes, const uint8_t* ks, const h8 (&hi)[QT][8],
                                             const uint32_t (*lo)[8][64][4], f4 (&s)[QT][2]) {
   const int l = threadIdx.x & 63;
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int q = 0; q < QT; q++) s[q][0] = s[q][1] = zero;
   h8 ql[2], x[2][2];
-  u2 sc[2][2];
+  u2 sc[2][2], k[2];
   f4 c[2][2];  // of this step and the one before
+  const uint8_t* row = codes + (l & 15) * kRow + 8 * (l >> 4);
   auto ask_q = [&](int i) { ql[i & 1] = *(const h8*)lo[i % QT][i / QT][l]; };
   auto ask_s = [&](int b) {
 #pragma unroll
     for (int u = 0; u < 2; u++) sc[b & 1][u] = scales_of(ks, b, u);
   };
-  auto turn = [&](int b, int u) { x[b & 1][u] = codes8(k[u][b].x, k[u][b].y); };
+  auto ask_k = [&](int b, int u) { k[u] = *(const u2*)(row + kUpper * u + 32 * b); };
+  auto turn = [&](int b, int u) { x[b & 1][u] = codes8(k[u].x, k[u].y); };
   auto scale = [&](int i) {
     const int b = i / QT, q = i % QT;
 #pragma unroll
@@ -508,25 +501,30 @@ __device__ __forceinline__ void wide_scores(const u2 (&k)[2][8], const uint8_t* 
       asm("" : "+v"(s[q][u]));
     }
   };
+  ask_k(0, 0);
+  ask_k(0, 1);
   ask_q(0);
   ask_s(0);
   turn(0, 0);
   turn(0, 1);
+  ask_k(1, 0);
+  ask_k(1, 1);
 #pragma unroll
   for (int i = 0; i < 8 * QT; i++) {
     const int b = i / QT, q = i % QT;
     __builtin_amdgcn_sched_barrier(0);
     if (i + 1 < 8 * QT) ask_q(i + 1);
-    if (q == 0 && b < 7 && QT == 1) ask_s(b + 1);
 #pragma unroll
     for (int u = 0; u < 2; u++) c[i & 1][u] = mfma16(x[b & 1][u], ql[i & 1], zero);
 #pragma unroll
     for (int u = 0; u < 2; u++) c[i & 1][u] = mfma16(x[b & 1][u], hi[q][b], c[i & 1][u]);
     if (i) scale(i - 1);
-    if (q == QT - 1 && b < 7 && QT > 1) ask_s(b + 1);  // behind the last use of the block's before
-    if (b < 7) {
-      if (QT == 1 || q == 0) turn(b + 1, 0);
-      if (QT == 1 || q == 1) turn(b + 1, 1);
+    if (q == QT - 1 && b < 7) ask_s(b + 1);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      if (b >= 7 || (QT > 1 && q != u)) continue;
+      turn(b + 1, u);
+      if (b < 6) ask_k(b + 2, u);
     }
     interleave<QT == 1 ? 7 : 4>();
   }
@@ -539,7 +537,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   __shared__ WideLds<QT> sh;
   const Part pt = part_of<kWaves * 64>(a, kRows);
   if (pt.seq < 0) return;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15;
   const int group = a.nqh / a.pg.nkvh;
   const Tokens tk = pt.tk;
   const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
@@ -547,12 +545,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   const int tiles = a.pg.n_pages ? (vis.end + kTileKeys - 1) / kTileKeys : 0;  // without a page there is nothing to read
   const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
   auto row = [&](int r) {  // the global row (token * nqh + head) of the unit's query row r, or -1
+    int by = group;
+    asm volatile("" : "+s"(by));  // what the division takes is formed where it is used, see `lane`
     r += first;
-    return r < rows ? (tk.t0 + r / group) * a.nqh + kh * group + r % group : -1;
+    return r < rows ? (tk.t0 + r / by) * a.nqh + kh * group + r % by : -1;
   };
   const int* table = a.pg.table + (size_t)pt.seq * a.pg.max_pages;
   const int prow = 1 << a.pg.shift;
-  int page[kWaves];
+  int page[kWaves];  // of the tile's four groups of 32 rows
   auto ask_pages = [&](int t) {
 #pragma unroll
     for (int k = 0; k < kWaves; k++) page[k] = t + k < t1 ? uniform_load(table + ((t + k) >> (a.pg.shift - 5))) : -1;
@@ -561,28 +561,27 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   bool whole;  // every row of the tile is seen by every query
   auto place = [&](int t) {
     whole = (t + kWaves) * kTileKeys <= vis.n && t + kWaves <= t1;
-    wt.j0 = t * kTileKeys;
+    int mine = page[0];
 #pragma unroll
     for (int k = 0; k < kWaves; k++) {
-      const int j0 = (t + k) * kTileKeys;
-      const bool is = (unsigned)page[k] < (unsigned)a.pg.n_pages;
-      whole = whole && is;
-      wt.left[k] = is ? (vis.end - j0 < kTileKeys ? vis.end - j0 : kTileKeys) : 0;
-      wt.page[k] = is ? page[k] : 0;
-      if (k != w) continue;
-      const size_t at = (size_t)kh * prow + (j0 & (prow - 1)), p = wt.page[k];
-      wt.mine = wt.left[k];
-      wt.k = a.pg.k + p * a.pg.kb + at * kHD;
-      wt.ks = a.pg.k + p * a.pg.kb + (size_t)a.pg.nkvh * prow * kHD + at * 16;
-      wt.vs = a.pg.v + p * a.pg.vb + (size_t)a.pg.nkvh * prow * kV + at * 16;
+      whole = whole && (unsigned)page[k] < (unsigned)a.pg.n_pages;
+      mine = k == w ? page[k] : mine;
     }
+    const int j0 = (t + w) * kTileKeys;
+    const bool is = (unsigned)mine < (unsigned)a.pg.n_pages;
+    wt.left = is ? (vis.end - j0 < kTileKeys ? vis.end - j0 : kTileKeys) : 0;
+    const size_t at = (size_t)kh * prow + (j0 & (prow - 1)), p = is ? mine : 0;
+    wt.k = a.pg.k + p * a.pg.kb + at * kHD;
+    wt.v = a.pg.v + p * a.pg.vb + at * kV;
+    wt.ks = a.pg.k + p * a.pg.kb + (size_t)a.pg.nkvh * prow * kHD + at * 16;
+    wt.vs = a.pg.v + p * a.pg.vb + (size_t)a.pg.nkvh * prow * kV + at * 16;
   };
   WideRegs<TYPE> r;
   if (t0 < t1) {
     ask_pages(t0);
     place(t0);
     wide_load_k(r, wt, l);
-    wide_load_v(r, wt, a.pg, kh, w, l);
+    wide_load_v(r, wt, l);
     ask_pages(t0 + kWaves);
   }
   load_queries<true, kWaves, QT>(sh.q, a.scale * kLog2e, [&](int r) {
@@ -606,15 +605,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   }
   __syncthreads();
 
-  int t = t0;
+  int t = t0, left = wt.left;  // of the tile in work, where wt is the next one's
   auto step = [&](auto hidden) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(hidden)::value;
-    const int left = wt.mine;
     f4 s[QT][2];
     int lane = l;
     asm volatile("" : "+v"(lane));  // addresses are formed for each tile: kept over the loop they would spill
     const int n = lane & 15, g = lane >> 4;
-    wide_stage_v(r, sh.v[w], lane);
+    left = wt.left;
+    wide_stage_k(r, sh.codes[w], lane);
     if (kPart && (lane >> 1) >= left) r.ks = r.vs = (u2){0u, 0u};
     put_scales(r.ks, sh.ks[w]);
     // V's scales: f, and what is left of them
@@ -631,43 +630,48 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
 #pragma unroll
       for (int i = 0; i < 4; i++) x[i] = m > 0.0f ? __builtin_amdgcn_ldexpf(x[i], -ex) : x[i];
       vs = (u2){pk_rtz(x[0], x[1]), pk_rtz(x[2], x[3])};
-      const int lf = m > 0.0f ? ex : -25;
-      if (!(lane & 1)) sh.lf[w][lane >> 1] = (float)lf, sh.f[w][lane >> 1] = exp2i((uint32_t)(127 + lf));
+      if (!(lane & 1)) sh.lf[w][lane >> 1] = m > 0.0f ? ex : -25;
     }
+    const int j0 = (t + w) * kTileKeys;
     t += kWaves;
     if (t < t1) {
       place(t);
-      wide_load_v(r, wt, a.pg, kh, w, lane);
+      wide_load_k(r, wt, lane);
       ask_pages(t + kWaves);
     }
     loads_issued();
-    wide_scores<QT>(r.k, sh.ks[w], hi, sh.lo, s);
-    if (t < t1) wide_load_k(r, wt, lane);
-    loads_issued();
+    wide_scores<QT>(sh.codes[w], sh.ks[w], hi, sh.lo, s);
     if (kPart) {
       Vis mine = vis;
-      int m = n;
-      asm volatile("" : "+v"(m));
       uint64_t chain[QT];
 #pragma unroll
-      for (int q = 0; q < QT; q++) chain[q] = row(16 * q + m) >= 0 ? ~0ull >> (63 - (first + 16 * q + m) / group) : 0ull;
+      for (int q = 0; q < QT; q++) {
+        int by = group;
+        asm volatile("" : "+s"(by));
+        const int at = first + 16 * q + n;
+        chain[q] = at < rows ? ~0ull >> (63 - at / by) : 0ull;
+      }
       if (left <= 0) mine.n = mine.end = 0;
-      hide<QT, kHidden>(s, mine, chain, (t - kWaves + w) * kTileKeys);
+      hide<QT, kHidden>(s, mine, chain, j0);
     }
-    const f4 lf[2] = {*(const f4*)&sh.lf[w][4 * g], *(const f4*)&sh.lf[w][16 + 4 * g]};
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    const i4 lf[2] = {*(const i4*)&sh.lf[w][4 * g], *(const i4*)&sh.lf[w][16 + 4 * g]};
 #pragma unroll
     for (int q = 0; q < QT; q++) {
       float mx = -3.0e38f;
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, __builtin_fmaf(s[q][u][i], c[q], lf[u][i]));
+        for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, __builtin_fmaf(s[q][u][i], c[q], (float)lf[u][i]));
       mx = __builtin_fmaxf(mx, lane_xor<16>(mx));
       mx = __builtin_fmaxf(mx, lane_xor32(mx));
       if (g == 0) sh.mx[w][q][n] = mx;
     }
-    __syncthreads();  // the outputs of the tile before are formed: what the waves share is free
-    const f4 f[2] = {*(const f4*)&sh.f[w][4 * g], *(const f4*)&sh.f[w][16 + 4 * g]};
+    wide_stage_v(r, sh.codes[w], lane);  // K's rows are read
+    if (t < t1) wide_load_v(r, wt, lane);
+    loads_issued();
+    put_scales(vs, sh.vs[w]);
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < QT; q++) {
       const float mx = __builtin_fmaxf(__builtin_fmaxf(sh.mx[0][q][n], sh.mx[1][q][n]), __builtin_fmaxf(sh.mx[2][q][n], sh.mx[3][q][n]));
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
           const float x = s[q][u][i], y = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[q], -e[q]));
           const float z = kPart && __builtin_bit_cast(uint32_t, x) == kHidden ? -0.0f : y;
           add += z;
-          p[u][i] = z * f[u][i];
+          p[u][i] = __builtin_amdgcn_ldexpf(z, lf[u][i]);
         }
       sum[q] += add;
       u4 ph, pl;
@@ -701,13 +705,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       *(u4*)sh.p[q][w][0][lane] = ph;
       *(u4*)sh.p[q][w][1][lane] = pl;
     }
-    put_scales(vs, sh.vs[w]);
     __syncthreads();
-    // O += P V: the wave's two blocks of 32 dims
-    const int vrow = (n >> 1) >= 4 ? 12 + 4 * g + (n >> 1) : 4 * g + (n >> 1);  // the transposing read, see attn_core.h
-    const uint8_t* vbase = sh.v[w] + vrow * 64 + 8 * (n & 1);
-    const int vx = (vrow >> 2 & 1) | (vrow >> 3 & 2);
-    // a step per (group, block): its products, the next step's weights and codes between them
+    // O += P V: the wave's two blocks of 32 dims; the transposing read as in attn_core.h. A step per (group, block): its
+    // products, the next step's weights and codes between them
+    const uint8_t* vbase = sh.codes[0] + ((n >> 1) >= 4 ? kUpper + (4 * g + (n >> 1) - 4) * kRow : (4 * g + (n >> 1)) * kRow) + 8 * (n & 1) + 64 * w;
     u4 ph[QT], pl[QT], wh[2][QT], wl[2][QT];
     typedef int v2i __attribute__((ext_vector_type(2)));
     v2i x[2];
@@ -723,8 +724,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       for (int u = 0; u < 2; u++) d[u] = scales_of(sh.vs[k], 2 * w + b, u);
 #pragma unroll
       for (int h = 0; h < 2; h++)
-        x[h] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (__attribute__((address_space(3))) v2i*)(vbase + 2048 * k + ((2 * b + h) ^ vx) * 16));
+        x[h] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(vbase + kCodes * k + 32 * b + 16 * h));
     };
     auto turn = [&](int i) {
 #pragma unroll
@@ -758,24 +758,28 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
         if (QT == 2) interleave<5>();
       }
     }
+    __syncthreads();  // V's rows are read: K's take their place
   };
   while (t < t1) {
     while (t < t1 && whole) step(std::false_type());
     if (t < t1) step(std::true_type());
   }
+  int end = l;
+  asm volatile("" : "+v"(end));
+  const int n1 = end & 15, g1 = end >> 4;
 #pragma unroll
   for (int q = 0; q < QT; q++) {
     sum[q] += lane_xor<16>(sum[q]);
     sum[q] += lane_xor32(sum[q]);
-    if (g == 0) sh.l[w][q][n] = sum[q];
+    if (g1 == 0) sh.mx[w][q][n1] = sum[q];
   }
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < QT; q++) {
-    const int gr = row(16 * q + n);
+    const int gr = row(16 * q + n1);
     if (gr < 0) continue;
-    const float total = (sh.l[0][q][n] + sh.l[1][q][n]) + (sh.l[2][q][n] + sh.l[3][q][n]);
-    const bool lead = w == 0 && g == 0;
+    const float total = (sh.mx[0][q][n1] + sh.mx[1][q][n1]) + (sh.mx[2][q][n1] + sh.mx[3][q][n1]);
+    const bool lead = w == 0 && g1 == 0;
     float x = 512.0f;  // codes8's 2^-9
     float* dst;
     if (pt.parts == 1) {
@@ -783,12 +787,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       dst = a.o + (size_t)gr * kHD;
       if (a.lse && lead) a.lse[gr] = total == 0.0f ? -__builtin_huge_valf() : (e[q] + __builtin_amdgcn_logf(total)) * kLn2;
     } else {
-      const size_t at = (size_t)pt.place * kRows + 16 * q + n;
+      const size_t at = (size_t)pt.place * kRows + 16 * q + n1;
       dst = a.part + at * kHD;
       if (lead) *(float2*)(a.ml + at * 2) = make_float2(e[q], total);
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) *(f4*)(dst + 64 * w + 16 * i + 4 * g) = o[q][i] * x;
+    for (int i = 0; i < 4; i++) *(f4*)(dst + 64 * w + 16 * i + 4 * g1) = o[q][i] * x;
   }
 }
 
@@ -871,7 +875,9 @@ Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   const int rows = max_tokens * (nqh / nkvh);
   y.wr = rows <= 16 ? 1 : 2;
   y.threads = y.wr == 2 && type == Q27H_KV_F16 ? 512 : 256;
-  y.slots = 2 * kCUs * 256 / y.threads;
+  // the kernel of more than 16 query rows over codes is bound by arithmetic: half as many parts more leave less of it to the
+  // last ones (48 sequences of 4 drafts, 371589 rows: 237 -> 218 us; of one token, bound by HBM: 51.0 -> 52.0)
+  y.slots = y.wr == 2 && type != Q27H_KV_F16 ? 3 * kCUs : 2 * kCUs * 256 / y.threads;
   // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has two
   // parts at least and not two more than its share
   const int units = n_seqs * nkvh * ((rows + 16 * y.wr - 1) / (16 * y.wr));

@@ -39,8 +39,8 @@ Pages pages_of(const q27h_kv_pages* kv) {
 
 namespace {
 
-constexpr int kChunk = 32;    // rows of a piece
-constexpr int kBlocks = 8 * kCUs;
+constexpr int kChunk = 16;    // rows of a piece
+constexpr int kBlocks = 16 * kCUs;
 
 struct ReadArgs {
   Pages pg;
@@ -55,7 +55,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 // Values as they are stored: 16 bytes a lane and store, so that the 16 lanes of a row write 256 bytes that lie together (a
 // lane's values one behind the other in several stores would leave every cache line to be written in pieces: 8 sequences
-// of 81250 rows, K in 8 bits and V in 4, to f16: 167 us, @@ so).
+// with 81250 rows in all, K in 8 bits and V in 4, to f16: 167 us, 112 so).
 struct AsF32 {
   typedef float type;
   static constexpr int kN = 4;
@@ -119,8 +119,8 @@ struct Piece {
   }
 };
 
-// A workgroup takes a chunk of 32 rows in two steps of 16, K and V of a step requested together. Rows of a page that is none
-// of the cache's are zeros.
+// A workgroup takes a chunk of 16 rows, K and V requested together, and then the next. Twice the rows in twice the loads,
+// and half the workgroups, were slower (to f16: 112 us against 104). Rows of a page that is none of the cache's are zeros.
 template <int KB, int VB, typename OUT>
 __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
   typedef typename OUT::type O;
@@ -142,44 +142,32 @@ __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
     sp.x++;
     const long long from = a.from ? a.from[b] : 0;
     constexpr int N = OUT::kN;
-    Piece<KB, N> k[2];
-    Piece<VB, N> v[2];
-    bool is[2];
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int i = i0 + 16 * s + r;
-      const long long j = from + i;
-      const long long pi = j >> a.pg.shift;
-      int page = -1;
-      if (i < count && pi >= 0 && pi < a.pg.max_pages) page = a.pg.table[(size_t)b * a.pg.max_pages + pi];
-      is[s] = (unsigned)page < (unsigned)a.pg.n_pages;
-      if (!is[s]) continue;
+    Piece<KB, N> k;
+    Piece<VB, N> v;
+    const int i = i0 + r;
+    if (i >= count) continue;
+    const long long j = from + i, pi = j >> a.pg.shift;
+    const int page = pi >= 0 && pi < a.pg.max_pages ? a.pg.table[(size_t)b * a.pg.max_pages + pi] : -1;
+    const bool is = (unsigned)page < (unsigned)a.pg.n_pages;
+    if (is) {
       const size_t rows = (size_t)a.pg.nkvh * n, row = (size_t)kh * n + (size_t)(j & (n - 1));
-      if (a.kout) k[s].load(a.pg.k + (size_t)page * a.pg.kb, rows, row, l);
-      if (a.vout) v[s].load(a.pg.v + (size_t)page * a.pg.vb, rows, row, l);
+      if (a.kout) k.load(a.pg.k + (size_t)page * a.pg.kb, rows, row, l);
+      if (a.vout) v.load(a.pg.v + (size_t)page * a.pg.vb, rows, row, l);
     }
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int i = i0 + 16 * s + r;
-      if (i >= count) continue;
-      const size_t o = (((size_t)b * a.pg.nkvh + kh) * a.n_out + i) * kHeadDim + N * l;
+    const size_t o = (((size_t)b * a.pg.nkvh + kh) * a.n_out + i) * kHeadDim + N * l;
+    auto give = [&](const auto& x, void* out) {
+      if (!out) return;
 #pragma unroll
       for (int h = 0; h < 16 / N; h++) {
         float y[N];
-        if (a.kout) {
-          k[s].values(h, l, y);
+        x.values(h, l, y);
 #pragma unroll
-          for (int e = 0; e < N; e++) y[e] = is[s] ? y[e] : 0.0f;
-          put<OUT>((O*)a.kout + o + 16 * N * h, y);
-        }
-        if (a.vout) {
-          v[s].values(h, l, y);
-#pragma unroll
-          for (int e = 0; e < N; e++) y[e] = is[s] ? y[e] : 0.0f;
-          put<OUT>((O*)a.vout + o + 16 * N * h, y);
-        }
+        for (int e = 0; e < N; e++) y[e] = is ? y[e] : 0.0f;
+        put<OUT>((O*)out + o + 16 * N * h, y);
       }
-    }
+    };
+    give(k, a.kout);
+    give(v, a.vout);
   }
 }
 

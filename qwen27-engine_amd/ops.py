@@ -10,11 +10,7 @@ from ._lib import check, lib
 
 
 def _ptr(t):
-    if t is None:
-        return None
-    if isinstance(t, int):
-        return t
-    return t.data_ptr()
+    return t if t is None or isinstance(t, int) else t.data_ptr()
 
 
 _raw_stream = None
