@@ -1,5 +1,6 @@
 // Attention over the K/V cache that attn_prep writes, and the cache's keeping, in namespace q27 over include/q27h.h: a tree
-// of drafted tokens, attention weights per row and eviction, blocks chosen per token. No counterparts in the reference's
+// of drafted tokens, attention weights per row and eviction, blocks chosen per token; a batch of sequences over a cache in
+// pages, and the verification of drafts. No counterparts in the reference's
 // headers. The contracts stand in q27h.h; a bad shape or argument throws std::runtime_error.
 #pragma once
 #include "ops.h"
@@ -45,6 +46,32 @@ inline void attn_blocks(const float* qn, const void* kcache, const void* vcache,
                         float scale, int nqh, int nkvh, int n_ctx, bool q8, float* o, void* ws, size_t ws_bytes, hipStream_t s,
                         float* lse = nullptr) {
   q27h_check(q27h_attn_blocks(qn, kcache, vcache, pos0, idx, T, nsel, scale, nqh, nkvh, n_ctx, q8 ? 1 : 0, o, lse, ws, ws_bytes, s));
+}
+
+// A batch of sequences over a cache in pages
+using KvPages = q27h_kv_pages;
+inline size_t kv_page_bytes(int nkvh, int page_rows, int type, bool v) { return q27h_kv_page_bytes(nkvh, page_rows, type, v ? 1 : 0); }
+inline void attn_prep_paged(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm, float* qn,
+                            const KvPages& kv, const int* pos, const int* cu, int T, float eps, float theta_scale, int nqh, hipStream_t s,
+                            const int* rope3 = nullptr, const int* rdelta = nullptr) {
+  q27h_check(q27h_attn_prep_paged(qg, k, v, q_norm, k_norm, qn, &kv, pos, cu, T, eps, theta_scale, nqh, s, rope3, rdelta));
+}
+inline size_t attn_paged_ws_bytes(const KvPages& kv, int T, int max_tokens, int nqh) {
+  return q27h_attn_paged_ws_bytes(&kv, T, max_tokens, nqh);
+}
+inline void attn_paged(const float* qn, const KvPages& kv, const int* pos, const int* cu, int T, int max_tokens, float scale, int nqh,
+                       float* o, void* ws, size_t ws_bytes, hipStream_t s, float* lse = nullptr) {
+  q27h_check(q27h_attn_paged(qn, &kv, pos, cu, T, max_tokens, scale, nqh, o, lse, ws, ws_bytes, s));
+}
+inline void kv_pages_read(const KvPages& kv, const int* from, const int* count, int n_out, int out_type, void* kout, void* vout,
+                          hipStream_t s) {
+  q27h_check(q27h_kv_pages_read(&kv, from, count, n_out, out_type, kout, vout, s));
+}
+inline size_t draft_verify_ws_bytes(int n_seqs, int V) { return q27h_draft_verify_ws_bytes(n_seqs, V); }
+inline void draft_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, const int* ids, const int* parent, const float* u,
+                         const float* u_last, const int* cu, int n_seqs, int T, int V, int* out, int* path, int* n_path, void* ws,
+                         size_t ws_bytes, hipStream_t s, int* pos = nullptr) {
+  q27h_check(q27h_draft_verify(p, ldp, q, ldq, ids, parent, u, u_last, cu, n_seqs, T, V, out, path, n_path, pos, ws, ws_bytes, s));
 }
 
 }  // namespace q27

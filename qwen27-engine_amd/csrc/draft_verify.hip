@@ -1,7 +1,7 @@
 // Verification of drafted tokens against the target's probabilities (draft_verify), for a ragged batch of sequences.
 //
 // Which drafts stand is a walk over at most 64 tokens, whose probabilities one round of gathers brings: every workgroup of a
-// sequence does it for itself (lane t holds token t). What remains is a draw from the row where the walk ended, over the
+// sequence does it for itself (lane t holds token t), and one leaves it for the second launch. What remains is a draw from the row where the walk ended, over the
 // whole vocabulary: the sum S of the row's weights, and the first token whose sum up to it passes u S. The row is cut in
 // chunks; the first launch leaves each chunk's sum, the second finds the chunk and then the token in it. Bound by HBM: a row
 // of p and, behind a refusal in a chain with probabilities, one of q.
@@ -18,6 +18,7 @@ namespace {
 constexpr int kMostTokens = 64;
 constexpr int kPerThread = 16, kThreads = 256, kChunk = kThreads * kPerThread;  // values of a chunk
 
+struct Walk;
 struct VerifyArgs {
   const float *p, *q;  // q null: drafts without probabilities
   const int *ids, *parent;
@@ -25,18 +26,18 @@ struct VerifyArgs {
   const int* cu;
   int *out, *path, *n_path, *pos;  // pos may be null
   double2* sums;                   // [n_seqs][chunks]: of max(p - q, 0), and of p
+  Walk* walks;                     // [n_seqs], for the second launch
   long long ldp, ldq;
   int T, V, chunks;
 };
 
 // Where a sequence's walk ended.
 struct Walk {
-  int t0, nt;
   uint64_t path;   // its accepted tokens, token 0 among them
   uint64_t tried;  // the children of the last one that were refused (drafts without probabilities)
+  int t0, nt;
   int node;        // the last one
-  bool refused;    // a chain with probabilities: token node + 1 was refused, q's row of it is to be taken off
-  int id;          // lane t: token t
+  int refused;     // a chain with probabilities: token node + 1 was refused, q's row of it is to be taken off
 };
 
 __device__ __forceinline__ float read_lane(float x, int l) {
@@ -55,16 +56,16 @@ __device__ __forceinline__ Walk walk_of(const VerifyArgs& a, int b) {
   w.path = w.nt ? 1ull : 0ull;
   w.tried = 0;
   w.node = 0;
-  w.refused = false;
+  w.refused = 0;
   const bool draft = l >= 1 && l < w.nt;
-  w.id = l < w.nt ? a.ids[w.t0 + l] : -1;
+  const int mine = l < w.nt ? a.ids[w.t0 + l] : -1;
   int parent = l - 1;
   if (a.parent && draft) parent = a.parent[w.t0 + l];
-  const bool sound = draft && parent >= 0 && parent < l && (unsigned)w.id < (unsigned)a.V;
+  const bool sound = draft && parent >= 0 && parent < l && (unsigned)mine < (unsigned)a.V;
   const float u = draft ? a.u[w.t0 + l] : 0.0f;
-  const float p = sound ? a.p[(size_t)(w.t0 + parent) * a.ldp + w.id] : 0.0f;
+  const float p = sound ? a.p[(size_t)(w.t0 + parent) * a.ldp + mine] : 0.0f;
   if (a.q) {  // a chain: the first draft that is refused ends it. The products of two floats are exact in 64 bits.
-    const float q = sound ? a.q[(size_t)(w.t0 + l) * a.ldq + w.id] : 0.0f;
+    const float q = sound ? a.q[(size_t)(w.t0 + l) * a.ldq + mine] : 0.0f;
     const uint64_t yes = __ballot(draft && (double)u * q < (double)p) | 1ull;
     const int n = yes == ~0ull ? 64 : __builtin_ctzll(~yes);  // tokens accepted, the first among them
     if (w.nt) w.path = n == 64 ? ~0ull : (1ull << n) - 1;
@@ -77,8 +78,8 @@ __device__ __forceinline__ Walk walk_of(const VerifyArgs& a, int b) {
   for (uint64_t todo = drafts & __ballot(parent == 0); todo;) {
     const int t = __builtin_ctzll(todo);
     todo &= todo - 1;
-    const int id = __builtin_amdgcn_readlane(w.id, t);
-    const bool again = (__ballot(w.id == id) & w.tried) != 0;  // a token that was refused already
+    const int id = __builtin_amdgcn_readlane(mine, t);
+    const bool again = (__ballot(mine == id) & w.tried) != 0;  // a token that was refused already
     const double x = again ? 0.0 : (double)read_lane(p, t);
     if ((double)read_lane(u, t) * rest < x) {
       w.node = t, w.path |= 1ull << t, w.tried = 0, rest = 1.0;
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
   __shared__ double s_red[2][kThreads / 64];
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, w = threadIdx.x >> 6;
   const Walk k = walk_of(a, b);
+  if (chunk == 0 && threadIdx.x == 0) a.walks[b] = k;
   if (!k.nt) return;
   float p[kPerThread], q[kPerThread];
   load_chunk(a.p + (size_t)(k.t0 + k.node) * a.ldp, chunk, a.V, p);
@@ -174,26 +176,27 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   __shared__ int s_bad[kMostTokens];
   __shared__ double s_takes[kMostTokens];
   const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63;
-  const Walk k = walk_of(a, b);
+  const Walk k = a.walks[b];
   if (!k.nt) {
     if (tid == 0) a.n_path[b] = 0;
     return;
   }
+  const int id = l < k.nt ? a.ids[k.t0 + l] : -1;  // lane t: token t
   const float* prow = a.p + (size_t)(k.t0 + k.node) * a.ldp;
   const float* qrow = a.q ? a.q + (size_t)(k.t0 + k.node + 1) * a.ldq : nullptr;
   // the refused children weigh nothing: their ids, each once, and what they take from their chunks' sums, exactly
   if (tid < 64) {
     const bool bad = k.tried >> l & 1;
-    bool first = bad && (unsigned)k.id < (unsigned)a.V;
+    bool first = bad && (unsigned)id < (unsigned)a.V;
     for (uint64_t m = k.tried; m; m &= m - 1) {
-      const int t = __builtin_ctzll(m);
-      if (__builtin_amdgcn_readlane(k.id, t) == k.id && t < l) first = false;
+      const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+      if (__builtin_amdgcn_readlane(id, t) == id && t < l) first = false;
     }
     const uint64_t each = __ballot(first);
     if (first) {
       const int at = __builtin_popcountll(each & ((1ull << l) - 1));
-      s_bad[at] = k.id;
-      s_takes[at] = weight_of(prow[k.id]);
+      s_bad[at] = id;
+      s_takes[at] = weight_of(prow[id]);
     }
     if (l == 0) s_n = __builtin_popcountll(each), s_chunk = s_token = -1;
   }
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   const bool on = k.path >> l & 1;
   if (on) {
     a.path[k.t0 + rank] = l;
-    if (rank) a.out[k.t0 + rank - 1] = k.id;
+    if (rank) a.out[k.t0 + rank - 1] = id;
   }
   if (l >= n && l < k.nt) a.path[k.t0 + l] = a.out[k.t0 + l] = -1;
   if (l == 0) {
@@ -295,7 +298,7 @@ int chunks_of(int V) { return (V + kChunk - 1) / kChunk; }
 using namespace q27h;
 
 extern "C" size_t q27h_draft_verify_ws_bytes(int n_seqs, int V) {
-  return n_seqs <= 0 || V <= 0 || V > 1 << 24 ? 0 : (size_t)n_seqs * chunks_of(V) * sizeof(double2);
+  return n_seqs <= 0 || V <= 0 || V > 1 << 24 ? 0 : (size_t)n_seqs * (chunks_of(V) * sizeof(double2) + sizeof(Walk));
 }
 
 extern "C" int q27h_draft_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, const int* ids, const int* parent,
@@ -316,7 +319,9 @@ extern "C" int q27h_draft_verify(const float* p, int64_t ldp, const float* q, in
   if (outputs_overlap({{out, tb}, {path, tb}, {n_path, B}, {pos, B}, {ws, need}},
                       {{p, pb}, {q, qb}, {ids, tb}, {parent, tb}, {u, tb}, {u_last, B}, {cu, B + 4}}))
     return fail(Q27H_ERR_ARG, "draft_verify: a result, pos or ws overlaps another argument");
-  VerifyArgs a = {p, q, ids, parent, u, u_last, cu, out, path, n_path, pos, (double2*)ws, (long long)ldp, (long long)ldq, T, V, chunks_of(V)};
+  double2* sums = (double2*)ws;
+  VerifyArgs a = {p, q, ids, parent, u, u_last, cu, out, path, n_path, pos, sums, (Walk*)(sums + (size_t)n_seqs * chunks_of(V)),
+                  (long long)ldp, (long long)ldq, T, V, chunks_of(V)};
   hipLaunchKernelGGL(draft_sums_kernel, dim3((unsigned)(n_seqs * a.chunks)), dim3(kThreads), 0, stream_of(s), a);
   hipLaunchKernelGGL(draft_pick_kernel, dim3((unsigned)n_seqs), dim3(kThreads), 0, stream_of(s), a);
   return check_launch("draft_verify");

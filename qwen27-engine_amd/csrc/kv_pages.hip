@@ -12,19 +12,19 @@
 namespace q27h {
 
 int check_pages(const q27h_kv_pages* kv, const char* what) {
-  const std::string w = what;
-  if (!kv) return fail(Q27H_ERR_ARG, w + ": null handle of pages");
+  auto bad = [&](int code, const char* why) { return fail(code, std::string(what) + why); };
+  if (!kv) return bad(Q27H_ERR_ARG, ": null handle of pages");
   if (kv->type != Q27H_KV_F16 && kv->type != Q27H_KV_Q8 && kv->type != Q27H_KV_Q8_Q4)
-    return fail(Q27H_ERR_SHAPE, w + ": unknown type of cache");
+    return bad(Q27H_ERR_SHAPE, ": unknown type of cache");
   if (kv->page_rows < 32 || kv->page_rows > 65536 || (kv->page_rows & (kv->page_rows - 1)))
-    return fail(Q27H_ERR_SHAPE, w + ": the rows of a page must be a power of two, 32 to 65536");
+    return bad(Q27H_ERR_SHAPE, ": the rows of a page must be a power of two, 32 to 65536");
   if (kv->nkvh <= 0 || kv->nkvh > 4096 || kv->n_seqs < 0 || kv->n_pages < 0 || kv->max_pages < 0 ||
       (long long)kv->max_pages * kv->page_rows > 1 << 30)
-    return fail(Q27H_ERR_SHAPE, w + ": bad sizes of the paged cache (at most 2^30 rows a sequence)");
+    return bad(Q27H_ERR_SHAPE, ": bad sizes of the paged cache (at most 2^30 rows a sequence)");
   if ((kv->n_pages && (!kv->k || !kv->v)) || (kv->n_seqs && kv->max_pages && !kv->table))
-    return fail(Q27H_ERR_ARG, w + ": null pointer in the handle of pages");
+    return bad(Q27H_ERR_ARG, ": null pointer in the handle of pages");
   if (!aligned16(kv->k) || !aligned16(kv->v) || !aligned4(kv->table))
-    return fail(Q27H_ERR_ARG, w + ": pages need 16-byte alignment, their table 4-byte");
+    return bad(Q27H_ERR_ARG, ": pages need 16-byte alignment, their table 4-byte");
   return Q27H_OK;
 }
 

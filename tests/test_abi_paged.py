@@ -154,7 +154,7 @@ def test_sizes(q27):
     assert o.attn_paged_ws_bytes(KV(), 10, 4, 24) > 0
     assert o.attn_paged_ws_bytes(KV(), 0, 4, 24) == o.attn_paged_ws_bytes(KV(rows=48), 10, 4, 24) == 0
     assert o.attn_paged_ws_bytes(KV(), 10, 65, 24) == o.attn_paged_ws_bytes(KV(), 10, 4, 25) == 0
-    assert o.draft_verify_ws_bytes(3, 248320) == 3 * 61 * 16
+    assert o.draft_verify_ws_bytes(3, 248320) >= 3 * 61 * 16
     assert o.draft_verify_ws_bytes(0, 10) == o.draft_verify_ws_bytes(1, 0) == o.draft_verify_ws_bytes(1, (1 << 24) + 1) == 0
 
 
@@ -167,3 +167,51 @@ def test_a_handle_needs_a_whole_table(q27):
     for table in (torch.zeros(3, 8, dtype=torch.int64), torch.zeros(8, 3, dtype=torch.int32).t(), torch.zeros(24, dtype=torch.int32)):
         with pytest.raises(ValueError):
             q27.ops.KvPages(k, v, table, 4, 64, q27.ops.KV_Q8_Q4)
+
+
+def test_cpp_header_forwards(tmp_path):
+    """include/q27/attn.h: every function compiles in a caller, and a refusal arrives as an exception."""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "qwen27-engine_amd", "lib")
+    src, exe = tmp_path / "caller.cpp", tmp_path / "caller"
+    src.write_text(r'''
+#include <cstdio>
+#include "q27/attn.h"
+void step(const float* x, const q27::KvPages& kv, int* pos, const int* cu, int* out, float* o, float* lse, void* ws, size_t n,
+          hipStream_t s) {
+  q27::attn_prep_paged(x, x, x, x, x, o, kv, pos, cu, 9, 1e-6f, 0.6f, 24, s, nullptr, pos);
+  q27::attn_paged(x, kv, pos, cu, 9, 4, 0.0625f, 24, o, ws, n, s, lse);
+  q27::kv_pages_read(kv, nullptr, pos, 100, Q27H_F16, ws, ws, s);
+  q27::draft_verify(x, 100, x, 100, pos, nullptr, x, x, cu, 3, 9, 100, out, out, out, ws, n, s, pos);
+}
+int main(int argc, char**) {
+  q27::KvPages kv = {nullptr, nullptr, nullptr, 3, 8, 50, 4, 64, Q27H_KV_Q8_Q4};
+  if (argc > 9) step(nullptr, kv, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr);
+  size_t n = q27::kv_page_bytes(4, 64, kv.type, true) + q27::attn_paged_ws_bytes(kv, 9, 4, 24) + q27::draft_verify_ws_bytes(3, 100);
+  try {
+    q27::attn_paged(nullptr, kv, nullptr, nullptr, 9, 4, 1.0f, 24, nullptr, nullptr, 0, nullptr);
+  } catch (const std::runtime_error& e) {
+    std::printf("%d %s\n", n > 0, e.what());
+    return 0;
+  }
+  return 1;
+}
+''')
+    subprocess.run(["/opt/rocm/llvm/bin/clang++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    f"-I{root}/include", str(src), f"-L{lib}", "-lq27h", "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{lib}",
+                    "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)], check=True, capture_output=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout
+    assert out.startswith("1 ") and "null pointer" in out
+
+
+def test_header_is_c(tmp_path):
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "caller.c"
+    src.write_text('#include "q27h.h"\nint main(void) { q27h_kv_pages kv = {0}; return q27h_kv_pages_read(&kv, 0, 0, 0, Q27H_F32, 0, 0, 0) == 0; }\n')
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", f"-I{root}/include", "-c", str(src), "-o", str(tmp_path / "o")], check=True)
