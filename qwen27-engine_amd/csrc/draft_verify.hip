@@ -116,10 +116,27 @@ __device__ __forceinline__ void load_chunk(const float* row, int chunk, int n, f
   }
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+// Sums over the lanes up to each one; 0 comes from lanes that do not exist.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lanes(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lanes_before(double x) {
+  x += from_lanes<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
+  x += from_lanes<0x112, 0xf>(x);
+  x += from_lanes<0x114, 0xf>(x);
+  x += from_lanes<0x118, 0xf>(x);
+  x += from_lanes<0x142, 0xa>(x);  // row_bcast 15, 31: the rows before
+  x += from_lanes<0x143, 0xc>(x);
   return x;
+}
+__device__ __forceinline__ double read_lane(double x, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
@@ -138,9 +155,9 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
 #pragma unroll
     for (int i = 0; i < kPerThread; i++) left += weight_of((double)p[i] - q[i]);
   }
-  left = wave_sum(left);
-  all = wave_sum(all);
-  if ((threadIdx.x & 63) == 0) s_red[0][w] = left, s_red[1][w] = all;
+  all = lanes_before(all);
+  if (k.refused) left = lanes_before(left);
+  if ((threadIdx.x & 63) == 63) s_red[0][w] = left, s_red[1][w] = all;
   __syncthreads();
   if (threadIdx.x) return;
   left = (s_red[0][0] + s_red[0][1]) + (s_red[0][2] + s_red[0][3]);
@@ -148,78 +165,44 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
   a.sums[(size_t)b * a.chunks + chunk] = make_double2(left, all);
 }
 
-// Exclusive sum over the workgroup's threads, and the whole sum.
-__device__ __forceinline__ double before_of(double x, double* red, double& total) {
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double s = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double y = __shfl_up(s, d);
-    s += l >= d ? y : 0.0;
-  }
-  __syncthreads();
-  if (l == 63) red[w] = s;
-  __syncthreads();
-  total = 0.0;
-  double before = s - x;
-#pragma unroll
-  for (int k = 0; k < kThreads / 64; k++) {
-    before += k < w ? red[k] : 0.0;
-    total += red[k];
-  }
-  return before;
-}
-
+// Every wave finds the chunk by itself, 64 chunks at a time; then a thread has 16 neighbouring values of it.
 __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
-  __shared__ double s_red[kThreads / 64], s_before;
-  __shared__ int s_chunk, s_token, s_n;
-  __shared__ int s_bad[kMostTokens];
-  __shared__ double s_takes[kMostTokens];
-  const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63;
+  __shared__ double s_sum[kThreads / 64];
+  const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const double2* sums = a.sums + (size_t)b * a.chunks;
+  double left0 = 0.0, all0 = 0.0;  // of the first 64 chunks, on their way with the walk
+  if (l < a.chunks) left0 = sums[l].x, all0 = sums[l].y;
   const Walk k = a.walks[b];
+  const int n = __builtin_popcountll(k.path);
   if (!k.nt) {
     if (tid == 0) a.n_path[b] = 0;
     return;
   }
   const int id = l < k.nt ? a.ids[k.t0 + l] : -1;  // lane t: token t
   const float* prow = a.p + (size_t)(k.t0 + k.node) * a.ldp;
-  const float* qrow = a.q ? a.q + (size_t)(k.t0 + k.node + 1) * a.ldq : nullptr;
-  // the refused children weigh nothing: their ids, each once, and what they take from their chunks' sums, exactly
-  if (tid < 64) {
-    const bool bad = k.tried >> l & 1;
-    bool first = bad && (unsigned)id < (unsigned)a.V;
-    for (uint64_t m = k.tried; m; m &= m - 1) {
-      const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
-      if (__builtin_amdgcn_readlane(id, t) == id && t < l) first = false;
-    }
-    const uint64_t each = __ballot(first);
-    if (first) {
-      const int at = __builtin_popcountll(each & ((1ull << l) - 1));
-      s_bad[at] = id;
-      s_takes[at] = weight_of(prow[id]);
-    }
-    if (l == 0) s_n = __builtin_popcountll(each), s_chunk = s_token = -1;
+  const float* qrow = k.refused ? a.q + (size_t)(k.t0 + k.node + 1) * a.ldq : prow;
+  // the refused children weigh nothing: each id once (lanes of `bad`), and what it takes from its chunk's sum, exactly
+  bool lead = (k.tried >> l & 1) && (unsigned)id < (unsigned)a.V;
+  for (uint64_t m = k.tried; m; m &= m - 1) {
+    const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+    if (__builtin_amdgcn_readlane(id, t) == id && t < l) lead = false;
   }
-  __syncthreads();
-  const int n_bad = s_n;
-  auto is_bad = [&](int i) {
-    bool bad = false;
-    for (int j = 0; j < n_bad; j++) bad |= s_bad[j] == i;
-    return bad;
-  };
-  const double2* sums = a.sums + (size_t)b * a.chunks;
-  auto taken = [&](int chunk) {
-    double t = 0.0;
-    for (int j = 0; j < n_bad; j++) t += s_bad[j] / kChunk == chunk ? s_takes[j] : 0.0;
-    return t;
-  };
-  // the chunk: 256 of them at a time, first their whole sum
+  const uint64_t bad = __ballot(lead);
+  const double takes = lead ? weight_of(prow[id]) : 0.0;
   bool use_q = k.refused;
+  auto sum_of = [&](int c) {  // of chunk c
+    double x = use_q ? left0 : all0;
+    if (c != l) x = c >= a.chunks ? 0.0 : use_q ? sums[c].x : sums[c].y;
+    for (uint64_t m = bad; m; m &= m - 1) {
+      const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+      x -= __builtin_amdgcn_readlane(id, t) / kChunk == c ? read_lane(takes, t) : 0.0;
+    }
+    return x;
+  };
   double total = 0.0;
   for (int pass = 0; pass < 2; pass++) {
-    double mine = 0.0;
-    for (int c = tid; c < a.chunks; c += kThreads) mine += use_q ? sums[c].x : sums[c].y - taken(c);
-    before_of(mine, s_red, total);
+    total = 0.0;
+    for (int c0 = 0; c0 < a.chunks; c0 += 64) total += read_lane(lanes_before(sum_of(c0 + l)), 63);
     if (total > 0.0 || !use_q) break;
     use_q = false;  // p nowhere above q: the target's own distribution
   }
@@ -228,27 +211,28 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   u = u < 0x1.fffffep-1 ? u : 0x1.fffffep-1;
   const double want = u * total;
   double base = 0.0;
-  for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
-    const int c = c0 + tid;
-    const double x = c < a.chunks ? (use_q ? sums[c].x : sums[c].y - taken(c)) : 0.0;
-    double part;
-    const double before = base + before_of(x, s_red, part);
-    if (before <= want && want < before + x) s_chunk = c, s_before = before;
-    base += part;
+  int chunk = -1;
+  for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
+    const double x = sum_of(c0 + l), to = base + lanes_before(x);
+    const uint64_t hit = __ballot(to - x <= want && want < to);
+    if (hit) {
+      const int t = __builtin_ctzll(hit);
+      chunk = c0 + t;
+      base = read_lane(to - x, t);
+    } else {
+      base = read_lane(to, 63);
+    }
   }
-  __syncthreads();
-  const int chunk = s_chunk;
+  if (tid == 0) a.out[k.t0 + n - 1] = -1;  // unless there is a token, below and behind the barrier
   if (chunk >= 0) {
-    // its values in order, 16 neighbours a thread
     const int i0 = chunk * kChunk + tid * kPerThread;
     double wt[kPerThread], mine = 0.0;
     if (i0 + kPerThread <= a.V) {
       f4u pv[kPerThread / 4], qv[kPerThread / 4];
 #pragma unroll
-      for (int g = 0; g < kPerThread / 4; g++) pv[g] = *(const f4u*)(prow + i0 + 4 * g);
-      if (use_q) {
-#pragma unroll
-        for (int g = 0; g < kPerThread / 4; g++) qv[g] = *(const f4u*)(qrow + i0 + 4 * g);
+      for (int g = 0; g < kPerThread / 4; g++) {
+        pv[g] = *(const f4u*)(prow + i0 + 4 * g);
+        if (use_q) qv[g] = *(const f4u*)(qrow + i0 + 4 * g);
       }
 #pragma unroll
       for (int i = 0; i < kPerThread; i++) wt[i] = weight_of(use_q ? (double)pv[i >> 2][i & 3] - qv[i >> 2][i & 3] : (double)pv[i >> 2][i & 3]);
@@ -257,34 +241,35 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
       for (int i = 0; i < kPerThread; i++)
         wt[i] = i0 + i < a.V ? weight_of(use_q ? (double)prow[i0 + i] - qrow[i0 + i] : (double)prow[i0 + i]) : 0.0;
     }
-    if (n_bad) {
+    for (uint64_t m = bad; m; m &= m - 1) {
+      const int at = __builtin_amdgcn_readlane(id, __builtin_amdgcn_readfirstlane(__builtin_ctzll(m))) - i0;
 #pragma unroll
-      for (int i = 0; i < kPerThread; i++) wt[i] = is_bad(i0 + i) ? 0.0 : wt[i];
+      for (int i = 0; i < kPerThread; i++) wt[i] = at == i ? 0.0 : wt[i];
     }
 #pragma unroll
     for (int i = 0; i < kPerThread; i++) mine += wt[i];
-    double part;
-    double at = s_before + before_of(mine, s_red, part);
+    double at = lanes_before(mine);
+    if (l == 63) s_sum[w] = at;
+    __syncthreads();
+    at += base - mine;
+#pragma unroll
+    for (int j = 0; j < kThreads / 64; j++) at += j < w ? s_sum[j] : 0.0;
 #pragma unroll
     for (int i = 0; i < kPerThread; i++) {
       const double to = at + wt[i];
-      if (at <= want && want < to) s_token = i0 + i;
+      if (at <= want && want < to) a.out[k.t0 + n - 1] = i0 + i;  // one thread's one value
       at = to;
     }
-    __syncthreads();
   }
   if (tid >= 64) return;
   // token l of the walk's path goes to its place among them
-  const int n = __builtin_popcountll(k.path);
   const int rank = __builtin_popcountll(k.path & ((1ull << l) - 1));
-  const bool on = k.path >> l & 1;
-  if (on) {
+  if (k.path >> l & 1) {
     a.path[k.t0 + rank] = l;
     if (rank) a.out[k.t0 + rank - 1] = id;
   }
   if (l >= n && l < k.nt) a.path[k.t0 + l] = a.out[k.t0 + l] = -1;
   if (l == 0) {
-    a.out[k.t0 + n - 1] = s_token;
     a.n_path[b] = n;
     if (a.pos) a.pos[b] += n;
   }
