@@ -187,7 +187,7 @@ __device__ __forceinline__ int size_of(int total, int slots) {
 // The part that a workgroup has: sequence, unit of it, the part's number in the unit and how many it has, their size, and
 // the part's place in the workspace. seq < 0: none. Whole parts come before those that are left over, and of these the ones
 // over half the size before the others: workgroups start in this order as others end, so that the last to end are short (48
-// sequences of 500 to 32768 rows, 704 parts in any order: @@, so @@). The first workgroup leaves for the join where the
+// sequences of 500 to 32768 rows, 4 tokens each: 293 us with parts in any order, 250 so). The first workgroup leaves for the join where the
 // places of each sequence begin, and the size behind them.
 struct Part {
   int seq, unit, k, parts, size, place;
