@@ -23,8 +23,8 @@ struct PagedArgs {
   const int *pos, *cu;
   float *o, *lse;        // lse may be null
   float *part, *ml;      // [place][row of its unit][256], [..][2]
-  int* starts;           // [n_seqs + 1]: each sequence's first place; the size of a part
-  int T, most, nqh, slots;  // slots: shares of the whole work, see Part
+  int* starts;           // [n_seqs][2]: each sequence's first place, and the parts of each of its units
+  int T, most, nqh, slots;  // slots: shares of the whole work, about the workgroups that run at a time
   float scale;
 };
 
@@ -178,7 +178,7 @@ __device__ __forceinline__ Demand demand_of(const PagedArgs& a, int nt, const Vi
   const int tiles = vis.end > 0 ? (vis.end + kTileKeys - 1) / kTileKeys : 1;
   return {a.pg.nkvh * ((nt * (a.nqh / a.pg.nkvh) + rows - 1) / rows), (tiles + kWaves - 1) / kWaves * kWaves};
 }
-// Every unit is cut in parts of one size, its last one what is left: the total by the workgroups that run at a time.
+// Every unit is cut in parts of one size, its last one what is left: the total by the shares.
 __device__ __forceinline__ int size_of(int total, int slots) {
   const int each = (total + slots - 1) / slots;
   return each ? (each + kWaves - 1) / kWaves * kWaves : kWaves;
@@ -188,7 +188,7 @@ __device__ __forceinline__ int size_of(int total, int slots) {
 // the part's place in the workspace. seq < 0: none. Whole parts come before those that are left over, and of these the ones
 // over half the size before the others: workgroups start in this order as others end, so that the last to end are short (48
 // sequences of 500 to 32768 rows, 4 tokens each: 293 us with parts in any order, 250 so). The first workgroup leaves for the join where the
-// places of each sequence begin, and the size behind them.
+// places of each sequence begin and how many parts its units have.
 struct Part {
   int seq, unit, k, parts, size, place;
   Tokens tk;
@@ -225,8 +225,7 @@ __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   const int s0 = lanes_before(n0), s1 = lanes_before(n1), s2 = lanes_before(n2), sp = lanes_before(np);
   const int all0 = __builtin_amdgcn_readlane(s0, 63), all1 = __builtin_amdgcn_readlane(s1, 63);
   if (blockIdx.x == 0 && threadIdx.x < 64) {
-    if (is) a.starts[l] = sp - np;
-    if (l == 0) a.starts[a.pg.n_seqs] = p.size;
+    if (is) *(int2*)(a.starts + 2 * l) = make_int2(sp - np, parts);
   }
   int me = (int)blockIdx.x, kind = 0;
   if (me >= all0) me -= all0, kind = 1;
@@ -308,12 +307,12 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   auto of_kind = [&](const Counts& c) { return kind == 0 ? (int)c.a : kind == 1 ? (int)c.b : (int)(c.b >> 32); };
   const int lo = of_kind(at);
   const bool lead = blockIdx.x == 0, here = lo <= me && me < lo + of_kind(mine);
-  if (lead && tid == 0) a.starts[a.pg.n_seqs] = p.size;
   if (lead || here) {
     for (int b = b0; b < b1; b++) {
-      const Counts c = count(b == b0 ? first : demand(b));
+      const Demand d = b == b0 ? first : demand(b);
+      const Counts c = count(d);
       const int x = of_kind(at);
-      if (lead) a.starts[b] = (int)(at.a >> 32);
+      if (lead) *(int2*)(a.starts + 2 * b) = make_int2((int)(at.a >> 32), (d.span + p.size - 1) / p.size);
       if (x <= me && me < x + of_kind(c)) s_part[0] = b, s_part[1] = me - x, s_part[2] = (int)(at.a >> 32);
       at.a += c.a, at.b += c.b;
     }
@@ -796,24 +795,19 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   }
 }
 
-// Joins the parts of one query row (token t of sequence b, query head h), in order: wave w of WAVES takes every WAVES-th
-// part, a lane four dims; then the waves' sums are added in order. 16 waves where there are few rows, which may have many
-// parts; 4 where there are many.
-template <int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArgs a, int rows) {
-  __shared__ f4 s_o[WAVES][64];
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  const int h = blockIdx.x % a.nqh, t = (int)(blockIdx.x / a.nqh) % a.most, b = (int)(blockIdx.x / a.nqh) / a.most;
-  const int start = uniform_load(a.starts + b), size = uniform_load(a.starts + a.pg.n_seqs), pos = uniform_load(a.pos + b);
-  const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
-  if (t >= tk.nt) return;
-  const Vis vis = vis_of(pos, tk.nt, a.pg.max_pages << a.pg.shift);
-  const int n = (demand_of(a, tk.nt, vis, rows).span + size - 1) / size;
-  if (n == 1) return;
-  const int group = a.nqh / a.pg.nkvh, r = t * group + h % group, groups = (tk.nt * group + rows - 1) / rows;
-  const size_t place = ((size_t)start + (size_t)(h / group * groups + r / rows) * n) * rows + r % rows;
-  const f4* part = (const f4*)(a.part + place * kHD) + l;  // part k: k * rows rows on
-  const float2* ml = (const float2*)a.ml + place;
+// ---------------------------------------------------------------- the join
+// A query row whose unit was cut: its first part in the workspace, and how many.
+struct Cut {
+  int n;         // 0 or 1: there is nothing to join
+  size_t place;  // part k: k * rows rows on
+  size_t row;    // its place in the results
+};
+// Wave w's share of a row, every WAVES-th part in order: a lane four dims; m and sum are the whole row's.
+template <int WAVES, int rows>
+__device__ __forceinline__ f4 join_of(const PagedArgs& a, const Cut& c, int w, float& m, float& sum) {
+  const int l = threadIdx.x & 63, n = c.n;
+  const f4* part = (const f4*)(a.part + c.place * kHD) + l;
+  const float2* ml = (const float2*)a.ml + c.place;
   constexpr int kBatch = 4;
   f4 x[kBatch];
 #pragma unroll
@@ -828,12 +822,12 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
     return op(y, lane_xor32(y));
   };
   // every wave for itself, lane l parts l, l + 64, ..
-  float2 v = l < n ? ml[l * rows] : make_float2(-3.0e38f, 0.0f);
-  float m = v.x;
+  const float2 v = l < n ? ml[l * rows] : make_float2(-3.0e38f, 0.0f);
+  m = v.x;
   for (int k = l + 64; k < n; k += 64) m = __builtin_fmaxf(m, ml[k * rows].x);
   m = all(m, [](float p, float q) { return __builtin_fmaxf(p, q); });
   const float f = __builtin_amdgcn_exp2f(v.x - m);
-  float sum = v.y * f;
+  sum = v.y * f;
   for (int k = l + 64; k < n; k += 64) sum += ml[k * rows].y * __builtin_amdgcn_exp2f(ml[k * rows].x - m);
   sum = all(sum, [](float p, float q) { return p + q; });
   auto factor = [&](int k) {  // of part k, the same in the whole wave
@@ -841,11 +835,10 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
                   : __builtin_amdgcn_exp2f(ml[k * rows].x - m);
   };
   f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int w0 = __builtin_amdgcn_readfirstlane(w);
 #pragma unroll
   for (int k = 0; k < kBatch; k++)
-    if (w0 + WAVES * k < n) o += x[k] * factor(w0 + WAVES * k);
-  for (int k0 = w0 + WAVES * kBatch; k0 < n; k0 += WAVES * kBatch) {
+    if (w + WAVES * k < n) o += x[k] * factor(w + WAVES * k);
+  for (int k0 = w + WAVES * kBatch; k0 < n; k0 += WAVES * kBatch) {
 #pragma unroll
     for (int k = 0; k < kBatch; k++)
       if (k0 + WAVES * k < n) x[k] = part[(size_t)(k0 + WAVES * k) * rows * 64];
@@ -853,15 +846,30 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
     for (int k = 0; k < kBatch; k++)
       if (k0 + WAVES * k < n) o += x[k] * factor(k0 + WAVES * k);
   }
+  return o;
+}
+// A workgroup joins a row: sequence blockIdx.x, token y, query head z. 16 waves where there are few rows, which may have many
+// parts; 4 where there are many (a row to each wave was slower: 32 sequences 14 us, with 4 waves to a row 5.9).
+template <int WAVES, int ROWS>
+__global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArgs a) {
+  __shared__ f4 s_o[WAVES][64];
+  const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.x, t = blockIdx.y, h = blockIdx.z;
+  const int start = uniform_load(a.starts + 2 * b), n = uniform_load(a.starts + 2 * b + 1);
+  const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
+  if (t >= tk.nt || n <= 1) return;
+  const int group = a.nqh / a.pg.nkvh, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + ROWS - 1) / ROWS;
+  const Cut c = {n, ((size_t)start + (size_t)(kh * groups + r / ROWS) * n) * ROWS + r % ROWS, (size_t)(tk.t0 + t) * a.nqh + h};
+  float m, sum;
+  f4 o = join_of<WAVES, ROWS>(a, c, w, m, sum);
   s_o[w][l] = o;
   __syncthreads();
   if (w) return;
 #pragma unroll
   for (int k = 1; k < WAVES; k++) o += s_o[k][l];
-  const size_t gr = (size_t)(tk.t0 + t) * a.nqh + h;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  *((f4*)(a.o + gr * kHD) + l) = o * inv;
-  if (a.lse && l == 0) a.lse[gr] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  *((f4*)(a.o + c.row * kHD) + l) = o * inv;
+  if (a.lse && l == 0) a.lse[c.row] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 struct Layout {
@@ -875,15 +883,17 @@ Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   const int rows = max_tokens * (nqh / nkvh);
   y.wr = rows <= 16 ? 1 : 2;
   y.threads = y.wr == 2 && type == Q27H_KV_F16 ? 512 : 256;
-  // the kernel of more than 16 query rows over codes is bound by arithmetic: half as many parts more leave less of it to the
-  // last ones (48 sequences of 4 drafts, 371589 rows: 237 -> 218 us; of one token, bound by HBM: 51.0 -> 52.0)
-  y.slots = y.wr == 2 && type != Q27H_KV_F16 ? 3 * kCUs : 2 * kCUs * 256 / y.threads;
-  // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has two
-  // parts at least and not two more than its share
   const int units = n_seqs * nkvh * ((rows + 16 * y.wr - 1) / (16 * y.wr));
+  y.slots = 2 * kCUs * 256 / y.threads;
+  // over codes, more than 16 query rows are bound by arithmetic: with units of many lengths, half as many shares more leave
+  // the last workgroups less of it (200 sequences of 300 to 4096 rows, 4 tokens: 184 -> 173 us); one sequence is cut evenly,
+  // and a second round of workgroups costs it (150000 rows: 82 -> 91 us)
+  if (y.wr == 2 && type != Q27H_KV_F16 && units >= kCUs / 2) y.slots = 3 * kCUs;
+  // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has less than
+  // twice its share of parts
   y.grid = units + y.slots;
   y.places = (size_t)(y.grid < 2 * y.slots ? y.grid : 2 * y.slots) * 16 * y.wr;
-  y.bytes = y.places * (kHD + 2) * sizeof(float) + ((size_t)n_seqs + 1) * sizeof(int);
+  y.bytes = y.places * (kHD + 2) * sizeof(float) + (size_t)n_seqs * 2 * sizeof(int);
   return y;
 }
 bool shape_ok(const q27h_kv_pages* kv, int max_tokens, int nqh) {
@@ -934,9 +944,9 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
   else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_wide_kernel<Q27H_KV_Q8, 2>);
   else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_wide_kernel<Q27H_KV_Q8_Q4, 2>);
   const int qrows = kv->n_seqs * max_tokens * nqh;
-  if (qrows <= 2 * kCUs)
-    hipLaunchKernelGGL(attn_paged_join_kernel<16>, dim3((unsigned)qrows), dim3(1024), 0, stream_of(s), a, 16 * y.wr);
-  else
-    hipLaunchKernelGGL(attn_paged_join_kernel<4>, dim3((unsigned)qrows), dim3(256), 0, stream_of(s), a, 16 * y.wr);
+  const dim3 all((unsigned)kv->n_seqs, (unsigned)max_tokens, (unsigned)nqh);
+  auto join = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, all, dim3(64 * waves), 0, stream_of(s), a); };
+  if (qrows <= 2 * kCUs) join(y.wr == 1 ? attn_paged_join_kernel<16, 16> : attn_paged_join_kernel<16, 32>, 16);
+  else join(y.wr == 1 ? attn_paged_join_kernel<4, 16> : attn_paged_join_kernel<4, 32>, 4);
   return check_launch("attn_paged");
 }

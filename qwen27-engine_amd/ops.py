@@ -270,11 +270,14 @@ def draft_verify(p, q, ids, parent, u, u_last, cu, n_seqs, V, out, path, n_path,
     """Which drafted tokens stand and the token after them (out), their rows (path, n_path: kv_accept's), by the uniform numbers u
     and u_last. p, q: f32 rows of V values, one per token; q None: drafts without probabilities, a tree by parent (None: a
     chain). pos int32 [n_seqs] (may be None) grows by n_path."""
-    for x in (p, q):
-        if x is not None and x.dim() == 2 and x.stride(1) != 1:
-            raise ValueError("draft_verify: rows of p and q are contiguous")
     T = ids.numel()
-    ld = lambda x: x.stride(0) if x is not None and x.dim() == 2 and T > 1 else V  # noqa: E731
+
+    def ld(x):
+        at = (1,) if x is None else x.stride()
+        if at[-1] != 1:
+            raise ValueError("draft_verify: rows of p and q are contiguous")
+        return at[0] if len(at) == 2 and T > 1 else V
+
     check(lib().q27h_draft_verify(_ptr(p), ld(p), _ptr(q), ld(q), _ptr(ids), _ptr(parent), _ptr(u), _ptr(u_last), _ptr(cu), n_seqs, T, V,
                                   _ptr(out), _ptr(path), _ptr(n_path), _ptr(pos), _ptr(ws), _bytes(ws), _stream(s)))
 
