@@ -3,9 +3,11 @@
 //
 // A unit of work is (sequence, kv head, 16 or 32 query rows): query rows are tokens x query heads of the kv head, as in
 // attn_tree. Sequences are of any length, so a unit's tiles of 32 cache rows are cut in parts none of which is longer than a
-// fixed share of the tiles of all units. Every workgroup has a part, which it finds from the lengths of all sequences itself;
-// its four waves each walk tiles of their own with the online softmax of attn_core.h. The parts of a unit that was cut go to
-// the workspace, and a second launch joins those of each query row in order.
+// fixed share of the tiles of all units. Every workgroup has a part, which it finds from the lengths of all sequences
+// itself. Up to 16 query rows, and over f16, its waves each walk tiles of their own with the online softmax of attn_core.h,
+// bound by HBM (128 sequences of 4096 q8_0 rows, one token: 5.4 TB/s; f16, 2048 rows, four tokens: 5.0); more over codes share
+// them, see below. The parts of a unit that was cut go to the workspace, and a second launch joins those of each query
+// row in order.
 #include <type_traits>
 
 #include "attn_wave.h"
@@ -14,8 +16,8 @@
 namespace q27h {
 namespace {
 
-constexpr int kWaves = 4;          // waves that share a segment's tiles
-constexpr int kMostTokens = 64;    // tokens of one sequence: hide()'s 64-bit masks
+constexpr int kWaves = 4;        // waves that share a part's tiles
+constexpr int kMostTokens = 64;  // tokens of one sequence: hide()'s 64-bit masks
 
 struct PagedArgs {
   Pages pg;
@@ -396,12 +398,15 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
 // A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
 // of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
 // query rows, and a wave holds a quarter of the outputs. The weights and the V rows go from the one to the other through LDS.
+// 48 sequences of 500 to 32768 rows with 4 tokens each, V in 4 bits: 180 us of its own, where waves with tiles of their own
+// take 270. What bounds it is no one thing: it runs at 3.4 TB/s, its vector instructions fill half the cycles; without the
+// weights' scaling it would be 9% faster, without the second f16 terms 16%, without its loads 12%.
 //
 // One reference E for each query row, the same in all waves: a row's product of weight and V scale is 2^(s - E) f d, f the
 // power of two above the V row's scales and d what is left of each (at most 1). E moves when a row's s + log2 f passes
 // E + 15, to 12 below it, so that what enters the product as two f16 terms is in their range, as in attn_core.h; the sum of
 // the weights is kept in units of 2^E as well. Rows whose V scales are all 0 count as f = 2^-25.
-template <int QT>
+constexpr int QT = 2;  // row tiles of a unit
 struct WideLds {
   union {
     QTile q[QT];
@@ -470,10 +475,8 @@ __device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* c
   }
 }
 
-// Scores of the wave's 32 rows and QT row tiles, as attn_core.h's. A step is (block, row tile): its four matrix
-// instructions, and between them the scaling of the step before and a share of the next block's codes, since a wave
-// issues in order and a matrix instruction takes four times a vector one.
-template <int QT>
+// Scores of the wave's 32 rows for the two row tiles, as attn_core.h's. A step is (block, row tile): its four matrix instructions
+// with the scaling of the step before and a share of the next block's codes beside them.
 __device__ __forceinline__ void wide_scores(const uint8_t* codes, const uint8_t* ks, const h8 (&hi)[QT][8],
                                             const uint32_t (*lo)[8][64][4], f4 (&s)[QT][2]) {
   const int l = threadIdx.x & 63;
@@ -519,21 +522,18 @@ __device__ __forceinline__ void wide_scores(const uint8_t* codes, const uint8_t*
     for (int u = 0; u < 2; u++) c[i & 1][u] = mfma16(x[b & 1][u], hi[q][b], c[i & 1][u]);
     if (i) scale(i - 1);
     if (q == QT - 1 && b < 7) ask_s(b + 1);
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      if (b >= 7 || (QT > 1 && q != u)) continue;
-      turn(b + 1, u);
-      if (b < 6) ask_k(b + 2, u);
+    if (b < 7) {  // a row tile's step: one half of the next block's rows
+      turn(b + 1, q);
+      if (b < 6) ask_k(b + 2, q);
     }
-    interleave<QT == 1 ? 7 : 4>();
   }
   scale(8 * QT - 1);
 }
 
-template <int TYPE, int QT>
+template <int TYPE>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedArgs a) {
   constexpr int kRows = 16 * QT, kV = TYPE == Q27H_KV_Q8_Q4 ? kHD / 2 : kHD, kBias = TYPE == Q27H_KV_Q8_Q4 ? 8 : 128;
-  __shared__ WideLds<QT> sh;
+  __shared__ WideLds sh;
   const Part pt = part_of<kWaves * 64>(a, kRows);
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15;
@@ -639,7 +639,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
       ask_pages(t + kWaves);
     }
     loads_issued();
-    wide_scores<QT>(sh.codes[w], sh.ks[w], hi, sh.lo, s);
+    __builtin_amdgcn_s_setprio(1);  // products before the other workgroup's staging (128 sequences of 4096 rows: 269 -> 263 us)
+    wide_scores(sh.codes[w], sh.ks[w], hi, sh.lo, s);
+    __builtin_amdgcn_s_setprio(0);
     if (kPart) {
       Vis mine = vis;
       uint64_t chain[QT];
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
     }
     __syncthreads();
     // O += P V: the wave's two blocks of 32 dims; the transposing read as in attn_core.h. A step per (group, block): its
-    // products, the next step's weights and codes between them
+    // products, and the next step's weights and codes beside them
     const uint8_t* vbase = sh.codes[0] + ((n >> 1) >= 4 ? kUpper + (4 * g + (n >> 1) - 4) * kRow : (4 * g + (n >> 1)) * kRow) + 8 * (n & 1) + 64 * w;
     u4 ph[QT], pl[QT], wh[2][QT], wl[2][QT];
     typedef int v2i __attribute__((ext_vector_type(2)));
@@ -731,6 +733,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
 #pragma unroll
       for (int h = 0; h < 2; h++) v[i & 1][h] = codes8<kBias>((uint32_t)x[h].x, (uint32_t)x[h].y);
     };
+    __builtin_amdgcn_s_setprio(1);
     ask_p(0);
     ask(0);
     turn(0);
@@ -753,10 +756,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
           if (!b) ask_p((i + 2) >> 1);
           ask(i + 2);
         }
-        interleave<5>();
-        if (QT == 2) interleave<5>();
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();  // V's rows are read: K's take their place
   };
   while (t < t1) {
@@ -896,8 +898,17 @@ Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   y.bytes = y.places * (kHD + 2) * sizeof(float) + (size_t)n_seqs * 2 * sizeof(int);
   return y;
 }
-bool shape_ok(const q27h_kv_pages* kv, int max_tokens, int nqh) {
-  return max_tokens >= 1 && max_tokens <= kMostTokens && nqh > 0 && nqh <= 4096 && nqh % kv->nkvh == 0;
+// Why a call of these sizes is refused, or null.
+const char* refusal(const q27h_kv_pages* kv, int T, int max_tokens, int nqh) {
+  if (T < 0 || max_tokens < 1 || max_tokens > kMostTokens || nqh <= 0 || nqh > 4096 || nqh % kv->nkvh)
+    return "attn_paged: bad shape (1 to 64 tokens a sequence, at most 4096 query heads)";
+  // the tiles of all units are counted in 31 bits
+  const int group = nqh / kv->nkvh;
+  const long long tiles = ((long long)kv->max_pages * kv->page_rows / kTileKeys + kWaves) / kWaves * kWaves;
+  if ((double)kv->n_seqs * kv->nkvh * ((max_tokens * group + 15) / 16) * (double)tiles > 2.0e9) return "attn_paged: too many rows in all";
+  if ((long long)kv->n_seqs * max_tokens * nqh > 0x7fffffffLL / 256 || (long long)T * nqh > 0x7fffffffLL / 256)
+    return "attn_paged: too many query rows";
+  return nullptr;
 }
 
 }  // namespace
@@ -906,22 +917,15 @@ bool shape_ok(const q27h_kv_pages* kv, int max_tokens, int nqh) {
 using namespace q27h;
 
 extern "C" size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int max_tokens, int nqh) {
-  if (check_pages(kv, "attn_paged") != Q27H_OK || T <= 0 || !shape_ok(kv, max_tokens, nqh)) return 0;
+  if (check_pages(kv, "attn_paged") != Q27H_OK || T <= 0 || refusal(kv, T, max_tokens, nqh)) return 0;
   return layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh, kv->type).bytes;
 }
 
 extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens,
                                float scale, int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s) {
   if (const int bad = check_pages(kv, "attn_paged")) return bad;
-  if (T < 0 || !shape_ok(kv, max_tokens, nqh))
-    return fail(Q27H_ERR_SHAPE, "attn_paged: bad shape (1 to 64 tokens a sequence, at most 4096 query heads)");
+  if (const char* why = refusal(kv, T, max_tokens, nqh)) return fail(Q27H_ERR_SHAPE, why);
   if (!cu && T != kv->n_seqs) return fail(Q27H_ERR_SHAPE, "attn_paged: without cu there is one token for each sequence");
-  const int group = nqh / kv->nkvh;
-  const long long tiles = ((long long)kv->max_pages * kv->page_rows / kTileKeys + kWaves - 1) / kWaves * kWaves;
-  if ((double)kv->n_seqs * kv->nkvh * ((max_tokens * group + 15) / 16) * (double)tiles > 2.0e9)
-    return fail(Q27H_ERR_SHAPE, "attn_paged: too many rows in all");
-  if ((long long)kv->n_seqs * max_tokens * nqh > 0x7fffffffLL / 256 || (long long)T * nqh > 0x7fffffffLL / 256)
-    return fail(Q27H_ERR_SHAPE, "attn_paged: too many query rows");
   if (T == 0 || kv->n_seqs == 0) return Q27H_OK;
   if (!qn || !pos || !o) return fail(Q27H_ERR_ARG, "attn_paged: null pointer");
   if (!aligned16(qn) || !aligned16(o) || !aligned16(ws)) return fail(Q27H_ERR_ARG, "attn_paged: tensors need 16-byte alignment");
@@ -941,8 +945,8 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
   const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);
   auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.wr == 1 ? one : two), grid, block, 0, stream_of(s), a); };
   if (kv->type == Q27H_KV_F16) launch(attn_paged_kernel<Q27H_KV_F16, 1>, attn_paged_kernel<Q27H_KV_F16, 2>);
-  else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_wide_kernel<Q27H_KV_Q8, 2>);
-  else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_wide_kernel<Q27H_KV_Q8_Q4, 2>);
+  else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_wide_kernel<Q27H_KV_Q8>);
+  else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_wide_kernel<Q27H_KV_Q8_Q4>);
   const int qrows = kv->n_seqs * max_tokens * nqh;
   const dim3 all((unsigned)kv->n_seqs, (unsigned)max_tokens, (unsigned)nqh);
   auto join = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, all, dim3(64 * waves), 0, stream_of(s), a); };
