@@ -189,8 +189,8 @@ __device__ __forceinline__ int size_of(int total, int slots) {
 // The part that a workgroup has: sequence, unit of it, the part's number in the unit and how many it has, their size, and
 // the part's place in the workspace. seq < 0: none. Whole parts come before those that are left over, and of these the ones
 // over half the size before the others: workgroups start in this order as others end, so that the last to end are short (48
-// sequences of 500 to 32768 rows, 4 tokens each: 293 us with parts in any order, 250 so). The first workgroup leaves for the join where the
-// places of each sequence begin and how many parts its units have.
+// sequences of 500 to 32768 rows, 4 tokens each, with the kernel of that time: 293 us with parts in any order, 250 so). The
+// first workgroup leaves for the join where the places of each sequence begin and how many parts its units have.
 struct Part {
   int seq, unit, k, parts, size, place;
   Tokens tk;
@@ -475,8 +475,8 @@ __device__ __forceinline__ void wide_stage_v(const WideRegs<TYPE>& r, uint8_t* c
   }
 }
 
-// Scores of the wave's 32 rows for the two row tiles, as attn_core.h's. A step is (block, row tile): its four matrix instructions
-// with the scaling of the step before and a share of the next block's codes beside them.
+// Scores of the wave's 32 rows for the two row tiles, as attn_core.h's. A step is (block, row tile): its four matrix
+// instructions with the scaling of the step before and a share of the next block's codes beside them.
 __device__ __forceinline__ void wide_scores(const uint8_t* codes, const uint8_t* ks, const h8 (&hi)[QT][8],
                                             const uint32_t (*lo)[8][64][4], f4 (&s)[QT][2]) {
   const int l = threadIdx.x & 63;
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   }
   __syncthreads();
 
-  int t = t0, left = wt.left;  // of the tile in work, where wt is the next one's
+  int t = t0, left = 0;  // of the tile in work, where wt is the next one's
   auto step = [&](auto hidden) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(hidden)::value;
     f4 s[QT][2];

@@ -260,7 +260,7 @@ struct PagedCache {
   static constexpr bool kRagged = true;
   Pages pg;
   const int *pos, *cu, *rdelta;
-  int T, type;
+  int type;
   int end;  // lane l: where sequence l's tokens end
   struct At {
     void *k, *v;
@@ -377,7 +377,7 @@ extern "C" int q27h_attn_prep_paged(const float* qg, const float* k, const float
   if (!aligned4(pos) || !aligned4(cu) || !aligned4(rope3) || !aligned4(rdelta))
     return fail(Q27H_ERR_ARG, "attn_prep_paged: pos, cu, rope3 and rdelta need 4-byte alignment");
   PagedCache c = {};
-  c.pg = pages_of(kv), c.pos = pos, c.cu = cu, c.rdelta = rdelta, c.T = T, c.type = kv->type;
+  c.pg = pages_of(kv), c.pos = pos, c.cu = cu, c.rdelta = rdelta, c.type = kv->type;
   const size_t B = (size_t)kv->n_seqs, kvb = (size_t)T * kv->nkvh * 1024;
   if (outputs_overlap({{qn, (size_t)T * nqh * 1024}, {c.pg.k, c.pg.kb * kv->n_pages}, {c.pg.v, c.pg.vb * kv->n_pages}},
                       {{qg, (size_t)T * nqh * 2048}, {k, kvb}, {v, kvb}, {q_norm, 1024}, {k_norm, 1024}, {pos, B * 4}, {cu, B * 4 + 4},

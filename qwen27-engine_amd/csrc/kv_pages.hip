@@ -119,6 +119,54 @@ struct Piece {
   }
 };
 
+// Work of unequal sequences in equal shares: cost(b) >= 0 of each sequence, laid end to end, is cut in `gridDim.x` parts.
+// Gives every thread of the workgroup its part [x, end), the sequence that x lies in and where that one begins.
+struct Share {
+  int x, end, seq, start;
+};
+template <int THREADS, typename F>
+__device__ __forceinline__ Share share_of(int n_seqs, F cost) {
+  __shared__ int s_sum[THREADS / 64], s_at[2];
+  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const int each = (n_seqs + THREADS - 1) / THREADS, b0 = tid * each, b1 = b0 + each < n_seqs ? b0 + each : n_seqs;
+  int mine = 0;
+  for (int b = b0; b < b1; b++) mine += cost(b);
+  int before = mine;  // inclusive sums of the wave
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(before, d);
+    before += l >= d ? y : 0;
+  }
+  if (l == 63) s_sum[w] = before;
+  __syncthreads();
+  int total = 0;
+  before -= mine;
+#pragma unroll
+  for (int k = 0; k < THREADS / 64; k++) {
+    before += k < w ? s_sum[k] : 0;
+    total += s_sum[k];
+  }
+  Share s;
+  const int parts = (int)gridDim.x, per = (total + parts - 1) / parts;
+  // a workgroup behind the last part: its product may pass 31 bits
+  s.x = (long long)blockIdx.x * per < total ? (int)blockIdx.x * per : total;
+  s.end = total - s.x < per ? total : s.x + per;
+  if (before <= s.x && s.x < before + mine) {
+    int at = before;
+    for (int b = b0; b < b1; b++) {
+      const int c = cost(b);
+      if (at <= s.x && s.x < at + c) s_at[0] = b, s_at[1] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  s.x = __builtin_amdgcn_readfirstlane(s.x);
+  s.end = __builtin_amdgcn_readfirstlane(s.end);
+  s.seq = __builtin_amdgcn_readfirstlane(s_at[0]);
+  s.start = __builtin_amdgcn_readfirstlane(s_at[1]);
+  return s;
+}
+
 // A workgroup takes a chunk of 16 rows, K and V requested together, and then the next. Twice the rows in twice the loads,
 // and half the workgroups, were slower (to f16: 112 us against 104). Rows of a page that is none of the cache's are zeros.
 template <int KB, int VB, typename OUT>
@@ -129,7 +177,7 @@ __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
     const int n = a.count[b];
     return n < 0 ? 0 : n < a.n_out ? n : a.n_out;
   };
-  Share sp = share_of<256>(a.pg.n_seqs, 1, nullptr, [&](int b) { return a.pg.nkvh * ((rows_of(b) + kChunk - 1) / kChunk); });
+  Share sp = share_of<256>(a.pg.n_seqs, [&](int b) { return a.pg.nkvh * ((rows_of(b) + kChunk - 1) / kChunk); });
   const int n = 1 << a.pg.shift;
   while (sp.x < sp.end) {
     const int b = sp.seq, count = rows_of(b), chunks = (count + kChunk - 1) / kChunk;

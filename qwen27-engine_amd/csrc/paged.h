@@ -45,57 +45,4 @@ __device__ __forceinline__ Tokens tokens_of(const int* cu, int b, int T, int mos
   return cu ? tokens_of(uniform_load(cu + b), uniform_load(cu + b + 1), T, most) : tokens_of(b, b + 1, T, most);
 }
 
-// Work of unequal sequences in equal shares: cost(b) >= 0 of each sequence, laid end to end, is cut in `gridDim.x` parts of
-// a multiple of `unit`. Gives every thread of the workgroup its part [x, end), the sequence that x lies in and where that
-// one begins; where `starts` is given, the first workgroup also leaves the beginnings there, and the total behind them.
-struct Share {
-  int x, end, per, seq, start;
-};
-template <int THREADS, typename F>
-__device__ __forceinline__ Share share_of(int n_seqs, int unit, int* starts, F cost) {
-  __shared__ int s_sum[THREADS / 64], s_at[2];
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  const int each = (n_seqs + THREADS - 1) / THREADS, b0 = tid * each, b1 = b0 + each < n_seqs ? b0 + each : n_seqs;
-  int mine = 0;
-  for (int b = b0; b < b1; b++) mine += cost(b);
-  int before = mine;  // inclusive sums of the wave
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(before, d);
-    before += l >= d ? y : 0;
-  }
-  if (l == 63) s_sum[w] = before;
-  __syncthreads();
-  int total = 0;
-  before -= mine;
-#pragma unroll
-  for (int k = 0; k < THREADS / 64; k++) {
-    before += k < w ? s_sum[k] : 0;
-    total += s_sum[k];
-  }
-  Share s;
-  const int parts = (int)gridDim.x;
-  s.per = ((total + parts - 1) / parts + unit - 1) / unit * unit;
-  // a workgroup behind the last part: its product may pass 31 bits
-  s.x = (long long)blockIdx.x * s.per < total ? (int)blockIdx.x * s.per : total;
-  s.end = total - s.x < s.per ? total : s.x + s.per;
-  if (starts && blockIdx.x == 0 && tid == 0) starts[n_seqs] = total;
-  if ((starts && blockIdx.x == 0) || (before <= s.x && s.x < before + mine)) {
-    int at = before;
-    for (int b = b0; b < b1; b++) {
-      const int c = cost(b);
-      if (starts && blockIdx.x == 0) starts[b] = at;
-      if (at <= s.x && s.x < at + c) s_at[0] = b, s_at[1] = at;
-      at += c;
-    }
-  }
-  __syncthreads();
-  s.x = __builtin_amdgcn_readfirstlane(s.x);
-  s.end = __builtin_amdgcn_readfirstlane(s.end);
-  s.per = __builtin_amdgcn_readfirstlane(s.per);
-  s.seq = __builtin_amdgcn_readfirstlane(s_at[0]);
-  s.start = __builtin_amdgcn_readfirstlane(s_at[1]);
-  return s;
-}
-
 }  // namespace q27h

@@ -226,8 +226,10 @@ class KvPages:
 
         kb, vb = kv_page_bytes(nkvh, page_rows, type, False), kv_page_bytes(nkvh, page_rows, type, True)
         n = min(_bytes(k) // kb, _bytes(v) // vb) if kb else 0
-        if not table.is_contiguous() or table.dim() != 2 or table.element_size() != 4:
+        if not table.is_contiguous() or table.dim() != 2 or table.element_size() != 4 or table.is_floating_point():
             raise ValueError("KvPages: the table is a contiguous int32 tensor [n_seqs][max_pages]")
+        if not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("KvPages: pages lie one behind the other in contiguous tensors")
         self.k, self.v, self.table = k, v, table
         self.c = KvPagesC(_ptr(k), _ptr(v), _ptr(table), table.shape[0], table.shape[1], n, nkvh, page_rows, type)
         self.ref = ctypes.addressof(self.c)

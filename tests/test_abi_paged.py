@@ -169,6 +169,15 @@ def test_a_handle_needs_a_whole_table(q27):
             q27.ops.KvPages(k, v, table, 4, 64, q27.ops.KV_Q8_Q4)
 
 
+def test_a_handle_refuses_other_numbers_and_pages_apart(q27):
+    import torch
+
+    k, v, table = torch.zeros(2, KB, dtype=torch.uint8), torch.zeros(2, VB, dtype=torch.uint8), torch.zeros(3, 8, dtype=torch.int32)
+    for bad in ((k, v, table.float()), (k.t(), v, table), (k, v[:, ::2], table)):
+        with pytest.raises(ValueError):
+            q27.ops.KvPages(*bad, 4, 64, q27.ops.KV_Q8_Q4)
+
+
 def test_cpp_header_forwards(tmp_path):
     """include/q27/attn.h: every function compiles in a caller, and a refusal arrives as an exception."""
     import os
