@@ -60,8 +60,8 @@ inline size_t attn_paged_ws_bytes(const KvPages& kv, int T, int max_tokens, int 
   return q27h_attn_paged_ws_bytes(&kv, T, max_tokens, nqh);
 }
 inline void attn_paged(const float* qn, const KvPages& kv, const int* pos, const int* cu, int T, int max_tokens, float scale, int nqh,
-                       float* o, void* ws, size_t ws_bytes, hipStream_t s, float* lse = nullptr) {
-  q27h_check(q27h_attn_paged(qn, &kv, pos, cu, T, max_tokens, scale, nqh, o, lse, ws, ws_bytes, s));
+                       float* o, void* ws, size_t ws_bytes, hipStream_t s, float* lse = nullptr, const uint64_t* tree = nullptr) {
+  q27h_check(q27h_attn_paged(qn, &kv, pos, cu, T, max_tokens, scale, nqh, o, lse, ws, ws_bytes, s, tree));
 }
 inline void kv_pages_read(const KvPages& kv, const int* from, const int* count, int n_out, int out_type, void* kout, void* vout,
                           hipStream_t s) {
@@ -72,6 +72,10 @@ inline void draft_verify(const float* p, int64_t ldp, const float* q, int64_t ld
                          const float* u_last, const int* cu, int n_seqs, int T, int V, int* out, int* path, int* n_path, void* ws,
                          size_t ws_bytes, hipStream_t s, int* pos = nullptr) {
   q27h_check(q27h_draft_verify(p, ldp, q, ldq, ids, parent, u, u_last, cu, n_seqs, T, V, out, path, n_path, pos, ws, ws_bytes, s));
+}
+inline void kv_accept_paged(const KvPages* layers, int n_layers, const int* pos, const int* cu, const int* path, const int* n_path, int T,
+                            hipStream_t s) {
+  q27h_check(q27h_kv_accept_paged(layers, n_layers, pos, cu, path, n_path, T, s));
 }
 
 }  // namespace q27

@@ -285,14 +285,15 @@ size_t q27h_kv_page_bytes(int nkvh, int page_rows, int type, int v);
 int q27h_attn_prep_paged(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm, float* qn,
                          const q27h_kv_pages* kv, const int* pos, const int* cu, int T, float eps, float theta_scale, int nqh,
                          q27h_stream_t s, const int* rope3, const int* rdelta);
-/* attn_paged: o [T][nqh][256] and lse [T][nqh] (may be NULL), as attn_tree's, of every token over the rows of its sequence up
- * to its own; with attn_tree's arithmetic and bounds, 4-bit codes entering exactly as q8_0's do. At most max_tokens (1 to 64)
- * tokens of a sequence are taken; those behind them are left out. A token that sees no row gets zeros and -inf. The same call
+/* attn_paged: o [T][nqh][256] and lse [T][nqh] (may be NULL), as attn_tree's, of every token over the rows of its sequence: all
+ * before pos[b], and of the new ones row pos[b] + u where bit u of tree[token] (device, 64-bit, 8-byte aligned, [T]; NULL: those
+ * up to its own) is set; with attn_tree's arithmetic and bounds, 4-bit codes entering exactly as q8_0's do. At most max_tokens
+ * (1 to 64) tokens of a sequence are taken; those behind them are left out. A token that sees no row gets zeros and -inf. The same call
  * gives the same bits; how a sequence's rows are split, and so the order of its sums, hangs on the lengths of all sequences.
  * ws: q27h_attn_paged_ws_bytes of the same handle's sizes, T, max_tokens and nqh. */
 size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int max_tokens, int nqh);
 int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens, float scale,
-                    int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s);
+                    int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s, const uint64_t* tree);
 /* kv_pages_read: rows from[b] .. from[b] + count[b] - 1 (from NULL: 0; count cut to 0 .. n_out; both device, [n_seqs]) as
  * values in kout and vout [n_seqs][nkvh][n_out][256] (either may be NULL), Q27H_F32, Q27H_F16 or Q27H_BF16 (rounded to the
  * nearest once), from row 0 on; rows behind them are left as they were. The f16 form of one sequence is an f16 cache of
@@ -307,8 +308,8 @@ int q27h_kv_pages_read(const q27h_kv_pages* kv, const int* from, const int* coun
  *   u[t] * q[t][id] < p[t - 1][id]. Behind the last one that stands, the next token is drawn from max(p - q, 0), q the row of
  *   the refused token (from p where that is 0 everywhere), or from p where none was refused.
  * Without q: the drafts are a tree, parent[t] < t (NULL: t - 1; a token whose parent is none of them is left out). From token
- *   0 on, the children of the last one that stands are tried in order: a child stands if u * rest < p[id], p the parent's, rest = 1 -
- *   the p[id] of those refused before it (in 64 bits); one that repeats a refused id is refused. The next token is drawn from p
+ *   0 on, the children of the last one that stands are tried in order: a child stands if u * rest < p[id], p the parent's,
+ *   rest = 1 - the p[id] of those refused before it (in 64 bits); one that repeats a refused id is refused. The next token is drawn from p
  *   without the refused ids.
  * A draw: the least x with sum of w over 0 .. x > u_last * S, S the sum over all, w clamped to [0, 1] (NaN: 0) and rounded to
  * multiples of 2^-40: exact, the same in any order. No weight at all: -1. An id outside [0, V) is refused.
@@ -318,6 +319,13 @@ size_t q27h_draft_verify_ws_bytes(int n_seqs, int V);
 int q27h_draft_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, const int* ids, const int* parent, const float* u,
                       const float* u_last, const int* cu, int n_seqs, int T, int V, int* out, int* path, int* n_path, int* pos,
                       void* ws, size_t ws_bytes, q27h_stream_t s);
+/* kv_accept_paged: moves the accepted path of each sequence's verified tree to its place in the pages of every layer: row
+ * p0 + path[i] to row p0 + i, for i < n_path[b], with pos, path and n_path as draft_verify leaves them (p0 = pos[b] - n_path[b],
+ * the rows before the batch; path [T] by cu). layers: n_layers handles, alike but for their k and v, no two of which may
+ * overlap; one launch for up to 32. The path ends at its first entry that is none of the sequence's tokens. A row stays where
+ * it or its place does not exist. Pages of new rows belong to one sequence alone. */
+int q27h_kv_accept_paged(const q27h_kv_pages* layers, int n_layers, const int* pos, const int* cu, const int* path,
+                         const int* n_path, int T, q27h_stream_t s);
 
 /* ---------------------------------------------------------------- quantized embedding gather */
 /* get_rows_iq2_s (src/ops.h:22-23, src/ops.cu:756-766): rows ids[t] (device) of an IQ2_S table (82-byte

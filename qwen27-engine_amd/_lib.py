@@ -84,8 +84,9 @@ SIGNATURES = {
     "q27h_kv_page_bytes": [_i, _i, _i, _i],
     "q27h_attn_prep_paged": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _f, _i, _p, _p, _p],
     "q27h_attn_paged_ws_bytes": [_p, _i, _i, _i],
-    "q27h_attn_paged": [_p, _p, _p, _p, _i, _i, _f, _i, _p, _p, _p, _sz, _p],
+    "q27h_attn_paged": [_p, _p, _p, _p, _i, _i, _f, _i, _p, _p, _p, _sz, _p, _p],
     "q27h_kv_pages_read": [_p, _p, _p, _i, _i, _p, _p, _p],
+    "q27h_kv_accept_paged": [_p, _i, _p, _p, _p, _p, _i, _p],
     "q27h_draft_verify_ws_bytes": [_i, _i],
     "q27h_draft_verify": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _p, _p, _sz, _p],
     "q27h_get_rows_iq2_s": [_p, _i64, _p, _i, _p, _i, _p, _p],

@@ -1,5 +1,5 @@
 // Attention of a batch of sequences over a K/V cache in pages (attn_paged): the new tokens of each sequence, one for plain
-// decoding or a few with drafts, over all of its rows.
+// decoding or a few with drafts (a chain or a tree), over all of its rows.
 //
 // A unit of work is (sequence, kv head, 16 or 32 query rows): query rows are tokens x query heads of the kv head, as in
 // attn_tree. Sequences are of any length, so a unit's tiles of 32 cache rows are cut in parts none of which is longer than a
@@ -23,12 +23,18 @@ struct PagedArgs {
   Pages pg;
   const float* qn;
   const int *pos, *cu;
+  const uint64_t* tree;  // may be null
   float *o, *lse;        // lse may be null
   float *part, *ml;      // [place][row of its unit][256], [..][2]
   int* starts;           // [n_seqs][2]: each sequence's first place, and the parts of each of its units
   int T, most, nqh, slots;  // slots: shares of the whole work, about the workgroups that run at a time
   float scale;
 };
+
+// Which of its sequence's new tokens token t of them sees: a bit for each.
+__device__ __forceinline__ uint64_t tree_of(const PagedArgs& a, const Tokens& tk, int t) {
+  return a.tree ? a.tree[tk.t0 + t] : ~0ull >> (63 - t);
+}
 
 // V in 4 bits: rows of 128 bytes as they lie, 16 a lane (row 8 r + (l >> 3), block l & 7).
 struct QRows4 {
@@ -369,10 +375,10 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   int mine = wr * 16 + (threadIdx.x & 15);
   asm volatile("" : "+v"(mine));  // the lane's row is formed here: kept over the tiles it would take registers that they need
   const int gr = row(mine);
-  const uint64_t chain = gr >= 0 ? ~0ull >> (63 - (first + mine) / group) : 0ull;
+  const uint64_t tree = gr >= 0 ? tree_of(a, tk, (first + mine) / group) : 0ull;
   for (TileAt at = walk.next(t1); at.j0 >= 0; at = walk.next(t1)) {
-    if constexpr (TYPE == Q27H_KV_Q8_Q4) tail_tile<QRows4>(st, at.k, at.v, q, sh.w[w], vis, chain, at.j0);
-    else tail_tile(st, at.k, at.v, q, sh.w[w], vis, chain, at.j0);
+    if constexpr (TYPE == Q27H_KV_Q8_Q4) tail_tile<QRows4>(st, at.k, at.v, q, sh.w[w], vis, tree, at.j0);
+    else tail_tile(st, at.k, at.v, q, sh.w[w], vis, tree, at.j0);
   }
   const bool whole = pt.parts == 1;
   const size_t place = (size_t)pt.place * kRows + mine;
@@ -417,6 +423,7 @@ struct WideLds {
   alignas(16) uint8_t ks[kWaves][kScales], vs[kWaves][kScales];
   alignas(16) int lf[kWaves][kTileKeys];  // the logarithms of f
   float mx[kWaves][QT][16];               // of the scores; in the end the sums of the weights
+  uint64_t tree[QT][16];                  // which of the new tokens a query row sees
 };
 
 // A wave's rows on their way. Rows behind the last one that exists are read from it, those of a group without any from row 0
@@ -587,6 +594,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
     const int gr = row(r);
     return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
   });
+  if (threadIdx.x < kRows) {
+    const int at = first + (int)threadIdx.x;
+    sh.tree[threadIdx.x >> 4][threadIdx.x & 15] = at < rows ? tree_of(a, tk, at / group) : 0ull;
+  }
   __syncthreads();
   h8 hi[QT][8];
   float c[QT], e[QT], sum[QT];
@@ -644,16 +655,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
     __builtin_amdgcn_s_setprio(0);
     if (kPart) {
       Vis mine = vis;
-      uint64_t chain[QT];
+      uint64_t tree[QT];
 #pragma unroll
-      for (int q = 0; q < QT; q++) {
-        int by = group;
-        asm volatile("" : "+s"(by));
-        const int at = first + 16 * q + n;
-        chain[q] = at < rows ? ~0ull >> (63 - at / by) : 0ull;
-      }
+      for (int q = 0; q < QT; q++) tree[q] = sh.tree[q][n];
       if (left <= 0) mine.n = mine.end = 0;
-      hide<QT, kHidden>(s, mine, chain, j0);
+      hide<QT, kHidden>(s, mine, tree, j0);
     }
     typedef int i4 __attribute__((ext_vector_type(4)));
     const i4 lf[2] = {*(const i4*)&sh.lf[w][4 * g], *(const i4*)&sh.lf[w][16 + 4 * g]};
@@ -922,24 +928,26 @@ extern "C" size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int m
 }
 
 extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens,
-                               float scale, int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s) {
+                               float scale, int nqh, float* o, float* lse, void* ws, size_t ws_bytes, q27h_stream_t s,
+                               const uint64_t* tree) {
   if (const int bad = check_pages(kv, "attn_paged")) return bad;
   if (const char* why = refusal(kv, T, max_tokens, nqh)) return fail(Q27H_ERR_SHAPE, why);
   if (!cu && T != kv->n_seqs) return fail(Q27H_ERR_SHAPE, "attn_paged: without cu there is one token for each sequence");
   if (T == 0 || kv->n_seqs == 0) return Q27H_OK;
   if (!qn || !pos || !o) return fail(Q27H_ERR_ARG, "attn_paged: null pointer");
   if (!aligned16(qn) || !aligned16(o) || !aligned16(ws)) return fail(Q27H_ERR_ARG, "attn_paged: tensors need 16-byte alignment");
-  if (!aligned4(pos) || !aligned4(cu) || !aligned4(lse)) return fail(Q27H_ERR_ARG, "attn_paged: pos, cu and lse need 4-byte alignment");
+  if (!aligned8(tree) || !aligned4(pos) || !aligned4(cu) || !aligned4(lse))
+    return fail(Q27H_ERR_ARG, "attn_paged: tree needs 8-byte alignment, pos, cu and lse 4-byte");
   const Layout y = layout_of(kv->n_seqs, max_tokens, nqh, kv->nkvh, kv->type);
   if (ws_bytes < y.bytes || !ws) return fail(Q27H_ERR_ARG, "attn_paged: workspace too small");
   const Pages pg = pages_of(kv);
   const size_t qb = (size_t)T * nqh * kHD * 4, B = (size_t)kv->n_seqs;
   if (outputs_overlap({{o, qb}, {lse, (size_t)T * nqh * 4}, {ws, y.bytes}},
                       {{qn, qb}, {pg.k, pg.kb * pg.n_pages}, {pg.v, pg.vb * pg.n_pages}, {pg.table, B * pg.max_pages * 4},
-                       {pos, B * 4}, {cu, (B + 1) * 4}}))
+                       {pos, B * 4}, {cu, (B + 1) * 4}, {tree, (size_t)T * 8}}))
     return fail(Q27H_ERR_ARG, "attn_paged: o, lse or ws overlaps another argument");
   PagedArgs a = {};
-  a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
+  a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.tree = tree, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
   a.slots = y.slots;
   a.part = (float*)ws, a.ml = a.part + y.places * kHD, a.starts = (int*)(a.ml + y.places * 2);
   const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);

@@ -1,4 +1,5 @@
-// A K/V cache in pages: its handle's checks, and its rows read back as values (kv_pages_read).
+// A K/V cache in pages: its handle's checks, its rows read back as values (kv_pages_read), and the rows of accepted paths moved
+// to their places (kv_accept_paged).
 //
 // Reading back is a copy that widens: rows x nkvh x (144 to 512 bytes in, 512 or 1024 out) for each of K and V, no arithmetic
 // but one product a value, so it is bound by HBM. A piece of work is kChunk rows of one head; the sequences' pieces are laid
@@ -219,6 +220,71 @@ __global__ void __launch_bounds__(256) kv_pages_read_kernel(ReadArgs a) {
   }
 }
 
+// kv_accept_paged: a workgroup for (sequence, kv head, K or V of a layer). Of a path that is a prefix of the drafts nothing moves,
+// which is all that a chain's workgroups find out; otherwise all the rows that move are held in registers before the first
+// is written, so a path in any order is right. At most 64 rows of 512 bytes each: bound by its round trips.
+constexpr int kMostPath = 64, kMostPools = 64;
+struct AcceptArgs {
+  Pages pg;                   // of every layer, but for k and v
+  uint8_t* pool[kMostPools];  // a layer's K, its V, the next one's K, ..
+  const int *pos, *cu, *path, *n_path;
+  int T;
+};
+__global__ void __launch_bounds__(256) kv_accept_paged_kernel(AcceptArgs a) {
+  __shared__ long long s_from[kMostPath], s_to[kMostPath];  // row i of the path: rows of the pool, counted over its pages; -1: stays
+  __shared__ int s_any;
+  const int b = blockIdx.x, kh = blockIdx.y, tid = threadIdx.x, n = 1 << a.pg.shift;
+  const bool v = blockIdx.z & 1;
+  if (tid < 64) {
+    const Tokens tk = tokens_of(a.cu, b, a.T, kMostPath);
+    const int got = uniform_load(a.n_path + b), want = got < tk.nt ? got : tk.nt;
+    const long long base = (long long)uniform_load(a.pos + b) - got;  // the sequence's rows before the batch
+    const int p = tid < want ? a.path[tk.t0 + tid] : -1;
+    const uint64_t good = __ballot(p >= 0 && p < tk.nt);
+    const int len = good == ~0ull ? 64 : __builtin_ctzll(~good);  // the path ends at its first entry that is no token
+    auto place = [&](long long j) {
+      const long long i = j >> a.pg.shift;
+      const int page = i >= 0 && i < a.pg.max_pages ? a.pg.table[(size_t)b * a.pg.max_pages + i] : -1;
+      return (unsigned)page < (unsigned)a.pg.n_pages ? (long long)page << a.pg.shift | (j & (n - 1)) : -1ll;
+    };
+    long long from = -1, to = -1;
+    if (tid < len && p != tid) from = place(base + p), to = place(base + tid);
+    const bool moves = from >= 0 && to >= 0;
+    s_from[tid] = moves ? from : -1;
+    s_to[tid] = to;
+    const uint64_t any = __ballot(moves);
+    if (tid == 0) s_any = any != 0;
+  }
+  __syncthreads();
+  if (!s_any) return;
+  uint8_t* c = a.pool[blockIdx.z];
+  const bool f16 = a.pg.type == Q27H_KV_F16;
+  const int log = f16 ? 5 : v && a.pg.type == Q27H_KV_Q8_Q4 ? 3 : 4;  // 16 bytes a lane: the lanes of a row
+  const int sub = tid & ((1 << log) - 1), step = 256 >> log;
+  const size_t bytes = v ? a.pg.vb : a.pg.kb, row = (size_t)16 << log;
+  auto codes = [&](long long j) {
+    return (w4*)(c + (size_t)(j >> a.pg.shift) * bytes + ((size_t)kh * n + (size_t)(j & (n - 1))) * row + 16 * sub);
+  };
+  auto scales = [&](long long j) {
+    return (w4*)(c + (size_t)(j >> a.pg.shift) * bytes + (size_t)a.pg.nkvh * n * row + ((size_t)kh * n + (size_t)(j & (n - 1))) * 16);
+  };
+  const bool has_d = !f16 && tid < kMostPath && s_from[tid & 63] >= 0;
+  w4 x[8], d = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const int i = k * step + (tid >> log);
+    if (i < kMostPath && s_from[i & 63] >= 0) x[k] = *codes(s_from[i & 63]);
+  }
+  if (has_d) d = *scales(s_from[tid & 63]);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const int i = k * step + (tid >> log);
+    if (i < kMostPath && s_from[i & 63] >= 0) *codes(s_to[i & 63]) = x[k];
+  }
+  if (has_d) *scales(s_to[tid & 63]) = d;
+}
+
 }  // namespace
 }  // namespace q27h
 
@@ -258,4 +324,42 @@ extern "C" int q27h_kv_pages_read(const q27h_kv_pages* kv, const int* from, cons
   else
     launch(kv_pages_read_kernel<8, 4, AsF32>, kv_pages_read_kernel<8, 4, AsF16>, kv_pages_read_kernel<8, 4, AsBf16>);
   return check_launch("kv_pages_read");
+}
+
+extern "C" int q27h_kv_accept_paged(const q27h_kv_pages* layers, int n_layers, const int* pos, const int* cu, const int* path,
+                                    const int* n_path, int T, q27h_stream_t s) {
+  if (T < 0 || n_layers < 0) return fail(Q27H_ERR_SHAPE, "kv_accept_paged: bad shape");
+  if (n_layers == 0) return Q27H_OK;
+  if (!layers) return fail(Q27H_ERR_ARG, "kv_accept_paged: null pointer");
+  const q27h_kv_pages& one = layers[0];
+  for (int i = 0; i < n_layers; i++) {
+    const q27h_kv_pages& kv = layers[i];
+    if (const int bad = check_pages(&kv, "kv_accept_paged")) return bad;
+    if (kv.table != one.table || kv.n_seqs != one.n_seqs || kv.max_pages != one.max_pages || kv.n_pages != one.n_pages ||
+        kv.nkvh != one.nkvh || kv.page_rows != one.page_rows || kv.type != one.type)
+      return fail(Q27H_ERR_ARG, "kv_accept_paged: layers of different sizes, types or tables");
+  }
+  if ((long long)one.n_seqs * one.nkvh > 1 << 17) return fail(Q27H_ERR_SHAPE, "kv_accept_paged: too many sequences");
+  if (T == 0 || one.n_seqs == 0) return Q27H_OK;
+  if (!pos || !cu || !path || !n_path) return fail(Q27H_ERR_ARG, "kv_accept_paged: null pointer");
+  if (!aligned4(pos) || !aligned4(cu) || !aligned4(path) || !aligned4(n_path))
+    return fail(Q27H_ERR_ARG, "kv_accept_paged: pos, cu, path and n_path need 4-byte alignment");
+  AcceptArgs a = {};
+  a.pg = pages_of(&one), a.pos = pos, a.cu = cu, a.path = path, a.n_path = n_path, a.T = T;
+  const size_t B = (size_t)one.n_seqs * 4, kb = a.pg.kb * one.n_pages, vb = a.pg.vb * one.n_pages;
+  auto pool = [&](int i) { return i & 1 ? Bytes{layers[i >> 1].v, vb} : Bytes{layers[i >> 1].k, kb}; };
+  bool twice = false;  // a row moved twice, by workgroups that run at once
+  for (int i = 0; i < 2 * n_layers; i++) {
+    const Bytes x = pool(i);
+    for (int j = 0; j < i; j++) twice |= overlaps(x.p, x.n, pool(j).p, pool(j).n);
+    twice |= outputs_overlap({x}, {{pos, B}, {cu, B + 4}, {path, (size_t)T * 4}, {n_path, B}, {one.table, B * one.max_pages}});
+  }
+  if (twice) return fail(Q27H_ERR_ARG, "kv_accept_paged: pages overlap each other or another argument");
+  for (int i = 0; i < n_layers; i += kMostPools / 2) {
+    const int n = n_layers - i < kMostPools / 2 ? n_layers - i : kMostPools / 2;
+    for (int j = 0; j < n; j++) a.pool[2 * j] = (uint8_t*)layers[i + j].k, a.pool[2 * j + 1] = (uint8_t*)layers[i + j].v;
+    hipLaunchKernelGGL(kv_accept_paged_kernel, dim3((unsigned)one.n_seqs, (unsigned)one.nkvh, (unsigned)(2 * n)), dim3(256), 0,
+                       stream_of(s), a);
+  }
+  return check_launch("kv_accept_paged");
 }

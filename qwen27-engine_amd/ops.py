@@ -245,11 +245,12 @@ def attn_paged_ws_bytes(kv, T, max_tokens, nqh):
     return int(lib().q27h_attn_paged_ws_bytes(kv.ref, T, max_tokens, nqh))
 
 
-def attn_paged(qn, kv, pos, cu, T, max_tokens, scale, nqh, o, ws, s=None, lse=None):
+def attn_paged(qn, kv, pos, cu, T, max_tokens, scale, nqh, o, ws, s=None, lse=None, tree=None):
     """Attention of each sequence's new tokens (at most max_tokens <= 64 each) over its rows in the pages: o f32 [T][nqh][256],
-    lse f32 [T][nqh]; ws: a tensor of attn_paged_ws_bytes() bytes, one per call that may run at a time."""
+    lse f32 [T][nqh]; tree (int64 / uint64 [T]): the new tokens of its sequence that each one sees, bit u the u-th (None: a
+    chain); ws: a tensor of attn_paged_ws_bytes() bytes, one per call that may run at a time."""
     check(lib().q27h_attn_paged(_ptr(qn), kv.ref, _ptr(pos), _ptr(cu), T, max_tokens, scale, nqh, _ptr(o), _ptr(lse), _ptr(ws),
-                                _bytes(ws), _stream(s)))
+                                _bytes(ws), _stream(s), _ptr(tree)))
 
 
 def kv_pages_read(kv, start, count, n_out, kout, vout, s=None):
@@ -282,6 +283,27 @@ def draft_verify(p, q, ids, parent, u, u_last, cu, n_seqs, V, out, path, n_path,
 
     check(lib().q27h_draft_verify(_ptr(p), ld(p), _ptr(q), ld(q), _ptr(ids), _ptr(parent), _ptr(u), _ptr(u_last), _ptr(cu), n_seqs, T, V,
                                   _ptr(out), _ptr(path), _ptr(n_path), _ptr(pos), _ptr(ws), _bytes(ws), _stream(s)))
+
+
+class KvLayers:
+    """The layers' KvPages for kv_accept_paged, listed once; holds them."""
+
+    def __init__(self, layers):
+        from ._lib import KvPagesC
+
+        self.layers, self.n = list(layers), len(layers)
+        self.c = (KvPagesC * max(1, self.n))(*(x.c for x in self.layers))
+
+
+def kv_layers(layers):
+    return KvLayers(layers)
+
+
+def kv_accept_paged(layers, pos, cu, path, n_path, T, s=None):
+    """The accepted path of each sequence to its place in the pages of every layer (KvLayers, or a list of KvPages that are alike
+    but for their pages); pos, path and n_path as draft_verify leaves them."""
+    x = layers if isinstance(layers, KvLayers) else KvLayers(layers)
+    check(lib().q27h_kv_accept_paged(x.c, x.n, _ptr(pos), _ptr(cu), _ptr(path), _ptr(n_path), T, _stream(s)))
 
 
 def rmsnorm_q8(x, w, h, xq, xd, n, rows, eps, s=None, xs=None):

@@ -114,8 +114,8 @@ def cu_of(new):
     return np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
 
 
-def attend(q, kp, vp, table, pos, new, scale):
-    """o, lse and their bounds for all tokens of the batch (R.attend's for each sequence)."""
+def attend(q, kp, vp, table, pos, new, scale, tree=None):
+    """o, lse and their bounds for all tokens of the batch (R.attend's for each sequence); tree: a mask for each token."""
     parts = []
     cu = cu_of(new)
     for b, n in enumerate(new):
@@ -124,7 +124,7 @@ def attend(q, kp, vp, table, pos, new, scale):
         end = max(0, min(pos[b] + n, table.shape[1] * kp.page))
         k, there = kp.values(table[b], end)
         v, _ = vp.values(table[b], end)
-        vis = R.visible(n, pos[b], end, None) & there
+        vis = R.visible(n, pos[b], end, None if tree is None else tree[cu[b]:cu[b + 1]]) & there
         k[:, ~there] = v[:, ~there] = 0
         if end == 0:
             k = v = np.zeros((kp.nkvh, 1, HD))
@@ -194,3 +194,25 @@ def verify(p, q, ids, parent, u, u_last, cu, V, out, path, n_path, pos):
         n_path[b] = n
         pos[b] += n
     return out, path, n_path, pos
+
+
+def accept(pool, table, pos, cu, path, n_path):
+    """kv_accept_paged in place on a pool's codes and scales; pos as draft_verify leaves it."""
+    def place(b, j):
+        i = j // pool.page
+        p = int(table[b, i]) if 0 <= i < table.shape[1] else -1
+        return (p, slice(None), j % pool.page) if 0 <= p < len(pool.buf) else None
+
+    for b in range(len(cu) - 1):
+        nt = min(64, cu[b + 1] - cu[b])
+        moves = []
+        for i in range(min(n_path[b], nt)):
+            t = int(path[cu[b] + i])
+            if not 0 <= t < nt:
+                break
+            a, z = (place(b, pos[b] - int(n_path[b]) + x) for x in (t, i))
+            if a and z:
+                moves.append((z, [x[a].copy() for x in (pool.codes, pool.scales) if x is not None]))
+        for z, rows in moves:
+            for x, row in zip((pool.codes, pool.scales), rows):
+                x[z] = row

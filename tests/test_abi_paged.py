@@ -64,6 +64,18 @@ def verify(ops, n_seqs=B, tokens=T, vocab=V, parent=None, ldp=V, ldq=V, ws_bytes
                                   a["path"], a["n_path"], a["pos"], a["ws"], ws_bytes, None))
 
 
+def accept(ops, kv=None, layers=2, tokens=T, other=None, **at):
+    """Two layers, the second one's pages 100 places on; `other`: what it has of its own."""
+    from qwen27_engine_amd._lib import KvPagesC, check, lib
+
+    a = PLACES | at
+    one = {"k": a["k"], "v": a["v"], "table": a["table"]} | (kv or {})
+    two = one | {"k": 101 * G4, "v": 102 * G4} | (other or {})
+    hs = [KV(**one), KV(**two)]
+    c = (KvPagesC * 2)(*(h.c for h in hs))
+    check(lib().q27h_kv_accept_paged(c if layers else None, layers, a["pos"], a["cu"], a["path"], a["n_path"], tokens, None))
+
+
 def refused(q27, call, code, needle, **args):
     with pytest.raises(q27.Q27Error) as ei:
         call(q27.ops, **args)
@@ -178,6 +190,42 @@ def test_a_handle_refuses_other_numbers_and_pages_apart(q27):
             q27.ops.KvPages(*bad, 4, 64, q27.ops.KV_Q8_Q4)
 
 
+ACCEPT = dict(SIZES, path=T * 4, n_path=B * 4)
+
+
+@pytest.mark.parametrize("args,code,needle", [
+    (dict(tokens=-1), -1, "bad shape"), (dict(layers=-1), -1, "bad shape"), (dict(kv=dict(rows=48)), -1, "power of two"),
+    (dict(kv=dict(k=None)), -4, "null pointer"), (dict(other=dict(v=None)), -4, "null pointer"),
+    (dict(kv=dict(n_seqs=40000)), -1, "too many sequences"), (dict(other=dict(type=1)), -4, "different"),
+    (dict(other=dict(n_seqs=2)), -4, "different"), (dict(other=dict(max_pages=9)), -4, "different"),
+    (dict(other=dict(n_pages=49)), -4, "different"), (dict(other=dict(nkvh=2)), -4, "different"),
+    (dict(other=dict(rows=32)), -4, "different"), (dict(other=dict(table=4 * G4)), -4, "different"),
+    (dict(other=dict(k=G4 + 16)), -4, "overlap"), (dict(other=dict(v=G4)), -4, "overlap"),
+    (dict(other=dict(k=101 * G4, v=101 * G4 + PAGES * KB - 16)), -4, "overlap")] +
+    [({n: None}, -4, "null pointer") for n in ("pos", "cu", "path", "n_path")] +
+    [({n: PLACES[n] + 2}, -4, "alignment") for n in ("pos", "cu", "path", "n_path")] +
+    [({o: PLACES[n] + (ACCEPT[n] - 1) // 16 * 16}, -4, "overlap") for o in ("k", "v") for n in ACCEPT if n != o])
+def test_accept_refusals(q27, args, code, needle):
+    refused(q27, accept, code, needle, **args)
+
+
+def test_accept_with_nothing_to_do(q27):
+    accept(q27.ops, layers=0)
+    accept(q27.ops, tokens=0)
+    accept(q27.ops, kv=dict(k=None, v=None, table=None, n_seqs=0, max_pages=0, n_pages=0), other=dict(k=None, v=None))
+
+
+def attn_of_trees(ops, tree, **at):
+    a = PLACES | at
+    ops.attn_paged(a["qn"], KV(), a["pos"], a["cu"], T, 4, 0.0625, 24, a["o"], WS(1 << 30, a["ws"]), 0, a["lse"], tree)
+
+
+def test_masks_are_checked(q27):
+    refused(q27, attn_of_trees, -4, "alignment", tree=60 * G4 + 4)
+    for out in ("o", "lse", "ws"):
+        refused(q27, attn_of_trees, -4, "overlap", tree=60 * G4, **{out: 60 * G4 + T * 8 - 16})
+
+
 def test_cpp_header_forwards(tmp_path):
     """include/q27/attn.h: every function compiles in a caller, and a refusal arrives as an exception."""
     import os
@@ -195,6 +243,8 @@ void step(const float* x, const q27::KvPages& kv, int* pos, const int* cu, int* 
   q27::attn_paged(x, kv, pos, cu, 9, 4, 0.0625f, 24, o, ws, n, s, lse);
   q27::kv_pages_read(kv, nullptr, pos, 100, Q27H_F16, ws, ws, s);
   q27::draft_verify(x, 100, x, 100, pos, nullptr, x, x, cu, 3, 9, 100, out, out, out, ws, n, s, pos);
+  q27::kv_accept_paged(&kv, 1, pos, cu, out, out, 9, s);
+  q27::attn_paged(x, kv, pos, cu, 9, 4, 0.0625f, 24, o, ws, n, s, lse, (const uint64_t*)out);
 }
 int main(int argc, char**) {
   q27::KvPages kv = {nullptr, nullptr, nullptr, 3, 8, 50, 4, 64, Q27H_KV_Q8_Q4};
