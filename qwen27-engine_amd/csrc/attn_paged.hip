@@ -4,12 +4,13 @@
 // A unit of work is (sequence, kv head, 16 or 32 query rows): query rows are tokens x query heads of the kv head, as in
 // attn_tree. Sequences are of any length, so a unit's tiles of 32 cache rows are cut in parts none of which is longer than a
 // fixed share of the tiles of all units. Every workgroup has a part, which it finds from the lengths of all sequences
-// itself. Up to 16 query rows, and over f16, its waves each walk tiles of their own with the online softmax of attn_core.h,
-// bound by HBM (128 sequences of 4096 q8_0 rows, one token: 5.4 TB/s; f16, 2048 rows, four tokens: 5.0); more over codes share
+// itself. Up to 16 query rows (over f16 32), its waves each walk tiles of their own with the online softmax of attn_core.h,
+// bound by HBM (128 sequences of 4096 q8_0 rows, one token: 5.4 TB/s; f16, 2048 rows, four tokens: 5.0); with more they share
 // them, see below. The parts of a unit that was cut go to the workspace, and a second launch joins those of each query
 // row in order.
 #include <type_traits>
 
+#include "attn_shared.h"
 #include "attn_wave.h"
 #include "paged.h"
 
@@ -28,6 +29,7 @@ struct PagedArgs {
   float *part, *ml;      // [place][row of its unit][256], [..][2]
   int* starts;           // [n_seqs][2]: each sequence's first place, and the parts of each of its units
   int T, most, nqh, slots;  // slots: shares of the whole work, about the workgroups that run at a time
+  int rows;                 // query rows of a unit
   float scale;
 };
 
@@ -77,9 +79,9 @@ struct TileAt {
   int j0;  // -1: none
 };
 
-// The tiles of one wave, t, t + kWaves, ... up to `end`. The page of the next one is asked for a tile ahead. A tile whose
+// The tiles of one wave, or of a workgroup whose waves share them: t, t + STEP, ... up to `end`. The page of the next one is asked for a tile ahead. A tile whose
 // page is none of the cache's is passed over: its rows do not exist.
-template <int TYPE>
+template <int TYPE, int STEP = kWaves>
 struct PageWalk {
   const Pages& pg;
   const int* table;
@@ -96,7 +98,7 @@ struct PageWalk {
     a.j0 = -1;
     while (t < limit) {
       const int cur = t, p = page;
-      t += kWaves;
+      t += STEP;
       ask();
       if ((unsigned)p >= (unsigned)pg.n_pages) continue;
       a.j0 = cur * kTileKeys;
@@ -202,6 +204,21 @@ struct Part {
   Tokens tk;
   int pos;
 };
+// The i-th of a sequence's parts of one kind, of which each unit has n. The units of a kv head read the same rows: theirs
+// follow each other 8 workgroups apart, which is on one XCD (16 sequences of 32768 q8_0 rows, 12 tokens: 650 -> 632 us).
+__device__ __forceinline__ void place_of(const PagedArgs& a, int i, int n, int units, int& unit, int& k) {
+  const int groups = units / a.pg.nkvh;
+  int at = i, g = 0;
+  if (groups > 1) {
+    const int all = a.pg.nkvh * n, round = i / (8 * groups), j = i - round * 8 * groups;
+    const int wide = all - 8 * round < 8 ? all - 8 * round : 8;
+    g = j / wide;
+    at = 8 * round + j - g * wide;
+  }
+  unit = at / n;
+  k = at - unit * n;
+  unit = unit * groups + g;
+}
 struct Counts {
   uint64_t a, b;  // whole parts, and above them places of parts that are joined; large rests, and above them small ones
 };
@@ -244,10 +261,10 @@ __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   if (!here) return p;
   p.seq = __builtin_ctzll(here);
   auto of = [&](int y) { return __builtin_amdgcn_readlane(y, p.seq); };
-  const int i = me - of(x), w = of(whole);
+  const int w = of(whole);
   p.parts = of(parts);
-  p.unit = kind == 0 ? i / w : i;
-  p.k = kind == 0 ? i - p.unit * w : w;
+  place_of(a, me - of(x), kind == 0 ? w : 1, of(d.units), p.unit, p.k);
+  if (kind) p.k = w;
   p.place = of(sp - np) + p.unit * p.parts + p.k;
   p.tk = {of(tk.t0), of(tk.nt)};
   p.pos = of(pos);
@@ -333,10 +350,11 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   kind = __builtin_amdgcn_readfirstlane(kind);
   p.tk = tokens_of(a.cu, p.seq, a.T, a.most);
   p.pos = uniform_load(a.pos + p.seq);
-  const int span = demand_of(a, p.tk.nt, vis_of(p.pos, p.tk.nt, cap), rows).span, whole = span / p.size;
-  p.parts = (span + p.size - 1) / p.size;
-  p.unit = kind == 0 ? i / whole : i;
-  p.k = kind == 0 ? i - p.unit * whole : whole;
+  const Demand d = demand_of(a, p.tk.nt, vis_of(p.pos, p.tk.nt, cap), rows);
+  const int whole = d.span / p.size;
+  p.parts = (d.span + p.size - 1) / p.size;
+  place_of(a, i, kind == 0 ? whole : 1, d.units, p.unit, p.k);
+  if (kind) p.k = whole;
   p.place = __builtin_amdgcn_readfirstlane(s_part[2]) + p.unit * p.parts + p.k;
   return p;
 }
@@ -400,7 +418,122 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   });
 }
 
-// ---------------------------------------------------------------- more than 16 query rows
+// ---------------------------------------------------------------- more than 32 query rows over f16
+// A row tile for each wave, the cache rows shared through LDS as in attn_tree (attn_shared.h): a tile is worked on while the
+// next one or two are on their way through registers. 16 sequences of 32768 rows, 6 and 12 tokens: 390 and 493 us, where
+// units of 32 query rows that each read the rows take 923 and 1409 (the bytes' floor is 424: at 6 tokens reading alone is
+// faster than a copy); 8 sequences, 64 tokens: 898 for 2462, of which the products with two terms need 701. One sequence of
+// 2000 rows, whose workgroups have four tiles one after the other here: 19.5 and 25.4 for 15.9 and 18.5.
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) attn_paged_shared_kernel(PagedArgs a) {
+  constexpr size_t kTiles = sizeof(SharedTile) * 2, kImages = sizeof(QTile) * WAVES;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kTiles > kImages ? kTiles : kImages];  // the queries' image, then the tiles
+  __shared__ int s_odd[2];
+  QTile* im = (QTile*)s_mem;
+  SharedTile* buf = (SharedTile*)s_mem;
+  const Part pt = part_of<WAVES * 64>(a, a.rows);
+  if (pt.seq < 0) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = a.nqh / a.pg.nkvh;
+  const Tokens tk = pt.tk;
+  const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
+  const int rows = tk.nt * group, groups = (rows + a.rows - 1) / a.rows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * a.rows;
+  const int tiles = (vis.end + kTileKeys - 1) / kTileKeys;
+  const int t0 = pt.k * pt.size, t1 = t0 + pt.size < tiles ? t0 + pt.size : tiles;
+  auto row = [&](int r) {  // the global row of the unit's query row r, or -1
+    const int at = first + r;
+    return r < a.rows && at < rows ? (tk.t0 + at / group) * a.nqh + kh * group + at % group : -1;
+  };
+  PageWalk<Q27H_KV_F16, 1> walk(a.pg, pt.seq, kh, t0, t1);
+  auto left_of = [&](const TileAt& at) { return vis.end - at.j0 < kTileKeys ? vis.end - at.j0 : kTileKeys; };
+  auto part_of_it = [&](const TileAt& at) { return at.j0 + kTileKeys > vis.n; };
+  auto ask = [&](Staged<false, WAVES>& n, TileAt& at) __attribute__((always_inline)) {
+    at = walk.next(t1);
+    if (at.j0 >= 0) request<false, WAVES, true, true>(n, at.k, at.v, at.j0, left_of(at));
+  };
+  // 8 waves have two tiles on their way; 4 carry twice as much each: one
+  constexpr bool kTwo = WAVES == 8;
+  Staged<false, WAVES> even, odd;
+  TileAt at, te, to;
+  ask(even, at);
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  load_queries<false, WAVES, WAVES>(im, a.scale * kLog2e, [&](int r) {
+    const int gr = row(r);
+    return gr < 0 ? nullptr : a.qn + (size_t)gr * kHD;
+  });
+  __syncthreads();
+  QRegs q;
+  take_queries(q, im[w]);
+  Rows st;
+  rows_init<false>(st, im[w]);
+  const int mine = w * 16 + (threadIdx.x & 15), gr = row(mine);
+  const uint64_t tree[1] = {gr >= 0 ? tree_of(a, tk, (first + mine) / group) : 0ull};
+  const bool active = w * 16 < a.rows && first + w * 16 < rows;
+  __syncthreads();
+  int b = 0;
+  auto put = [&](Staged<false, WAVES>& n, const TileAt& x, int b) __attribute__((always_inline)) {
+    if (x.j0 >= 0) stage<false, WAVES, true, true>(n, buf[b], part_of_it(x), left_of(x), &s_odd[b]);
+  };
+  put(even, at, 0);
+  ask(even, te);
+  if (kTwo) ask(odd, to);
+  __syncthreads();
+  // `at` is in LDS, `x` the next one in `next`, which is then given the one behind those on their way. Two loops, as in
+  // attn_tree; the first takes an even number of tiles.
+  auto step = [&](auto hidden, Staged<false, WAVES>& next, TileAt& x) __attribute__((always_inline)) {
+    constexpr bool kPart = decltype(hidden)::value;
+    if (active) {
+      f4 s[1][2];
+      __builtin_amdgcn_s_setprio(1);
+      scores<false>(buf[b], &q, s);
+      if (kPart) hide<1, kHidden>(s, vis, tree, at.j0);
+      weights<false, kPart>(st, s[0]);
+      accumulate<false, kPart>(st, s[0], buf[b]);
+      if (kPart && s_odd[b]) add_odd(st, s[0], at.v, at.j0, left_of(at));
+    }
+    __builtin_amdgcn_s_setprio(0);
+    b ^= 1;
+    put(next, x, b);
+    at = x;
+    ask(next, x);
+    __syncthreads();
+  };
+  auto full = [&](const TileAt& x) { return x.j0 >= 0 && !part_of_it(x); };
+  if constexpr (kTwo) {
+    while (full(at) && full(te)) {
+      step(std::false_type(), even, te);
+      step(std::false_type(), odd, to);
+    }
+    while (at.j0 >= 0) {
+      step(std::true_type(), even, te);
+      if (at.j0 < 0) break;
+      step(std::true_type(), odd, to);
+    }
+  } else {
+    while (full(at)) step(std::false_type(), even, te);
+    while (at.j0 >= 0) step(std::true_type(), even, te);
+  }
+  if (!active) return;
+  st.l += lane_xor<16>(st.l);
+  st.l += lane_xor32(st.l);
+  if (gr < 0) return;
+  const bool lead = (threadIdx.x & 63) < 16;
+  float* dst;
+  if (pt.parts == 1) {
+    const float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+#pragma unroll
+    for (int i = 0; i < 16; i++) st.o[i] *= inv;
+    dst = a.o + (size_t)gr * kHD;
+    if (a.lse && lead) a.lse[gr] = st.l == 0.0f ? -__builtin_huge_valf() : (st.m + __builtin_amdgcn_logf(st.l)) * kLn2;
+  } else {
+    const size_t place = (size_t)pt.place * a.rows + mine;
+    dst = a.part + place * kHD;
+    if (lead) *(float2*)(a.ml + place * 2) = make_float2(st.m, st.l);
+  }
+  store_rows<true>(st, dst);
+}
+
+// ---------------------------------------------------------------- more than 16 query rows over codes
 // A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
 // of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
 // query rows, and a wave holds a quarter of the outputs. The weights and the V rows go from the one to the other through LDS.
@@ -811,8 +944,8 @@ struct Cut {
   size_t row;    // its place in the results
 };
 // Wave w's share of a row, every WAVES-th part in order: a lane four dims; m and sum are the whole row's.
-template <int WAVES, int rows>
-__device__ __forceinline__ f4 join_of(const PagedArgs& a, const Cut& c, int w, float& m, float& sum) {
+template <int WAVES>
+__device__ __forceinline__ f4 join_of(const PagedArgs& a, const Cut& c, int rows, int w, float& m, float& sum) {
   const int l = threadIdx.x & 63, n = c.n;
   const f4* part = (const f4*)(a.part + c.place * kHD) + l;
   const float2* ml = (const float2*)a.ml + c.place;
@@ -858,7 +991,7 @@ __device__ __forceinline__ f4 join_of(const PagedArgs& a, const Cut& c, int w, f
 }
 // A workgroup joins a row: sequence blockIdx.x, token y, query head z. 16 waves where there are few rows, which may have many
 // parts; 4 where there are many (a row to each wave was slower: 32 sequences 14 us, with 4 waves to a row 5.9).
-template <int WAVES, int ROWS>
+template <int WAVES, int ROWS>  // query rows of a unit; 0: a.rows
 __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArgs a) {
   __shared__ f4 s_o[WAVES][64];
   const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -866,10 +999,11 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
   const int start = uniform_load(a.starts + 2 * b), n = uniform_load(a.starts + 2 * b + 1);
   const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
   if (t >= tk.nt || n <= 1) return;
-  const int group = a.nqh / a.pg.nkvh, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + ROWS - 1) / ROWS;
-  const Cut c = {n, ((size_t)start + (size_t)(kh * groups + r / ROWS) * n) * ROWS + r % ROWS, (size_t)(tk.t0 + t) * a.nqh + h};
+  const int rows = ROWS ? ROWS : a.rows;
+  const int group = a.nqh / a.pg.nkvh, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + rows - 1) / rows;
+  const Cut c = {n, ((size_t)start + (size_t)(kh * groups + r / rows) * n) * rows + r % rows, (size_t)(tk.t0 + t) * a.nqh + h};
   float m, sum;
-  f4 o = join_of<WAVES, ROWS>(a, c, w, m, sum);
+  f4 o = join_of<WAVES>(a, c, rows, w, m, sum);
   s_o[w][l] = o;
   __syncthreads();
   if (w) return;
@@ -881,26 +1015,31 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
 }
 
 struct Layout {
-  int wr, threads, slots, grid;
+  int rows, threads, slots, grid;
   size_t places, bytes;
 };
-// Up to 16 query rows a kv head: one row tile. Two workgroups of four waves run on a compute unit, or one of eight (f16,
-// two row tiles, whose waves read the same cache rows).
+// Units of 16 query rows where a kv head has no more, of 32 otherwise; over f16, where a unit's cache rows would be read again
+// for each 32 query rows, of up to 128, in equal groups. Two workgroups of four waves run on a compute unit, or one of eight.
 Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   Layout y;
-  const int rows = max_tokens * (nqh / nkvh);
-  y.wr = rows <= 16 ? 1 : 2;
-  y.threads = y.wr == 2 && type == Q27H_KV_F16 ? 512 : 256;
-  const int units = n_seqs * nkvh * ((rows + 16 * y.wr - 1) / (16 * y.wr));
+  const int tiles = (max_tokens * (nqh / nkvh) + 15) / 16;
+  y.rows = tiles == 1 ? 16 : 32;
+  y.threads = y.rows == 32 && type == Q27H_KV_F16 ? 512 : 256;
+  if (type == Q27H_KV_F16 && tiles > 2) {
+    const int groups = (tiles + 7) / 8;
+    y.rows = 16 * ((tiles + groups - 1) / groups);
+    y.threads = y.rows <= 64 ? 256 : 512;
+  }
+  const int units = n_seqs * nkvh * ((16 * tiles + y.rows - 1) / y.rows);
   y.slots = 2 * kCUs * 256 / y.threads;
   // over codes, more than 16 query rows are bound by arithmetic: with units of many lengths, half as many shares more leave
   // the last workgroups less of it (200 sequences of 300 to 4096 rows, 4 tokens: 184 -> 173 us); one sequence is cut evenly,
   // and a second round of workgroups costs it (150000 rows: 82 -> 91 us)
-  if (y.wr == 2 && type != Q27H_KV_F16 && units >= kCUs / 2) y.slots = 3 * kCUs;
+  if (y.rows == 32 && type != Q27H_KV_F16 && units >= kCUs / 2) y.slots = 3 * kCUs;
   // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has less than
   // twice its share of parts
   y.grid = units + y.slots;
-  y.places = (size_t)(y.grid < 2 * y.slots ? y.grid : 2 * y.slots) * 16 * y.wr;
+  y.places = (size_t)(y.grid < 2 * y.slots ? y.grid : 2 * y.slots) * y.rows;
   y.bytes = y.places * (kHD + 2) * sizeof(float) + (size_t)n_seqs * 2 * sizeof(int);
   return y;
 }
@@ -948,17 +1087,20 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
     return fail(Q27H_ERR_ARG, "attn_paged: o, lse or ws overlaps another argument");
   PagedArgs a = {};
   a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.tree = tree, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
-  a.slots = y.slots;
+  a.slots = y.slots, a.rows = y.rows;
   a.part = (float*)ws, a.ml = a.part + y.places * kHD, a.starts = (int*)(a.ml + y.places * 2);
   const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);
-  auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.wr == 1 ? one : two), grid, block, 0, stream_of(s), a); };
-  if (kv->type == Q27H_KV_F16) launch(attn_paged_kernel<Q27H_KV_F16, 1>, attn_paged_kernel<Q27H_KV_F16, 2>);
+  auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.rows == 16 ? one : two), grid, block, 0, stream_of(s), a); };
+  auto shared = y.threads == 256 ? attn_paged_shared_kernel<4> : attn_paged_shared_kernel<8>;
+  if (y.rows > 32) hipLaunchKernelGGL(shared, grid, block, 0, stream_of(s), a);
+  else if (kv->type == Q27H_KV_F16) launch(attn_paged_kernel<Q27H_KV_F16, 1>, attn_paged_kernel<Q27H_KV_F16, 2>);
   else if (kv->type == Q27H_KV_Q8) launch(attn_paged_kernel<Q27H_KV_Q8, 1>, attn_paged_wide_kernel<Q27H_KV_Q8>);
   else launch(attn_paged_kernel<Q27H_KV_Q8_Q4, 1>, attn_paged_wide_kernel<Q27H_KV_Q8_Q4>);
   const int qrows = kv->n_seqs * max_tokens * nqh;
   const dim3 all((unsigned)kv->n_seqs, (unsigned)max_tokens, (unsigned)nqh);
   auto join = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, all, dim3(64 * waves), 0, stream_of(s), a); };
-  if (qrows <= 2 * kCUs) join(y.wr == 1 ? attn_paged_join_kernel<16, 16> : attn_paged_join_kernel<16, 32>, 16);
-  else join(y.wr == 1 ? attn_paged_join_kernel<4, 16> : attn_paged_join_kernel<4, 32>, 4);
+  auto pick = [&](auto r16, auto r32, auto any) { return y.rows == 16 ? r16 : y.rows == 32 ? r32 : any; };
+  if (qrows <= 2 * kCUs) join(pick(attn_paged_join_kernel<16, 16>, attn_paged_join_kernel<16, 32>, attn_paged_join_kernel<16, 0>), 16);
+  else join(pick(attn_paged_join_kernel<4, 16>, attn_paged_join_kernel<4, 32>, attn_paged_join_kernel<4, 0>), 4);
   return check_launch("attn_paged");
 }
