@@ -253,20 +253,34 @@ def attn_paged(qn, kv, pos, cu, T, max_tokens, scale, nqh, o, ws, s=None, lse=No
                                 _bytes(ws), _stream(s), _ptr(tree)))
 
 
+_value_types = {}  # of kv_pages_read, filled at its first call
+
+
 def kv_pages_read(kv, start, count, n_out, kout, vout, s=None):
     """Rows start[b] .. start[b] + count[b] - 1 (start None: 0) of each sequence as values in kout and vout, float32, float16 or
     bfloat16 [n_seqs][nkvh][n_out][256] (either may be None)."""
-    import torch
+    if not _value_types:
+        import torch
 
-    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    kinds = {types.get(t.dtype, -1) for t in (kout, vout) if t is not None} or {0}
-    if len(kinds) != 1:
+        _value_types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    one = vout if kout is None else kout
+    if vout is not None and vout.dtype != one.dtype:
         raise ValueError("kv_pages_read: kout and vout have one type")
-    check(lib().q27h_kv_pages_read(kv.ref, _ptr(start), _ptr(count), n_out, kinds.pop(), _ptr(kout), _ptr(vout), _stream(s)))
+    kind = 0 if one is None else _value_types.get(one.dtype, -1)
+    check(lib().q27h_kv_pages_read(kv.ref, _ptr(start), _ptr(count), n_out, kind, _ptr(kout), _ptr(vout), _stream(s)))
 
 
 def draft_verify_ws_bytes(n_seqs, V):
     return int(lib().q27h_draft_verify_ws_bytes(n_seqs, V))
+
+
+def _row_stride(x, T, V):
+    if x is None:
+        return V
+    at = x.stride()
+    if at[-1] != 1:
+        raise ValueError("draft_verify: rows of p and q are contiguous")
+    return at[0] if len(at) == 2 and T > 1 else V
 
 
 def draft_verify(p, q, ids, parent, u, u_last, cu, n_seqs, V, out, path, n_path, ws, s=None, pos=None):
@@ -274,15 +288,9 @@ def draft_verify(p, q, ids, parent, u, u_last, cu, n_seqs, V, out, path, n_path,
     and u_last. p, q: f32 rows of V values, one per token; q None: drafts without probabilities, a tree by parent (None: a
     chain). pos int32 [n_seqs] (may be None) grows by n_path."""
     T = ids.numel()
-
-    def ld(x):
-        at = (1,) if x is None else x.stride()
-        if at[-1] != 1:
-            raise ValueError("draft_verify: rows of p and q are contiguous")
-        return at[0] if len(at) == 2 and T > 1 else V
-
-    check(lib().q27h_draft_verify(_ptr(p), ld(p), _ptr(q), ld(q), _ptr(ids), _ptr(parent), _ptr(u), _ptr(u_last), _ptr(cu), n_seqs, T, V,
-                                  _ptr(out), _ptr(path), _ptr(n_path), _ptr(pos), _ptr(ws), _bytes(ws), _stream(s)))
+    check(lib().q27h_draft_verify(_ptr(p), _row_stride(p, T, V), _ptr(q), _row_stride(q, T, V), _ptr(ids), _ptr(parent), _ptr(u),
+                                  _ptr(u_last), _ptr(cu), n_seqs, T, V, _ptr(out), _ptr(path), _ptr(n_path), _ptr(pos), _ptr(ws),
+                                  _bytes(ws), _stream(s)))
 
 
 class KvLayers:
