@@ -30,6 +30,7 @@ struct PagedArgs {
   int* starts;           // [n_seqs][2]: each sequence's first place, and the parts of each of its units
   int T, most, nqh, slots;  // slots: shares of the whole work, about the workgroups that run at a time
   int rows;                 // query rows of a unit
+  int group;                // query heads of a kv head
   float scale;
 };
 
@@ -186,7 +187,7 @@ struct Demand {
 };
 __device__ __forceinline__ Demand demand_of(const PagedArgs& a, int nt, const Vis& vis, int rows) {
   const int tiles = vis.end > 0 ? (vis.end + kTileKeys - 1) / kTileKeys : 1;
-  return {a.pg.nkvh * ((nt * (a.nqh / a.pg.nkvh) + rows - 1) / rows), (tiles + kWaves - 1) / kWaves * kWaves};
+  return {a.pg.nkvh * ((nt * a.group + rows - 1) / rows), (tiles + kWaves - 1) / kWaves * kWaves};
 }
 // Every unit is cut in parts of one size, its last one what is left: the total by the shares.
 __device__ __forceinline__ int size_of(int total, int slots) {
@@ -206,8 +207,7 @@ struct Part {
 };
 // The i-th of a sequence's parts of one kind, of which each unit has n. The units of a kv head read the same rows: theirs
 // follow each other 8 workgroups apart, which is on one XCD (16 sequences of 32768 q8_0 rows, 12 tokens: 650 -> 632 us).
-__device__ __forceinline__ void place_of(const PagedArgs& a, int i, int n, int units, int& unit, int& k) {
-  const int groups = units / a.pg.nkvh;
+__device__ __forceinline__ void place_of(const PagedArgs& a, int i, int n, int groups, int& unit, int& k) {
   int at = i, g = 0;
   if (groups > 1) {
     const int all = a.pg.nkvh * n, round = i / (8 * groups), j = i - round * 8 * groups;
@@ -263,10 +263,10 @@ __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   auto of = [&](int y) { return __builtin_amdgcn_readlane(y, p.seq); };
   const int w = of(whole);
   p.parts = of(parts);
-  place_of(a, me - of(x), kind == 0 ? w : 1, of(d.units), p.unit, p.k);
+  p.tk = {of(tk.t0), of(tk.nt)};
+  place_of(a, me - of(x), kind == 0 ? w : 1, (p.tk.nt * a.group + rows - 1) / rows, p.unit, p.k);
   if (kind) p.k = w;
   p.place = of(sp - np) + p.unit * p.parts + p.k;
-  p.tk = {of(tk.t0), of(tk.nt)};
   p.pos = of(pos);
   return p;
 }
@@ -353,7 +353,7 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
   const Demand d = demand_of(a, p.tk.nt, vis_of(p.pos, p.tk.nt, cap), rows);
   const int whole = d.span / p.size;
   p.parts = (d.span + p.size - 1) / p.size;
-  place_of(a, i, kind == 0 ? whole : 1, d.units, p.unit, p.k);
+  place_of(a, i, kind == 0 ? whole : 1, (p.tk.nt * a.group + rows - 1) / rows, p.unit, p.k);
   if (kind) p.k = whole;
   p.place = __builtin_amdgcn_readfirstlane(s_part[2]) + p.unit * p.parts + p.k;
   return p;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
   const Part pt = part_of<WR * kWaves * 64>(a, kRows);
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = w % WR, wk = w / WR;
-  const int group = a.nqh / a.pg.nkvh;
+  const int group = a.group;
   const Tokens tk = pt.tk;
   const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_paged_shared_kernel(PagedA
   const Part pt = part_of<WAVES * 64>(a, a.rows);
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = a.nqh / a.pg.nkvh;
+  const int group = a.group;
   const Tokens tk = pt.tk;
   const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + a.rows - 1) / a.rows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * a.rows;
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedAr
   const Part pt = part_of<kWaves * 64>(a, kRows);
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15;
-  const int group = a.nqh / a.pg.nkvh;
+  const int group = a.group;
   const Tokens tk = pt.tk;
   const Vis vis = vis_of(pt.pos, tk.nt, a.pg.max_pages << a.pg.shift);
   const int rows = tk.nt * group, groups = (rows + kRows - 1) / kRows, kh = pt.unit / groups, first = (pt.unit - kh * groups) * kRows;
@@ -1000,7 +1000,7 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
   const Tokens tk = tokens_of(a.cu, b, a.T, a.most);
   if (t >= tk.nt || n <= 1) return;
   const int rows = ROWS ? ROWS : a.rows;
-  const int group = a.nqh / a.pg.nkvh, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + rows - 1) / rows;
+  const int group = a.group, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + rows - 1) / rows;
   const Cut c = {n, ((size_t)start + (size_t)(kh * groups + r / rows) * n) * rows + r % rows, (size_t)(tk.t0 + t) * a.nqh + h};
   float m, sum;
   f4 o = join_of<WAVES>(a, c, rows, w, m, sum);
@@ -1087,7 +1087,7 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
     return fail(Q27H_ERR_ARG, "attn_paged: o, lse or ws overlaps another argument");
   PagedArgs a = {};
   a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.tree = tree, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
-  a.slots = y.slots, a.rows = y.rows;
+  a.slots = y.slots, a.rows = y.rows, a.group = nqh / kv->nkvh;
   a.part = (float*)ws, a.ml = a.part + y.places * kHD, a.starts = (int*)(a.ml + y.places * 2);
   const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);
   auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.rows == 16 ? one : two), grid, block, 0, stream_of(s), a); };

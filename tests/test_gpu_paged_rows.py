@@ -90,3 +90,43 @@ def test_nothing_behind_the_workspace_is_written(G, most, type):  # noqa: F811
         assert (G.down(ws[n:]) == 0xA5).all()
         if len(pos) == 1 and most < 64:
             check(G, q, kp, vp, table, type, pos, new, most, 6, got=(o, lse))
+
+
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("most", [1, 4, 12])
+def test_a_captured_call_follows_the_lengths(G, most, type):  # noqa: F811
+    """Captured at short lengths, replayed as lengths, tokens and the table change: the eager call's bits each time."""
+    import torch
+
+    r = np.random.default_rng(most)
+    nqh, nkvh, B = 24, 4, 5
+    kp, vp, table = P.make_pages(r, [6000, 700, 64, 31, 3000], [most] * B, 64, nkvh, type)
+    kv = handle(G, kp, vp, table, type)
+    T = B * most
+    q = G.up(r.standard_normal((T, nqh, 256)).astype(np.float32))
+    pos, cu = G.i32(*[3] * B), G.up(P.cu_of([1] * B))
+    ws = G.ws(G.ops.attn_paged_ws_bytes(kv, T, most, nqh))
+    out = [G.full((T, nqh, 256), 7.0), G.full((T, nqh), 7.0)]
+
+    def call():
+        G.ops.attn_paged(q, kv, pos, cu, T, most, SCALE, nqh, out[0], ws, lse=out[1])
+
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    steps = [([6000, 700, 64, 31, 3000], [most] * B, None), ([0, 699, 2, 30, 1000], [1, 0, most, most, 0], None),
+             ([5000, 0, 0, 0, 0], [0, most, 1, 0, 0], None), ([700, 6000, 31, 64, 3000], [most] * B, [1, 0, 3, 2, 4])]
+    for at, new, order in steps:
+        pos.copy_(G.i32(*at)), cu.copy_(G.up(P.cu_of(new)))
+        kv.table.copy_(G.up(table if order is None else table[order]))
+        got = []
+        for run in (call, g.replay):
+            for x in out:
+                x.fill_(7.0)
+            run()
+            got.append([G.down(x).copy() for x in out])
+        for a, b in zip(*got):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+        assert np.isfinite(got[1][0]).all()
