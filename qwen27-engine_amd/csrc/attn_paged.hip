@@ -29,6 +29,7 @@ struct PagedArgs {
   float *part, *ml;      // [place][row of its unit][256], [..][2]
   int* starts;           // [n_seqs][2]: each sequence's first place, and the parts of each of its units
   int T, most, nqh, slots;  // slots: shares of the whole work, about the workgroups that run at a time
+  int least;                // tiles; 0: parts are total / slots, else down to half of that where they are no shorter than this
   int rows;                 // query rows of a unit
   int group;                // query heads of a kv head
   float scale;
@@ -189,9 +190,14 @@ __device__ __forceinline__ Demand demand_of(const PagedArgs& a, int nt, const Vi
   const int tiles = vis.end > 0 ? (vis.end + kTileKeys - 1) / kTileKeys : 1;
   return {a.pg.nkvh * ((nt * a.group + rows - 1) / rows), (tiles + kWaves - 1) / kWaves * kWaves};
 }
-// Every unit is cut in parts of one size, its last one what is left: the total by the shares.
-__device__ __forceinline__ int size_of(int total, int slots) {
-  const int each = (total + slots - 1) / slots;
+// Every unit is cut in parts of one size, its last one what is left: the total by the shares. FINE: see a.least.
+template <bool FINE>
+__device__ __forceinline__ int size_of(const PagedArgs& a, int total) {
+  int each = (total + a.slots - 1) / a.slots;
+  if (FINE && a.least) {
+    const int half = (each + 1) / 2;
+    each = half >= a.least ? half : each < a.least ? each : a.least;
+  }
   return each ? (each + kWaves - 1) / kWaves * kWaves : kWaves;
 }
 
@@ -233,6 +239,7 @@ __device__ __forceinline__ int lanes_before(int x) {
   return x;
 }
 // Up to 64 sequences: every wave finds the part by itself, a sequence in each lane, without a barrier.
+template <bool FINE>
 __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   const int l = threadIdx.x & 63, cap = a.pg.max_pages << a.pg.shift;
   const bool is = l < a.pg.n_seqs;
@@ -244,7 +251,7 @@ __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   const Tokens tk = tokens_of(c0, c1, a.T, a.most);
   const Demand d = is ? demand_of(a, tk.nt, vis_of(pos, tk.nt, cap), rows) : Demand{0, kWaves};
   Part p;
-  p.size = size_of(__builtin_amdgcn_readlane(lanes_before(d.units * d.span), 63), a.slots);
+  p.size = size_of<FINE>(a, __builtin_amdgcn_readlane(lanes_before(d.units * d.span), 63));
   const int whole = d.span / p.size, rest = d.span - whole * p.size, parts = whole + (rest > 0);
   const int n0 = d.units * whole, n1 = 2 * rest > p.size ? d.units : 0, n2 = rest && !n1 ? d.units : 0, np = parts > 1 ? d.units * parts : 0;
   const int s0 = lanes_before(n0), s1 = lanes_before(n1), s2 = lanes_before(n2), sp = lanes_before(np);
@@ -270,9 +277,9 @@ __device__ __forceinline__ Part part_of_64(const PagedArgs& a, int rows) {
   p.pos = of(pos);
   return p;
 }
-template <int THREADS>
+template <int THREADS, bool FINE = false>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
-  if (a.pg.n_seqs <= 64) return part_of_64(a, rows);
+  if (a.pg.n_seqs <= 64) return part_of_64<FINE>(a, rows);
   constexpr int kW = THREADS / 64;
   __shared__ int s_total[kW], s_part[3];
   __shared__ Counts s_count[kW];
@@ -298,7 +305,7 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, int rows) {
 #pragma unroll
   for (int k = 0; k < kW; k++) total += s_total[k];
   Part p;
-  p.size = size_of(total, a.slots);
+  p.size = size_of<FINE>(a, total);
   auto count = [&](const Demand& d) {
     const int whole = d.span / p.size, rest = d.span - whole * p.size;
     const uint32_t u = (uint32_t)d.units, parts = whole + (rest > 0);
@@ -674,7 +681,7 @@ template <int TYPE>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_paged_wide_kernel(PagedArgs a) {
   constexpr int kRows = 16 * QT, kV = TYPE == Q27H_KV_Q8_Q4 ? kHD / 2 : kHD, kBias = TYPE == Q27H_KV_Q8_Q4 ? 8 : 128;
   __shared__ WideLds sh;
-  const Part pt = part_of<kWaves * 64>(a, kRows);
+  const Part pt = part_of<kWaves * 64, true>(a, kRows);
   if (pt.seq < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15;
   const int group = a.group;
@@ -1015,7 +1022,7 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
 }
 
 struct Layout {
-  int rows, threads, slots, grid;
+  int rows, threads, slots, least, grid;
   size_t places, bytes;
 };
 // Units of 16 query rows where a kv head has no more, of 32 otherwise; over f16, where a unit's cache rows would be read again
@@ -1032,14 +1039,17 @@ Layout layout_of(int n_seqs, int max_tokens, int nqh, int nkvh, int type) {
   }
   const int units = n_seqs * nkvh * ((16 * tiles + y.rows - 1) / y.rows);
   y.slots = 2 * kCUs * 256 / y.threads;
-  // over codes, more than 16 query rows are bound by arithmetic: with units of many lengths, half as many shares more leave
-  // the last workgroups less of it (200 sequences of 300 to 4096 rows, 4 tokens: 184 -> 173 us); one sequence is cut evenly,
-  // and a second round of workgroups costs it (150000 rows: 82 -> 91 us)
-  if (y.rows == 32 && type != Q27H_KV_F16 && units >= kCUs / 2) y.slots = 3 * kCUs;
-  // beside the whole parts, of which there are `slots` at the most, each unit leaves one; a unit that is cut has less than
+  // over codes, more than 16 query rows are bound by arithmetic: with units of many lengths, parts of half the size leave the
+  // last workgroups less of it (33 sequences of 64 to 131072 rows, 4 tokens: 243 -> 236 us; 64 of 300 to 8000, 8 tokens:
+  // 150 -> 139; equal ones, 100 of 4096: 210 -> 212), but none under 32 tiles, where its start costs more (48 of 200 to 8000:
+  // 65, and 71 with all parts halved). One sequence is cut evenly, and a second round of workgroups costs it (150000 rows:
+  // 82 -> 91 us)
+  y.least = y.rows == 32 && type != Q27H_KV_F16 && units >= kCUs / 2 ? 32 : 0;
+  // beside the whole parts, of which there are `most` at the most, each unit leaves one; a unit that is cut has less than
   // twice its share of parts
-  y.grid = units + y.slots;
-  y.places = (size_t)(y.grid < 2 * y.slots ? y.grid : 2 * y.slots) * y.rows;
+  const int most = y.least ? 2 * y.slots : y.slots;
+  y.grid = units + most;
+  y.places = (size_t)(y.grid < 2 * most ? y.grid : 2 * most) * y.rows;
   y.bytes = y.places * (kHD + 2) * sizeof(float) + (size_t)n_seqs * 2 * sizeof(int);
   return y;
 }
@@ -1087,7 +1097,7 @@ extern "C" int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const i
     return fail(Q27H_ERR_ARG, "attn_paged: o, lse or ws overlaps another argument");
   PagedArgs a = {};
   a.pg = pg, a.qn = qn, a.pos = pos, a.cu = cu, a.tree = tree, a.o = o, a.lse = lse, a.T = T, a.most = max_tokens, a.nqh = nqh, a.scale = scale;
-  a.slots = y.slots, a.rows = y.rows, a.group = nqh / kv->nkvh;
+  a.slots = y.slots, a.least = y.least, a.rows = y.rows, a.group = nqh / kv->nkvh;
   a.part = (float*)ws, a.ml = a.part + y.places * kHD, a.starts = (int*)(a.ml + y.places * 2);
   const dim3 grid((unsigned)y.grid), block((unsigned)y.threads);
   auto launch = [&](auto one, auto two) { hipLaunchKernelGGL((y.rows == 16 ? one : two), grid, block, 0, stream_of(s), a); };
