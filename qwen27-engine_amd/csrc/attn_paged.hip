@@ -544,8 +544,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_paged_shared_kernel(PagedA
 // A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
 // of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
 // query rows, and a wave holds a quarter of the outputs. The weights and the V rows go from the one to the other through LDS.
-// 48 sequences of 500 to 32768 rows with 4 tokens each, V in 4 bits: 180 us of its own, where waves with tiles of their own
-// take 270. What bounds it is no one thing: it runs at 3.4 TB/s, its vector instructions fill half the cycles; without the
+// 48 sequences of 500 to 32768 rows with 4 tokens each, V in 4 bits: 170 us of its own, where waves with tiles of their own
+// take 270. What bounds it is no one thing: it runs at 3.6 TB/s, its vector instructions fill half the cycles; without the
 // weights' scaling it would be 9% faster, without the second f16 terms 16%, without its loads 12%.
 //
 // One reference E for each query row, the same in all waves: a row's product of weight and V scale is 2^(s - E) f d, f the
@@ -997,7 +997,8 @@ __device__ __forceinline__ f4 join_of(const PagedArgs& a, const Cut& c, int rows
   return o;
 }
 // A workgroup joins a row: sequence blockIdx.x, token y, query head z. 16 waves where there are few rows, which may have many
-// parts; 4 where there are many (a row to each wave was slower: 32 sequences 14 us, with 4 waves to a row 5.9).
+// parts; 4 where there are many, of which the first joins a few parts alone, so that the others' places are free for other
+// rows (200 sequences of 300 to 4096 rows, 4 tokens: 17.5 -> 11.8 us; 48 of 500 to 32768: 12.7 -> 11.6).
 template <int WAVES, int ROWS>  // query rows of a unit; 0: a.rows
 __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArgs a) {
   __shared__ f4 s_o[WAVES][64];
@@ -1009,13 +1010,20 @@ __global__ void __launch_bounds__(WAVES * 64, 8) attn_paged_join_kernel(PagedArg
   const int rows = ROWS ? ROWS : a.rows;
   const int group = a.group, kh = h / group, r = t * group + h - kh * group, groups = (tk.nt * group + rows - 1) / rows;
   const Cut c = {n, ((size_t)start + (size_t)(kh * groups + r / rows) * n) * rows + r % rows, (size_t)(tk.t0 + t) * a.nqh + h};
+  const bool alone = WAVES == 4 && n <= 12;
+  if (alone && w) return;
   float m, sum;
-  f4 o = join_of<WAVES>(a, c, rows, w, m, sum);
-  s_o[w][l] = o;
-  __syncthreads();
-  if (w) return;
+  f4 o;
+  if (alone) {
+    o = join_of<1>(a, c, rows, 0, m, sum);
+  } else {
+    o = join_of<WAVES>(a, c, rows, w, m, sum);
+    s_o[w][l] = o;
+    __syncthreads();
+    if (w) return;
 #pragma unroll
-  for (int k = 1; k < WAVES; k++) o += s_o[k][l];
+    for (int k = 1; k < WAVES; k++) o += s_o[k][l];
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   *((f4*)(a.o + c.row * kHD) + l) = o * inv;
   if (a.lse && l == 0) a.lse[c.row] = sum == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
