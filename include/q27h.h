@@ -312,7 +312,8 @@ int q27h_kv_pages_read(const q27h_kv_pages* kv, const int* from, const int* coun
  *   rest = 1 - the p[id] of those refused before it (in 64 bits); one that repeats a refused id is refused. The next token is drawn from p
  *   without the refused ids.
  * A draw: the least x with sum of w over 0 .. x > u_last * S, S the sum over all, w clamped to [0, 1] (NaN: 0) and rounded to
- * multiples of 2^-40: exact, the same in any order. No weight at all: -1. An id outside [0, V) is refused.
+ * multiples of 2^-40. The sums and u_last * S are exact, whatever the row sums to, and so the token is the same in any order.
+ * No weight at all: -1. An id outside [0, V) is refused.
  * out [T]: the tokens that stand behind token 0, then the next one, -1 behind it; path [T]: the rows t that stand (0 first),
  * -1 behind them; n_path [n_seqs]: how many (path and n_path are kv_accept's); pos [n_seqs] (may be NULL) grows by n_path. */
 size_t q27h_draft_verify_ws_bytes(int n_seqs, int V);

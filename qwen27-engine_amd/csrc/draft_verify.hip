@@ -7,9 +7,9 @@
 // the token in it. Bound by HBM: a row of p and, behind a refusal in a chain with probabilities, one of q (64 sequences,
 // 95 MB: 15.5 us, 6.2 TB/s, and 4.4 for the second launch); one sequence by its round trips (3.9 and 3.4).
 //
-// Which token that is must not hang on the order of additions, so weights are brought to multiples of 2^-40 in [0, 1]
-// (adding and taking away 1.5 * 2^12 in 64 bits does that, to the nearest): sums below 4096 are exact in 64 bits, in any
-// order, and the draw is the same in every program that follows the definition.
+// Which token that is must not hang on the order of additions, so weights are whole numbers of 2^-40 in [0, 1] and their sums
+// 64-bit whole numbers, whatever the row sums to: at most 2^24 weights of at most 2^40. u S is formed exactly as well, and the
+// draw is the same in every program that follows the definition.
 #include "q27h_device.h"
 #include "q27h_internal.h"
 
@@ -26,7 +26,7 @@ struct VerifyArgs {
   const float *u, *u_last;
   const int* cu;
   int *out, *path, *n_path, *pos;  // pos may be null
-  double2* sums;                   // [n_seqs][chunks]: of max(p - q, 0), and of p
+  ulonglong2* sums;                // [n_seqs][chunks]: of max(p - q, 0), and of p
   Walk* walks;                     // [n_seqs], for the second launch
   long long ldp, ldq;
   int T, V, chunks;
@@ -92,10 +92,18 @@ __device__ __forceinline__ Walk walk_of(const VerifyArgs& a, int b) {
   return w;
 }
 
-__device__ __forceinline__ double weight_of(double x) {
+// To the nearest whole number of 2^-40: that is the last bit of a number in 64 bits from 4096 to 8192.
+__device__ __forceinline__ uint64_t weight_of(double x) {
   x = x > 0.0 ? x : 0.0;  // NaN: 0
   x = x < 1.0 ? x : 1.0;
-  return (x + 6144.0) - 6144.0;
+  return __builtin_bit_cast(uint64_t, x + 6144.0) - __builtin_bit_cast(uint64_t, 6144.0);
+}
+// floor(u s) for u in [0, 1), s = 2^64 where `over`: a sum of whole numbers exceeds u s where it exceeds this.
+__device__ __forceinline__ uint64_t share_of(float u, uint64_t s, bool over) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, u);
+  const uint32_t m = b >> 23 ? (b & 0x7fffff) | 0x800000 : b, e = b >> 23 ? 150 - (b >> 23) : 149;  // u = m 2^-e, e >= 24
+  const uint64_t lo = (s & 0xffffffff) * m, hi = (s >> 32) * m + (lo >> 32) + (over ? (uint64_t)m << 32 : 0);  // m s = hi 2^32 + lo's low half
+  return e < 32 ? hi << (32 - e) | (lo & 0xffffffff) >> e : e < 96 ? hi >> (e - 32) : 0;
 }
 
 // Four neighbouring values from any address of a float: rows of an odd vocabulary begin anywhere.
@@ -119,13 +127,12 @@ __device__ __forceinline__ void load_chunk(const float* row, int chunk, int n, f
 
 // Sums over the lanes up to each one; 0 comes from lanes that do not exist.
 template <int CTRL, int ROWS>
-__device__ __forceinline__ double from_lanes(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+__device__ __forceinline__ uint64_t from_lanes(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ double lanes_before(double x) {
+__device__ __forceinline__ uint64_t lanes_before(uint64_t x) {
   x += from_lanes<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
   x += from_lanes<0x112, 0xf>(x);
   x += from_lanes<0x114, 0xf>(x);
@@ -134,14 +141,13 @@ __device__ __forceinline__ double lanes_before(double x) {
   x += from_lanes<0x143, 0xc>(x);
   return x;
 }
-__device__ __forceinline__ double read_lane(double x, int l) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint32_t lo = __builtin_amdgcn_readlane((int)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+__device__ __forceinline__ uint64_t read_lane(uint64_t x, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)x, l), hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
+  return (uint64_t)hi << 32 | lo;
 }
 
 __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
-  __shared__ double s_red[2][kThreads / 64];
+  __shared__ uint64_t s_red[2][kThreads / 64];
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, w = threadIdx.x >> 6;
   const Walk k = walk_of(a, b);
   if (chunk == 0 && threadIdx.x == 0) a.walks[b] = k;
@@ -149,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
   float p[kPerThread], q[kPerThread];
   load_chunk(a.p + (size_t)(k.t0 + k.node) * a.ldp, chunk, a.V, p);
   if (k.refused) load_chunk(a.q + (size_t)(k.t0 + k.node + 1) * a.ldq, chunk, a.V, q);
-  double left = 0.0, all = 0.0;
+  uint64_t left = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; i++) all += weight_of(p[i]);
   if (k.refused) {
@@ -163,15 +169,15 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(VerifyArgs a) {
   if (threadIdx.x) return;
   left = (s_red[0][0] + s_red[0][1]) + (s_red[0][2] + s_red[0][3]);
   all = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-  a.sums[(size_t)b * a.chunks + chunk] = make_double2(left, all);
+  a.sums[(size_t)b * a.chunks + chunk] = make_ulonglong2(left, all);
 }
 
 // Every wave finds the chunk by itself, 64 chunks at a time; then a thread has 16 neighbouring values of it.
 __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
-  __shared__ double s_sum[kThreads / 64];
+  __shared__ uint64_t s_sum[kThreads / 64];
   const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  const double2* sums = a.sums + (size_t)b * a.chunks;
-  double left0 = 0.0, all0 = 0.0;  // of the first 64 chunks, on their way with the walk
+  const ulonglong2* sums = a.sums + (size_t)b * a.chunks;
+  uint64_t left0 = 0, all0 = 0;  // of the first 64 chunks, on their way with the walk
   if (l < a.chunks) left0 = sums[l].x, all0 = sums[l].y;
   const Walk k = a.walks[b];
   const int n = __builtin_popcountll(k.path);
@@ -182,40 +188,44 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   const int id = l < k.nt ? a.ids[k.t0 + l] : -1;  // lane t: token t
   const float* prow = a.p + (size_t)(k.t0 + k.node) * a.ldp;
   const float* qrow = k.refused ? a.q + (size_t)(k.t0 + k.node + 1) * a.ldq : prow;
-  // the refused children weigh nothing: each id once (lanes of `bad`), and what it takes from its chunk's sum, exactly
+  // the refused children weigh nothing: each id once (lanes of `bad`), and what it takes from its chunk's sum
   bool lead = (k.tried >> l & 1) && (unsigned)id < (unsigned)a.V;
   for (uint64_t m = k.tried; m; m &= m - 1) {
     const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
     if (__builtin_amdgcn_readlane(id, t) == id && t < l) lead = false;
   }
   const uint64_t bad = __ballot(lead);
-  const double takes = lead ? weight_of(prow[id]) : 0.0;
+  const uint64_t takes = lead ? weight_of(prow[id]) : 0;
   bool use_q = k.refused;
   auto sum_of = [&](int c) {  // of chunk c
-    double x = use_q ? left0 : all0;
-    if (c != l) x = c >= a.chunks ? 0.0 : use_q ? sums[c].x : sums[c].y;
+    uint64_t x = use_q ? left0 : all0;
+    if (c != l) x = c >= a.chunks ? 0 : use_q ? sums[c].x : sums[c].y;
     for (uint64_t m = bad; m; m &= m - 1) {
       const int t = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
-      x -= __builtin_amdgcn_readlane(id, t) / kChunk == c ? read_lane(takes, t) : 0.0;
+      x -= __builtin_amdgcn_readlane(id, t) / kChunk == c ? read_lane(takes, t) : 0;
     }
     return x;
   };
-  double total = 0.0;
+  uint64_t total = 0;
+  bool over = false;  // it is 2^64: every weight of 2^24 is 1
   for (int pass = 0; pass < 2; pass++) {
-    total = 0.0;
+    total = 0;
     for (int c0 = 0; c0 < a.chunks; c0 += 64) total += read_lane(lanes_before(sum_of(c0 + l)), 63);
-    if (total > 0.0 || !use_q) break;
+    if (!total) over = read_lane(sum_of(l), 0) != 0;
+    if (total || over || !use_q) break;
     use_q = false;  // p nowhere above q: the target's own distribution
   }
-  double u = a.u_last[b];
-  u = u > 0.0 ? u : 0.0;
-  u = u < 0x1.fffffep-1 ? u : 0x1.fffffep-1;
-  const double want = u * total;
-  double base = 0.0;
+  float u = a.u_last[b];
+  u = u > 0.0f ? u : 0.0f;
+  u = u < 0x1.fffffep-1f ? u : 0x1.fffffep-1f;
+  const uint64_t want = share_of(u, total, over);
+  // The token, as its chunk, is the one with a weight x behind a sum y such that y <= want < y + x: one alone.
+  auto holds = [want](uint64_t y, uint64_t x) { return y <= want && want - y < x; };
+  uint64_t base = 0;
   int chunk = -1;
   for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
-    const double x = sum_of(c0 + l), to = base + lanes_before(x);
-    const uint64_t hit = __ballot(to - x <= want && want < to);
+    const uint64_t x = sum_of(c0 + l), to = base + lanes_before(x);
+    const uint64_t hit = __ballot(holds(to - x, x));
     if (hit) {
       const int t = __builtin_ctzll(hit);
       chunk = c0 + t;
@@ -227,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
   if (tid == 0) a.out[k.t0 + n - 1] = -1;  // unless there is a token, below and behind the barrier
   if (chunk >= 0) {
     const int i0 = chunk * kChunk + tid * kPerThread;
-    double wt[kPerThread], mine = 0.0;
+    uint64_t wt[kPerThread], mine = 0;
     if (i0 + kPerThread <= a.V) {
       f4u pv[kPerThread / 4], qv[kPerThread / 4];
 #pragma unroll
@@ -240,26 +250,31 @@ __global__ void __launch_bounds__(kThreads) draft_pick_kernel(VerifyArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < kPerThread; i++)
-        wt[i] = i0 + i < a.V ? weight_of(use_q ? (double)prow[i0 + i] - qrow[i0 + i] : (double)prow[i0 + i]) : 0.0;
+        wt[i] = i0 + i < a.V ? weight_of(use_q ? (double)prow[i0 + i] - qrow[i0 + i] : (double)prow[i0 + i]) : 0;
     }
     for (uint64_t m = bad; m; m &= m - 1) {
       const int at = __builtin_amdgcn_readlane(id, __builtin_amdgcn_readfirstlane(__builtin_ctzll(m))) - i0;
 #pragma unroll
-      for (int i = 0; i < kPerThread; i++) wt[i] = at == i ? 0.0 : wt[i];
+      for (int i = 0; i < kPerThread; i++) wt[i] = at == i ? 0 : wt[i];
     }
 #pragma unroll
     for (int i = 0; i < kPerThread; i++) mine += wt[i];
-    double at = lanes_before(mine);
+    uint64_t at = lanes_before(mine);
     if (l == 63) s_sum[w] = at;
     __syncthreads();
     at += base - mine;
 #pragma unroll
-    for (int j = 0; j < kThreads / 64; j++) at += j < w ? s_sum[j] : 0.0;
+    for (int j = 0; j < kThreads / 64; j++) at += j < w ? s_sum[j] : 0;
+    if (holds(at, mine)) {  // one thread: behind its values whose sums are no more than what is left of `want`
+      const uint64_t left = want - at;
+      uint64_t to = 0;
+      int i = i0;
 #pragma unroll
-    for (int i = 0; i < kPerThread; i++) {
-      const double to = at + wt[i];
-      if (at <= want && want < to) a.out[k.t0 + n - 1] = i0 + i;  // one thread's one value
-      at = to;
+      for (int e = 0; e < kPerThread; e++) {
+        to += wt[e];
+        i += to <= left;
+      }
+      a.out[k.t0 + n - 1] = i;
     }
   }
   if (tid >= 64) return;
@@ -284,7 +299,7 @@ int chunks_of(int V) { return (V + kChunk - 1) / kChunk; }
 using namespace q27h;
 
 extern "C" size_t q27h_draft_verify_ws_bytes(int n_seqs, int V) {
-  return n_seqs <= 0 || V <= 0 || V > 1 << 24 ? 0 : (size_t)n_seqs * (chunks_of(V) * sizeof(double2) + sizeof(Walk));
+  return n_seqs <= 0 || V <= 0 || V > 1 << 24 ? 0 : (size_t)n_seqs * (chunks_of(V) * sizeof(ulonglong2) + sizeof(Walk));
 }
 
 extern "C" int q27h_draft_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, const int* ids, const int* parent,
@@ -305,7 +320,7 @@ extern "C" int q27h_draft_verify(const float* p, int64_t ldp, const float* q, in
   if (outputs_overlap({{out, tb}, {path, tb}, {n_path, B}, {pos, B}, {ws, need}},
                       {{p, pb}, {q, qb}, {ids, tb}, {parent, tb}, {u, tb}, {u_last, B}, {cu, B + 4}}))
     return fail(Q27H_ERR_ARG, "draft_verify: a result, pos or ws overlaps another argument");
-  double2* sums = (double2*)ws;
+  ulonglong2* sums = (ulonglong2*)ws;
   VerifyArgs a = {p, q, ids, parent, u, u_last, cu, out, path, n_path, pos, sums, (Walk*)(sums + (size_t)n_seqs * chunks_of(V)),
                   (long long)ldp, (long long)ldq, T, V, chunks_of(V)};
   hipLaunchKernelGGL(draft_sums_kernel, dim3((unsigned)(n_seqs * a.chunks)), dim3(kThreads), 0, stream_of(s), a);
