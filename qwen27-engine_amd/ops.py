@@ -280,6 +280,11 @@ def _row_stride(x, T, V):
     at = x.stride()
     if at[-1] != 1:
         raise ValueError("draft_verify: rows of p and q are contiguous")
+    if len(at) > 2:
+        try:
+            at = x.view(-1, x.shape[-1]).stride()
+        except RuntimeError:
+            raise ValueError("draft_verify: rows of p and q lie evenly apart") from None
     return at[0] if len(at) == 2 and T > 1 else V
 
 
