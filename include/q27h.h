@@ -289,7 +289,8 @@ int q27h_attn_prep_paged(const float* qg, const float* k, const float* v, const 
  * before pos[b], and of the new ones row pos[b] + u where bit u of tree[token] (device, 64-bit, 8-byte aligned, [T]; NULL: those
  * up to its own) is set; with attn_tree's arithmetic and bounds, 4-bit codes entering exactly as q8_0's do. At most max_tokens
  * (1 to 64) tokens of a sequence are taken; those behind them are left out. A token that sees no row gets zeros and -inf. The same call
- * gives the same bits; how a sequence's rows are split, and so the order of its sums, hangs on the lengths of all sequences.
+ * gives the same bits; how a sequence's rows are split, and so the order of its sums, hangs on the lengths and tokens of all
+ * sequences, on n_seqs, max_tokens and the heads: more sequences without tokens may change the last bits.
  * ws: q27h_attn_paged_ws_bytes of the same handle's sizes, T, max_tokens and nqh. */
 size_t q27h_attn_paged_ws_bytes(const q27h_kv_pages* kv, int T, int max_tokens, int nqh);
 int q27h_attn_paged(const float* qn, const q27h_kv_pages* kv, const int* pos, const int* cu, int T, int max_tokens, float scale,

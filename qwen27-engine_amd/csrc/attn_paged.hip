@@ -5,7 +5,7 @@
 // attn_tree. Sequences are of any length, so a unit's tiles of 32 cache rows are cut in parts none of which is longer than a
 // fixed share of the tiles of all units. Every workgroup has a part, which it finds from the lengths of all sequences
 // itself. Up to 16 query rows (over f16 32), its waves each walk tiles of their own with the online softmax of attn_core.h,
-// bound by HBM (128 sequences of 4096 q8_0 rows, one token: 5.4 TB/s; f16, 2048 rows, four tokens: 5.0); with more they share
+// bound by HBM (128 sequences of 4096 q8_0 rows, one token: 5.3 TB/s; f16, 2048 rows, four tokens: 5.0); with more they share
 // them, see below. The parts of a unit that was cut go to the workspace, and a second launch joins those of each query
 // row in order.
 #include <type_traits>
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(WR * kWaves * 64, 2) attn_paged_kernel(PagedAr
 // ---------------------------------------------------------------- more than 32 query rows over f16
 // A row tile for each wave, the cache rows shared through LDS as in attn_tree (attn_shared.h): a tile is worked on while the
 // next one or two are on their way through registers. 16 sequences of 32768 rows, 6 and 12 tokens: 390 and 493 us, where
-// units of 32 query rows that each read the rows take 923 and 1409 (the bytes' floor is 424: at 6 tokens reading alone is
-// faster than a copy); 8 sequences, 64 tokens: 898 for 2462, of which the products with two terms need 701. One sequence of
+// units of 32 query rows that each read the rows take 923 and 1409 (the bytes alone take 311 at a large read's rate);
+// 8 sequences, 64 tokens: 898 for 2462, of which the products with two terms need 701. One sequence of
 // 2000 rows, whose workgroups have four tiles one after the other here: 19.5 and 25.4 for 15.9 and 18.5.
 template <int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) attn_paged_shared_kernel(PagedArgs a) {
@@ -544,8 +544,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_paged_shared_kernel(PagedA
 // A workgroup's four waves share each tile of 128 cache rows. For the scores a wave takes 32 of the rows, for the outputs 64
 // of the 256 dims, both for all of the unit's query rows: no code is turned to a half twice, whatever the number of
 // query rows, and a wave holds a quarter of the outputs. The weights and the V rows go from the one to the other through LDS.
-// 48 sequences of 500 to 32768 rows with 4 tokens each, V in 4 bits: 170 us of its own, where waves with tiles of their own
-// take 270. What bounds it is no one thing: it runs at 3.6 TB/s, its vector instructions fill half the cycles; without the
+// 48 sequences of 500 to 32768 rows with 4 tokens each, V in 4 bits: 178 us of its own, where waves with tiles of their own
+// take 270. What bounds it is no one thing: it runs at 3.5 TB/s, its vector instructions fill half the cycles; without the
 // weights' scaling it would be 9% faster, without the second f16 terms 16%, without its loads 12%.
 //
 // One reference E for each query row, the same in all waves: a row's product of weight and V scale is 2^(s - E) f d, f the

@@ -5,7 +5,7 @@
 // the row where the walk ended, over the whole vocabulary: the sum S of the row's weights, and the first token whose sum up
 // to it passes u S. The row is cut in chunks; the first launch leaves each chunk's sum, the second finds the chunk and then
 // the token in it. Bound by HBM: a row of p and, behind a refusal in a chain with probabilities, one of q (64 sequences,
-// 95 MB: 15.5 us, 6.2 TB/s, and 4.4 for the second launch); one sequence by its round trips (3.9 and 3.4).
+// 95 MB: 15.0 us, 6.4 TB/s, and 4.4 for the second launch); one sequence by its round trips (3.9 and 3.4).
 //
 // Which token that is must not hang on the order of additions, so weights are whole numbers of 2^-40 in [0, 1] and their sums
 // 64-bit whole numbers, whatever the row sums to: at most 2^24 weights of at most 2^40. u S is formed exactly as well, and the
